@@ -275,6 +275,113 @@ KUDACUDA_API int kudacuda_lm_head_argmax_bf16(void* handle, uint64_t input, uint
                                               float epsilon, uint64_t stream);
 KUDACUDA_API int64_t kudacuda_lm_head_workspace_floats(void);
 
+/* ------------------------------------- several sequences, paged KV cache */
+/* NEW — what serving several sequences takes beside the one-sequence path (one
+ * contiguous cache, greedy argmax; the reference serves one sequence,
+ * README.md:170).  Types: dtype 1 = bf16, 2 = fp16 (logits also 0 = fp32).
+ *
+ * A paged cache is a pool of num_pages pages of page_size tokens (a power of two,
+ * 1..4096) for keys and one for values: the head_dim elements of (page, head,
+ * token in the page) begin at page * page_stride + head * head_stride + token *
+ * token_stride elements, the same in both pools.  [pages, heads, page_size, dim]
+ * and [pages, page_size, heads, dim] are both such pools.  Slot page * page_size
+ * + token names a token's place.
+ *
+ * These calls use the caller's buffers only (no scratch of the handle), run on
+ * the handle's device, whichever is current, and may be captured; a workspace
+ * must not be in use by another call or graph replay at the same time. */
+
+/* Rotary positions: output = the rows of input [tokens, heads, head_dim] with the
+ * first rotary_dim dims of every head turned, pair i by positions[token] *
+ * inv_freq[i] (float64 [rotary_dim / 2]; the product is formed in 64 bits, so
+ * far positions and any scaling of the frequencies hold), times amplitude.  Pairs
+ * are dims i and i + rotary_dim / 2, or 2 i and 2 i + 1 with interleaved = 1.
+ * positions int32.  Strides are elements between tokens; output may be input
+ * (same stride), else they must not overlap.  Contract: tokens>=0, heads 1..4096,
+ * head_dim even, 2..256, rotary_dim even, 2..head_dim.  Rows, strides and
+ * rotary_dim in whole 16-byte pieces (rotary_dim a multiple of 16) run faster. */
+KUDACUDA_API int kudacuda_rope(void* handle, uint64_t input, uint64_t inv_freq, uint64_t positions, uint64_t output,
+                               int64_t dtype, int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim,
+                               int64_t interleaved, int64_t input_stride, int64_t output_stride, float amplitude,
+                               uint64_t stream);
+
+/* Rotary positions and the append to a paged cache in one pass: query rows are
+ * turned into query_output [tokens, query_heads, head_dim] (may be query), key rows
+ * turned and value rows copied into the pools at slots[token] (int64).  A token
+ * whose slot is negative or past the pool is padding: nothing of it is written.
+ * Slots of one call must differ.  Contract as for kudacuda_rope, kv_heads 1..4096;
+ * query, key and value may be parts of one projection's rows (strides). */
+KUDACUDA_API int kudacuda_rope_paged_append(
+    void* handle, uint64_t query, uint64_t key, uint64_t value, uint64_t inv_freq, uint64_t positions, uint64_t slots,
+    uint64_t query_output, uint64_t key_pages, uint64_t value_pages, int64_t dtype, int64_t tokens,
+    int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t interleaved,
+    int64_t query_stride, int64_t key_stride, int64_t value_stride, int64_t output_stride, int64_t num_pages,
+    int64_t page_size, int64_t page_stride, int64_t head_stride, int64_t token_stride, float amplitude,
+    uint64_t stream);
+
+/* Causal attention of new tokens over a paged cache.  Sequence i's new tokens are
+ * rows query_starts[i] .. query_starts[i + 1] of query (int32 [sequences + 1],
+ * ascending); it has kv_lens[i] cached tokens (int32), the new ones the last of
+ * them, token j in page page_table[i * table_stride + j / page_size] (int32).  New
+ * token t sees the keys up to its own, kv_lens[i] - q_len + t; a row that sees none
+ * is zero.  Rows of no sequence are left as they were.  A sequence whose kv_len is
+ * negative or past its table row, and a row that sees a page id outside the pool,
+ * become NaN; such pages are not read.
+ * max_query_len and max_kv_len say how long the longest sequence may be; they
+ * choose kernels and key splits, results hold whatever they are.  Long caches with
+ * few rows are split over the chip through the workspace:
+ * kudacuda_paged_attention_workspace_bytes() of the same sizes, or less (fewer
+ * splits), or none (0, 0).
+ * Contract: head_dim 64 or 128, query_heads a multiple of kv_heads (both 1..1024),
+ * 1..65536 sequences, tokens * query_heads <= 2^30, table_stride * page_size <=
+ * 2^30, strides multiples of 8, buffers (but the int32 ones) on 16-byte
+ * boundaries, positive finite scale. */
+KUDACUDA_API int kudacuda_paged_attention(void* handle, uint64_t query, uint64_t key_pages, uint64_t value_pages,
+                                          uint64_t page_table, uint64_t query_starts, uint64_t kv_lens, uint64_t output,
+                                          uint64_t workspace, int64_t workspace_bytes, int64_t dtype, int64_t tokens,
+                                          int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
+                                          int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t query_stride, int64_t output_stride, int64_t num_pages,
+                                          int64_t page_size, int64_t table_stride, int64_t page_stride,
+                                          int64_t head_stride, int64_t token_stride, float scale, uint64_t stream);
+KUDACUDA_API int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences, int64_t max_query_len,
+                                                              int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
+                                                              int64_t head_dim);
+
+/* Copies pages inside a cache: for every pair (source, destination) of `pairs`
+ * (int32 [count][2] in HOST memory, read before the call returns) and each of
+ * `pools` pools (layers' keys and values) page_bytes bytes at pool + i *
+ * pool_stride + page * page_stride (bytes).  Forking copies a shared last page,
+ * compaction moves high pages to free low ones; the bookkeeping is the caller's
+ * (kudacuda_amd/paged_cache.py).  Destinations must differ from each other and
+ * from the sources of other pairs; other lists are refused.  Contract: page ids in
+ * [0, num_pages), everything in whole 16-byte pieces on 16-byte boundaries,
+ * page_stride and (pools > 1) pool_stride >= page_bytes.  A captured call keeps
+ * its pairs. */
+KUDACUDA_API int kudacuda_copy_pages(void* handle, uint64_t pool, uint64_t pairs, int64_t count, int64_t pools,
+                                     int64_t num_pages, int64_t page_bytes, int64_t page_stride, int64_t pool_stride,
+                                     uint64_t stream);
+
+/* Next tokens of rows of logits, drawn with one uniform number u = random[row]
+ * (fp32, [0, 1)) each; the sampling counterpart of kudacuda_lm_head_argmax_bf16.
+ * With w = exp((logit - max) / temperature) and tokens ordered by (logit
+ * descending, id ascending), top_k keeps the first k (k <= 0: all), top_p of these
+ * the ones before which the weights sum to less than p times the weight of these
+ * (p >= 1: all), min_p of these the ones with w >= min_p; the first token is always
+ * kept.  tokens_out (int32) is the lowest id whose kept weights, summed by id, pass
+ * u times their sum; chances (fp32, may be 0) its share of that sum.  Weights are
+ * formed in 64 bits and summed exactly, so equal inputs give equal tokens.
+ * temperature <= 0 takes the first token (chance 1).  temperature, top_k (int32),
+ * top_p and min_p are arrays of one value a row, each may be 0 (off).  NaN logits
+ * count as -inf; a row of nothing else gives token 0 with chance 0.
+ * Contract: rows 0..65535, vocab 1..2^20, stride >= vocab; workspace of
+ * kudacuda_sample_workspace_bytes(rows, vocab) bytes on a 16-byte boundary. */
+KUDACUDA_API int kudacuda_sample_tokens(void* handle, uint64_t logits, uint64_t random, uint64_t temperature,
+                                        uint64_t top_k, uint64_t top_p, uint64_t min_p, uint64_t tokens_out,
+                                        uint64_t chances, uint64_t workspace, int64_t workspace_bytes, int64_t dtype,
+                                        int64_t rows, int64_t vocab, int64_t stride, uint64_t stream);
+KUDACUDA_API int64_t kudacuda_sample_workspace_bytes(int64_t rows, int64_t vocab);
+
 /* ------------------------------------------------------------- graphs */
 /* reference include/kudacuda.h:257-263 — capture the caller's stream (global
  * mode), instantiate on end, replay with hipGraphLaunch, reset.  A replay of

@@ -63,6 +63,13 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "kudacuda_gqa_workspace_floats": ([_i64], _i64),
     "kudacuda_lm_head_argmax_bf16": ([_vp] + [_u64] * 5 + [_i64, _i64, _f, _u64], _i),
     "kudacuda_lm_head_workspace_floats": ([], _i64),
+    "kudacuda_rope": ([_vp] + [_u64] * 4 + [_i64] * 8 + [_f, _u64], _i),
+    "kudacuda_rope_paged_append": ([_vp] + [_u64] * 9 + [_i64] * 16 + [_f, _u64], _i),
+    "kudacuda_paged_attention": ([_vp] + [_u64] * 8 + [_i64] * 17 + [_f, _u64], _i),
+    "kudacuda_paged_attention_workspace_bytes": ([_i64] * 7, _i64),
+    "kudacuda_copy_pages": ([_vp, _u64, _u64] + [_i64] * 6 + [_u64], _i),
+    "kudacuda_sample_tokens": ([_vp] + [_u64] * 9 + [_i64] * 5 + [_u64], _i),
+    "kudacuda_sample_workspace_bytes": ([_i64] * 2, _i64),
     "kudacuda_begin_capture": ([_vp, _u64], _i),
     "kudacuda_end_capture": ([_vp, _u64], _i),
     "kudacuda_replay_graph": ([_vp, _u64], _i),

@@ -305,6 +305,99 @@ struct LmHeadArgs {
 hipError_t launch_lm_head_argmax(const LmHeadArgs& args, hipStream_t stream);
 int64_t lm_head_workspace_floats();  // size of block_best
 
+// ----------------------------------------------- several sequences, paged cache
+// The pools of a paged cache: row (page, head, offset) of kv_heads rows of
+// head_dim elements begins at page * page_stride + head * head_stride + offset *
+// token_stride; a page holds 1 << page_shift tokens.
+
+// Rotary positions of q and k, values beside them; with slots (page << page_shift
+// | offset) keys and values go into the pools, without (k, v null) only q is turned.
+constexpr int kRopeMaxDim = 256;
+struct RopeArgs {
+    const uint16_t* q = nullptr;
+    const uint16_t* k = nullptr;
+    const uint16_t* v = nullptr;
+    const double* inv_freq = nullptr;  // [rotary_dim / 2]
+    const int32_t* positions = nullptr;
+    const int64_t* slots = nullptr;
+    uint16_t* q_out = nullptr;
+    uint16_t* k_pages = nullptr;
+    uint16_t* v_pages = nullptr;
+    int64_t tokens = 0;
+    int q_heads = 0;
+    int kv_heads = 0;  // 0 without slots
+    int head_dim = 0;
+    int rotary_dim = 0;
+    bool interleaved = false;
+    int page_shift = 0;
+    int64_t q_stride = 0, k_stride = 0, v_stride = 0, out_stride = 0;  // elements between tokens
+    int64_t num_pages = 0;
+    int64_t page_stride = 0, head_stride = 0, token_stride = 0;
+    float amplitude = 1.0f;
+};
+hipError_t launch_rope(Act act, const RopeArgs& args, hipStream_t stream);
+
+struct PagedAttnArgs {
+    const uint16_t* q = nullptr;
+    const uint16_t* k = nullptr;
+    const uint16_t* v = nullptr;
+    const int32_t* table = nullptr;    // [sequences, table_stride] page ids
+    const int32_t* starts = nullptr;   // [sequences + 1] first rows
+    const int32_t* kv_lens = nullptr;  // [sequences]
+    uint16_t* out = nullptr;
+    float* partials = nullptr;  // [tokens, q_heads, splits, head_dim], then (max, sum) of each
+    int64_t tokens = 0;
+    int64_t sequences = 0;
+    int64_t q_heads = 0, kv_heads = 0, group = 0, head_dim = 0;
+    int64_t q_stride = 0, out_stride = 0;
+    int64_t num_pages = 0, table_stride = 0;
+    int64_t page_stride = 0, head_stride = 0, token_stride = 0;
+    int page_shift = 0;
+    float scale_log2 = 0.0f;  // scale * log2(e)
+};
+// Which kernels a call takes and over how many key splits: the few-row kernel for
+// sequences with few rows, the tile kernel for the others (0: not launched).
+struct PagedAttnPlan {
+    int64_t few_splits = 0;
+    int64_t tile_splits = 0;
+    int64_t slots = 0;   // tile slots of the tile kernel's grid
+    int64_t splits = 0;  // the larger: row length of the partials
+    int64_t workspace_bytes = 0;
+};
+PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
+                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t workspace_bytes);
+hipError_t launch_paged_attention(Act act, const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t stream);
+
+constexpr int kPagePairs = 448;  // pairs of a launch: 3584 bytes of kernel arguments
+struct CopyPagesArgs {
+    uint8_t* pool = nullptr;
+    const int32_t* pairs = nullptr;  // host memory, [count][2]
+    int64_t count = 0;
+    int64_t pools = 0;
+    int64_t page_bytes = 0, page_stride = 0, pool_stride = 0;
+};
+hipError_t launch_copy_pages(const CopyPagesArgs& args, hipStream_t stream);
+
+// Next tokens of rows of logits (kc_sample.hip).
+struct SampleArgs {
+    const void* logits = nullptr;
+    const float* random = nullptr;
+    const float* temperature = nullptr;  // the settings may be null: off
+    const int32_t* top_k = nullptr;
+    const float* top_p = nullptr;
+    const float* min_p = nullptr;
+    int32_t* tokens = nullptr;
+    float* chances = nullptr;  // may be null
+    uint8_t* workspace = nullptr;
+    int64_t rows = 0;
+    int64_t vocab = 0;
+    int64_t stride = 0;
+};
+constexpr int64_t kSampleMaxVocab = int64_t{1} << 20;
+int64_t sample_workspace_bytes(int64_t rows, int64_t vocab);
+// dtype: 0 = fp32, 1 = bf16, 2 = fp16
+hipError_t launch_sample(int dtype, const SampleArgs& args, hipStream_t stream);
+
 // ------------------------------------------------------------------ misc ops
 hipError_t launch_vector_add(const float* a, const float* b, float* out, int64_t n, hipStream_t stream);
 hipError_t launch_rmsnorm_f32(const float* x, const float* w, float* y, int64_t rows, int64_t hidden, float eps,

@@ -1,0 +1,859 @@
+// Attention of a ragged batch of new tokens over a paged KV cache.
+//
+// Sequence i brings q_len new tokens (rows query_starts[i] .. query_starts[i + 1]
+// of the queries) and has kv_len cached rows, its new tokens' among them; token t
+// of it stands at position kv_len - q_len + t and sees the keys up to there:
+//     out = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - max)
+// in one pass over the keys with a running maximum and sum (fp32).  A row that
+// sees no key is zero.
+//
+// The query heads of a KV head share its keys, so the rows of one (sequence, KV
+// head) are its tokens times those heads, row r = token r / G, head r % G, and a
+// block takes a tile of them as the columns of S^T = K Q^T and O^T = V^T P^T.  In
+// that orientation a lane's scores belong to one column, and they lie in the
+// order in which the second product takes its weights if V's keys are read in
+// the same order: the weights never leave their lane.  V's rows go to LDS as they
+// are and are read transposed (ds_read_b64_tr_b16: a group of 16 lanes reads 4
+// keys x 16 dims and each lane receives the 4 keys of one dim).
+#include "kc_device.h"
+#include "kc_kernels.h"
+
+namespace kc {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr int kThreads = 256;
+
+// ------------------------------------------------------------ element types
+__device__ __forceinline__ floatx4 mfma16(Bf16, uint4 a, uint4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mfma16(F16, uint4 a, uint4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mfma32(Bf16, uint4 a, uint4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mfma32(F16, uint4 a, uint4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+// Two fp32 values rounded to nearest, the first in the low half; and back.
+__device__ __forceinline__ uint32_t pack(Bf16, float lo, float hi) { return pack2(lo, hi); }
+__device__ __forceinline__ uint32_t pack(F16, float lo, float hi) {
+    typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+    const halfx2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+template <typename T>
+__device__ __forceinline__ float low(uint32_t v) {
+    return T::load(static_cast<uint16_t>(v & 0xffffu));
+}
+template <typename T>
+__device__ __forceinline__ float high(uint32_t v) {
+    return T::load(static_cast<uint16_t>(v >> 16));
+}
+
+// Transposed read of 4 keys x 16 dims by 16 lanes (each lane: 8 bytes of a row).
+__device__ __forceinline__ uint2 read_transposed(const uint8_t* p) {
+    const auto lds = (__attribute__((address_space(3))) shortx4*)(__attribute__((address_space(3))) const uint8_t*)p;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds));
+}
+
+// ------------------------------------------------------------- the sequence
+// What a block needs of its sequence.  Lengths come from device memory; whatever
+// they hold, rows stay inside [0, tokens) and keys inside the sequence's table
+// row.  A kv_len that does not fit the table row gives NaN rows.
+struct Sequence {
+    int first;     // row of the first new token
+    int q_len;
+    int kv_len;
+    bool bad;
+};
+__device__ __forceinline__ Sequence sequence(const PagedAttnArgs& a, int index) {
+    Sequence s;
+    const int tokens = static_cast<int>(a.tokens);
+    const int begin = a.starts[index];
+    const int end = a.starts[index + 1];
+    s.first = begin < 0 ? 0 : (begin < tokens ? begin : tokens);
+    const int last = end < tokens ? end : tokens;
+    s.q_len = last > s.first ? last - s.first : 0;
+    const int kv = a.kv_lens[index];
+    s.bad = kv < 0 || kv > (a.table_stride << a.page_shift);
+    s.kv_len = s.bad ? 0 : kv;
+    return s;
+}
+
+// Key j of a sequence: element offset of its row in the pools, and whether its
+// page exists (a page id outside the pool is read as page 0 and reported).
+__device__ __forceinline__ int64_t key_row(const PagedAttnArgs& a, int page, int key, bool& bad) {
+    bad |= static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.num_pages);
+    const int64_t id = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages) ? page : 0;
+    return id * a.page_stride + static_cast<int64_t>(key & ((1 << a.page_shift) - 1)) * a.token_stride;
+}
+
+// ----------------------------------------------------------- careful columns
+// Columns [c0, c0 + count) of a (sequence, KV head) over keys [begin, end) in
+// plain fp32, 16 lanes a column: where a product met an infinity or NaN of a key
+// that a column does not see (0 * inf), or a page id is outside the pool (the
+// columns that see it become NaN).
+template <typename T, int D>
+__device__ __forceinline__ void careful_columns(const PagedAttnArgs& a, const Sequence& s, const int32_t* table, int g,
+                                                int c0, int count, int begin, int end, int split, int splits) {
+    constexpr int kDims = D / 16;
+    const int G = static_cast<int>(a.group);
+    const int d0 = static_cast<int>(threadIdx.x) % 16 * kDims;
+    for (int c = c0 + static_cast<int>(threadIdx.x) / 16; c < c0 + count; c += kThreads / 16) {
+        const int token = c / G;
+        const int head = g * G + c % G;
+        const int pos = s.kv_len - s.q_len + token;
+        const int stop = end < pos + 1 ? end : pos + 1;
+        const int64_t row = s.first + token;
+        const uint16_t* qp = a.q + row * a.q_stride + head * D + d0;
+        float acc[kDims] = {};
+        float m = kNegInf;
+        float l = 0.0f;
+        for (int key = begin; key < stop; ++key) {
+            bool bad = false;
+            const int64_t at = key_row(a, table[key >> a.page_shift], key, bad) + g * a.head_stride + d0;
+            float dot = 0.0f;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                dot = fmaf(T::load(qp[d]), T::load(a.k[at + d]), dot);
+            }
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1) {
+                dot += __shfl_xor(dot, o, 16);
+            }
+            const float sc = bad ? __builtin_nanf("") : dot * a.scale_log2;
+            const float m_new = fmaxf(m, sc);
+            const float m_sub = m_new == kNegInf ? 0.0f : m_new;
+            const float corr = __builtin_amdgcn_exp2f(m - m_sub);
+            const float p = __builtin_amdgcn_exp2f(sc - m_sub);
+            l = l * corr + p;
+            m = m_new;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                // (a weight of zero takes nothing from an infinite value)
+                acc[d] = acc[d] * corr + (p == 0.0f ? 0.0f : p * T::load(a.v[at + d]));
+            }
+        }
+        if (splits == 1) {
+            uint16_t* out = a.out + row * a.out_stride + head * D + d0;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                out[d] = T::store(l == 0.0f ? 0.0f : acc[d] / l);
+            }
+        } else {
+            const int64_t at = (row * a.q_heads + head) * splits + split;
+            float* part = a.partials + at * D + d0;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                part[d] = acc[d];
+            }
+            if (d0 == 0) {
+                float* ml = a.partials + a.tokens * a.q_heads * splits * D + 2 * at;
+                ml[0] = m;
+                ml[1] = l;
+            }
+        }
+    }
+}
+
+// Rows of a sequence whose kv_len does not fit its table.
+template <typename T, int D>
+__device__ __forceinline__ void nan_columns(const PagedAttnArgs& a, const Sequence& s, int g, int c0, int count,
+                                            int splits) {
+    const int G = static_cast<int>(a.group);
+    for (int i = threadIdx.x; i < count * D; i += kThreads) {
+        const int c = c0 + i / D;
+        const int64_t row = s.first + c / G;
+        const int head = g * G + c % G;
+        if (splits == 1) {
+            a.out[row * a.out_stride + head * D + i % D] = T::store(__builtin_nanf(""));
+        } else if (i % D == 0) {
+            float* ml = a.partials + a.tokens * a.q_heads * splits * D + 2 * ((row * a.q_heads + head) * splits);
+            for (int k = 0; k < splits; ++k) {
+                ml[2 * k] = 0.0f;
+                ml[2 * k + 1] = __builtin_nanf("");
+            }
+        }
+    }
+}
+
+// One column's merged result: 8 consecutive dims from d0.
+template <typename T, int D>
+__device__ __forceinline__ void put_column(const PagedAttnArgs& a, int64_t row, int head, int d0, const float (&v)[8],
+                                           float m, float l, int split, int splits) {
+    if (splits == 1) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = l == 0.0f ? 0u : pack(T{}, v[2 * i] / l, v[2 * i + 1] / l);
+        }
+        *reinterpret_cast<uint4*>(a.out + row * a.out_stride + head * D + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+        return;
+    }
+    const int64_t at = (row * a.q_heads + head) * splits + split;
+    float* part = a.partials + at * D + d0;
+    *reinterpret_cast<float4*>(part) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(part + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    if (d0 == 0) {
+        *reinterpret_cast<float2*>(a.partials + a.tokens * a.q_heads * splits * D + 2 * at) = make_float2(m, l);
+    }
+}
+
+// Splits of a column that no block of its kind writes weigh nothing.
+template <int D>
+__device__ __forceinline__ void clear_splits(const PagedAttnArgs& a, const Sequence& s, int g, int c0, int count,
+                                             int from, int splits) {
+    const int G = static_cast<int>(a.group);
+    const int n = splits - from;
+    for (int i = threadIdx.x; i < count * n; i += kThreads) {
+        const int c = c0 + i / n;
+        const int64_t at = ((s.first + c / G) * a.q_heads + g * G + c % G) * splits + from + i % n;
+        *reinterpret_cast<float2*>(a.partials + a.tokens * a.q_heads * splits * D + 2 * at) = make_float2(kNegInf, 0.0f);
+    }
+}
+
+// ------------------------------------------------------------------ few rows
+// A (sequence, KV head) with at most kFewRows rows, the form of single tokens:
+// the four waves take alternate units of 32 keys, 16 columns at a time, K straight
+// from memory into the first product's operand, V through the wave's own LDS.
+constexpr int kFewRows = 32;
+constexpr int kUnit = 32;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttnArgs a, int few_splits, int splits,
+                                                                       int few_rows) {
+    constexpr int kSteps = D / 32;   // products of 32 dims a score
+    constexpr int kPieces = D / 8;   // 16-byte pieces of a row
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
+    __shared__ float s_ml[4][16][2];
+    __shared__ int s_redo;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15;
+    const int q = lane >> 4;
+    const int split = static_cast<int>(blockIdx.x) % few_splits;
+    const int g = static_cast<int>(blockIdx.x) / few_splits % static_cast<int>(a.kv_heads);
+    const int index = static_cast<int>(blockIdx.x) / few_splits / static_cast<int>(a.kv_heads);
+    const Sequence s = sequence(a, index);
+    const int G = static_cast<int>(a.group);
+    const int rows = s.q_len * G;
+    if (rows == 0 || rows > few_rows) {
+        return;
+    }
+    if (s.bad) {
+        if (split == 0) {
+            nan_columns<T, D>(a, s, g, 0, rows, splits);
+        }
+        return;
+    }
+    if (split == 0 && splits > few_splits) {
+        clear_splits<D>(a, s, g, 0, rows, few_splits, splits);
+    }
+    const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
+    const uint16_t* const kbase = a.k + g * a.head_stride;
+    const uint16_t* const vbase = a.v + g * a.head_stride;
+    uint8_t* const s_v = s_mem + wave * (kUnit * D * 2);
+
+    for (int c0 = 0; c0 < rows; c0 += 16) {
+        const int count = rows - c0 < 16 ? rows - c0 : 16;
+        const int column = c0 + (r < count ? r : count - 1);
+        const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
+        const int head = g * G + column % G;
+        const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
+        const int keys = ends > 0 ? ends : 0;
+        const int units = (keys + kUnit - 1) / kUnit;
+        const int per_split = ((units + 3) / 4 + few_splits - 1) / few_splits * 4;
+        const int u_end = (split + 1) * per_split < units ? (split + 1) * per_split : units;
+        int unit = split * per_split + wave;
+
+        uint4 qf[kSteps];
+        {
+            const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D + 8 * q;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                qf[i] = *reinterpret_cast<const uint4*>(src + 32 * i);
+            }
+        }
+        bool bad = false;
+        int64_t at[2];
+        const auto place = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int key = u * kUnit + 16 * t + r;
+                const int k = key < keys ? key : keys - 1;
+                at[t] = key_row(a, table[k >> a.page_shift], k, bad) + 8 * q;
+            }
+        };
+        uint4 kf[2][kSteps], vf[2][kSteps];
+        const auto fetch = [&](uint4 (&f)[2][kSteps], const uint16_t* base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    f[t][i] = load_stream(reinterpret_cast<const uint4*>(base + at[t] + 32 * i));
+                }
+            }
+        };
+        floatx4 acc[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            acc[i] = floatx4{};
+        }
+        float m_run = kNegInf;
+        float l_run = 0.0f;
+        if (unit < u_end) {
+            place(unit);
+            fetch(kf, kbase);
+            fetch(vf, vbase);
+        }
+        for (; unit < u_end; unit += 4) {
+            // V's rows, their 16-byte pieces swizzled so that the 8 rows of a
+            // transposed half-wave read lie in different banks
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int row = 16 * t + r;
+                    const int piece = (4 * i + q) ^ (((row & 7) << 1) % kPieces);
+                    *reinterpret_cast<uint4*>(s_v + row * (D * 2) + piece * 16) = vf[t][i];
+                }
+            }
+            const bool more = unit + 4 < u_end;
+            if (more) {
+                place(unit + 4);
+                fetch(vf, vbase);
+            }
+            floatx4 sc[2] = {floatx4{}, floatx4{}};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                sc[0] = mfma16(T{}, kf[0][i], qf[i], sc[0]);
+                sc[1] = mfma16(T{}, kf[1][i], qf[i], sc[1]);
+            }
+            if (more) {
+                fetch(kf, kbase);
+            }
+            // sc[t][i]: key 16 t + 4 q + i of the unit
+            const int rel = pos - unit * kUnit - 4 * q;
+            float mx = kNegInf;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[t][i] = 16 * t + i <= rel ? sc[t][i] * a.scale_log2 : kNegInf;
+                    mx = fmaxf(mx, sc[t][i]);
+                }
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float m_new = fmaxf(m_run, mx);
+            const float m_sub = m_new == kNegInf ? 0.0f : m_new;
+            const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+            m_run = m_new;
+            l_run *= corr;
+            // weights as two 16-bit parts (16 bits of the fp32 weight in bf16, 22
+            // in fp16): this form waits for memory, the second product is free
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_sub);
+                const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_sub);
+                l_run += p0 + p1;
+                hi[e] = pack(T{}, p0, p1);
+                lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
+            }
+            const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint2 part[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int row = 16 * t + 4 * q + r / 4;
+                    const int piece = (2 * i + (r & 3) / 2) ^ (((row & 7) << 1) % kPieces);
+                    part[t] = read_transposed(s_v + row * (D * 2) + piece * 16 + (r & 1) * 8);
+                }
+                const uint4 vt = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[i][e] *= corr;
+                }
+                acc[i] = mfma16(T{}, vt, ph, acc[i]);
+                acc[i] = mfma16(T{}, vt, pl, acc[i]);
+            }
+        }
+        l_run += __shfl_xor(l_run, 16, 64);
+        l_run += __shfl_xor(l_run, 32, 64);
+        // the waves' columns meet in LDS, each in the wave's own part: [column][dim]
+        __syncthreads();
+        if (tid == 0) {
+            s_redo = 0;
+        }
+        float* const s_acc = reinterpret_cast<float*>(s_mem);  // [wave][16][D / 2]: half of the dims a round
+        if (q == 0) {
+            s_ml[wave][r][0] = m_run;
+            s_ml[wave][r][1] = l_run;
+        }
+        bool redo = bad;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            __syncthreads();
+            // a padded, rotated row: the 16 columns of a store start in different banks
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const int dim = 16 * i + 4 * q;
+                *reinterpret_cast<float4*>(s_acc + (wave * 16 + r) * (D / 2) + (dim ^ ((r & 7) * 4))) =
+                    make_float4(acc[half * (D / 32) + i][0], acc[half * (D / 32) + i][1], acc[half * (D / 32) + i][2],
+                                acc[half * (D / 32) + i][3]);
+            }
+            __syncthreads();
+            constexpr int kChunks = D / 16;  // 8 dims of a half row
+            if (tid < 16 * kChunks) {
+                const int c = tid / kChunks;
+                const int d = tid % kChunks * 8;
+                float m = s_ml[0][c][0];
+#pragma unroll
+                for (int w = 1; w < 4; ++w) {
+                    m = fmaxf(m, s_ml[w][c][0]);
+                }
+                const float m_sub = m == kNegInf ? 0.0f : m;
+                float l = 0.0f;
+                float v[8] = {};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(s_ml[w][c][0] - m_sub);
+                    l = fmaf(s_ml[w][c][1], f, l);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float4 p = *reinterpret_cast<const float4*>(s_acc + (w * 16 + c) * (D / 2) +
+                                                                         ((d + 4 * j) ^ ((c & 7) * 4)));
+                        v[4 * j] = fmaf(p.x, f, v[4 * j]);
+                        v[4 * j + 1] = fmaf(p.y, f, v[4 * j + 1]);
+                        v[4 * j + 2] = fmaf(p.z, f, v[4 * j + 2]);
+                        v[4 * j + 3] = fmaf(p.w, f, v[4 * j + 3]);
+                    }
+                }
+                float zero = l * 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    zero = fmaf(v[j], 0.0f, zero);
+                }
+                redo |= zero != zero;
+                if (c < count) {
+                    const int col = c0 + c;
+                    put_column<T, D>(a, s.first + col / G, g * G + col % G, half * (D / 2) + d, v, m, l, split, splits);
+                }
+            }
+        }
+        if (redo) {
+            s_redo = 1;
+        }
+        __syncthreads();
+        if (s_redo != 0) {
+            const int begin = split * per_split * kUnit;
+            careful_columns<T, D>(a, s, table, g, c0, count, begin, u_end * kUnit, split, splits);
+        }
+        __syncthreads();
+    }
+}
+
+// ----------------------------------------------------------------- row tiles
+// 128 columns of a (sequence, KV head): four waves of 32 over the same 64 keys,
+// whose K and V rows go straight to LDS, one window ahead.
+constexpr int kTileRows = 128;
+constexpr int kWindow = 64;
+
+__device__ __forceinline__ void load_lds16(const uint16_t* src, uint8_t* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+__device__ __forceinline__ float halves_max(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// Tile slots: sequence i owns slots from floor(starts[i] G / 128) + i on, at least
+// as many as it has tiles, so the grid follows from the token count alone.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(PagedAttnArgs a, int slots, int tile_splits,
+                                                                           int splits, int few_rows) {
+    constexpr int kSteps = D / 16;
+    constexpr int kRowBytes = D * 2;
+    constexpr int kPieces = D / 8;
+    constexpr int kTileBytes = kWindow * kRowBytes;
+    constexpr int kLoadRows = 1024 / kRowBytes;      // rows of a wave's load
+    constexpr int kLoads = kWindow / (4 * kLoadRows);  // loads of a wave for a tile of K (and of V)
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[2][2 * kTileBytes];
+    __shared__ int s_index;
+    __shared__ int s_redo;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31;
+    const int q = lane >> 5;
+    const int G = static_cast<int>(a.group);
+    const int kv_heads = static_cast<int>(a.kv_heads);
+    // later tiles see more keys: they start first
+    const int g = static_cast<int>(blockIdx.x) % kv_heads;
+    const int split = static_cast<int>(blockIdx.x) / kv_heads % tile_splits;
+    const int slot = slots - 1 - static_cast<int>(blockIdx.x) / kv_heads / tile_splits;
+    if (tid == 0) {
+        s_index = 0;
+        s_redo = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < static_cast<int>(a.sequences); i += kThreads) {
+        const int64_t base = static_cast<int64_t>(a.starts[i]) * G / kTileRows + i;
+        if (base <= slot) {
+            atomicMax(&s_index, i);
+        }
+    }
+    __syncthreads();
+    const int index = s_index;
+    const Sequence s = sequence(a, index);
+    const int64_t total = static_cast<int64_t>(s.q_len) * G;
+    const int64_t tile = slot - (static_cast<int64_t>(s.first) * G / kTileRows + index);
+    const int64_t c0 = tile * kTileRows;
+    if (tile < 0 || c0 >= total || total <= few_rows) {
+        return;
+    }
+    const int count = static_cast<int>(total - c0 < kTileRows ? total - c0 : kTileRows);
+    if (s.bad) {
+        if (split == 0) {
+            nan_columns<T, D>(a, s, g, static_cast<int>(c0), count, splits);
+        }
+        return;
+    }
+    if (split == 0 && splits > tile_splits) {
+        clear_splits<D>(a, s, g, static_cast<int>(c0), count, tile_splits, splits);
+    }
+    const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
+    const uint16_t* const kbase = a.k + g * a.head_stride;
+    const uint16_t* const vbase = a.v + g * a.head_stride;
+    const int before = s.kv_len - s.q_len;  // position of the first new token
+    const int ends = before + (static_cast<int>(c0) + count - 1) / G + 1;
+    const int keys = ends > 0 ? ends : 0;
+    const int windows = (keys + kWindow - 1) / kWindow;
+    const int per_split = (windows + tile_splits - 1) / tile_splits;
+    const int w_begin = split * per_split;
+    const int w_end = w_begin + per_split < windows ? w_begin + per_split : windows;
+
+    const int local = wave * 32 + r;
+    const int column = static_cast<int>(c0) + (local < count ? local : count - 1);
+    const int head = g * G + column % G;
+    const int pos = before + column / G;
+    const int wave_column = static_cast<int>(c0) + (wave * 32 < count ? wave * 32 : count - 1);
+    const int first_pos = before + wave_column / G;  // lowest and highest positions of the wave's columns
+    const int wave_last = wave * 32 + 31 < count ? wave * 32 + 31 : count - 1;
+    const int last_pos = wave * 32 < count ? before + (static_cast<int>(c0) + wave_last) / G : -1;
+
+    uint4 qf[kSteps];
+    {
+        const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D + 8 * q;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            qf[i] = *reinterpret_cast<const uint4*>(src + 16 * i);
+        }
+    }
+    bool bad = false;
+    int page[kLoads];
+    const auto pages = [&](int w) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int key = w * kWindow + (j * 4 + wave) * kLoadRows + lane / kPieces;
+            page[j] = table[(key < keys ? key : keys - 1) >> a.page_shift];
+        }
+    };
+    // K's pieces are swizzled by row against the 16 (D = 64: 8) rows that a read
+    // takes together, V's so that the 4 rows of a transposed half-wave read lie
+    // in different banks; the lane fetches the piece that belongs in its place
+    const auto fetch = [&](int w) __attribute__((always_inline)) {
+        uint8_t* const dst = s_mem[w & 1];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int row = (j * 4 + wave) * kLoadRows + lane / kPieces;
+            const int key = w * kWindow + row;
+            const int64_t at = key_row(a, page[j], key < keys ? key : keys - 1, bad);
+            const int kp = (lane % kPieces) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
+            const int vp = (lane % kPieces) ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
+            load_lds16(kbase + at + 8 * kp, dst + (j * 4 + wave) * 1024);
+            load_lds16(vbase + at + 8 * vp, dst + kTileBytes + (j * 4 + wave) * 1024);
+        }
+    };
+    floatx16 acc[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        acc[i] = floatx16{};
+    }
+    float m_run = kNegInf;
+    float l_run = 0.0f;
+    if (w_begin < w_end) {
+        pages(w_begin);
+        fetch(w_begin);
+        if (w_begin + 1 < w_end) {
+            pages(w_begin + 1);
+        }
+    }
+    for (int w = w_begin; w < w_end; ++w) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the window is in LDS
+        __syncthreads();
+        if (w + 1 < w_end) {
+            fetch(w + 1);
+            if (w + 2 < w_end) {
+                pages(w + 2);
+            }
+        }
+        const int key0 = w * kWindow;
+        if (key0 > last_pos) {
+            continue;  // no column of this wave sees the window
+        }
+        const uint8_t* const s_k = s_mem[w & 1];
+        const uint8_t* const s_v = s_k + kTileBytes;
+        floatx16 sc[2] = {floatx16{}, floatx16{}};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int row = 32 * t + r;
+                const int piece = (2 * i + q) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
+                const uint4 kf = *reinterpret_cast<const uint4*>(s_k + row * kRowBytes + piece * 16);
+                sc[t] = mfma32(T{}, kf, qf[i], sc[t]);
+            }
+        }
+        // sc[t][e]: key 32 t + 8 (e / 4) + 4 q + e % 4 of the window
+        if (__builtin_amdgcn_readfirstlane(static_cast<int>(key0 + kWindow > first_pos + 1)) != 0) {
+            const int rel = pos - key0 - 4 * q;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[t][e] = 32 * t + 8 * (e / 4) + e % 4 <= rel ? sc[t][e] : kNegInf;
+                }
+            }
+        }
+        float mx = kNegInf;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                mx = fmaxf(mx, sc[t][e]);
+            }
+        }
+        const float m_new = fmaxf(m_run, halves_max(mx) * a.scale_log2);
+        const float m_sub = m_new == kNegInf ? 0.0f : m_new;
+        if (__any(m_new != m_run)) {
+            const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+            l_run *= corr;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    acc[i][e] *= corr;
+                }
+            }
+            m_run = m_new;
+        }
+        // steps of 16 keys: the lane's weights of scores 8 (n % 2) .. + 7 of half n / 2
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            uint32_t p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e], a.scale_log2, -m_sub));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e + 1], a.scale_log2, -m_sub));
+                l_run += p0 + p1;
+                p[e] = pack(T{}, p0, p1);
+            }
+            const uint4 pf = make_uint4(p[0], p[1], p[2], p[3]);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                uint2 part[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    // 16 lanes: keys 16 n + 8 t + 4 q .. + 3, dims 32 i + 16 (lane / 16 % 2) .. + 15
+                    const int row = 16 * n + 8 * t + 4 * q + (lane & 15) / 4;
+                    const int piece = (4 * i + 2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^
+                                      (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
+                    part[t] = read_transposed(s_v + row * kRowBytes + piece * 16 + (lane & 1) * 8);
+                }
+                acc[i] = mfma32(T{}, make_uint4(part[0].x, part[0].y, part[1].x, part[1].y), pf, acc[i]);
+            }
+        }
+    }
+    l_run = halves_sum(l_run);
+    {
+        float zero = l_run * 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                zero = fmaf(acc[i][e], 0.0f, zero);
+            }
+        }
+        if (bad || zero != zero) {
+            s_redo = 1;
+        }
+    }
+    __syncthreads();
+    if (s_redo != 0) {
+        careful_columns<T, D>(a, s, table, g, static_cast<int>(c0), count, w_begin * kWindow, w_end * kWindow, split,
+                              splits);
+        return;
+    }
+    if (local >= count) {
+        return;
+    }
+    // acc[i][e]: dim 32 i + 8 (e / 4) + 4 q + e % 4 of the lane's column
+    const int64_t row = s.first + column / G;
+    if (splits == 1) {
+        uint16_t* const out = a.out + row * a.out_stride + head * D + 4 * q;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool none = l_run == 0.0f;
+                const uint32_t x = none ? 0u : pack(T{}, acc[i][4 * j] / l_run, acc[i][4 * j + 1] / l_run);
+                const uint32_t y = none ? 0u : pack(T{}, acc[i][4 * j + 2] / l_run, acc[i][4 * j + 3] / l_run);
+                *reinterpret_cast<uint2*>(out + 32 * i + 8 * j) = make_uint2(x, y);
+            }
+        }
+        return;
+    }
+    const int64_t at = (row * a.q_heads + head) * splits + split;
+    float* const part = a.partials + at * D + 4 * q;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            *reinterpret_cast<float4*>(part + 32 * i + 8 * j) =
+                make_float4(acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
+        }
+    }
+    if (q == 0) {
+        *reinterpret_cast<float2*>(a.partials + a.tokens * a.q_heads * splits * D + 2 * at) = make_float2(m_run, l_run);
+    }
+}
+
+// -------------------------------------------------------------------- merge
+// One row and head: D / 8 lanes of 8 dims each over its splits.  Rows outside
+// [starts[0], starts[sequences]) belong to no sequence and are left alone.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_attention_merge_kernel(PagedAttnArgs a, int splits) {
+    constexpr int kLanes = D / 8;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
+    const int64_t row = unit / a.q_heads;
+    const int head = static_cast<int>(unit % a.q_heads);
+    if (row >= a.tokens || row < a.starts[0] || row >= a.starts[a.sequences]) {
+        return;
+    }
+    const int d0 = static_cast<int>(threadIdx.x) % kLanes * 8;
+    const float* const ml = a.partials + a.tokens * a.q_heads * splits * D + 2 * unit * splits;
+    const float* const src = a.partials + unit * splits * D + d0;
+    float m = kNegInf;
+    for (int s = 0; s < splits; ++s) {
+        m = fmaxf(m, ml[2 * s]);
+    }
+    const float m_sub = m == kNegInf ? 0.0f : m;
+    float l = 0.0f;
+    float v[8] = {};
+    for (int s = 0; s < splits; ++s) {
+        const float ls = ml[2 * s + 1];
+        if (ls == 0.0f) {
+            continue;  // no key of the row in this split: its sums were not written
+        }
+        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m_sub);
+        l = fmaf(ls, f, l);
+        const float4 x = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D);
+        const float4 y = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D + 4);
+        v[0] = fmaf(x.x, f, v[0]);
+        v[1] = fmaf(x.y, f, v[1]);
+        v[2] = fmaf(x.z, f, v[2]);
+        v[3] = fmaf(x.w, f, v[3]);
+        v[4] = fmaf(y.x, f, v[4]);
+        v[5] = fmaf(y.y, f, v[5]);
+        v[6] = fmaf(y.z, f, v[6]);
+        v[7] = fmaf(y.w, f, v[7]);
+    }
+    put_column<T, D>(a, row, head, d0, v, m, l, 0, 1);
+}
+
+template <typename T, int D>
+hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
+    if (plan.few_splits > 0) {
+        const int64_t blocks = a.sequences * a.kv_heads * plan.few_splits;
+        hipLaunchKernelGGL((paged_attention_few_kernel<T, D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                           stream, a, static_cast<int>(plan.few_splits), static_cast<int>(plan.splits),
+                           plan.tile_splits > 0 ? kFewRows : 0x7fffffff);
+        const hipError_t status = hipGetLastError();
+        if (status != hipSuccess) {
+            return status;
+        }
+    }
+    if (plan.tile_splits > 0) {
+        const int64_t blocks = plan.slots * a.kv_heads * plan.tile_splits;
+        hipLaunchKernelGGL((paged_attention_tile_kernel<T, D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                           stream, a, static_cast<int>(plan.slots), static_cast<int>(plan.tile_splits),
+                           static_cast<int>(plan.splits), plan.few_splits > 0 ? kFewRows : 0);
+        const hipError_t status = hipGetLastError();
+        if (status != hipSuccess) {
+            return status;
+        }
+    }
+    if (plan.splits > 1) {
+        const int64_t units = a.tokens * a.q_heads;
+        constexpr int kUnits = kThreads / (D / 8);
+        hipLaunchKernelGGL((paged_attention_merge_kernel<T, D>), dim3(static_cast<unsigned>((units + kUnits - 1) / kUnits)),
+                           dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits));
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
+                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t workspace_bytes) {
+    const int64_t group = q_heads / kv_heads;
+    PagedAttnPlan p;
+    const int64_t longest = max_query_len < tokens ? max_query_len : tokens;
+    const int64_t rows = longest * group;
+    const auto cap = [](int64_t v, int64_t most) { return v < 1 ? int64_t{1} : (v < most ? v : most); };
+    // few rows: four blocks a CU; a split is at least 128 keys, one unit a wave
+    if (rows <= kFewRows || tokens != sequences * max_query_len) {
+        p.few_splits = cap(1024 / (sequences * kv_heads), cap((max_kv_len + 127) / 128, 256));
+    }
+    if (rows > kFewRows) {
+        p.slots = tokens * group / kTileRows + sequences;
+        p.tile_splits = cap(512 / (p.slots * kv_heads), cap((max_kv_len + 2 * kWindow - 1) / (2 * kWindow), 32));
+    }
+    const int64_t unit = tokens * q_heads * (head_dim + 2) * 4;
+    const int64_t room = unit > 0 ? workspace_bytes / unit : 0;
+    const int64_t most = room > 1 ? room : 1;
+    p.few_splits = p.few_splits < most ? p.few_splits : most;
+    p.tile_splits = p.tile_splits < most ? p.tile_splits : most;
+    p.splits = p.few_splits > p.tile_splits ? p.few_splits : p.tile_splits;
+    p.workspace_bytes = p.splits > 1 ? unit * p.splits : 0;
+    return p;
+}
+
+hipError_t launch_paged_attention(Act act, const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
+    if (a.head_dim == 64) {
+        return act == Act::kBf16 ? launch<Bf16, 64>(a, plan, stream) : launch<F16, 64>(a, plan, stream);
+    }
+    return act == Act::kBf16 ? launch<Bf16, 128>(a, plan, stream) : launch<F16, 128>(a, plan, stream);
+}
+
+}  // namespace kc

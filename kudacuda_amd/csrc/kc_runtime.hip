@@ -860,6 +860,124 @@ hipError_t model_step(const Model& m, hipStream_t stream, int form = -1) {
     return model_op(m, 5, 0, true, stream);
 }
 
+// ------------------------------------------ several sequences, paged KV cache
+
+// The handle's device for a call's launches, whichever device is current.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        status_ = hipGetDevice(&before_);
+        if (status_ == hipSuccess && before_ != device) {
+            status_ = hipSetDevice(device);
+            changed_ = status_ == hipSuccess;
+        }
+    }
+    ~OnDevice() {
+        if (changed_) {
+            (void)hipSetDevice(before_);
+        }
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+    hipError_t status() const { return status_; }
+
+private:
+    int before_ = 0;
+    bool changed_ = false;
+    hipError_t status_ = hipSuccess;
+};
+
+template <typename Launch>
+int launch_on(Handle* h, const char* symbol, Launch launch) {
+    const OnDevice device(h->device_id);
+    return finish(h, symbol, device.status() == hipSuccess ? launch() : device.status());
+}
+
+bool refuse(Handle* h, const char* symbol, const char* reason) {
+    h->set_error(std::string(symbol) + " requires " + reason);
+    return false;
+}
+
+// log2 of a page size the cache takes, or -1.
+int page_shift_of(int64_t page_size) {
+    for (int shift = 0; shift <= 12; ++shift) {
+        if (page_size == int64_t{1} << shift) {
+            return shift;
+        }
+    }
+    return -1;
+}
+
+bool within(int64_t v, int64_t low, int64_t high) { return v >= low && v <= high; }
+bool multiple(uint64_t v, uint64_t n) { return v % n == 0; }
+constexpr int64_t kInt32Max = 0x7fffffff;
+
+bool rope_shape_ok(Handle* h, const char* symbol, int64_t dtype, int64_t tokens, int64_t heads, int64_t head_dim,
+                   int64_t rotary_dim, int64_t interleaved, float amplitude) {
+    if (dtype != 1 && dtype != 2) {
+        return refuse(h, symbol, "dtype 1 (bf16) or 2 (fp16)");
+    }
+    if (!within(tokens, 0, kInt32Max) || !within(heads, 1, 4096) || !within(head_dim, 2, kRopeMaxDim) ||
+        !within(rotary_dim, 2, head_dim) || head_dim % 2 != 0 || rotary_dim % 2 != 0 || !within(interleaved, 0, 1)) {
+        return refuse(h, symbol,
+                      "tokens>=0, heads 1..4096, even head_dim 2..256, even rotary_dim 2..head_dim and interleaved 0 or 1");
+    }
+    if (!std::isfinite(amplitude)) {
+        return refuse(h, symbol, "a finite amplitude");
+    }
+    return true;
+}
+
+// Every page id in range, no destination twice or another pair's source.  The
+// destinations, and the sources of pairs that move, go into an open hash table.
+bool pairs_ok(Handle* h, const char* symbol, const int32_t* pairs, int64_t count, int64_t num_pages) {
+    uint64_t size = 16;
+    while (size < 4 * static_cast<uint64_t>(count)) {
+        size *= 2;
+    }
+    // entries: page + 1 in the low 32 bits, 1 << 32 as destination, 1 << 33 as source
+    struct Free {
+        uint64_t* p;
+        ~Free() { delete[] p; }
+    } table{new (std::nothrow) uint64_t[size]()};
+    if (table.p == nullptr) {
+        h->set_error(std::string(symbol) + ": out of host memory");
+        return false;
+    }
+    const auto find = [&](int32_t page) -> uint64_t& {
+        const uint64_t key = static_cast<uint64_t>(page) + 1;
+        uint64_t i = key * 0x9e3779b97f4a7c15ull >> 20 & (size - 1);
+        while (table.p[i] != 0 && (table.p[i] & 0xffffffffu) != key) {
+            i = (i + 1) & (size - 1);
+        }
+        table.p[i] |= key;
+        return table.p[i];
+    };
+    constexpr uint64_t kDestination = uint64_t{1} << 32;
+    constexpr uint64_t kSource = uint64_t{1} << 33;
+    for (int64_t i = 0; i < count; ++i) {
+        const int32_t from = pairs[2 * i];
+        const int32_t to = pairs[2 * i + 1];
+        if (from < 0 || from >= num_pages || to < 0 || to >= num_pages) {
+            return refuse(h, symbol, "page ids in [0, num_pages)");
+        }
+        uint64_t& entry = find(to);
+        if ((entry & kDestination) != 0) {
+            return refuse(h, symbol, "destinations that differ from each other");
+        }
+        entry |= kDestination;
+        if (from != to) {
+            find(from) |= kSource;
+        }
+    }
+    for (int64_t i = 0; i < count; ++i) {
+        if (pairs[2 * i] != pairs[2 * i + 1] && (find(pairs[2 * i + 1]) & kSource) != 0) {
+            return refuse(h, symbol, "destinations that are no pair's source");
+        }
+    }
+    return true;
+}
+
 }  // namespace
 }  // namespace kc
 
@@ -872,6 +990,14 @@ using kc::ptr;
 using kc::ready;
 using kc::claim_scratch;
 using kc::scratch_launched;
+using kc::kInt32Max;
+using kc::launch_on;
+using kc::multiple;
+using kc::page_shift_of;
+using kc::pairs_ok;
+using kc::refuse;
+using kc::rope_shape_ok;
+using kc::within;
 
 extern "C" {
 
@@ -1462,6 +1588,315 @@ int kudacuda_lm_head_argmax_bf16(void* raw, uint64_t input, uint64_t norm_weight
 }
 
 int64_t kudacuda_lm_head_workspace_floats(void) { return kc::lm_head_workspace_floats(); }
+
+// ------------------------------------------ several sequences, paged KV cache
+int kudacuda_rope(void* raw, uint64_t input, uint64_t inv_freq, uint64_t positions, uint64_t output, int64_t dtype,
+                  int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim, int64_t interleaved,
+                  int64_t input_stride, int64_t output_stride, float amplitude, uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "rope";
+    if (!ready(h, "kudacuda_rope")) {
+        return 1;
+    }
+    if (input == 0 || inv_freq == 0 || positions == 0 || output == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (!rope_shape_ok(h, symbol, dtype, tokens, heads, head_dim, rotary_dim, interleaved, amplitude)) {
+        return 1;
+    }
+    if (input_stride < heads * head_dim || output_stride < heads * head_dim) {
+        refuse(h, symbol, "strides of at least heads * head_dim");
+        return 1;
+    }
+    if (!multiple(input | output, 2) || !multiple(inv_freq, 8) || !multiple(positions, 4)) {
+        refuse(h, symbol, "buffers aligned to their elements");
+        return 1;
+    }
+    if (tokens == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::RopeArgs a;
+    a.q = ptr<const uint16_t>(input);
+    a.inv_freq = ptr<const double>(inv_freq);
+    a.positions = ptr<const int32_t>(positions);
+    a.q_out = ptr<uint16_t>(output);
+    a.tokens = tokens;
+    a.q_heads = static_cast<int>(heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.rotary_dim = static_cast<int>(rotary_dim);
+    a.interleaved = interleaved != 0;
+    a.q_stride = input_stride;
+    a.out_stride = output_stride;
+    a.amplitude = amplitude;
+    return launch_on(h, symbol,
+                     [&] { return kc::launch_rope(dtype == 1 ? Act::kBf16 : Act::kF16, a, as_stream(stream)); });
+}
+
+int kudacuda_rope_paged_append(void* raw, uint64_t query, uint64_t key, uint64_t value, uint64_t inv_freq,
+                               uint64_t positions, uint64_t slots, uint64_t query_output, uint64_t key_pages,
+                               uint64_t value_pages, int64_t dtype, int64_t tokens, int64_t query_heads,
+                               int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t interleaved,
+                               int64_t query_stride, int64_t key_stride, int64_t value_stride, int64_t output_stride,
+                               int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t head_stride,
+                               int64_t token_stride, float amplitude, uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "rope_paged_append";
+    if (!ready(h, "kudacuda_rope_paged_append")) {
+        return 1;
+    }
+    if (query == 0 || key == 0 || value == 0 || inv_freq == 0 || positions == 0 || slots == 0 || query_output == 0 ||
+        key_pages == 0 || value_pages == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (!rope_shape_ok(h, symbol, dtype, tokens, query_heads, head_dim, rotary_dim, interleaved, amplitude)) {
+        return 1;
+    }
+    const int shift = page_shift_of(page_size);
+    if (!within(kv_heads, 1, 4096) || !within(num_pages, 1, kInt32Max) || shift < 0) {
+        refuse(h, symbol, "kv_heads 1..4096, num_pages>=1 and a page_size that is a power of two, 1..4096");
+        return 1;
+    }
+    if (query_stride < query_heads * head_dim || output_stride < query_heads * head_dim ||
+        key_stride < kv_heads * head_dim || value_stride < kv_heads * head_dim) {
+        refuse(h, symbol, "strides of at least heads * head_dim");
+        return 1;
+    }
+    if (page_stride < head_dim || head_stride < head_dim || token_stride < head_dim) {
+        refuse(h, symbol, "pool strides of at least head_dim");
+        return 1;
+    }
+    if (!multiple(query | key | value | query_output | key_pages | value_pages, 2) || !multiple(inv_freq | slots, 8) ||
+        !multiple(positions, 4)) {
+        refuse(h, symbol, "buffers aligned to their elements");
+        return 1;
+    }
+    if (tokens == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::RopeArgs a;
+    a.q = ptr<const uint16_t>(query);
+    a.k = ptr<const uint16_t>(key);
+    a.v = ptr<const uint16_t>(value);
+    a.inv_freq = ptr<const double>(inv_freq);
+    a.positions = ptr<const int32_t>(positions);
+    a.slots = ptr<const int64_t>(slots);
+    a.q_out = ptr<uint16_t>(query_output);
+    a.k_pages = ptr<uint16_t>(key_pages);
+    a.v_pages = ptr<uint16_t>(value_pages);
+    a.tokens = tokens;
+    a.q_heads = static_cast<int>(query_heads);
+    a.kv_heads = static_cast<int>(kv_heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.rotary_dim = static_cast<int>(rotary_dim);
+    a.interleaved = interleaved != 0;
+    a.page_shift = shift;
+    a.q_stride = query_stride;
+    a.k_stride = key_stride;
+    a.v_stride = value_stride;
+    a.out_stride = output_stride;
+    a.num_pages = num_pages;
+    a.page_stride = page_stride;
+    a.head_stride = head_stride;
+    a.token_stride = token_stride;
+    a.amplitude = amplitude;
+    return launch_on(h, symbol,
+                     [&] { return kc::launch_rope(dtype == 1 ? Act::kBf16 : Act::kF16, a, as_stream(stream)); });
+}
+
+int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences, int64_t max_query_len,
+                                                 int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
+                                                 int64_t head_dim) {
+    if (tokens < 1 || sequences < 1 || max_query_len < 1 || max_kv_len < 1 || query_heads < 1 || kv_heads < 1 ||
+        head_dim < 1 || query_heads % kv_heads != 0) {
+        return 0;
+    }
+    return kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len, query_heads, kv_heads, head_dim, INT64_MAX)
+        .workspace_bytes;
+}
+
+int kudacuda_paged_attention(void* raw, uint64_t query, uint64_t key_pages, uint64_t value_pages, uint64_t page_table,
+                             uint64_t query_starts, uint64_t kv_lens, uint64_t output, uint64_t workspace,
+                             int64_t workspace_bytes, int64_t dtype, int64_t tokens, int64_t sequences,
+                             int64_t max_query_len, int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
+                             int64_t head_dim, int64_t query_stride, int64_t output_stride, int64_t num_pages,
+                             int64_t page_size, int64_t table_stride, int64_t page_stride, int64_t head_stride,
+                             int64_t token_stride, float scale, uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "paged_attention";
+    if (!ready(h, "kudacuda_paged_attention")) {
+        return 1;
+    }
+    if (query == 0 || key_pages == 0 || value_pages == 0 || page_table == 0 || query_starts == 0 || kv_lens == 0 ||
+        output == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (dtype != 1 && dtype != 2) {
+        refuse(h, symbol, "dtype 1 (bf16) or 2 (fp16)");
+        return 1;
+    }
+    if ((head_dim != 64 && head_dim != 128) || !within(query_heads, 1, 1024) || !within(kv_heads, 1, query_heads) ||
+        query_heads % kv_heads != 0) {
+        refuse(h, symbol, "head_dim 64 or 128 and query_heads (1..1024) a multiple of kv_heads");
+        return 1;
+    }
+    const int shift = page_shift_of(page_size);
+    if (!within(tokens, 0, (int64_t{1} << 30) / query_heads) || !within(sequences, 1, 65536) ||
+        !within(num_pages, 1, kInt32Max) || shift < 0 || !within(table_stride, 1, (int64_t{1} << 30) >> shift)) {
+        refuse(h, symbol,
+               "0 <= tokens * query_heads <= 2^30, 1..65536 sequences, num_pages>=1, page_size a power of two (1..4096) "
+               "and 1 <= table_stride * page_size <= 2^30");
+        return 1;
+    }
+    if (max_query_len < 1 || max_kv_len < 1) {
+        refuse(h, symbol, "max_query_len>=1 and max_kv_len>=1");
+        return 1;
+    }
+    if (query_stride < query_heads * head_dim || output_stride < query_heads * head_dim || page_stride < head_dim ||
+        head_stride < head_dim || token_stride < head_dim ||
+        (query_stride | output_stride | page_stride | head_stride | token_stride) % 8 != 0) {
+        refuse(h, symbol, "strides of at least a row, multiples of 8");
+        return 1;
+    }
+    if (!multiple(query | key_pages | value_pages | output | workspace, 16) ||
+        !multiple(page_table | query_starts | kv_lens, 4)) {
+        refuse(h, symbol, "buffers on 16-byte boundaries");
+        return 1;
+    }
+    if (workspace_bytes < 0) {
+        refuse(h, symbol, "workspace_bytes>=0");
+        return 1;
+    }
+    if (!(scale > 0.0f) || !std::isfinite(scale)) {
+        refuse(h, symbol, "a positive finite scale");
+        return 1;
+    }
+    if (tokens == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::PagedAttnArgs a;
+    a.q = ptr<const uint16_t>(query);
+    a.k = ptr<const uint16_t>(key_pages);
+    a.v = ptr<const uint16_t>(value_pages);
+    a.table = ptr<const int32_t>(page_table);
+    a.starts = ptr<const int32_t>(query_starts);
+    a.kv_lens = ptr<const int32_t>(kv_lens);
+    a.out = ptr<uint16_t>(output);
+    a.partials = ptr<float>(workspace);
+    a.tokens = tokens;
+    a.sequences = sequences;
+    a.q_heads = query_heads;
+    a.kv_heads = kv_heads;
+    a.group = query_heads / kv_heads;
+    a.head_dim = head_dim;
+    a.q_stride = query_stride;
+    a.out_stride = output_stride;
+    a.num_pages = num_pages;
+    a.table_stride = table_stride;
+    a.page_stride = page_stride;
+    a.head_stride = head_stride;
+    a.token_stride = token_stride;
+    a.page_shift = shift;
+    a.scale_log2 = scale * kc::kLog2e;
+    const int64_t longest = table_stride << shift;
+    const kc::PagedAttnPlan plan =
+        kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len < longest ? max_kv_len : longest, query_heads,
+                                 kv_heads, head_dim, workspace != 0 ? workspace_bytes : 0);
+    return launch_on(h, symbol, [&] {
+        return kc::launch_paged_attention(dtype == 1 ? Act::kBf16 : Act::kF16, a, plan, as_stream(stream));
+    });
+}
+
+int kudacuda_copy_pages(void* raw, uint64_t pool, uint64_t pairs, int64_t count, int64_t pools, int64_t num_pages,
+                        int64_t page_bytes, int64_t page_stride, int64_t pool_stride, uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "copy_pages";
+    if (!ready(h, "kudacuda_copy_pages")) {
+        return 1;
+    }
+    if (pool == 0 || (pairs == 0 && count > 0)) {
+        h->set_error(std::string(symbol) + " requires a non-null pool and pairs");
+        return 1;
+    }
+    if (!within(count, 0, num_pages) || !within(pools, 1, 65536) || !within(num_pages, 1, kInt32Max) ||
+        !within(page_bytes, 16, int64_t{1} << 28)) {
+        refuse(h, symbol, "0 <= count <= num_pages, 1..65536 pools, num_pages>=1 and page_bytes 16..2^28");
+        return 1;
+    }
+    if (!multiple(pool | static_cast<uint64_t>(page_bytes | page_stride | pool_stride), 16) || !multiple(pairs, 4) ||
+        (num_pages > 1 && page_stride < page_bytes) || (pools > 1 && pool_stride < page_bytes)) {
+        refuse(h, symbol, "whole 16-byte pieces on 16-byte boundaries and strides of at least page_bytes");
+        return 1;
+    }
+    const int32_t* const list = ptr<const int32_t>(pairs);
+    if (!pairs_ok(h, symbol, list, count, num_pages)) {
+        return 1;
+    }
+    kc::CopyPagesArgs a;
+    a.pool = ptr<uint8_t>(pool);
+    a.pairs = list;
+    a.count = count;
+    a.pools = pools;
+    a.page_bytes = page_bytes;
+    a.page_stride = page_stride;
+    a.pool_stride = pool_stride;
+    return launch_on(h, symbol, [&] { return kc::launch_copy_pages(a, as_stream(stream)); });
+}
+
+int64_t kudacuda_sample_workspace_bytes(int64_t rows, int64_t vocab) {
+    return rows < 1 || vocab < 1 ? 0 : kc::sample_workspace_bytes(rows, vocab);
+}
+
+int kudacuda_sample_tokens(void* raw, uint64_t logits, uint64_t random, uint64_t temperature, uint64_t top_k,
+                           uint64_t top_p, uint64_t min_p, uint64_t tokens_out, uint64_t chances, uint64_t workspace,
+                           int64_t workspace_bytes, int64_t dtype, int64_t rows, int64_t vocab, int64_t stride,
+                           uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "sample_tokens";
+    if (!ready(h, "kudacuda_sample_tokens")) {
+        return 1;
+    }
+    if (logits == 0 || random == 0 || tokens_out == 0 || workspace == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (!within(dtype, 0, 2)) {
+        refuse(h, symbol, "dtype 0 (fp32), 1 (bf16) or 2 (fp16)");
+        return 1;
+    }
+    if (!within(rows, 0, 65535) || !within(vocab, 1, kc::kSampleMaxVocab) || stride < vocab) {
+        refuse(h, symbol, "rows 0..65535, vocab 1..2^20 and stride >= vocab");
+        return 1;
+    }
+    if (!multiple(logits, dtype == 0 ? 4 : 2) ||
+        !multiple(random | temperature | top_k | top_p | min_p | tokens_out | chances, 4) || !multiple(workspace, 16)) {
+        refuse(h, symbol, "buffers aligned to their elements and a workspace on a 16-byte boundary");
+        return 1;
+    }
+    if (workspace_bytes < kudacuda_sample_workspace_bytes(rows, vocab)) {
+        refuse(h, symbol, "a workspace of kudacuda_sample_workspace_bytes(rows, vocab)");
+        return 1;
+    }
+    if (rows == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::SampleArgs a;
+    a.logits = ptr<const void>(logits);
+    a.random = ptr<const float>(random);
+    a.temperature = ptr<const float>(temperature);
+    a.top_k = ptr<const int32_t>(top_k);
+    a.top_p = ptr<const float>(top_p);
+    a.min_p = ptr<const float>(min_p);
+    a.tokens = ptr<int32_t>(tokens_out);
+    a.chances = ptr<float>(chances);
+    a.workspace = ptr<uint8_t>(workspace);
+    a.rows = rows;
+    a.vocab = vocab;
+    a.stride = stride;
+    return launch_on(h, symbol, [&] { return kc::launch_sample(static_cast<int>(dtype), a, as_stream(stream)); });
+}
 
 int kudacuda_begin_capture(void* raw, uint64_t stream) {
     Handle* h = as_handle(raw);

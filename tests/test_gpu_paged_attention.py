@@ -1,0 +1,227 @@
+"""GPU: attention of new tokens over a paged cache (kudacuda_paged_attention) against softmax in 64 bits.
+
+Rows of the pools that no sequence has hold NaN, table entries behind a sequence's pages no valid id."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from tests._paged_ref import Paged, f64
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _check(batch, out, rows=None):
+    want, size = batch.want()
+    got = f64(out)
+    rows = np.arange(int(batch.starts[-1])) if rows is None else rows
+    off = np.abs(got[rows] - want[rows])
+    assert np.isfinite(got[rows]).all()
+    bound = batch.bound(want, size)[rows]
+    assert (off <= bound).all(), float((off / np.maximum(bound, 1e-30)).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,kv,heads,kv_heads,page,layout", [
+    # single tokens: one key, the ends of units of 32 keys and of the waves' rounds of 128
+    ([1], [1], 1, 1, 1, "hnd"),
+    ([1, 1, 1, 1], [1, 31, 32, 33], 16, 2, 16, "hnd"),
+    ([1, 1, 1], [127, 129, 1000], 7, 1, 16, "nhd"),
+    ([1] * 9, [5, 700, 1, 64, 65, 333, 16, 17, 2000], 12, 4, 64, "hnd"),
+    ([1, 1], [300, 40], 32, 1, 8, "nhd"),            # 32 heads of a KV head: two rounds of columns
+    ([1, 1], [70, 3], 64, 1, 16, "hnd"),             # 64: past the few-row form
+    # few new tokens: drafts, more columns than 16
+    ([3, 2, 4], [3, 100, 260], 8, 2, 16, "hnd"),
+    # chunks: first ones (no cache before), later ones, ends inside a tile and a window
+    ([17], [17], 4, 2, 16, "hnd"),
+    ([128], [128], 2, 2, 64, "nhd"),
+    ([33, 200, 1, 64], [33, 500, 77, 64], 8, 4, 16, "hnd"),
+    ([250, 5], [1300, 5], 7, 7, 128, "nhd"),
+    ([1, 130, 1], [900, 131, 2], 16, 2, 4096, "hnd"),
+    # sequences without new tokens, without cache rows, and rows that see no key
+    ([0, 4, 0, 1, 40], [9, 4, 0, 0, 13], 4, 2, 16, "hnd"),
+    ([2, 60], [0, 1], 4, 4, 16, "hnd"),
+])
+def test_matches_fp64(torch_gpu, native, dtype, dim, new, kv, heads, kv_heads, page, layout):
+    batch = Paged(len(new) + sum(kv), new, kv, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype,
+                  layout=layout, q_extra=1)
+    print(f"paged attention {new} of {kv}, {heads}/{kv_heads} heads of {dim}, pages of {page}", flush=True)
+    _check(batch, batch.call(native, batch.device()))
+
+
+@pytest.mark.parametrize("new,kv", [([1, 1], [3000, 700]), ([60], [2500]), ([1, 90, 2], [4000, 1500, 1])])
+def test_splits_follow_the_workspace_and_the_hints(torch_gpu, native, new, kv):
+    """No workspace, a small one and a full one; hints that are too small and too large: the same results to rounding."""
+
+    batch = Paged(5, new, kv, heads=8, kv_heads=2, dim=128)
+    d = batch.device()
+    nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(batch.tokens, len(new), max(new), max(kv), 8, 2, 128)
+    assert nbytes > 0
+    row = batch.tokens * 8 * 130 * 4
+    for size in (0, row - 16, 2 * row, 3 * row + 16, nbytes):
+        d["out"].fill_(7.25)
+        _check(batch, batch.call(native, d, nbytes=size))
+    for max_new, max_kv in ((1, 1), (1, 1 << 20), (batch.tokens, 1), (1 << 20, 1 << 20)):
+        d["out"].fill_(7.25)
+        _check(batch, batch.call(native, d, max_new=max_new, max_kv=max_kv))
+
+
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [900, 33, 0]), ([70, 3], [200, 3])])
+def test_rows_behind_the_last_sequence_stay(torch_gpu, native, new, kv):
+    batch = Paged(6, new, kv, extra_rows=5)
+    for nbytes in (None, 0):
+        d = batch.device()
+        out = batch.call(native, d, nbytes=nbytes)
+        _check(batch, out)
+        assert (f64(out[-5:]) == 7.25).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("new,kv", [([4], [300]), ([150], [400])])
+def test_infinities_and_nan_of_hidden_keys_stay_hidden(torch_gpu, native, dtype, new, kv):
+    """The last key's K and V are NaN and infinite: only the row that sees it is not finite."""
+
+    batch = Paged(8, new, kv, dtype=dtype, dim=64)
+    last = kv[0] - 1
+    page, at = batch.table[0, last // 16], last % 16
+    for value in (float("inf"), float("nan")):
+        batch.k[page, :, at] = value if value != value else 3.0
+        batch.v[page, :, at] = value
+        d = batch.device()
+        for nbytes in (None, 0):
+            out = batch.call(native, d, nbytes=nbytes)
+            _check(batch, out, rows=np.arange(new[0] - 1))
+            assert not np.isfinite(f64(out[-1])).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_large_scores_and_lowest_values(torch_gpu, native, dtype):
+    """Scores of hundreds, keys at the type's lowest value, a first key that outweighs all others by far."""
+
+    batch = Paged(9, [1, 40], [600, 300], dtype=dtype, dim=64, junk=float("-inf"))
+    batch.k *= 12
+    page = batch.table[0, 0]
+    batch.k[page, :, 3] = 0
+    batch.v[page, :, 3] = torch.finfo(dtype).min / 4
+    batch.k[page, :, 4] = -batch.q[0, :2] * 8
+    want, size = batch.want()
+    out = f64(batch.call(native, batch.device()))
+    assert np.isfinite(out).all()
+    # scores of up to 64 * 12 * 4 * 1.5 / 8: 2^10 of them in fp32, off by 64 * 2^-24 * 2^10 = 2^-8
+    bound = batch.bound(want, size) + 2.0**-7 * size
+    assert (np.abs(out - want) <= bound).all()
+
+
+def test_pages_outside_the_pool_make_nan_rows(torch_gpu, native):
+    """A bad page id is not read; the rows that see one of its keys are NaN, the others hold."""
+
+    for new, kv in (([1, 1, 1], [500, 90, 33]), ([40, 1], [300, 20])):
+        for bad in (-1, 2**31 - 1, None):
+            batch = Paged(10, new, kv)
+            d = batch.device()
+            d["table"][0, (kv[0] - 1) // 16 - 1] = batch.num_pages if bad is None else bad
+            first = ((kv[0] - 1) // 16 - 1) * 16  # the first key of that page
+            for nbytes in (None, 0):
+                out = f64(batch.call(native, d, nbytes=nbytes))
+                for i in range(new[0]):
+                    seen = kv[0] - new[0] + i >= first
+                    assert np.isnan(out[i]).all() if seen else np.isfinite(out[i]).all(), (new, bad, i)
+                _check(batch, d["out"], rows=np.array([i for i in range(batch.tokens) if np.isfinite(out[i]).all()]))
+                assert np.isfinite(out[new[0]:]).all()
+
+
+def test_lengths_that_do_not_fit_the_table_make_nan_rows(torch_gpu, native):
+    for new, kv in (([1, 1], [64, 40]), ([50, 3], [64, 40])):
+        for bad in (-1, 4 * 16 + 1, 2**31 - 1):
+            batch = Paged(11, new, kv)
+            d = batch.device()
+            d["lens"][0] = bad
+            for nbytes in (None, 0, 1 << 20):
+                out = f64(batch.call(native, d, nbytes=nbytes))
+                assert np.isnan(out[:new[0]]).all()
+                _check(batch, d["out"], rows=np.arange(new[0], batch.tokens))
+
+
+def test_starts_outside_the_rows_stay_inside(torch_gpu, native):
+    """Starts past the tokens (and below zero) name no rows."""
+
+    batch = Paged(12, [2, 3], [40, 50])
+    d = batch.device()
+    d["starts"].copy_(torch.tensor([-4, 2, 2**31 - 1], dtype=torch.int32))
+    out = f64(batch.call(native, d, nbytes=0))
+    assert np.isfinite(out).all()
+
+
+def test_offsets_past_32_bits(torch_gpu, native):
+    """Pools of more than 2^32 elements: pages 2^25 elements apart, the values half a page behind the keys."""
+
+    stride, pages = 1 << 25, 130
+    batch = Paged(13, [1, 20], [700, 300], dim=64, kv_heads=2, heads=4, spare=pages - 3 - 44 - 19)
+    assert batch.num_pages == pages and int(batch.table.max()) > 127
+    d = batch.device()
+    pool = torch.zeros(pages * stride, dtype=BF16, device="cuda:0")
+    shape, inner = (pages, 2, 16, 64), (2 * 16 * 64) // 2
+    k = torch.as_strided(pool, shape, (stride, inner, 64, 1), 0)
+    v = torch.as_strided(pool, shape, (stride, inner, 64, 1), stride // 2)
+    k.copy_(d["k"])
+    v.copy_(d["v"])
+    d |= {"k": k, "v": v, "strides": (stride, inner, 64)}
+    _check(batch, batch.call(native, d))
+    del pool, k, v, d
+    torch.cuda.empty_cache()
+
+
+def test_two_streams_and_a_second_handle(torch_gpu, native):
+    from kudacuda_amd._native import Native
+
+    other = Native(0)
+    first, second = Paged(14, [1, 1], [2000, 900], dim=128), Paged(15, [100], [800], dim=128)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    ds = [first.device(), second.device()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        first.call(native, ds[0], stream=streams[0])
+        second.call(native, ds[1], stream=streams[1])
+        second.call(other, ds[1], stream=streams[1])
+    torch.cuda.synchronize()
+    _check(first, ds[0]["out"])
+    _check(second, ds[1]["out"])
+    other.close()
+
+
+def test_captured_call_follows_its_tables(torch_gpu, native):
+    """One capture, replayed while the sequences grow: lengths, tables and starts are read at replay time."""
+
+    batch = Paged(16, [1, 1, 1], [900, 600, 40], dim=128)
+    d = batch.device()
+    nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(3, 3, 1, 1024, 4, 2, 128)
+    workspace = torch.zeros(nbytes, dtype=torch.uint8, device="cuda:0")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        batch.call(native, d, stream=torch.cuda.current_stream(), workspace=workspace, nbytes=nbytes, max_kv=1024)
+    for kv in ([900, 600, 40], [1, 600, 39], [33, 0, 17], [899, 128, 40]):
+        batch.kv = kv
+        with torch.cuda.stream(side):
+            d["lens"].copy_(torch.tensor(kv, dtype=torch.int32))
+            d["out"].fill_(7.25)
+            graph.replay()
+        side.synchronize()
+        _check(batch, d["out"])
+        replayed = d["out"].clone()
+        batch.call(native, d, workspace=workspace, nbytes=nbytes, max_kv=1024)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, d["out"])
+
+
+def test_results_do_not_change_from_call_to_call(torch_gpu, native):
+    batch = Paged(17, [1, 200, 3], [3000, 900, 60], dim=128, heads=16)
+    d = batch.device()
+    first = batch.call(native, d).clone()
+    for _ in range(5):
+        assert torch.equal(batch.call(native, d), first)
