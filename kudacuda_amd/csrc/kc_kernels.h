@@ -355,17 +355,19 @@ struct PagedAttnArgs {
     int page_shift = 0;
     float scale_log2 = 0.0f;  // scale * log2(e)
 };
-// Which kernels a call takes and over how many key splits: the few-row kernel for
-// sequences with few rows, the tile kernel for the others (0: not launched).
+// Which kernels a call takes (0: not launched), the few-row kernel for sequences with
+// few rows, the tile kernel for the others, and over how many key splits.
 struct PagedAttnPlan {
-    int64_t few_splits = 0;
+    int64_t few_blocks = 0;
     int64_t tile_splits = 0;
     int64_t slots = 0;   // tile slots of the tile kernel's grid
-    int64_t splits = 0;  // the larger: row length of the partials
+    int64_t splits = 0;  // the most of either: row length of the partials
     int64_t workspace_bytes = 0;
 };
+// max_keys: what a table row holds, whatever the hints say.
 PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
-                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t workspace_bytes);
+                                   int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t workspace_bytes);
 hipError_t launch_paged_attention(Act act, const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t stream);
 
 constexpr int kPagePairs = 448;  // pairs of a launch: 3584 bytes of kernel arguments

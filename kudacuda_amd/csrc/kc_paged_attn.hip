@@ -89,6 +89,16 @@ __device__ __forceinline__ Sequence sequence(const PagedAttnArgs& a, int index) 
     return s;
 }
 
+// The same where the index is one for the whole wave.
+__device__ __forceinline__ Sequence wave_sequence(const PagedAttnArgs& a, int index) {
+    Sequence s = sequence(a, index);
+    s.first = __builtin_amdgcn_readfirstlane(s.first);
+    s.q_len = __builtin_amdgcn_readfirstlane(s.q_len);
+    s.kv_len = __builtin_amdgcn_readfirstlane(s.kv_len);
+    s.bad = __builtin_amdgcn_readfirstlane(s.bad) != 0;
+    return s;
+}
+
 // Key j of a sequence: element offset of its row in the pools, and whether its
 // page exists (a page id outside the pool is read as page 0 and reported).
 __device__ __forceinline__ int64_t key_row(const PagedAttnArgs& a, int page, int key, bool& bad) {
@@ -222,247 +232,385 @@ __device__ __forceinline__ void clear_splits(const PagedAttnArgs& a, const Seque
 }
 
 // ------------------------------------------------------------------ few rows
-// A (sequence, KV head) with at most kFewRows rows, the form of single tokens:
-// the four waves take alternate units of 32 keys, 16 columns at a time, K straight
-// from memory into the first product's operand, V through the wave's own LDS.
+// Sequences of which a KV head has at most kFewRows rows, the form of single tokens:
+// bound by the cache's bytes.  All blocks share the cached rows of all sequences
+// evenly: the work is the line of (sequence, KV head, tile of 16 rows, round of 128
+// keys), cut into one stretch a block, so a batch of unequal lengths ends everywhere
+// at once (a fixed number of splits a sequence: 64 sequences of up to 8192 tokens
+// 88 us instead of 70).  In a round the four waves take 32 keys each, K straight from
+// memory into the first product's operand, V through the wave's own LDS, the next
+// keys requested as soon as the registers of these are free.
 constexpr int kFewRows = 32;
 constexpr int kUnit = 32;
+constexpr int kRound = 4 * kUnit;
+constexpr int64_t kFewBlocks = 512;
+
+// A sequence's part of the line: tiles of 16 rows, rounds of each.  Without splits a
+// tile is one piece of work.
+struct Line {
+    int tiles;
+    int rounds;
+};
+__device__ __forceinline__ Line line_of(const PagedAttnArgs& a, const Sequence& s, int few_rows, int splits) {
+    const int64_t rows = static_cast<int64_t>(s.q_len) * a.group;
+    Line line;
+    line.tiles = rows <= few_rows ? static_cast<int>((rows + 15) / 16) : 0;
+    const int rounds = (s.kv_len + kRound - 1) / kRound;
+    line.rounds = splits > 1 && rounds > 1 ? rounds : 1;
+    return line;
+}
+__device__ __forceinline__ int length_of(const PagedAttnArgs& a, const Line& line) {
+    return static_cast<int>(a.kv_heads) * line.tiles * line.rounds;
+}
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttnArgs a, int few_splits, int splits,
-                                                                       int few_rows) {
+__device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequence& s, int index, int g, int c0,
+                                              int begin, int end, int split, int splits, uint8_t* s_mem,
+                                              float (*s_ml)[16][2], int* s_redo) {
     constexpr int kSteps = D / 32;   // products of 32 dims a score
     constexpr int kPieces = D / 8;   // 16-byte pieces of a row
-    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
-    __shared__ float s_ml[4][16][2];
-    __shared__ int s_redo;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15;
     const int q = lane >> 4;
-    const int split = static_cast<int>(blockIdx.x) % few_splits;
-    const int g = static_cast<int>(blockIdx.x) / few_splits % static_cast<int>(a.kv_heads);
-    const int index = static_cast<int>(blockIdx.x) / few_splits / static_cast<int>(a.kv_heads);
-    const Sequence s = sequence(a, index);
     const int G = static_cast<int>(a.group);
     const int rows = s.q_len * G;
-    if (rows == 0 || rows > few_rows) {
-        return;
-    }
-    if (s.bad) {
-        if (split == 0) {
-            nan_columns<T, D>(a, s, g, 0, rows, splits);
-        }
-        return;
-    }
-    if (split == 0 && splits > few_splits) {
-        clear_splits<D>(a, s, g, 0, rows, few_splits, splits);
-    }
     const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
     const uint16_t* const kbase = a.k + g * a.head_stride;
     const uint16_t* const vbase = a.v + g * a.head_stride;
     uint8_t* const s_v = s_mem + wave * (kUnit * D * 2);
 
-    for (int c0 = 0; c0 < rows; c0 += 16) {
-        const int count = rows - c0 < 16 ? rows - c0 : 16;
-        const int column = c0 + (r < count ? r : count - 1);
-        const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
-        const int head = g * G + column % G;
-        const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
-        const int keys = ends > 0 ? ends : 0;
-        const int units = (keys + kUnit - 1) / kUnit;
-        const int per_split = ((units + 3) / 4 + few_splits - 1) / few_splits * 4;
-        const int u_end = (split + 1) * per_split < units ? (split + 1) * per_split : units;
-        int unit = split * per_split + wave;
+    const int count = rows - c0 < 16 ? rows - c0 : 16;
+    const int column = c0 + (r < count ? r : count - 1);
+    const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
+    const int head = g * G + column % G;
+    const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
+    const int keys = ends > 0 ? ends : 0;
+    const int units = (keys + kUnit - 1) / kUnit;
+    const int u_end = end * 4 < units ? end * 4 : units;
+    int unit = begin * 4 + wave;
 
-        uint4 qf[kSteps];
-        {
-            const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D + 8 * q;
+    uint4 qf[kSteps];
+    {
+        const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D + 8 * q;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            qf[i] = *reinterpret_cast<const uint4*>(src + 32 * i);
+        }
+    }
+    bool bad = false;
+    int64_t at[2];
+    int page[2];
+    const auto pages = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key = u * kUnit + 16 * t + r;
+            page[t] = table[(key < keys ? key : keys - 1) >> a.page_shift];
+        }
+    };
+    const auto place = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key = u * kUnit + 16 * t + r;
+            at[t] = key_row(a, page[t], key < keys ? key : keys - 1, bad) + 8 * q;
+        }
+    };
+    uint4 kf[2][kSteps], vf[2][kSteps];
+    const auto fetch = [&](uint4 (&f)[2][kSteps], const uint16_t* base) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                qf[i] = *reinterpret_cast<const uint4*>(src + 32 * i);
+                f[t][i] = load_stream(reinterpret_cast<const uint4*>(base + at[t] + 32 * i));
             }
         }
-        bool bad = false;
-        int64_t at[2];
-        const auto place = [&](int u) __attribute__((always_inline)) {
+    };
+    floatx4 acc[D / 16];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int key = u * kUnit + 16 * t + r;
-                const int k = key < keys ? key : keys - 1;
-                at[t] = key_row(a, table[k >> a.page_shift], k, bad) + 8 * q;
+    for (int i = 0; i < D / 16; ++i) {
+        acc[i] = floatx4{};
+    }
+    float m_run = kNegInf;
+    float l_run = 0.0f;
+    if (unit < u_end) {
+        pages(unit);
+        place(unit);
+        fetch(kf, kbase);
+        fetch(vf, vbase);
+        pages(unit + 4);
+    }
+    for (; unit < u_end; unit += 4) {
+        // V's rows, their 16-byte pieces swizzled so that the 8 rows of a
+        // transposed half-wave read lie in different banks
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int row = 16 * t + r;
+                const int piece = (4 * i + q) ^ (((row & 7) << 1) % kPieces);
+                *reinterpret_cast<uint4*>(s_v + row * (D * 2) + piece * 16) = vf[t][i];
             }
-        };
-        uint4 kf[2][kSteps], vf[2][kSteps];
-        const auto fetch = [&](uint4 (&f)[2][kSteps], const uint16_t* base) __attribute__((always_inline)) {
+        }
+        const bool more = unit + 4 < u_end;
+        if (more) {
+            place(unit + 4);
+            fetch(vf, vbase);
+            pages(unit + 8);
+        }
+        floatx4 sc[2] = {floatx4{}, floatx4{}};
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+        for (int i = 0; i < kSteps; ++i) {
+            sc[0] = mfma16(T{}, kf[0][i], qf[i], sc[0]);
+            sc[1] = mfma16(T{}, kf[1][i], qf[i], sc[1]);
+        }
+        if (more) {
+            fetch(kf, kbase);
+        }
+        // sc[t][i]: key 16 t + 4 q + i of the unit
+        const int rel = pos - unit * kUnit - 4 * q;
+        float mx = kNegInf;
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    f[t][i] = load_stream(reinterpret_cast<const uint4*>(base + at[t] + 32 * i));
-                }
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[t][i] = 16 * t + i <= rel ? sc[t][i] * a.scale_log2 : kNegInf;
+                mx = fmaxf(mx, sc[t][i]);
             }
-        };
-        floatx4 acc[D / 16];
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_run, mx);
+        const float m_sub = m_new == kNegInf ? 0.0f : m_new;
+        const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+        m_run = m_new;
+        l_run *= corr;
+        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16, 22
+        // in fp16): this form waits for memory, the second product is free
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_sub);
+            const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_sub);
+            l_run += p0 + p1;
+            hi[e] = pack(T{}, p0, p1);
+            lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
+        }
+        const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-            acc[i] = floatx4{};
-        }
-        float m_run = kNegInf;
-        float l_run = 0.0f;
-        if (unit < u_end) {
-            place(unit);
-            fetch(kf, kbase);
-            fetch(vf, vbase);
-        }
-        for (; unit < u_end; unit += 4) {
-            // V's rows, their 16-byte pieces swizzled so that the 8 rows of a
-            // transposed half-wave read lie in different banks
+            uint2 part[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const int row = 16 * t + r;
-                    const int piece = (4 * i + q) ^ (((row & 7) << 1) % kPieces);
-                    *reinterpret_cast<uint4*>(s_v + row * (D * 2) + piece * 16) = vf[t][i];
-                }
+                const int row = 16 * t + 4 * q + r / 4;
+                const int piece = (2 * i + (r & 3) / 2) ^ (((row & 7) << 1) % kPieces);
+                part[t] = read_transposed(s_v + row * (D * 2) + piece * 16 + (r & 1) * 8);
             }
-            const bool more = unit + 4 < u_end;
-            if (more) {
-                place(unit + 4);
-                fetch(vf, vbase);
-            }
-            floatx4 sc[2] = {floatx4{}, floatx4{}};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                sc[0] = mfma16(T{}, kf[0][i], qf[i], sc[0]);
-                sc[1] = mfma16(T{}, kf[1][i], qf[i], sc[1]);
-            }
-            if (more) {
-                fetch(kf, kbase);
-            }
-            // sc[t][i]: key 16 t + 4 q + i of the unit
-            const int rel = pos - unit * kUnit - 4 * q;
-            float mx = kNegInf;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sc[t][i] = 16 * t + i <= rel ? sc[t][i] * a.scale_log2 : kNegInf;
-                    mx = fmaxf(mx, sc[t][i]);
-                }
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float m_new = fmaxf(m_run, mx);
-            const float m_sub = m_new == kNegInf ? 0.0f : m_new;
-            const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
-            m_run = m_new;
-            l_run *= corr;
-            // weights as two 16-bit parts (16 bits of the fp32 weight in bf16, 22
-            // in fp16): this form waits for memory, the second product is free
-            uint32_t hi[4], lo[4];
+            const uint4 vt = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_sub);
-                const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_sub);
-                l_run += p0 + p1;
-                hi[e] = pack(T{}, p0, p1);
-                lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
+                acc[i][e] *= corr;
             }
-            const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                uint2 part[2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int row = 16 * t + 4 * q + r / 4;
-                    const int piece = (2 * i + (r & 3) / 2) ^ (((row & 7) << 1) % kPieces);
-                    part[t] = read_transposed(s_v + row * (D * 2) + piece * 16 + (r & 1) * 8);
-                }
-                const uint4 vt = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    acc[i][e] *= corr;
-                }
-                acc[i] = mfma16(T{}, vt, ph, acc[i]);
-                acc[i] = mfma16(T{}, vt, pl, acc[i]);
-            }
+            acc[i] = mfma16(T{}, vt, ph, acc[i]);
+            acc[i] = mfma16(T{}, vt, pl, acc[i]);
         }
-        l_run += __shfl_xor(l_run, 16, 64);
-        l_run += __shfl_xor(l_run, 32, 64);
-        // the waves' columns meet in LDS, each in the wave's own part: [column][dim]
+    }
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    // the waves' columns meet in LDS, each in the wave's own part: [column][dim]
+    __syncthreads();
+    if (tid == 0) {
+        *s_redo = 0;
+    }
+    float* const s_acc = reinterpret_cast<float*>(s_mem);  // [wave][16][D / 2]: half of the dims a round
+    if (q == 0) {
+        s_ml[wave][r][0] = m_run;
+        s_ml[wave][r][1] = l_run;
+    }
+    bool redo = bad;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
         __syncthreads();
-        if (tid == 0) {
-            s_redo = 0;
-        }
-        float* const s_acc = reinterpret_cast<float*>(s_mem);  // [wave][16][D / 2]: half of the dims a round
-        if (q == 0) {
-            s_ml[wave][r][0] = m_run;
-            s_ml[wave][r][1] = l_run;
-        }
-        bool redo = bad;
+        // a padded, rotated row: the 16 columns of a store start in different banks
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            __syncthreads();
-            // a padded, rotated row: the 16 columns of a store start in different banks
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const int dim = 16 * i + 4 * q;
-                *reinterpret_cast<float4*>(s_acc + (wave * 16 + r) * (D / 2) + (dim ^ ((r & 7) * 4))) =
-                    make_float4(acc[half * (D / 32) + i][0], acc[half * (D / 32) + i][1], acc[half * (D / 32) + i][2],
-                                acc[half * (D / 32) + i][3]);
-            }
-            __syncthreads();
-            constexpr int kChunks = D / 16;  // 8 dims of a half row
-            if (tid < 16 * kChunks) {
-                const int c = tid / kChunks;
-                const int d = tid % kChunks * 8;
-                float m = s_ml[0][c][0];
-#pragma unroll
-                for (int w = 1; w < 4; ++w) {
-                    m = fmaxf(m, s_ml[w][c][0]);
-                }
-                const float m_sub = m == kNegInf ? 0.0f : m;
-                float l = 0.0f;
-                float v[8] = {};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(s_ml[w][c][0] - m_sub);
-                    l = fmaf(s_ml[w][c][1], f, l);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float4 p = *reinterpret_cast<const float4*>(s_acc + (w * 16 + c) * (D / 2) +
-                                                                         ((d + 4 * j) ^ ((c & 7) * 4)));
-                        v[4 * j] = fmaf(p.x, f, v[4 * j]);
-                        v[4 * j + 1] = fmaf(p.y, f, v[4 * j + 1]);
-                        v[4 * j + 2] = fmaf(p.z, f, v[4 * j + 2]);
-                        v[4 * j + 3] = fmaf(p.w, f, v[4 * j + 3]);
-                    }
-                }
-                float zero = l * 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    zero = fmaf(v[j], 0.0f, zero);
-                }
-                redo |= zero != zero;
-                if (c < count) {
-                    const int col = c0 + c;
-                    put_column<T, D>(a, s.first + col / G, g * G + col % G, half * (D / 2) + d, v, m, l, split, splits);
-                }
-            }
-        }
-        if (redo) {
-            s_redo = 1;
+        for (int i = 0; i < D / 32; ++i) {
+            const int dim = 16 * i + 4 * q;
+            *reinterpret_cast<float4*>(s_acc + (wave * 16 + r) * (D / 2) + (dim ^ ((r & 7) * 4))) =
+                make_float4(acc[half * (D / 32) + i][0], acc[half * (D / 32) + i][1], acc[half * (D / 32) + i][2],
+                            acc[half * (D / 32) + i][3]);
         }
         __syncthreads();
-        if (s_redo != 0) {
-            const int begin = split * per_split * kUnit;
-            careful_columns<T, D>(a, s, table, g, c0, count, begin, u_end * kUnit, split, splits);
+        constexpr int kChunks = D / 16;  // 8 dims of a half row
+        if (tid < 16 * kChunks) {
+            const int c = tid / kChunks;
+            const int d = tid % kChunks * 8;
+            float m = s_ml[0][c][0];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+                m = fmaxf(m, s_ml[w][c][0]);
+            }
+            const float m_sub = m == kNegInf ? 0.0f : m;
+            float l = 0.0f;
+            float v[8] = {};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(s_ml[w][c][0] - m_sub);
+                l = fmaf(s_ml[w][c][1], f, l);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float4 p = *reinterpret_cast<const float4*>(s_acc + (w * 16 + c) * (D / 2) +
+                                                                     ((d + 4 * j) ^ ((c & 7) * 4)));
+                    v[4 * j] = fmaf(p.x, f, v[4 * j]);
+                    v[4 * j + 1] = fmaf(p.y, f, v[4 * j + 1]);
+                    v[4 * j + 2] = fmaf(p.z, f, v[4 * j + 2]);
+                    v[4 * j + 3] = fmaf(p.w, f, v[4 * j + 3]);
+                }
+            }
+            float zero = l * 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                zero = fmaf(v[j], 0.0f, zero);
+            }
+            redo |= zero != zero;
+            if (c < count) {
+                const int col = c0 + c;
+                put_column<T, D>(a, s.first + col / G, g * G + col % G, half * (D / 2) + d, v, m, l, split, splits);
+            }
+        }
+    }
+    if (redo) {
+        *s_redo = 1;
+    }
+    __syncthreads();
+    if (*s_redo != 0) {
+        careful_columns<T, D>(a, s, table, g, c0, count, begin * kRound, u_end * kUnit, split, splits);
+    }
+    __syncthreads();
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttnArgs a, int splits, int few_rows) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
+    __shared__ float s_ml[4][16][2];
+    __shared__ int s_part[4], s_most[4];
+    __shared__ int s_found[6];
+    __shared__ int s_redo;
+    const int tid = threadIdx.x;
+    const int sequences = static_cast<int>(a.sequences);
+    // (the line's length fits in 31 bits: the plan splits nothing where it might not)
+    // a thread's run of sequences (one of up to 256): the run's part of the line, where
+    // it begins, and its first sequence
+    const int per_thread = (sequences + kThreads - 1) / kThreads;
+    int mine = 0;
+    int mine_before = 0;
+    Sequence own = {};
+    int total, most;
+    if (sequences == 1) {
+        const Line line = line_of(a, wave_sequence(a, 0), few_rows, splits);
+        total = length_of(a, line);
+        most = line.rounds;
+    } else {
+        const int run_end = (tid + 1) * per_thread < sequences ? (tid + 1) * per_thread : sequences;
+        int longest = 1;
+        for (int i = tid * per_thread; i < run_end; ++i) {
+            own = sequence(a, i);
+            const Line line = line_of(a, own, few_rows, splits);
+            mine += length_of(a, line);
+            longest = line.tiles > 0 && line.rounds > longest ? line.rounds : longest;
+        }
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int left = __shfl_up(sum, o, 64);
+            const int other = __shfl_xor(longest, o, 64);
+            sum += (tid & 63) >= o ? left : 0;
+            longest = other > longest ? other : longest;
+        }
+        if ((tid & 63) == 63) {
+            s_part[tid >> 6] = sum;
+            s_most[tid >> 6] = longest;
         }
         __syncthreads();
+        total = __builtin_amdgcn_readfirstlane(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+        most = __builtin_amdgcn_readfirstlane(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
+        mine_before = sum - mine;
+        for (int w = 0; w < (tid >> 6); ++w) {
+            mine_before += s_part[w];
+        }
+    }
+    // a stretch: an even share, and long enough that no tile lies in more than `splits`
+    const int blocks = static_cast<int>(gridDim.x);
+    int stretch = (total + blocks - 1) / blocks;
+    const int least = splits > 1 ? (most + splits - 2) / (splits - 1) : 1;
+    stretch = stretch > least ? stretch : least;
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * stretch;
+    if (begin >= total) {
+        return;
+    }
+    int at = static_cast<int>(begin);
+    const int stop = at + stretch < total ? at + stretch : total;
+    int index, before;
+    Sequence s;
+    if (sequences == 1) {
+        index = 0;
+        before = 0;
+        s = wave_sequence(a, 0);
+    } else {
+        // the thread whose sequences the stretch begins in tells which
+        if (mine_before <= at && at < mine_before + mine) {
+            int i = tid * per_thread;
+            for (; per_thread > 1; ++i) {
+                own = sequence(a, i);
+                const int next = mine_before + length_of(a, line_of(a, own, few_rows, splits));
+                if (at < next) {
+                    break;
+                }
+                mine_before = next;
+            }
+            s_found[0] = i;
+            s_found[1] = mine_before;
+            s_found[2] = own.first;
+            s_found[3] = own.q_len;
+            s_found[4] = own.kv_len;
+            s_found[5] = own.bad;
+        }
+        __syncthreads();
+        index = __builtin_amdgcn_readfirstlane(s_found[0]);
+        before = __builtin_amdgcn_readfirstlane(s_found[1]);
+        s.first = __builtin_amdgcn_readfirstlane(s_found[2]);
+        s.q_len = __builtin_amdgcn_readfirstlane(s_found[3]);
+        s.kv_len = __builtin_amdgcn_readfirstlane(s_found[4]);
+        s.bad = __builtin_amdgcn_readfirstlane(s_found[5]) != 0;
+    }
+    for (;;) {
+        const Line line = line_of(a, s, few_rows, splits);
+        const int next = before + length_of(a, line);
+        while (at < stop && at < next) {
+            const int piece = (at - before) / line.rounds;
+            const int first = before + piece * line.rounds;
+            const int to = stop - first < line.rounds ? stop - first : line.rounds;
+            const int g = piece / line.tiles;
+            const int c0 = piece % line.tiles * 16;
+            const int rest = s.q_len * static_cast<int>(a.group) - c0;
+            const int count = rest < 16 ? rest : 16;
+            const int split = splits > 1 ? static_cast<int>(blockIdx.x) - first / stretch : 0;
+            if (s.bad) {
+                nan_columns<T, D>(a, s, g, c0, count, splits);
+            } else {
+                if (to == line.rounds && split + 1 < splits) {
+                    clear_splits<D>(a, s, g, c0, count, split + 1, splits);
+                }
+                few_rows_tile<T, D>(a, s, index, g, c0, at - first, splits > 1 ? to : 0x7fffffff / kRound, split, splits,
+                                    s_mem, s_ml, &s_redo);
+            }
+            at = first + to;
+        }
+        if (at >= stop) {
+            return;
+        }
+        before = next;
+        s = wave_sequence(a, ++index);
     }
 }
 
@@ -522,8 +670,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         }
     }
     __syncthreads();
-    const int index = s_index;
-    const Sequence s = sequence(a, index);
+    const int index = __builtin_amdgcn_readfirstlane(s_index);
+    const Sequence s = wave_sequence(a, index);
     const int64_t total = static_cast<int64_t>(s.q_len) * G;
     const int64_t tile = slot - (static_cast<int64_t>(s.first) * G / kTileRows + index);
     const int64_t c0 = tile * kTileRows;
@@ -748,55 +896,127 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
 }
 
 // -------------------------------------------------------------------- merge
-// One row and head: D / 8 lanes of 8 dims each over its splits.  Rows outside
-// [starts[0], starts[sequences]) belong to no sequence and are left alone.
-template <typename T, int D>
+// One row and head: GROUPS groups of D / 8 lanes of 8 dims each, a group takes every
+// GROUPS-th split, four of them requested together, and the groups' sums meet in
+// LDS.  Rows outside [starts[0], starts[sequences]) belong to no sequence and are
+// left alone.
+template <typename T, int D, int GROUPS>
 __global__ __launch_bounds__(kThreads) void paged_attention_merge_kernel(PagedAttnArgs a, int splits) {
     constexpr int kLanes = D / 8;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
+    constexpr int kUnits = kThreads / (kLanes * GROUPS);  // rows and heads of a block
+    constexpr int kAhead = 4;
+    __shared__ __attribute__((aligned(16))) float s_v[GROUPS > 1 ? GROUPS : 1][kUnits][GROUPS > 1 ? D : 1];
+    __shared__ float s_ml[GROUPS][kUnits][2];
+    const int part = static_cast<int>(threadIdx.x) / kLanes;
+    const int mine = part % kUnits;
+    const int group = part / kUnits;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kUnits + mine;
     const int64_t row = unit / a.q_heads;
     const int head = static_cast<int>(unit % a.q_heads);
-    if (row >= a.tokens || row < a.starts[0] || row >= a.starts[a.sequences]) {
-        return;
-    }
+    const bool live = row < a.tokens && row >= a.starts[0] && row < a.starts[a.sequences];
     const int d0 = static_cast<int>(threadIdx.x) % kLanes * 8;
-    const float* const ml = a.partials + a.tokens * a.q_heads * splits * D + 2 * unit * splits;
-    const float* const src = a.partials + unit * splits * D + d0;
     float m = kNegInf;
-    for (int s = 0; s < splits; ++s) {
-        m = fmaxf(m, ml[2 * s]);
-    }
-    const float m_sub = m == kNegInf ? 0.0f : m;
     float l = 0.0f;
     float v[8] = {};
-    for (int s = 0; s < splits; ++s) {
-        const float ls = ml[2 * s + 1];
-        if (ls == 0.0f) {
-            continue;  // no key of the row in this split: its sums were not written
+    if (live) {
+        const float2* const ml = reinterpret_cast<const float2*>(a.partials + a.tokens * a.q_heads * splits * D) + unit * splits;
+        const float* const src = a.partials + unit * splits * D + d0;
+        for (int s0 = group; s0 < splits; s0 += kAhead * GROUPS) {
+            float2 w[kAhead];
+            float4 x[kAhead], y[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int s = s0 + j * GROUPS < splits ? s0 + j * GROUPS : splits - 1;
+                w[j] = ml[s];
+            }
+            float m_new = m;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                // a split without a key of the row has sum 0 and anything for its dims
+                w[j].y = s0 + j * GROUPS < splits ? w[j].y : 0.0f;
+                m_new = fmaxf(m_new, w[j].y != 0.0f ? w[j].x : kNegInf);
+                if (w[j].y != 0.0f) {
+                    x[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s0 + j * GROUPS) * D);
+                    y[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s0 + j * GROUPS) * D + 4);
+                }
+            }
+            const float m_sub = m_new == kNegInf ? 0.0f : m_new;
+            const float corr = __builtin_amdgcn_exp2f(m - m_sub);
+            m = m_new;
+            l *= corr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] *= corr;
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (w[j].y != 0.0f) {
+                    const float f = __builtin_amdgcn_exp2f(w[j].x - m_sub);
+                    l = fmaf(w[j].y, f, l);
+                    v[0] = fmaf(x[j].x, f, v[0]);
+                    v[1] = fmaf(x[j].y, f, v[1]);
+                    v[2] = fmaf(x[j].z, f, v[2]);
+                    v[3] = fmaf(x[j].w, f, v[3]);
+                    v[4] = fmaf(y[j].x, f, v[4]);
+                    v[5] = fmaf(y[j].y, f, v[5]);
+                    v[6] = fmaf(y[j].z, f, v[6]);
+                    v[7] = fmaf(y[j].w, f, v[7]);
+                }
+            }
         }
-        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m_sub);
-        l = fmaf(ls, f, l);
-        const float4 x = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D);
-        const float4 y = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D + 4);
-        v[0] = fmaf(x.x, f, v[0]);
-        v[1] = fmaf(x.y, f, v[1]);
-        v[2] = fmaf(x.z, f, v[2]);
-        v[3] = fmaf(x.w, f, v[3]);
-        v[4] = fmaf(y.x, f, v[4]);
-        v[5] = fmaf(y.y, f, v[5]);
-        v[6] = fmaf(y.z, f, v[6]);
-        v[7] = fmaf(y.w, f, v[7]);
     }
-    put_column<T, D>(a, row, head, d0, v, m, l, 0, 1);
+    if constexpr (GROUPS > 1) {
+        *reinterpret_cast<float4*>(&s_v[group][mine][d0]) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(&s_v[group][mine][d0 + 4]) = make_float4(v[4], v[5], v[6], v[7]);
+        if (d0 == 0) {
+            s_ml[group][mine][0] = m;
+            s_ml[group][mine][1] = l;
+        }
+        __syncthreads();
+        if (group != 0) {
+            return;
+        }
+        float m_all = m;
+#pragma unroll
+        for (int o = 1; o < GROUPS; ++o) {
+            m_all = fmaxf(m_all, s_ml[o][mine][0]);
+        }
+        const float m_sub = m_all == kNegInf ? 0.0f : m_all;
+        const float c = __builtin_amdgcn_exp2f(m - m_sub);
+        l *= c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] *= c;
+        }
+#pragma unroll
+        for (int o = 1; o < GROUPS; ++o) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[o][mine][0] - m_sub);
+            l = fmaf(s_ml[o][mine][1], f, l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = fmaf(s_v[o][mine][d0 + i], f, v[i]);
+            }
+        }
+    }
+    if (live) {
+        put_column<T, D>(a, row, head, d0, v, m, l, 0, 1);
+    }
+}
+
+template <typename T, int D, int GROUPS>
+hipError_t launch_merge(const PagedAttnArgs& a, int64_t splits, hipStream_t stream) {
+    constexpr int kUnits = kThreads / (D / 8 * GROUPS);
+    const int64_t blocks = (a.tokens * a.q_heads + kUnits - 1) / kUnits;
+    hipLaunchKernelGGL((paged_attention_merge_kernel<T, D, GROUPS>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                       stream, a, static_cast<int>(splits));
+    return hipGetLastError();
 }
 
 template <typename T, int D>
 hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
-    if (plan.few_splits > 0) {
-        const int64_t blocks = a.sequences * a.kv_heads * plan.few_splits;
-        hipLaunchKernelGGL((paged_attention_few_kernel<T, D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
-                           stream, a, static_cast<int>(plan.few_splits), static_cast<int>(plan.splits),
-                           plan.tile_splits > 0 ? kFewRows : 0x7fffffff);
+    if (plan.few_blocks > 0) {
+        hipLaunchKernelGGL((paged_attention_few_kernel<T, D>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(kThreads), 0,
+                           stream, a, static_cast<int>(plan.splits), plan.tile_splits > 0 ? kFewRows : 0x7fffffff);
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) {
             return status;
@@ -806,18 +1026,17 @@ hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t
         const int64_t blocks = plan.slots * a.kv_heads * plan.tile_splits;
         hipLaunchKernelGGL((paged_attention_tile_kernel<T, D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
                            stream, a, static_cast<int>(plan.slots), static_cast<int>(plan.tile_splits),
-                           static_cast<int>(plan.splits), plan.few_splits > 0 ? kFewRows : 0);
+                           static_cast<int>(plan.splits), plan.few_blocks > 0 ? kFewRows : 0);
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) {
             return status;
         }
     }
+    if (plan.splits > 4) {
+        return launch_merge<T, D, 16>(a, plan.splits, stream);
+    }
     if (plan.splits > 1) {
-        const int64_t units = a.tokens * a.q_heads;
-        constexpr int kUnits = kThreads / (D / 8);
-        hipLaunchKernelGGL((paged_attention_merge_kernel<T, D>), dim3(static_cast<unsigned>((units + kUnits - 1) / kUnits)),
-                           dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits));
-        return hipGetLastError();
+        return launch_merge<T, D, 1>(a, plan.splits, stream);
     }
     return hipSuccess;
 }
@@ -825,15 +1044,21 @@ hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t
 }  // namespace
 
 PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
-                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t workspace_bytes) {
+                                   int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t workspace_bytes) {
     const int64_t group = q_heads / kv_heads;
     PagedAttnPlan p;
     const int64_t longest = max_query_len < tokens ? max_query_len : tokens;
     const int64_t rows = longest * group;
     const auto cap = [](int64_t v, int64_t most) { return v < 1 ? int64_t{1} : (v < most ? v : most); };
-    // few rows: four blocks a CU; a split is at least 128 keys, one unit a wave
+    int64_t few_splits = 0;
     if (rows <= kFewRows || tokens != sequences * max_query_len) {
-        p.few_splits = cap(1024 / (sequences * kv_heads), cap((max_kv_len + 127) / 128, 256));
+        // two blocks a CU; a stretch of at least one round of keys.  The longest sequence
+        // may be cut into twice as many stretches as it were in a batch of such ones.
+        const int64_t tiles = sequences * kv_heads * (((rows < kFewRows ? rows : kFewRows) + 15) / 16);
+        const int64_t rounds = (max_kv_len + kRound - 1) / kRound;
+        p.few_blocks = rounds < kFewBlocks && tiles * rounds < kFewBlocks ? tiles * rounds : kFewBlocks;
+        few_splits = cap(2 * ((kFewBlocks + tiles - 1) / tiles) + 1, cap(rounds, 256));
     }
     if (rows > kFewRows) {
         p.slots = tokens * group / kTileRows + sequences;
@@ -841,10 +1066,13 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     }
     const int64_t unit = tokens * q_heads * (head_dim + 2) * 4;
     const int64_t room = unit > 0 ? workspace_bytes / unit : 0;
-    const int64_t most = room > 1 ? room : 1;
-    p.few_splits = p.few_splits < most ? p.few_splits : most;
+    // the few-row kernel counts its rounds in 31 bits
+    const int64_t rounds = (max_keys + kRound - 1) / kRound;
+    const bool countable = (tokens * q_heads / 16 + sequences * kv_heads) * rounds < (int64_t{1} << 31);
+    const int64_t most = room > 1 && countable ? room : 1;
+    few_splits = few_splits < most ? few_splits : most;
     p.tile_splits = p.tile_splits < most ? p.tile_splits : most;
-    p.splits = p.few_splits > p.tile_splits ? p.few_splits : p.tile_splits;
+    p.splits = few_splits > p.tile_splits ? few_splits : p.tile_splits;
     p.workspace_bytes = p.splits > 1 ? unit * p.splits : 0;
     return p;
 }

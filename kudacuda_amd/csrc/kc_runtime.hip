@@ -1712,7 +1712,8 @@ int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, int64_t sequenc
         head_dim < 1 || query_heads % kv_heads != 0) {
         return 0;
     }
-    return kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len, query_heads, kv_heads, head_dim, INT64_MAX)
+    return kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len, max_kv_len, query_heads, kv_heads, head_dim,
+                                    INT64_MAX)
         .workspace_bytes;
 }
 
@@ -1802,8 +1803,8 @@ int kudacuda_paged_attention(void* raw, uint64_t query, uint64_t key_pages, uint
     a.scale_log2 = scale * kc::kLog2e;
     const int64_t longest = table_stride << shift;
     const kc::PagedAttnPlan plan =
-        kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len < longest ? max_kv_len : longest, query_heads,
-                                 kv_heads, head_dim, workspace != 0 ? workspace_bytes : 0);
+        kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len < longest ? max_kv_len : longest, longest,
+                                 query_heads, kv_heads, head_dim, workspace != 0 ? workspace_bytes : 0);
     return launch_on(h, symbol, [&] {
         return kc::launch_paged_attention(dtype == 1 ? Act::kBf16 : Act::kF16, a, plan, as_stream(stream));
     });
