@@ -50,6 +50,15 @@ __device__ __forceinline__ uint32_t pack(F16, float lo, float hi) {
     const halfx2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
     return __builtin_bit_cast(uint32_t, v);
 }
+// sum + both halves of v, in fp32.
+__device__ __forceinline__ float add_pair(Bf16, uint32_t v, float sum) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+}
+__device__ __forceinline__ float add_pair(F16, uint32_t v, float sum) {
+    typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, v), __builtin_bit_cast(halfx2, 0x3c003c00u), sum, false);
+}
 template <typename T>
 __device__ __forceinline__ float low(uint32_t v) {
     return T::load(static_cast<uint16_t>(v & 0xffffu));
@@ -620,9 +629,18 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 constexpr int kTileRows = 128;
 constexpr int kWindow = 64;
 
-__device__ __forceinline__ void load_lds16(const uint16_t* src, uint8_t* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// 16 bytes a lane from base + offset straight into LDS, lane after lane from `lds`.
+// (As an instruction of its own: behind the builtin the compiler waits for the load
+// before the next LDS read, whatever that reads.  It writes no register; the wait is
+// the window's own.  Nothing else in these kernels keeps a value in m0.)
+__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void load_lds16(const uint16_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
 }
 __device__ __forceinline__ float halves_max(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -717,28 +735,66 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         }
     }
     bool bad = false;
-    int page[kLoads];
-    const auto pages = [&](int w) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const int key = w * kWindow + (j * 4 + wave) * kLoadRows + lane / kPieces;
-            page[j] = table[(key < keys ? key : keys - 1) >> a.page_shift];
-        }
-    };
     // K's pieces are swizzled by row against the 16 (D = 64: 8) rows that a read
     // takes together, V's so that the 4 rows of a transposed half-wave read lie
     // in different banks; the lane fetches the piece that belongs in its place
-    const auto fetch = [&](int w) __attribute__((always_inline)) {
-        uint8_t* const dst = s_mem[w & 1];
+    const int lane_row = lane / kPieces;  // of a load's kLoadRows rows, which begin at a multiple of that
+    const auto piece_of = [&](int row, bool value) __attribute__((always_inline)) {
+        const int k = D == 128 ? row & 15 : (row >> 1) & 7;
+        const int v = D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+        return (lane % kPieces) ^ (value ? v : k);
+    };
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(s_mem[0]) + wave * 1024);
+    // Whole windows of pages that hold a load's rows together (and begin within 4 GB
+    // of a pool's beginning times a page id): a load's base is the wave's, its lanes'
+    // offsets are the same in every window.  Bytes from here on.
+    const int page_mask = (1 << a.page_shift) - 1;
+    const bool together = page_mask + 1 >= kLoadRows && a.token_stride < (1 << 26) && a.page_stride < (1 << 30);
+    const uint32_t page_bytes = static_cast<uint32_t>(2 * a.page_stride);
+    const uint32_t token_bytes = static_cast<uint32_t>(2 * a.token_stride);
+    const uint8_t* k_at[kLoads];
+    const uint8_t* v_at[kLoads];
+    uint32_t k_lane[kLoads];
+    uint32_t v_lane[kLoads];
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const int row = (j * 4 + wave) * kLoadRows + lane / kPieces;
-            const int key = w * kWindow + row;
-            const int64_t at = key_row(a, page[j], key < keys ? key : keys - 1, bad);
-            const int kp = (lane % kPieces) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
-            const int vp = (lane % kPieces) ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
-            load_lds16(kbase + at + 8 * kp, dst + (j * 4 + wave) * 1024);
-            load_lds16(vbase + at + 8 * vp, dst + kTileBytes + (j * 4 + wave) * 1024);
+    for (int j = 0; j < kLoads; ++j) {
+        const int row0 = (j * 4 + wave) * kLoadRows;
+        const int64_t in_page = static_cast<int64_t>(row0 & page_mask) * token_bytes;
+        k_at[j] = reinterpret_cast<const uint8_t*>(kbase) + in_page;
+        v_at[j] = reinterpret_cast<const uint8_t*>(vbase) + in_page;
+        k_lane[j] = lane_row * token_bytes + 16 * piece_of(row0 + lane_row, false);
+        v_lane[j] = lane_row * token_bytes + 16 * piece_of(row0 + lane_row, true);
+    }
+    // pages of the window's groups of kLoadRows keys, one a lane
+    int pages = 0;
+    const auto look = [&](int w) __attribute__((always_inline)) {
+        const int key = w * kWindow + lane % (4 * kLoads) * kLoadRows;
+        pages = table[(key < keys ? key : keys - 1) >> a.page_shift];
+    };
+    const auto fetch = [&](int w) __attribute__((always_inline)) {
+        const uint32_t lds = lds0 + (w & 1) * (2 * kTileBytes);
+        if (together && (w + 1) * kWindow <= keys) {
+            const bool out = static_cast<uint32_t>(pages) >= static_cast<uint32_t>(a.num_pages);
+            bad |= out;
+            const int page = out ? 0 : pages;
+            // (pages of more than a window: where the window begins in its page)
+            const int64_t shift = static_cast<int64_t>((w * kWindow) & page_mask) * token_bytes;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const uint32_t id = __builtin_amdgcn_readlane(page, j * 4 + wave);
+                const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(id) * page_bytes) + shift;
+                load_lds16(k_at[j] + at, k_lane[j], lds + j * 4096);
+                load_lds16(v_at[j] + at, v_lane[j], lds + kTileBytes + j * 4096);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int row = (j * 4 + wave) * kLoadRows + lane_row;
+                const int key = w * kWindow + row < keys ? w * kWindow + row : keys - 1;
+                const int64_t at = key_row(a, table[key >> a.page_shift], key, bad);
+                load_lds16(kbase + at + 8 * piece_of(row, false), lds + j * 4096);
+                load_lds16(vbase + at + 8 * piece_of(row, true), lds + kTileBytes + j * 4096);
+            }
         }
     };
     floatx16 acc[D / 32];
@@ -749,20 +805,16 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
     float m_run = kNegInf;
     float l_run = 0.0f;
     if (w_begin < w_end) {
-        pages(w_begin);
+        look(w_begin);
         fetch(w_begin);
-        if (w_begin + 1 < w_end) {
-            pages(w_begin + 1);
-        }
+        look(w_begin + 1);
     }
     for (int w = w_begin; w < w_end; ++w) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the window is in LDS
         __syncthreads();
         if (w + 1 < w_end) {
             fetch(w + 1);
-            if (w + 2 < w_end) {
-                pages(w + 2);
-            }
+            look(w + 2);
         }
         const int key0 = w * kWindow;
         if (key0 > last_pos) {
@@ -770,16 +822,47 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         }
         const uint8_t* const s_k = s_mem[w & 1];
         const uint8_t* const s_v = s_k + kTileBytes;
-        floatx16 sc[2] = {floatx16{}, floatx16{}};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        const auto read_k = [&](uint4 (&k)[2], int i) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int row = 32 * t + r;
                 const int piece = (2 * i + q) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
-                const uint4 kf = *reinterpret_cast<const uint4*>(s_k + row * kRowBytes + piece * 16);
-                sc[t] = mfma32(T{}, kf, qf[i], sc[t]);
+                k[t] = *reinterpret_cast<const uint4*>(s_k + row * kRowBytes + piece * 16);
             }
+        };
+        const auto read_v = [&](uint4& v, int n, int i) __attribute__((always_inline)) {
+            uint2 part[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                // 16 lanes: keys 16 n + 8 t + 4 q .. + 3, dims 32 i + 16 (lane / 16 % 2) .. + 15
+                const int row = 16 * n + 8 * t + 4 * q + (lane & 15) / 4;
+                const int piece = (4 * i + 2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^
+                                  (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
+                part[t] = read_transposed(s_v + row * kRowBytes + piece * 16 + (lane & 1) * 8);
+            }
+            v = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+        };
+        // operands are read two steps ahead of their products, held there by the
+        // scheduling barriers
+        floatx16 sc[2] = {floatx16{}, floatx16{}};
+        uint4 kf[3][2], vf[D / 32];
+        read_k(kf[0], 0);
+        read_k(kf[1], 1);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (i + 2 < kSteps) {
+                read_k(kf[(i + 2) % 3], i + 2);
+            } else {
+#pragma unroll
+                for (int d = 0; d < D / 64; ++d) {
+                    read_v(vf[(i + 2 - kSteps) * (D / 64) + d], 0, (i + 2 - kSteps) * (D / 64) + d);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                sc[t] = mfma32(T{}, kf[i % 3][t], qf[i], sc[t]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         // sc[t][e]: key 32 t + 8 (e / 4) + 4 q + e % 4 of the window
         if (__builtin_amdgcn_readfirstlane(static_cast<int>(key0 + kWindow > first_pos + 1)) != 0) {
@@ -800,10 +883,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
                 mx = fmaxf(mx, sc[t][e]);
             }
         }
+        // the maximum may lag behind by 2^8 (weights up to 256 are as exact): sums are
+        // rescaled a few times a row, not in every window
         const float m_new = fmaxf(m_run, halves_max(mx) * a.scale_log2);
-        const float m_sub = m_new == kNegInf ? 0.0f : m_new;
-        if (__any(m_new != m_run)) {
-            const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+        if (__any(m_new > m_run + 8.0f)) {
+            const float corr = __builtin_amdgcn_exp2f(m_run - (m_new == kNegInf ? 0.0f : m_new));
             l_run *= corr;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
@@ -814,30 +898,35 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
             }
             m_run = m_new;
         }
-        // steps of 16 keys: the lane's weights of scores 8 (n % 2) .. + 7 of half n / 2
+        const float m_sub = m_run == kNegInf ? 0.0f : m_run;
+        // steps of 16 keys: the lane's weights of scores 8 (n % 2) .. + 7 of half n / 2;
+        // between the products of a step the next step's weights are formed and its V read
+        uint32_t p[2][4];
+        const auto weights = [&](int n, int e) __attribute__((always_inline)) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e], a.scale_log2, -m_sub));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e + 1], a.scale_log2, -m_sub));
+            p[n & 1][e] = pack(T{}, p0, p1);
+            l_run = add_pair(T{}, p[n & 1][e], l_run);
+        };
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            weights(0, e);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            uint32_t p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e], a.scale_log2, -m_sub));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e + 1], a.scale_log2, -m_sub));
-                l_run += p0 + p1;
-                p[e] = pack(T{}, p0, p1);
-            }
-            const uint4 pf = make_uint4(p[0], p[1], p[2], p[3]);
+            const uint4 pf = make_uint4(p[n & 1][0], p[n & 1][1], p[n & 1][2], p[n & 1][3]);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-                uint2 part[2];
+                acc[i] = mfma32(T{}, vf[i], pf, acc[i]);
+                if (n < 3) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    // 16 lanes: keys 16 n + 8 t + 4 q .. + 3, dims 32 i + 16 (lane / 16 % 2) .. + 15
-                    const int row = 16 * n + 8 * t + 4 * q + (lane & 15) / 4;
-                    const int piece = (4 * i + 2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^
-                                      (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
-                    part[t] = read_transposed(s_v + row * kRowBytes + piece * 16 + (lane & 1) * 8);
+                    for (int e = 0; e < 128 / D; ++e) {
+                        weights(n + 1, i * (128 / D) + e);
+                    }
+                    read_v(vf[i], n + 1, i);
                 }
-                acc[i] = mfma32(T{}, make_uint4(part[0].x, part[0].y, part[1].x, part[1].y), pf, acc[i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
