@@ -345,7 +345,7 @@ struct PagedAttnArgs {
     const int32_t* starts = nullptr;   // [sequences + 1] first rows
     const int32_t* kv_lens = nullptr;  // [sequences]
     uint16_t* out = nullptr;
-    float* partials = nullptr;  // [tokens, q_heads, splits, head_dim], then (max, sum) of each
+    float* partials = nullptr;  // the key splits' sums (16-byte aligned)
     int64_t tokens = 0;
     int64_t sequences = 0;
     int64_t q_heads = 0, kv_heads = 0, group = 0, head_dim = 0;
@@ -360,6 +360,7 @@ struct PagedAttnArgs {
 struct PagedAttnPlan {
     int64_t few_blocks = 0;
     int64_t tile_splits = 0;
+    int tile_groups = 1;  // K-groups of a tile's block
     int64_t slots = 0;   // tile slots of the tile kernel's grid
     int64_t splits = 0;  // the most of either: row length of the partials
     int64_t workspace_bytes = 0;

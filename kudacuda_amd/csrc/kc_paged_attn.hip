@@ -116,6 +116,15 @@ __device__ __forceinline__ int64_t key_row(const PagedAttnArgs& a, int page, int
     return id * a.page_stride + static_cast<int64_t>(key & ((1 << a.page_shift) - 1)) * a.token_stride;
 }
 
+// The partials' parts: sums [row, head, split, dim], (max, sum) [row, head, split],
+// and how many splits a row and head has [row, head].
+__device__ __forceinline__ float* split_stats(const PagedAttnArgs& a, int D, int splits) {
+    return a.partials + a.tokens * a.q_heads * splits * D;
+}
+__device__ __forceinline__ int32_t* split_counts(const PagedAttnArgs& a, int D, int splits) {
+    return reinterpret_cast<int32_t*>(a.partials + a.tokens * a.q_heads * splits * (D + 2));
+}
+
 // ----------------------------------------------------------- careful columns
 // Columns [c0, c0 + count) of a (sequence, KV head) over keys [begin, end) in
 // plain fp32, 16 lanes a column: where a product met an infinity or NaN of a key
@@ -127,7 +136,7 @@ __device__ __forceinline__ void careful_columns(const PagedAttnArgs& a, const Se
     constexpr int kDims = D / 16;
     const int G = static_cast<int>(a.group);
     const int d0 = static_cast<int>(threadIdx.x) % 16 * kDims;
-    for (int c = c0 + static_cast<int>(threadIdx.x) / 16; c < c0 + count; c += kThreads / 16) {
+    for (int c = c0 + static_cast<int>(threadIdx.x) / 16; c < c0 + count; c += static_cast<int>(blockDim.x) / 16) {
         const int token = c / G;
         const int head = g * G + c % G;
         const int pos = s.kv_len - s.q_len + token;
@@ -176,7 +185,7 @@ __device__ __forceinline__ void careful_columns(const PagedAttnArgs& a, const Se
                 part[d] = acc[d];
             }
             if (d0 == 0) {
-                float* ml = a.partials + a.tokens * a.q_heads * splits * D + 2 * at;
+                float* ml = split_stats(a, D, splits) + 2 * at;
                 ml[0] = m;
                 ml[1] = l;
             }
@@ -189,18 +198,16 @@ template <typename T, int D>
 __device__ __forceinline__ void nan_columns(const PagedAttnArgs& a, const Sequence& s, int g, int c0, int count,
                                             int splits) {
     const int G = static_cast<int>(a.group);
-    for (int i = threadIdx.x; i < count * D; i += kThreads) {
+    for (int i = threadIdx.x; i < count * D; i += blockDim.x) {
         const int c = c0 + i / D;
         const int64_t row = s.first + c / G;
         const int head = g * G + c % G;
         if (splits == 1) {
             a.out[row * a.out_stride + head * D + i % D] = T::store(__builtin_nanf(""));
         } else if (i % D == 0) {
-            float* ml = a.partials + a.tokens * a.q_heads * splits * D + 2 * ((row * a.q_heads + head) * splits);
-            for (int k = 0; k < splits; ++k) {
-                ml[2 * k] = 0.0f;
-                ml[2 * k + 1] = __builtin_nanf("");
-            }
+            const int64_t unit = row * a.q_heads + head;
+            *reinterpret_cast<float2*>(split_stats(a, D, splits) + 2 * unit * splits) = make_float2(0.0f, __builtin_nanf(""));
+            split_counts(a, D, splits)[unit] = 1;
         }
     }
 }
@@ -223,20 +230,18 @@ __device__ __forceinline__ void put_column(const PagedAttnArgs& a, int64_t row, 
     *reinterpret_cast<float4*>(part) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(part + 4) = make_float4(v[4], v[5], v[6], v[7]);
     if (d0 == 0) {
-        *reinterpret_cast<float2*>(a.partials + a.tokens * a.q_heads * splits * D + 2 * at) = make_float2(m, l);
+        *reinterpret_cast<float2*>(split_stats(a, D, splits) + 2 * at) = make_float2(m, l);
     }
 }
 
-// Splits of a column that no block of its kind writes weigh nothing.
+// How many splits columns [c0, c0 + count) have: told once, by the block with the last.
 template <int D>
-__device__ __forceinline__ void clear_splits(const PagedAttnArgs& a, const Sequence& s, int g, int c0, int count,
-                                             int from, int splits) {
+__device__ __forceinline__ void tell_splits(const PagedAttnArgs& a, const Sequence& s, int g, int c0, int count, int made,
+                                            int splits) {
     const int G = static_cast<int>(a.group);
-    const int n = splits - from;
-    for (int i = threadIdx.x; i < count * n; i += kThreads) {
-        const int c = c0 + i / n;
-        const int64_t at = ((s.first + c / G) * a.q_heads + g * G + c % G) * splits + from + i % n;
-        *reinterpret_cast<float2*>(a.partials + a.tokens * a.q_heads * splits * D + 2 * at) = make_float2(kNegInf, 0.0f);
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        const int c = c0 + i;
+        split_counts(a, D, splits)[(s.first + c / G) * a.q_heads + g * G + c % G] = made;
     }
 }
 
@@ -607,8 +612,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
             if (s.bad) {
                 nan_columns<T, D>(a, s, g, c0, count, splits);
             } else {
-                if (to == line.rounds && split + 1 < splits) {
-                    clear_splits<D>(a, s, g, c0, count, split + 1, splits);
+                if (to == line.rounds && splits > 1) {
+                    tell_splits<D>(a, s, g, c0, count, split + 1, splits);
                 }
                 few_rows_tile<T, D>(a, s, index, g, c0, at - first, splits > 1 ? to : 0x7fffffff / kRound, split, splits,
                                     s_mem, s_ml, &s_redo);
@@ -625,7 +630,22 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 
 // ----------------------------------------------------------------- row tiles
 // 128 columns of a (sequence, KV head): four waves of 32 over the same 64 keys,
-// whose K and V rows go straight to LDS, one window ahead.
+// whose K and V rows go straight to LDS, one window ahead.  Two waves a SIMD hide
+// each other's waits and arithmetic: from two such blocks on a CU, or, where there
+// are fewer tiles, from one block of two K-groups, which take alternate windows and
+// meet in LDS at the end.
+//
+// A wave takes 32 products of 32 cycles a window (D = 128) and about as long in fp32
+// arithmetic (exp of 32 scores a lane).  Weights enter the second product rounded to
+// 16 bits and their sum adds the rounded ones: half a step of the type a weight, at
+// random, next to the result's own half step (2-norm error of a prompt of 8192 bf16
+// tokens 1.9e-3, of the result's rounding alone 1.6e-3); a second part of each weight
+// would cost half as many products again.  Measured, 8192 tokens of 16 heads over 2
+// KV heads: 346 us at first, 318 with loads that bypass the compiler's waits, 293
+// with operands read ahead and the maximum allowed to lag, 287 with page bases as
+// scalars, 262 with the waves' priorities and the order of blocks (1050 TFLOP/s; a
+// library product of 8192^3 1405).  Forming the next window's scores between this
+// window's weights (250 VGPRs) took 293.
 constexpr int kTileRows = 128;
 constexpr int kWindow = 64;
 
@@ -653,35 +673,45 @@ __device__ __forceinline__ float halves_sum(float v) {
 
 // Tile slots: sequence i owns slots from floor(starts[i] G / 128) + i on, at least
 // as many as it has tiles, so the grid follows from the token count alone.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(PagedAttnArgs a, int slots, int tile_splits,
-                                                                           int splits, int few_rows) {
+template <typename T, int D, int GROUPS>
+__global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) void paged_attention_tile_kernel(PagedAttnArgs a, int slots,
+                                                                                    int tile_splits, int splits,
+                                                                                    int few_rows) {
     constexpr int kSteps = D / 16;
     constexpr int kRowBytes = D * 2;
     constexpr int kPieces = D / 8;
     constexpr int kTileBytes = kWindow * kRowBytes;
     constexpr int kLoadRows = 1024 / kRowBytes;      // rows of a wave's load
     constexpr int kLoads = kWindow / (4 * kLoadRows);  // loads of a wave for a tile of K (and of V)
-    __shared__ __attribute__((aligned(16))) uint8_t s_mem[2][2 * kTileBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[GROUPS][2][2 * kTileBytes];
+    __shared__ float s_stats[GROUPS > 1 ? kTileRows : 1][2];
     __shared__ int s_index;
     __shared__ int s_redo;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
+    const int group = __builtin_amdgcn_readfirstlane(tid >> 8);  // the K-group
     const int r = lane & 31;
     const int q = lane >> 5;
     const int G = static_cast<int>(a.group);
     const int kv_heads = static_cast<int>(a.kv_heads);
-    // later tiles see more keys: they start first
-    const int g = static_cast<int>(blockIdx.x) % kv_heads;
-    const int split = static_cast<int>(blockIdx.x) / kv_heads % tile_splits;
-    const int slot = slots - 1 - static_cast<int>(blockIdx.x) / kv_heads / tile_splits;
+    // Later tiles see more keys: they start first, and of the first two blocks of a CU
+    // the second is the lighter the heavier the first is.
+    int order = static_cast<int>(blockIdx.x);
+    if (GROUPS == 1) {
+        const int total = static_cast<int>(gridDim.x);
+        const int end = total < 512 ? total : 512;
+        order = order >= 256 && order < end ? 255 + end - order : order;
+    }
+    const int g = order % kv_heads;
+    const int split = order / kv_heads % tile_splits;
+    const int slot = slots - 1 - order / kv_heads / tile_splits;
     if (tid == 0) {
         s_index = 0;
         s_redo = 0;
     }
     __syncthreads();
-    for (int i = tid; i < static_cast<int>(a.sequences); i += kThreads) {
+    for (int i = tid; i < static_cast<int>(a.sequences); i += kThreads * GROUPS) {
         const int64_t base = static_cast<int64_t>(a.starts[i]) * G / kTileRows + i;
         if (base <= slot) {
             atomicMax(&s_index, i);
@@ -703,8 +733,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         }
         return;
     }
-    if (split == 0 && splits > tile_splits) {
-        clear_splits<D>(a, s, g, static_cast<int>(c0), count, tile_splits, splits);
+    if (split == 0 && splits > 1) {
+        tell_splits<D>(a, s, g, static_cast<int>(c0), count, tile_splits, splits);
     }
     const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
     const uint16_t* const kbase = a.k + g * a.head_stride;
@@ -744,7 +774,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         const int v = D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
         return (lane % kPieces) ^ (value ? v : k);
     };
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(s_mem[0]) + wave * 1024);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(s_mem[group][0]) + wave * 1024);
     // Whole windows of pages that hold a load's rows together (and begin within 4 GB
     // of a pool's beginning times a page id): a load's base is the wave's, its lanes'
     // offsets are the same in every window.  Bytes from here on.
@@ -771,8 +801,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         const int key = w * kWindow + lane % (4 * kLoads) * kLoadRows;
         pages = table[(key < keys ? key : keys - 1) >> a.page_shift];
     };
-    const auto fetch = [&](int w) __attribute__((always_inline)) {
-        const uint32_t lds = lds0 + (w & 1) * (2 * kTileBytes);
+    const auto fetch = [&](int w, int buffer) __attribute__((always_inline)) {
+        const uint32_t lds = lds0 + buffer * (2 * kTileBytes);
         if (together && (w + 1) * kWindow <= keys) {
             const bool out = static_cast<uint32_t>(pages) >= static_cast<uint32_t>(a.num_pages);
             bad |= out;
@@ -804,23 +834,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
     }
     float m_run = kNegInf;
     float l_run = 0.0f;
-    if (w_begin < w_end) {
-        look(w_begin);
-        fetch(w_begin);
-        look(w_begin + 1);
+    if (w_begin + group < w_end) {
+        look(w_begin + group);
+        fetch(w_begin + group, 0);
+        look(w_begin + group + GROUPS);
     }
-    for (int w = w_begin; w < w_end; ++w) {
+    int buffer = 0;
+    for (int w0 = w_begin; w0 < w_end; w0 += GROUPS, buffer ^= 1) {
+        const int w = w0 + group;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the window is in LDS
         __syncthreads();
-        if (w + 1 < w_end) {
-            fetch(w + 1);
-            look(w + 2);
+        if (w + GROUPS < w_end) {
+            fetch(w + GROUPS, buffer ^ 1);
+            look(w + 2 * GROUPS);
         }
         const int key0 = w * kWindow;
-        if (key0 > last_pos) {
-            continue;  // no column of this wave sees the window
+        if (w >= w_end || key0 > last_pos) {
+            continue;  // no window for this group, or no column of this wave sees it
         }
-        const uint8_t* const s_k = s_mem[w & 1];
+        const uint8_t* const s_k = s_mem[group][buffer];
         const uint8_t* const s_v = s_k + kTileBytes;
         const auto read_k = [&](uint4 (&k)[2], int i) __attribute__((always_inline)) {
 #pragma unroll
@@ -842,17 +874,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
             }
             v = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
         };
-        // operands are read two steps ahead of their products, held there by the
-        // scheduling barriers
+        // operands are read ahead of their products, held there by the scheduling
+        // barriers; a wave that multiplies goes before one that does arithmetic
         floatx16 sc[2] = {floatx16{}, floatx16{}};
-        uint4 kf[3][2], vf[D / 32];
-        read_k(kf[0], 0);
-        read_k(kf[1], 1);
+        constexpr int kAhead = D == 128 ? 2 : 1;
+        uint4 kf[kAhead + 1][2], vf[D / 32];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            read_k(kf[i], i);
+        }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            if (i + 2 < kSteps) {
-                read_k(kf[(i + 2) % 3], i + 2);
-            } else {
+            if (i + kAhead < kSteps) {
+                read_k(kf[(i + kAhead) % (kAhead + 1)], i + kAhead);
+            }
+            if (i + 2 >= kSteps) {
 #pragma unroll
                 for (int d = 0; d < D / 64; ++d) {
                     read_v(vf[(i + 2 - kSteps) * (D / 64) + d], 0, (i + 2 - kSteps) * (D / 64) + d);
@@ -860,10 +897,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                sc[t] = mfma32(T{}, kf[i % 3][t], qf[i], sc[t]);
+                sc[t] = mfma32(T{}, kf[i % (kAhead + 1)][t], qf[i], sc[t]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         // sc[t][e]: key 32 t + 8 (e / 4) + 4 q + e % 4 of the window
         if (__builtin_amdgcn_readfirstlane(static_cast<int>(key0 + kWindow > first_pos + 1)) != 0) {
             const int rel = pos - key0 - 4 * q;
@@ -913,6 +951,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
             weights(0, e);
         }
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const uint4 pf = make_uint4(p[n & 1][0], p[n & 1][1], p[n & 1][2], p[n & 1][3]);
@@ -929,6 +968,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     l_run = halves_sum(l_run);
     {
@@ -949,6 +989,44 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         careful_columns<T, D>(a, s, table, g, static_cast<int>(c0), count, w_begin * kWindow, w_end * kWindow, split,
                               splits);
         return;
+    }
+    if constexpr (GROUPS > 1) {
+        // the second group's columns meet the first's: [wave][4 values][lane]
+        float4* const s_acc = reinterpret_cast<float4*>(&s_mem[0][0][0]);
+        if (group == 1) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s_acc[(wave * (D / 8) + i * 4 + j) * 64 + lane] =
+                        make_float4(acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
+                }
+            }
+            s_stats[local][0] = m_run;  // (both halves of the wave hold it)
+            s_stats[local][1] = l_run;
+        }
+        __syncthreads();
+        if (group == 1) {
+            return;
+        }
+        const float m1 = s_stats[local][0];
+        const float m_all = fmaxf(m_run, m1);
+        const float m_sub = m_all == kNegInf ? 0.0f : m_all;
+        const float f0 = __builtin_amdgcn_exp2f(m_run - m_sub);
+        const float f1 = __builtin_amdgcn_exp2f(m1 - m_sub);
+        l_run = l_run * f0 + s_stats[local][1] * f1;
+        m_run = m_all;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 v = s_acc[(wave * (D / 8) + i * 4 + j) * 64 + lane];
+                acc[i][4 * j] = acc[i][4 * j] * f0 + v.x * f1;
+                acc[i][4 * j + 1] = acc[i][4 * j + 1] * f0 + v.y * f1;
+                acc[i][4 * j + 2] = acc[i][4 * j + 2] * f0 + v.z * f1;
+                acc[i][4 * j + 3] = acc[i][4 * j + 3] * f0 + v.w * f1;
+            }
+        }
     }
     if (local >= count) {
         return;
@@ -980,7 +1058,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_tile_kernel(Paged
         }
     }
     if (q == 0) {
-        *reinterpret_cast<float2*>(a.partials + a.tokens * a.q_heads * splits * D + 2 * at) = make_float2(m_run, l_run);
+        *reinterpret_cast<float2*>(split_stats(a, D, splits) + 2 * at) = make_float2(m_run, l_run);
     }
 }
 
@@ -1008,21 +1086,22 @@ __global__ __launch_bounds__(kThreads) void paged_attention_merge_kernel(PagedAt
     float l = 0.0f;
     float v[8] = {};
     if (live) {
-        const float2* const ml = reinterpret_cast<const float2*>(a.partials + a.tokens * a.q_heads * splits * D) + unit * splits;
+        const float2* const ml = reinterpret_cast<const float2*>(split_stats(a, D, splits)) + unit * splits;
         const float* const src = a.partials + unit * splits * D + d0;
-        for (int s0 = group; s0 < splits; s0 += kAhead * GROUPS) {
+        const int made = split_counts(a, D, splits)[unit];
+        for (int s0 = group; s0 < made; s0 += kAhead * GROUPS) {
             float2 w[kAhead];
             float4 x[kAhead], y[kAhead];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
-                const int s = s0 + j * GROUPS < splits ? s0 + j * GROUPS : splits - 1;
+                const int s = s0 + j * GROUPS < made ? s0 + j * GROUPS : made - 1;
                 w[j] = ml[s];
             }
             float m_new = m;
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
-                // a split without a key of the row has sum 0 and anything for its dims
-                w[j].y = s0 + j * GROUPS < splits ? w[j].y : 0.0f;
+                // (sum 0: no key of the row in this split)
+                w[j].y = s0 + j * GROUPS < made ? w[j].y : 0.0f;
                 m_new = fmaxf(m_new, w[j].y != 0.0f ? w[j].x : kNegInf);
                 if (w[j].y != 0.0f) {
                     x[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s0 + j * GROUPS) * D);
@@ -1112,20 +1191,26 @@ hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t
         }
     }
     if (plan.tile_splits > 0) {
-        const int64_t blocks = plan.slots * a.kv_heads * plan.tile_splits;
-        hipLaunchKernelGGL((paged_attention_tile_kernel<T, D>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
-                           stream, a, static_cast<int>(plan.slots), static_cast<int>(plan.tile_splits),
-                           static_cast<int>(plan.splits), plan.few_blocks > 0 ? kFewRows : 0);
+        const dim3 grid(static_cast<unsigned>(plan.slots * a.kv_heads * plan.tile_splits));
+        const int few_rows = plan.few_blocks > 0 ? kFewRows : 0;
+        if (plan.tile_groups == 1) {
+            hipLaunchKernelGGL((paged_attention_tile_kernel<T, D, 1>), grid, dim3(kThreads), 0, stream, a,
+                               static_cast<int>(plan.slots), static_cast<int>(plan.tile_splits),
+                               static_cast<int>(plan.splits), few_rows);
+        } else {
+            hipLaunchKernelGGL((paged_attention_tile_kernel<T, D, 2>), grid, dim3(2 * kThreads), 0, stream, a,
+                               static_cast<int>(plan.slots), static_cast<int>(plan.tile_splits),
+                               static_cast<int>(plan.splits), few_rows);
+        }
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) {
             return status;
         }
     }
-    if (plan.splits > 4) {
-        return launch_merge<T, D, 16>(a, plan.splits, stream);
-    }
     if (plan.splits > 1) {
-        return launch_merge<T, D, 1>(a, plan.splits, stream);
+        // many splits of few rows: the groups work on them side by side
+        return plan.splits > 4 && a.tokens * a.q_heads < 2048 ? launch_merge<T, D, 16>(a, plan.splits, stream)
+                                                              : launch_merge<T, D, 1>(a, plan.splits, stream);
     }
     return hipSuccess;
 }
@@ -1151,10 +1236,14 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     }
     if (rows > kFewRows) {
         p.slots = tokens * group / kTileRows + sequences;
-        p.tile_splits = cap(512 / (p.slots * kv_heads), cap((max_kv_len + 2 * kWindow - 1) / (2 * kWindow), 32));
+        // two blocks of one K-group a CU, or one of two; a split is at least four windows
+        p.tile_groups = p.slots * kv_heads >= 512 ? 1 : 2;
+        const int64_t tiles = p.slots * kv_heads;
+        p.tile_splits = cap(tiles > 128 && tiles <= 192 ? 2 : 256 / tiles, cap((max_kv_len + 4 * kWindow - 1) / (4 * kWindow), 32));
     }
     const int64_t unit = tokens * q_heads * (head_dim + 2) * 4;
-    const int64_t room = unit > 0 ? workspace_bytes / unit : 0;
+    const int64_t counts = tokens * q_heads * 4;
+    const int64_t room = unit > 0 ? (workspace_bytes - counts) / unit : 0;
     // the few-row kernel counts its rounds in 31 bits
     const int64_t rounds = (max_keys + kRound - 1) / kRound;
     const bool countable = (tokens * q_heads / 16 + sequences * kv_heads) * rounds < (int64_t{1} << 31);
@@ -1162,7 +1251,7 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     few_splits = few_splits < most ? few_splits : most;
     p.tile_splits = p.tile_splits < most ? p.tile_splits : most;
     p.splits = few_splits > p.tile_splits ? few_splits : p.tile_splits;
-    p.workspace_bytes = p.splits > 1 ? unit * p.splits : 0;
+    p.workspace_bytes = p.splits > 1 ? unit * p.splits + counts : 0;
     return p;
 }
 
