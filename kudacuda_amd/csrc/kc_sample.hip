@@ -12,16 +12,20 @@
 // tokens, and a sum over 2^20 tokens fits in 64 bits.  A token below 2^-43 of the
 // most likely one weighs nothing.
 //
-// No row is sorted.  Tokens fall into 2048 buckets by log2 w; which bucket ends
-// the kept tokens follows from the buckets' counts and sums, and only that
-// bucket's tokens (tens to hundreds of them) are ordered.  Launches, each over
-// (blocks of a row, rows):
-//   1. the row's largest logit;  2. buckets (for top-k and top-p);
-//   3. tokens of the deciding buckets to a list, sums of the surely kept tokens
-//      of each chunk of 2048 ids;  4. one block a row: the list ordered, the last
-//      kept token, the chunk and in it the token that u falls on.
+// No row is sorted.  Tokens fall into buckets of 1/64 in log2 w; which bucket ends
+// the kept tokens follows from the buckets' counts and sums, and only that bucket's
+// tokens (a few to some hundred) are ordered.  Launches, each over (blocks of a row,
+// rows):
+//   1. the row's largest logit, and the largest of every 128 ids;
+//   2. buckets (for top-k and top-p; with top-k only those down to the k-th of the
+//      largest of 128, below which no kept token lies);
+//   3. tokens of the deciding buckets to a list, sums of the surely kept tokens of
+//      each chunk of 2048 ids;
+//   4. one block a row: the list ordered, the last kept token, the chunk and in it
+//      the token that u falls on.
 // The row is read by the first three (once from memory, then from the caches) and
-// one chunk of it by the last.
+// one chunk of it by the last.  A logit is first compared with the least one that
+// matters, in 32 bits; 64-bit arithmetic is for those that do.
 #include "kc_device.h"
 #include "kc_kernels.h"
 
@@ -29,40 +33,71 @@ namespace kc {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
 constexpr int kChunk = 8 * kThreads;  // ids of a chunk: 8 a thread
-constexpr int kBuckets = 2048;
+constexpr int kAhead = 4;             // chunks that a block requests together
+constexpr int kGroups = kThreads / 16;  // groups of 128 ids of a chunk, 16 lanes each
+constexpr int kUnits = 64;            // buckets of a factor of two
+constexpr int kDepth = 43 * kUnits;   // buckets of the weights' range
+constexpr int kBuckets = 11 * kThreads;
 constexpr int kList = 2048;           // most tokens that are ordered in LDS
-constexpr int kFinish = 1024;         // threads of the last launch
 constexpr int kWeightBits = 42;
-constexpr double kDepth = 43.0;       // log2 of the weights' range
+#ifndef SBL
+#define SBL 1280
+#endif
+constexpr int64_t kSampleBlocks = SBL;
 constexpr int kMaxChunks = static_cast<int>(kSampleMaxVocab / kChunk);
 constexpr int kIdBits = 20;
 constexpr uint64_t kIdMask = (uint64_t{1} << kIdBits) - 1;
 static_assert(kSampleMaxVocab <= (int64_t{1} << kIdBits), "ids of an order word");
+static_assert(kDepth < kBuckets, "a bucket for every weight");
 
-// What launch 3 tells launch 4 of a row's deciding buckets.
-struct Decision {
-    int32_t low;         // tokens of buckets below are kept (if min_p lets them)
-    int32_t high;        // [low, high]: top-p, or the bucket of the k-th token, decides
-    int32_t k_bucket;    // bucket of the k-th token (kBuckets: top-k off or too large)
-    int32_t listed;      // tokens of these buckets
-    uint64_t k_weight;   // weights and tokens of the buckets before k_bucket (of all: top-k off)
-    int64_t k_count;
-    uint64_t low_weight;  // weights of the buckets before low
+// 2^(-j / 64).
+__device__ constexpr double kPowers[kUnits] = {
+    0x1.0000000000000p+0, 0x1.fa7c1819e90d8p-1, 0x1.f50765b6e4540p-1, 0x1.efa1bee615a27p-1,
+    0x1.ea4afa2a490dap-1, 0x1.e502ee78b3ff6p-1, 0x1.dfc97337b9b5fp-1, 0x1.da9e603db3285p-1,
+    0x1.d5818dcfba487p-1, 0x1.d072d4a07897cp-1, 0x1.cb720dcef9069p-1, 0x1.c67f12e57d14bp-1,
+    0x1.c199bdd85529cp-1, 0x1.bcc1e904bc1d2p-1, 0x1.b7f76f2fb5e47p-1, 0x1.b33a2b84f15fbp-1,
+    0x1.ae89f995ad3adp-1, 0x1.a9e6b5579fdbfp-1, 0x1.a5503b23e255dp-1, 0x1.a0c667b5de565p-1,
+    0x1.9c49182a3f090p-1, 0x1.97d829fde4e50p-1, 0x1.93737b0cdc5e5p-1, 0x1.8f1ae99157736p-1,
+    0x1.8ace5422aa0dbp-1, 0x1.868d99b4492edp-1, 0x1.82589994cce13p-1, 0x1.7e2f336cf4e62p-1,
+    0x1.7a11473eb0187p-1, 0x1.75feb564267c9p-1, 0x1.71f75e8ec5f74p-1, 0x1.6dfb23c651a2fp-1,
+    0x1.6a09e667f3bcdp-1, 0x1.6623882552225p-1, 0x1.6247eb03a5585p-1, 0x1.5e76f15ad2148p-1,
+    0x1.5ab07dd485429p-1, 0x1.56f4736b527dap-1, 0x1.5342b569d4f82p-1, 0x1.4f9b2769d2ca7p-1,
+    0x1.4bfdad5362a27p-1, 0x1.486a2b5c13cd0p-1, 0x1.44e086061892dp-1, 0x1.4160a21f72e2ap-1,
+    0x1.3dea64c123422p-1, 0x1.3a7db34e59ff7p-1, 0x1.371a7373aa9cbp-1, 0x1.33c08b26416ffp-1,
+    0x1.306fe0a31b715p-1, 0x1.2d285a6e4030bp-1, 0x1.29e9df51fdee1p-1, 0x1.26b4565e27cddp-1,
+    0x1.2387a6e756238p-1, 0x1.2063b88628cd6p-1, 0x1.1d4873168b9aap-1, 0x1.1a35beb6fcb75p-1,
+    0x1.172b83c7d517bp-1, 0x1.1429aaea92de0p-1, 0x1.11301d0125b51p-1, 0x1.0e3ec32d3d1a2p-1,
+    0x1.0b5586cf9890fp-1, 0x1.0874518759bc8p-1, 0x1.059b0d3158574p-1, 0x1.02c9a3e778061p-1,
 };
+
+// What launch 3 tells launch 4 of a row.
+struct Decision {
+    uint64_t best;        // order word of the row's largest logit
+    uint64_t k_weight;    // weights of the buckets before k_bucket (of all: top-k off)
+    uint64_t low_weight;  // weights of the buckets before low
+    int32_t k_count;      // tokens of the buckets before k_bucket
+    int32_t low;          // tokens of buckets below are kept (if min_p lets them)
+    int32_t high;         // [low, high]: top-p, or the bucket of the k-th token, decides
+    int32_t k_bucket;     // bucket of the k-th token (kBuckets: top-k off or too large)
+    int32_t listed;       // tokens of these buckets
+};
+static_assert(sizeof(Decision) <= 64, "the row's workspace");
 
 // Workspace of a row, in this order.
 struct RowSpace {
     uint64_t* weights;   // [kBuckets]
-    uint32_t* counts;    // [kBuckets]
     uint64_t* list;      // [kList] order words
     uint64_t* sums;      // [chunks]
     uint64_t* best;      // [chunks] order word of each block's largest logit
     Decision* decision;
     uint32_t* listed;
+    uint32_t* counts;    // [kBuckets]
+    float* largest;      // [chunks * kGroups] of 128 ids each
 };
 __host__ __device__ inline int64_t row_bytes(int64_t chunks) {
-    return kBuckets * 12 + kList * 8 + chunks * 16 + 64 + 16;
+    return kBuckets * 12 + kList * 8 + chunks * (16 + kGroups * 4) + 64 + 16;
 }
 __device__ __forceinline__ RowSpace row_space(uint8_t* base, int64_t row, int chunks) {
     uint8_t* p = base + row * row_bytes(chunks);
@@ -80,9 +115,10 @@ __device__ __forceinline__ RowSpace row_space(uint8_t* base, int64_t row, int ch
     s.listed = reinterpret_cast<uint32_t*>(p);
     p += 16;
     s.counts = reinterpret_cast<uint32_t*>(p);
+    p += kBuckets * 4;
+    s.largest = reinterpret_cast<float*>(p);
     return s;
 }
-static_assert(sizeof(Decision) <= 64, "the row's workspace");
 
 // ---------------------------------------------------------------- one logit
 struct F32 {
@@ -96,33 +132,70 @@ template <>
 struct Raw<F32> {
     typedef float type;
 };
+__device__ __forceinline__ uint16_t lowest(Bf16) { return 0xff80u; }
+__device__ __forceinline__ uint16_t lowest(F16) { return 0xfc00u; }
+__device__ __forceinline__ float lowest(F32) { return -__builtin_huge_valf(); }
 
-// 8 logits from id on; -inf where the row ends.  NaN counts as -inf, -0 as 0.
+// 8 logits from id on as they are stored; -inf where the row ends.
 template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const typename Raw<T>::type* row, int64_t id, int64_t vocab) {
-    typedef typename Raw<T>::type raw;
-    const raw* p = row + id;
+struct Piece {
+    uint4 w[sizeof(typename Raw<T>::type) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const typename Raw<T>::type* row, int64_t id, int64_t vocab) {
+    const auto* const p = row + id;
+    Piece<T> v;
     if (id + 8 <= vocab && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-        raw v[8];
-        uint4 w[sizeof(raw) / 2];
 #pragma unroll
-        for (unsigned i = 0; i < sizeof(raw) / 2; ++i) {
-            w[i] = reinterpret_cast<const uint4*>(p)[i];
-        }
-        __builtin_memcpy(v, w, sizeof(v));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = T::load(v[i]);
+        for (unsigned i = 0; i < sizeof(v) / 16; ++i) {
+            v.w[i] = reinterpret_cast<const uint4*>(p)[i];
         }
     } else {
+        typename Raw<T>::type x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            x[i] = id + i < vocab ? T::load(p[i]) : -__builtin_huge_valf();
+            x[i] = id + i < vocab ? p[i] : lowest(T{});
         }
+        __builtin_memcpy(&v, x, sizeof(v));
     }
+    return v;
+}
+// As fp32; NaN counts as -inf, -0 as 0.
+template <typename T>
+__device__ __forceinline__ void unpack(float (&x)[8], const Piece<T>& v) {
+    typename Raw<T>::type raw[8];
+    __builtin_memcpy(raw, &v, sizeof(v));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+        x[i] = T::load(raw[i]);
         x[i] = x[i] == x[i] ? x[i] + 0.0f : -__builtin_huge_valf();
+    }
+}
+template <typename T>
+__device__ __forceinline__ const typename Raw<T>::type* row_logits(const SampleArgs& a, int64_t row) {
+    return static_cast<const typename Raw<T>::type*>(a.logits) + row * a.stride;
+}
+
+// f(chunk, first id, the thread's 8 logits from there) for chunks [begin, end),
+// kAhead of them requested together.
+template <typename T, typename F>
+__device__ __forceinline__ void for_chunks(const typename Raw<T>::type* logits, int64_t vocab, int begin, int end, F f) {
+    for (int c0 = begin; c0 < end; c0 += kAhead) {
+        Piece<T> piece[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (c0 + j < end) {
+                piece[j] = load_piece<T>(logits, static_cast<int64_t>(c0 + j) * kChunk + threadIdx.x * 8, vocab);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (c0 + j < end) {
+                float x[8];
+                unpack<T>(x, piece[j]);
+                f(c0 + j, static_cast<int64_t>(c0 + j) * kChunk + threadIdx.x * 8, x);
+            }
+        }
     }
 }
 
@@ -142,9 +215,9 @@ __device__ __forceinline__ int64_t order_id(uint64_t word) { return static_cast<
 struct Row {
     bool greedy;
     float top;       // largest logit
-    double scale;    // log2(e) / T
-    int64_t k;       // 0: off
-    double p;        // >= 1: off
+    double scale;    // 64 log2(e) / T: buckets of a logit
+    int k;           // 0: off
+    double p;        // 1: off
     uint64_t least;  // smallest weight that min_p lets pass
 };
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
@@ -152,7 +225,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
     const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
     r.greedy = !(t > 0.0f);
     r.top = 0.0f;
-    r.scale = r.greedy ? 0.0 : 0x1.71547652b82fep+0 / static_cast<double>(t);
+    r.scale = r.greedy ? 0.0 : kUnits * 0x1.71547652b82fep+0 / static_cast<double>(t);
     const int32_t k = a.top_k != nullptr ? a.top_k[row] : 0;
     r.k = k > 0 && k < a.vocab ? k : 0;  // (a row of one token has nothing to decide)
     const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
@@ -168,46 +241,66 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
 }
 __device__ __forceinline__ bool decides(const Row& r) { return r.k > 0 || r.p < 1.0; }
 
-// How far a logit lies below the largest, in log2 of the weight; >= kDepth: no weight.
+// How far a logit lies below the largest, in buckets; kDepth: it weighs nothing.
 __device__ __forceinline__ double depth_of(const Row& r, float x) {
     if (x == r.top) {
         return 0.0;
     }
     const double d = (static_cast<double>(r.top) - static_cast<double>(x)) * r.scale;
-    return d == d && x > -__builtin_huge_valf() ? d : kDepth;
+    return d < kDepth && x > -__builtin_huge_valf() ? d : kDepth;  // (NaN: kDepth)
 }
-__device__ __forceinline__ int bucket_of(double depth) {
-    const int b = static_cast<int>(depth * (kBuckets / kDepth));
-    return b < kBuckets ? b : kBuckets - 1;  // (the product may round up to kBuckets)
+__device__ __forceinline__ int bucket_of(double depth) { return static_cast<int>(depth); }
+
+// The least logit that may lie in a bucket below `buckets` (rounded down: a filter).
+__device__ __forceinline__ float least_logit(const Row& r, int buckets) {
+    if (r.top == __builtin_huge_valf()) {
+        return r.top;
+    }
+    const double c = static_cast<double>(r.top) - (buckets + 1) / r.scale;
+    return static_cast<float>(c - fabs(c) * 0x1p-23);
+}
+// Bits of the logits that are at least `least` (and above -inf).
+__device__ __forceinline__ uint32_t passing(const float (&x)[8], float least) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        mask |= x[i] >= least && x[i] > -__builtin_huge_valf() ? 1u << i : 0u;
+    }
+    return mask;
+}
+// One of 8 values by a running index.
+__device__ __forceinline__ float pick(const float (&x)[8], int i) {
+    const float a = (i & 1) != 0 ? x[1] : x[0];
+    const float b = (i & 1) != 0 ? x[3] : x[2];
+    const float c = (i & 1) != 0 ? x[5] : x[4];
+    const float d = (i & 1) != 0 ? x[7] : x[6];
+    const float e = (i & 2) != 0 ? b : a;
+    const float f = (i & 2) != 0 ? d : c;
+    return (i & 4) != 0 ? f : e;
 }
 
-// 2^(42 - depth) rounded to a whole number, 0 <= depth < 43: e^z of the fraction
-// less a half by its Taylor polynomial of degree 12 (|z| <= 0.35: 2^-52).
-__device__ __forceinline__ uint64_t weight_of(double depth) {
-    const double y = kWeightBits - depth;
-    const double n = floor(y);
-    const double z = (y - n - 0.5) * 0x1.62e42fefa39efp-1;
-    double e = 1.0 / 479001600.0;
-    e = fma(e, z, 1.0 / 39916800.0);
-    e = fma(e, z, 1.0 / 3628800.0);
-    e = fma(e, z, 1.0 / 362880.0);
-    e = fma(e, z, 1.0 / 40320.0);
-    e = fma(e, z, 1.0 / 5040.0);
-    e = fma(e, z, 1.0 / 720.0);
-    e = fma(e, z, 1.0 / 120.0);
+// 2^(42 - depth / 64) rounded to a whole number, 0 <= depth < kDepth: a table's power
+// for the whole buckets of the fraction, the Taylor polynomial of degree 5 of e^z for
+// the rest (|z| <= ln 2 / 64: off by 2^-49), and the addition of 2^52 that rounds.
+__device__ __forceinline__ uint64_t weight_of(double depth, const double* powers) {
+    const int whole = static_cast<int>(depth);
+    const double z = (whole - depth) * (0x1.62e42fefa39efp-1 / kUnits);
+    double e = 1.0 / 120.0;
     e = fma(e, z, 1.0 / 24.0);
     e = fma(e, z, 1.0 / 6.0);
     e = fma(e, z, 0.5);
     e = fma(e, z, 1.0);
-    e = fma(e, z, 1.0) * 0x1.6a09e667f3bcdp+0;
-    return static_cast<uint64_t>(ldexp(e, static_cast<int>(n)) + 0.5);
+    e = fma(e, z, 1.0);
+    const double y = powers[whole % kUnits] * e;
+    const int64_t shift = static_cast<int64_t>(kWeightBits - whole / kUnits) << 52;
+    const double w = __longlong_as_double(__double_as_longlong(y) + shift) + 0x1p52;
+    return static_cast<uint64_t>(__double_as_longlong(w)) & ((uint64_t{1} << 52) - 1);
 }
 
 // ------------------------------------------------------------ block helpers
 __device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 // Largest of a block's values, in every thread.
-template <int WAVES>
 __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s_part) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
@@ -220,19 +313,24 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s_part) {
     __syncthreads();
     v = s_part[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) {
+    for (int w = 1; w < kWaves; ++w) {
         v = max_u64(v, s_part[w]);
     }
     return v;
 }
 
 // Sum of the values of the threads before this one; total in every thread.
-template <int WAVES>
-__device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t* s_part, uint64_t& total) {
-    uint64_t sum = v;
+template <typename V>
+__device__ __forceinline__ V block_before(V v, uint64_t* s_part, V& total) {
+    V sum = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t left = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(sum), o, 64));
+        V left;
+        if constexpr (sizeof(V) == 8) {
+            left = static_cast<V>(__shfl_up(static_cast<unsigned long long>(sum), o, 64));
+        } else {
+            left = static_cast<V>(__shfl_up(static_cast<unsigned int>(sum), o, 64));
+        }
         sum += static_cast<int>(threadIdx.x & 63) >= o ? left : 0;
     }
     __syncthreads();
@@ -240,35 +338,57 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t* s_part, u
         s_part[threadIdx.x >> 6] = sum;
     }
     __syncthreads();
-    uint64_t before = 0;
+    V before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        before += w < static_cast<int>(threadIdx.x >> 6) ? s_part[w] : 0;
-        total += s_part[w];
+    for (int w = 0; w < kWaves; ++w) {
+        before += w < static_cast<int>(threadIdx.x >> 6) ? static_cast<V>(s_part[w]) : 0;
+        total += static_cast<V>(s_part[w]);
     }
     return before + sum - v;
 }
-
-template <typename T>
-__device__ __forceinline__ const typename Raw<T>::type* row_logits(const SampleArgs& a, int64_t row) {
-    return static_cast<const typename Raw<T>::type*>(a.logits) + row * a.stride;
+// Sum of a block's values, in every thread.
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* s_part) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        v += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), o, 64));
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        s_part[threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        v += s_part[w];
+    }
+    return v;
 }
 
-// The row's largest logit and its order word from the first launch's blocks.
-template <int WAVES>
+// The order word of the row's largest logit from the first launch's blocks.
 __device__ __forceinline__ uint64_t row_best(const RowSpace& s, int blocks, uint64_t* s_part) {
     uint64_t v = 0;
-    for (int i = threadIdx.x; i < blocks; i += WAVES * 64) {
+    for (int i = threadIdx.x; i < blocks; i += kThreads) {
         v = max_u64(v, s.best[i]);
     }
-    return block_max<WAVES>(v, s_part);
+    return block_max(v, s_part);
+}
+// The block's copy of the powers.
+__device__ __forceinline__ void load_powers(double* s_powers) {
+    if (threadIdx.x < kUnits) {
+        s_powers[threadIdx.x] = kPowers[threadIdx.x];
+    }
+}
+__device__ __forceinline__ int chunks_end(int chunks, int per) {
+    const int end = (static_cast<int>(blockIdx.x) + 1) * per;
+    return end < chunks ? end : chunks;
 }
 
 // ---------------------------------------------------------------- launches
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int chunks, int per) {
-    __shared__ uint64_t s_part[kThreads / 64];
+    __shared__ uint64_t s_part[kWaves];
     const int64_t row = blockIdx.y;
     const RowSpace s = row_space(a.workspace, row, chunks);
     const int blocks = static_cast<int>(gridDim.x);
@@ -279,23 +399,32 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int 
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *s.listed = 0;
     }
-    const auto* const logits = row_logits<T>(a, row);
-    const int end = (static_cast<int>(blockIdx.x) + 1) * per < chunks ? (static_cast<int>(blockIdx.x) + 1) * per : chunks;
-    uint64_t best = 0;
-    for (int c = static_cast<int>(blockIdx.x) * per; c < end; ++c) {
-        const int64_t id = static_cast<int64_t>(c) * kChunk + threadIdx.x * 8;
-        if (id < a.vocab) {
-            float x[8];
-            load8<T>(x, logits, id, a.vocab);
+    float best = -__builtin_huge_valf();
+    int64_t best_id = -1;
+    for_chunks<T>(row_logits<T>(a, row), a.vocab, static_cast<int>(blockIdx.x) * per, chunks_end(chunks, per),
+                  [&](int c, int64_t id, const float(&x)[8]) {
+                      float most = x[0];
+                      int at = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                best = max_u64(best, id + i < a.vocab ? order_word(x[i], id + i) : 0);
-            }
-        }
-    }
-    best = block_max<kThreads / 64>(best, s_part);
+                      for (int i = 1; i < 8; ++i) {
+                          at = x[i] > most ? i : at;
+                          most = fmaxf(most, x[i]);
+                      }
+                      if (id < a.vocab && (best_id < 0 || most > best)) {
+                          best = most;
+                          best_id = id + at;
+                      }
+                      most = fmaxf(most, row_ror<8>(most));
+                      most = fmaxf(most, row_ror<4>(most));
+                      most = fmaxf(most, row_ror<2>(most));
+                      most = fmaxf(most, row_ror<1>(most));
+                      if (threadIdx.x % 16 == 0) {
+                          s.largest[c * kGroups + threadIdx.x / 16] = most;
+                      }
+                  });
+    const uint64_t word = block_max(best_id < 0 ? 0 : order_word(best, best_id), s_part);
     if (threadIdx.x == 0) {
-        s.best[blockIdx.x] = best;
+        s.best[blockIdx.x] = word;
     }
 }
 
@@ -303,37 +432,71 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_buckets_kernel(SampleArgs a, int chunks, int per) {
     __shared__ unsigned long long s_weights[kBuckets];
     __shared__ uint32_t s_counts[kBuckets];
-    __shared__ uint64_t s_part[kThreads / 64];
+    __shared__ uint64_t s_part[kWaves];
+    __shared__ double s_powers[kUnits];
+    __shared__ int s_limit;
     const int64_t row = blockIdx.y;
     Row r = row_of(a, row);
     if (r.greedy || !decides(r)) {
         return;
     }
+    constexpr int kPer = kBuckets / kThreads;
     for (int i = threadIdx.x; i < kBuckets; i += kThreads) {
         s_weights[i] = 0;
         s_counts[i] = 0;
     }
+    load_powers(s_powers);
     const RowSpace s = row_space(a.workspace, row, chunks);
-    r.top = order_logit(row_best<kThreads / 64>(s, static_cast<int>(gridDim.x), s_part));
-    const auto* const logits = row_logits<T>(a, row);
-    const int end = (static_cast<int>(blockIdx.x) + 1) * per < chunks ? (static_cast<int>(blockIdx.x) + 1) * per : chunks;
-    for (int c = static_cast<int>(blockIdx.x) * per; c < end; ++c) {
-        const int64_t id = static_cast<int64_t>(c) * kChunk + threadIdx.x * 8;
-        if (id < a.vocab) {
-            float x[8];
-            load8<T>(x, logits, id, a.vocab);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double d = depth_of(r, x[i]);
-                if (d < kDepth) {
-                    atomicAdd(&s_counts[bucket_of(d)], 1u);
-                    if (r.p < 1.0) {
-                        atomicAdd(&s_weights[bucket_of(d)], static_cast<unsigned long long>(weight_of(d)));
-                    }
-                }
+    r.top = order_logit(row_best(s, static_cast<int>(gridDim.x), s_part));
+    int limit = kDepth;
+    if (r.k > 0 && r.k <= chunks * kGroups) {
+        // k of the groups' largest logits are at least the k-th of them: the k-th token
+        // lies no deeper
+        if (threadIdx.x == 0) {
+            s_limit = kDepth;
+        }
+        for (int i = threadIdx.x; i < chunks * kGroups; i += kThreads) {
+            const double d = depth_of(r, s.largest[i]);
+            if (d < kDepth) {
+                atomicAdd(&s_counts[bucket_of(d)], 1u);
             }
         }
+        __syncthreads();
+        const int b0 = static_cast<int>(threadIdx.x) * kPer;
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            mine += s_counts[b0 + i];
+        }
+        uint32_t total;
+        uint32_t c = block_before<uint32_t>(mine, s_part, total);
+        if (c < static_cast<uint32_t>(r.k) && c + mine >= static_cast<uint32_t>(r.k)) {
+            int b = b0;
+            for (; c + s_counts[b] < static_cast<uint32_t>(r.k); ++b) {
+                c += s_counts[b];
+            }
+            s_limit = b + 1;
+        }
+        __syncthreads();
+        limit = s_limit;
+        for (int i = threadIdx.x; i < kBuckets; i += kThreads) {
+            s_counts[i] = 0;
+        }
+        __syncthreads();
     }
+    const float least = least_logit(r, limit);
+    for_chunks<T>(row_logits<T>(a, row), a.vocab, static_cast<int>(blockIdx.x) * per, chunks_end(chunks, per),
+                  [&](int, int64_t, const float(&x)[8]) {
+                      for (uint32_t mask = passing(x, least); mask != 0; mask &= mask - 1) {
+                          const double d = depth_of(r, pick(x, __builtin_ctz(mask)));
+                          if (d < limit) {
+                              atomicAdd(&s_counts[bucket_of(d)], 1u);
+                              if (r.p < 1.0) {
+                                  atomicAdd(&s_weights[bucket_of(d)], static_cast<unsigned long long>(weight_of(d, s_powers)));
+                              }
+                          }
+                      }
+                  });
     __syncthreads();
     for (int i = threadIdx.x; i < kBuckets; i += kThreads) {
         if (s_counts[i] != 0) {
@@ -346,51 +509,48 @@ __global__ __launch_bounds__(kThreads) void sample_buckets_kernel(SampleArgs a, 
 }
 
 // The deciding buckets, from the row's counts and weights (all threads of a block).
-__device__ __forceinline__ Decision decide(const Row& r, const RowSpace& s, uint64_t* s_part, Decision* s_decision) {
+__device__ __forceinline__ Decision decide(const Row& r, const RowSpace& s, uint64_t* s_part, Decision* s_decision,
+                                           uint64_t* s_upper) {
     constexpr int kPer = kBuckets / kThreads;
-    constexpr int kWaves = kThreads / 64;
     const int b0 = static_cast<int>(threadIdx.x) * kPer;
     uint32_t count[kPer];
     uint64_t weight[kPer];
-    uint64_t counts = 0;
+    uint32_t counts = 0;
     uint64_t weights = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         count[i] = s.counts[b0 + i];
-        weight[i] = s.weights[b0 + i];
+        weight[i] = r.p < 1.0 ? s.weights[b0 + i] : 0;
         counts += count[i];
         weights += weight[i];
     }
-    uint64_t all_counts, all_weights;
-    const uint64_t counts_before = block_before<kWaves>(counts, s_part, all_counts);
-    const uint64_t weights_before = block_before<kWaves>(weights, s_part, all_weights);
+    uint32_t all_counts;
+    uint64_t all_weights = 0;
+    const uint32_t counts_before = block_before<uint32_t>(counts, s_part, all_counts);
+    const uint64_t weights_before = r.p < 1.0 ? block_before<uint64_t>(weights, s_part, all_weights) : 0;
     if (threadIdx.x == 0) {
         s_decision->k_bucket = kBuckets;
         s_decision->k_weight = all_weights;
-        s_decision->k_count = static_cast<int64_t>(all_counts);
+        s_decision->k_count = static_cast<int32_t>(all_counts);
         s_decision->low = kBuckets;
         s_decision->high = kBuckets - 1;
         s_decision->low_weight = all_weights;
-        s_decision->listed = 0;
-    }
-    __shared__ uint64_t s_upper;  // the most that the first top_k tokens can weigh
-    if (threadIdx.x == 0) {
-        s_upper = all_weights;
+        *s_upper = all_weights;  // the most that the first top_k tokens can weigh
     }
     __syncthreads();
-    if (r.k > 0) {
-        uint64_t c = counts_before;
+    if (r.k > 0 && counts_before < static_cast<uint32_t>(r.k) && counts_before + counts >= static_cast<uint32_t>(r.k)) {
+        uint32_t c = counts_before;
         uint64_t w = weights_before;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            if (c < static_cast<uint64_t>(r.k) && c + count[i] >= static_cast<uint64_t>(r.k)) {
+            if (c < static_cast<uint32_t>(r.k) && c + count[i] >= static_cast<uint32_t>(r.k)) {
                 s_decision->k_bucket = b0 + i;
                 s_decision->k_weight = w;
-                s_decision->k_count = static_cast<int64_t>(c);
+                s_decision->k_count = static_cast<int32_t>(c);
                 s_decision->low = b0 + i;
                 s_decision->high = b0 + i;
                 s_decision->low_weight = w;
-                s_upper = w + weight[i];
+                *s_upper = w + weight[i];
             }
             c += count[i];
             w += weight[i];
@@ -400,46 +560,41 @@ __device__ __forceinline__ Decision decide(const Row& r, const RowSpace& s, uint
     if (r.p < 1.0) {
         // the k-th token's bucket holds some of its weight, at most all of it
         const double least = r.p * static_cast<double>(s_decision->k_weight);
-        const double most = r.p * static_cast<double>(s_upper);
+        const double most = r.p * static_cast<double>(*s_upper);
         uint64_t w = weights_before;
-        bool is_low[kPer], is_high[kPer];
+        int low = -1, high = -1;
         uint64_t low_weight = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const bool first = b0 + i == 0;
             const double before = static_cast<double>(w);
             const double after = static_cast<double>(w + weight[i]);
-            is_low[i] = after >= least && (first || before < least);
-            is_high[i] = after >= most && (first || before < most);
-            low_weight = is_low[i] ? w : low_weight;
+            const bool is_low = after >= least && (first || before < least);
+            low = is_low ? b0 + i : low;
+            low_weight = is_low ? w : low_weight;
+            high = after >= most && (first || before < most) ? b0 + i : high;
             w += weight[i];
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (is_low[i]) {
-                s_decision->low = b0 + i;
-                s_decision->low_weight = low_weight;
-            }
-            if (is_high[i]) {
-                s_decision->high = b0 + i;
-            }
+        if (low >= 0) {
+            s_decision->low = low;
+            s_decision->low_weight = low_weight;
         }
+        if (high >= 0) {
+            s_decision->high = high;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    uint64_t listed = 0;
+    uint32_t listed = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int b = b0 + i;
         listed += (b >= s_decision->low && b <= s_decision->high) || b == s_decision->k_bucket ? count[i] : 0;
     }
-    uint64_t all_listed;
-    (void)block_before<kWaves>(listed, s_part, all_listed);
-    if (threadIdx.x == 0) {
-        s_decision->listed = static_cast<int32_t>(all_listed);
-    }
-    __syncthreads();
-    return *s_decision;
+    const uint32_t all_listed = static_cast<uint32_t>(block_sum(listed, s_part));
+    Decision d = *s_decision;
+    d.listed = static_cast<int32_t>(all_listed);
+    return d;
 }
 
 __device__ __forceinline__ bool listed_bucket(const Decision& d, int b) {
@@ -448,66 +603,91 @@ __device__ __forceinline__ bool listed_bucket(const Decision& d, int b) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int chunks, int per) {
-    __shared__ uint64_t s_part[kThreads / 64];
+    __shared__ uint64_t s_part[kWaves];
     __shared__ uint64_t s_list[kList];
+    __shared__ uint64_t s_sums[kWaves * kAhead];
+    __shared__ double s_powers[kUnits];
     __shared__ Decision s_decision;
+    __shared__ uint64_t s_upper;
     __shared__ uint32_t s_listed, s_at;
     const int64_t row = blockIdx.y;
     Row r = row_of(a, row);
-    if (r.greedy) {
+    const RowSpace s = row_space(a.workspace, row, chunks);
+    if (r.greedy && blockIdx.x != 0) {
         return;
     }
-    const RowSpace s = row_space(a.workspace, row, chunks);
-    r.top = order_logit(row_best<kThreads / 64>(s, static_cast<int>(gridDim.x), s_part));
+    const uint64_t best = row_best(s, static_cast<int>(gridDim.x), s_part);
+    r.top = order_logit(best);
     Decision d{};
     d.low = kBuckets;
     d.high = kBuckets - 1;
     d.k_bucket = kBuckets;
-    if (decides(r)) {
-        d = decide(r, s, s_part, &s_decision);
+    if (!r.greedy && decides(r)) {
+        d = decide(r, s, s_part, &s_decision, &s_upper);
     }
+    d.best = best;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *s.decision = d;
+    }
+    if (r.greedy) {
+        return;
     }
     if (threadIdx.x == 0) {
         s_listed = 0;
     }
+    load_powers(s_powers);
     __syncthreads();
-    const auto* const logits = row_logits<T>(a, row);
-    const int end = (static_cast<int>(blockIdx.x) + 1) * per < chunks ? (static_cast<int>(blockIdx.x) + 1) * per : chunks;
-    for (int c = static_cast<int>(blockIdx.x) * per; c < end; ++c) {
-        const int64_t id = static_cast<int64_t>(c) * kChunk + threadIdx.x * 8;
+    const bool keep_list = d.listed <= kList;
+    const int deepest = d.low > kDepth ? kDepth : max(max(d.low, d.high), d.k_bucket < kBuckets ? d.k_bucket : 0) + 1;
+    const float least = least_logit(r, deepest);
+    int in_round = 0;
+    const int begin = static_cast<int>(blockIdx.x) * per;
+    const int end = chunks_end(chunks, per);
+    for_chunks<T>(row_logits<T>(a, row), a.vocab, begin, end, [&](int c, int64_t id, const float(&x)[8]) {
         uint64_t sum = 0;
-        if (id < a.vocab) {
-            float x[8];
-            load8<T>(x, logits, id, a.vocab);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double depth = depth_of(r, x[i]);
-                if (depth < kDepth) {
-                    const int b = bucket_of(depth);
-                    if (b < d.low) {
-                        const uint64_t w = weight_of(depth);
-                        sum += w >= r.least ? w : 0;
-                    } else if (d.listed <= kList && listed_bucket(d, b)) {
-                        s_list[atomicAdd(&s_listed, 1u) % kList] = order_word(x[i], id + i);
-                    }
+        for (uint32_t mask = passing(x, least); mask != 0; mask &= mask - 1) {
+            const int i = __builtin_ctz(mask);
+            const float v = pick(x, i);
+            const double depth = depth_of(r, v);
+            if (depth < kDepth) {
+                const int b = bucket_of(depth);
+                if (b < d.low) {
+                    const uint64_t w = weight_of(depth, s_powers);
+                    sum += w >= r.least ? w : 0;
+                } else if (keep_list && listed_bucket(d, b)) {
+                    s_list[atomicAdd(&s_listed, 1u) % kList] = order_word(v, id + i);
                 }
             }
         }
-        uint64_t total;
-        (void)block_before<kThreads / 64>(sum, s_part, total);
-        if (threadIdx.x == 0) {
-            s.sums[c] = total;
+        // the waves' sums of a round of chunks meet at its end
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            sum += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(sum), o, 64));
         }
-    }
+        if ((threadIdx.x & 63) == 0) {
+            s_sums[in_round * kWaves + (threadIdx.x >> 6)] = sum;
+        }
+        if (++in_round == kAhead || c + 1 == end) {
+            __syncthreads();
+            if (static_cast<int>(threadIdx.x) < in_round) {
+                uint64_t total = 0;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    total += s_sums[threadIdx.x * kWaves + w];
+                }
+                s.sums[c + 1 - in_round + threadIdx.x] = total;
+            }
+            in_round = 0;
+            __syncthreads();
+        }
+    });
     __syncthreads();
     if (threadIdx.x == 0 && s_listed != 0) {
         s_at = atomicAdd(s.listed, s_listed);
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < s_listed; i += kThreads) {
-        s.list[s_at + i] = s_list[i];
+        s.list[(s_at + i) % kList] = s_list[i];
     }
 }
 
@@ -517,47 +697,43 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
 // over buckets [low, high] reaches the target, digit by digit over the whole row;
 // 0: it is never reached.
 template <typename T>
-__device__ __noinline__ uint64_t select_in_row(const SampleArgs& a, const Row& r, const typename Raw<T>::type* logits,
-                                               int low, int high, uint64_t before, int64_t k, double target,
-                                               unsigned long long* s_bins, uint64_t* s_part) {
-    constexpr int kWaves = kFinish / 64;
+__device__ __forceinline__ uint64_t select_in_row(const SampleArgs& a, const Row& r, const typename Raw<T>::type* logits,
+                                               int low, int high, uint64_t before, int k, double target,
+                                               unsigned long long* s_bins, uint64_t* s_part, const double* s_powers) {
+    static_assert(kThreads == 256, "a thread a digit");
     __shared__ uint64_t s_prefix, s_before;
     __shared__ int s_found;
     uint64_t prefix = 0;
-    int shift = 52;
+    int shift = 32 + kIdBits;
     while (shift > 0) {
         const int bits = shift >= 8 ? 8 : shift;
         shift -= bits;
         __syncthreads();
-        if (threadIdx.x < 256) {
-            s_bins[threadIdx.x] = 0;
-        }
+        s_bins[threadIdx.x] = 0;
         if (threadIdx.x == 0) {
             s_found = 0;
         }
         __syncthreads();
-        for (int64_t id = threadIdx.x * 8; id < a.vocab; id += kFinish * 8) {
-            float x[8];
-            load8<T>(x, logits, id, a.vocab);
-            for (int i = 0; i < 8; ++i) {
-                const double depth = depth_of(r, x[i]);
-                if (depth < kDepth) {
-                    const int b = bucket_of(depth);
-                    const uint64_t word = order_word(x[i], id + i);
-                    if (b >= low && b <= high && (word >> shift) >> bits == prefix) {
-                        atomicAdd(&s_bins[(word >> shift) & ((1u << bits) - 1)],
-                                  static_cast<unsigned long long>(k > 0 ? 1 : weight_of(depth)));
-                    }
-                }
-            }
-        }
+        for_chunks<T>(logits, a.vocab, 0, static_cast<int>((a.vocab + kChunk - 1) / kChunk),
+                      [&](int, int64_t id, const float(&x)[8]) {
+                          for (int i = 0; i < 8; ++i) {
+                              const double depth = depth_of(r, x[i]);
+                              if (depth < kDepth) {
+                                  const int b = bucket_of(depth);
+                                  const uint64_t word = order_word(x[i], id + i);
+                                  if (b >= low && b <= high && (word >> shift) >> bits == prefix) {
+                                      atomicAdd(&s_bins[(word >> shift) & ((1u << bits) - 1)],
+                                                static_cast<unsigned long long>(k > 0 ? 1 : weight_of(depth, s_powers)));
+                                  }
+                              }
+                          }
+                      });
         __syncthreads();
         // bins from the highest digit down: thread i holds digit last - i
-        const int last = (1 << bits) - 1;
-        const int digit = last - static_cast<int>(threadIdx.x);
+        const int digit = (1 << bits) - 1 - static_cast<int>(threadIdx.x);
         const uint64_t mine = digit >= 0 ? s_bins[digit] : 0;
         uint64_t total;
-        const uint64_t until = before + block_before<kWaves>(mine, s_part, total);
+        const uint64_t until = before + block_before<uint64_t>(mine, s_part, total);
         const bool short_of = k > 0 ? until < static_cast<uint64_t>(k) : static_cast<double>(until) < target;
         const bool reaches = k > 0 ? until + mine >= static_cast<uint64_t>(k) : static_cast<double>(until + mine) >= target;
         if (mine != 0 && short_of && reaches) {
@@ -576,24 +752,27 @@ __device__ __noinline__ uint64_t select_in_row(const SampleArgs& a, const Row& r
 }
 
 template <typename T>
-__global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleArgs a, int chunks, int blocks) {
-    constexpr int kWaves = kFinish / 64;
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, int chunks) {
+    constexpr int kMine = kList / kThreads;  // list entries of a thread
     __shared__ uint64_t s_part[kWaves];
     __shared__ uint64_t s_list[kList];
+    __shared__ uint64_t s_weights[kThreads];
     __shared__ unsigned long long s_sums[kMaxChunks];
     __shared__ unsigned long long s_bins[256];
+    __shared__ double s_powers[kUnits];
     __shared__ uint64_t s_last, s_rest;
     __shared__ int s_chunk;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x;
     Row r = row_of(a, row);
     const RowSpace s = row_space(a.workspace, row, chunks);
-    const uint64_t best = row_best<kWaves>(s, blocks, s_part);
-    r.top = order_logit(best);
+    const Decision d = *s.decision;
+    const float u = a.random[row];
+    r.top = order_logit(d.best);
     if (r.greedy || r.top == -__builtin_huge_valf()) {
         if (tid == 0) {
             const bool none = r.top == -__builtin_huge_valf();  // no token: no logit above -inf
-            a.tokens[row] = none ? 0 : static_cast<int32_t>(order_id(best));
+            a.tokens[row] = none ? 0 : static_cast<int32_t>(order_id(d.best));
             if (a.chances != nullptr) {
                 a.chances[row] = none ? 0.0f : 1.0f;
             }
@@ -601,200 +780,219 @@ __global__ __launch_bounds__(kFinish) void sample_finish_kernel(SampleArgs a, in
         return;
     }
     const auto* const logits = row_logits<T>(a, row);
-    const Decision d = *s.decision;
     const int n = d.listed;
     uint64_t last = 0;  // order word of the last kept token
-    for (int c = tid; c < chunks; c += kFinish) {
+    load_powers(s_powers);
+    for (int c = tid; c < chunks; c += kThreads) {
         s_sums[c] = s.sums[c];
     }
-    if (n > 0 && n <= kList) {
+    if (tid == 0) {
+        s_last = 0;
+    }
+    if (n > 0 && n <= kThreads) {
+        // a token a thread: what comes before it, by comparing it with every other
+        const uint64_t word = tid < n ? s.list[tid] : 0;
+        __syncthreads();
+        const double depth = tid < n ? depth_of(r, order_logit(word)) : 0.0;
+        const uint64_t weight = tid < n ? weight_of(depth, s_powers) : 0;
+        const int b = tid < n ? bucket_of(depth) : -1;
+        const bool in_k = b == d.k_bucket;
+        const bool in_p = b >= d.low && b <= d.high;
+        s_list[tid] = word;
+        s_weights[tid] = weight | static_cast<uint64_t>(in_k) << 63 | static_cast<uint64_t>(in_p) << 62;
+        __syncthreads();
+        uint32_t rank = 0;
+        uint64_t before = d.low_weight;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const uint64_t w = s_weights[j];
+            const bool earlier = s_list[j] > word;
+            rank += earlier ? static_cast<uint32_t>(w >> 63) : 0;
+            before += earlier && (w >> 62 & 1) != 0 ? w & ((uint64_t{1} << 62) - 1) : 0;
+        }
+        uint64_t k_weight = d.k_weight;
+        if (d.k_bucket < kBuckets) {
+            const int place = d.k_count + static_cast<int>(rank);
+            k_weight += block_sum(in_k && place < r.k ? weight : 0, s_part);
+            if (in_k && place + 1 == r.k) {
+                s_last = word;
+            }
+        }
+        __syncthreads();
+        last = s_last;
+        if (r.p < 1.0) {
+            // the last token with less than the target before it: the smallest word
+            const bool under = in_p && static_cast<double>(before) < r.p * static_cast<double>(k_weight);
+            last = max_u64(last, ~block_max(under ? ~word : 0, s_part));
+        }
+    } else if (n > 0 && n <= kList) {
         // the list in order: a bitonic network over the next power of two
-        int size = 2;
+        int size = 2 * kThreads;
         while (size < n) {
             size *= 2;
         }
-        for (int i = tid; i < size; i += kFinish) {
+        for (int i = tid; i < kList; i += kThreads) {
             s_list[i] = i < n ? s.list[i] : 0;
         }
         for (int width = 2; width <= size; width *= 2) {
             for (int step = width / 2; step >= 1; step /= 2) {
                 __syncthreads();
-                for (int i = tid; i < size / 2; i += kFinish) {
+                for (int i = tid; i < size / 2; i += kThreads) {
                     const int x = 2 * i - (i & (step - 1));
                     const int y = x + step;
                     const bool down = (x & width) == 0;
-                    const uint64_t u = s_list[x];
-                    const uint64_t v = s_list[y];
-                    if ((u < v) == down) {
-                        s_list[x] = v;
-                        s_list[y] = u;
+                    const uint64_t v = s_list[x];
+                    const uint64_t w = s_list[y];
+                    if ((v < w) == down) {
+                        s_list[x] = w;
+                        s_list[y] = v;
                     }
                 }
             }
         }
-        if (tid == 0) {
-            s_last = 0;
-        }
         __syncthreads();
-        // two tokens a thread: weights, and which buckets they are in
-        uint64_t word[2], weight[2];
-        bool in_k[2], in_p[2];
+        uint64_t weight[kMine];
+        bool in_k[kMine], in_p[kMine];
+        uint32_t k_mine = 0;
+        uint64_t p_mine = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int i = 2 * tid + j;
-            word[j] = i < n ? s_list[i] : 0;
-            const double depth = i < n ? depth_of(r, order_logit(word[j])) : kDepth;
-            weight[j] = i < n ? weight_of(depth) : 0;
+        for (int j = 0; j < kMine; ++j) {
+            const int i = kMine * tid + j;
+            const double depth = i < n ? depth_of(r, order_logit(s_list[i])) : 0.0;
+            weight[j] = i < n ? weight_of(depth, s_powers) : 0;
             const int b = i < n ? bucket_of(depth) : -1;
             in_k[j] = b == d.k_bucket;
             in_p[j] = b >= d.low && b <= d.high;
+            k_mine += in_k[j] ? 1 : 0;
+            p_mine += in_p[j] ? weight[j] : 0;
         }
         uint64_t k_weight = d.k_weight;
         if (d.k_bucket < kBuckets) {
-            uint64_t all;
-            uint64_t rank = block_before<kWaves>((in_k[0] ? 1 : 0) + (in_k[1] ? 1 : 0), s_part, all);
+            uint32_t all;
+            int place = d.k_count + static_cast<int>(block_before<uint32_t>(k_mine, s_part, all));
             uint64_t mine = 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < kMine; ++j) {
                 if (in_k[j]) {
-                    const uint64_t place = static_cast<uint64_t>(d.k_count) + rank;
-                    mine += place < static_cast<uint64_t>(r.k) ? weight[j] : 0;
-                    if (place + 1 == static_cast<uint64_t>(r.k)) {
-                        s_last = word[j];
+                    mine += place < r.k ? weight[j] : 0;
+                    if (place + 1 == r.k) {
+                        s_last = s_list[kMine * tid + j];
                     }
-                    ++rank;
+                    ++place;
                 }
             }
-            (void)block_before<kWaves>(mine, s_part, all);
-            k_weight += all;
+            k_weight += block_sum(mine, s_part);
         }
         __syncthreads();
         last = s_last;
         if (r.p < 1.0) {
             const double target = r.p * static_cast<double>(k_weight);
             uint64_t all;
-            uint64_t before = d.low_weight + block_before<kWaves>((in_p[0] ? weight[0] : 0) + (in_p[1] ? weight[1] : 0),
-                                                                  s_part, all);
-            // the last token with less than the target before it
+            uint64_t before = d.low_weight + block_before<uint64_t>(p_mine, s_part, all);
             uint64_t mine = ~uint64_t{0};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < kMine; ++j) {
                 if (in_p[j]) {
-                    mine = static_cast<double>(before) < target ? word[j] : mine;
+                    mine = static_cast<double>(before) < target ? s_list[kMine * tid + j] : mine;
                     before += weight[j];
                 }
             }
-            // order words fall along the list: the smallest is the last
-            const uint64_t p_last = ~block_max<kWaves>(~mine, s_part);
-            last = max_u64(last, p_last);
+            last = max_u64(last, ~block_max(~mine, s_part));
         }
     } else if (n > kList) {
+        __syncthreads();
         uint64_t k_weight = d.k_weight;
         if (d.k_bucket < kBuckets) {
-            last = select_in_row<T>(a, r, logits, d.k_bucket, d.k_bucket, static_cast<uint64_t>(d.k_count), r.k, 0.0,
-                                    s_bins, s_part);
+            last = select_in_row<T>(a, r, logits, d.k_bucket, d.k_bucket, static_cast<uint64_t>(d.k_count), r.k, 0.0, s_bins,
+                                    s_part, s_powers);
             uint64_t mine = 0;
-            for (int64_t id = tid * 8; id < a.vocab; id += kFinish * 8) {
-                float x[8];
-                load8<T>(x, logits, id, a.vocab);
+            for_chunks<T>(logits, a.vocab, 0, chunks, [&](int, int64_t id, const float(&x)[8]) {
                 for (int i = 0; i < 8; ++i) {
                     const double depth = depth_of(r, x[i]);
                     if (depth < kDepth && bucket_of(depth) == d.k_bucket && order_word(x[i], id + i) >= last) {
-                        mine += weight_of(depth);
+                        mine += weight_of(depth, s_powers);
                     }
                 }
-            }
-            uint64_t all;
-            (void)block_before<kWaves>(mine, s_part, all);
-            k_weight += all;
+            });
+            k_weight += block_sum(mine, s_part);
         }
         if (r.p < 1.0) {
             last = max_u64(last, select_in_row<T>(a, r, logits, d.low, d.high, d.low_weight, 0,
-                                                  r.p * static_cast<double>(k_weight), s_bins, s_part));
+                                                  r.p * static_cast<double>(k_weight), s_bins, s_part, s_powers));
         }
     }
     // the first token stays, whatever the settings
-    last = last < best ? last : best;
+    last = last < d.best ? last : d.best;
     __syncthreads();
     if (n > 0 && n <= kList) {
-        for (int i = tid; i < n; i += kFinish) {
+        for (int i = tid; i < n; i += kThreads) {
             const uint64_t word = s_list[i];
-            const double depth = depth_of(r, order_logit(word));
-            const uint64_t w = weight_of(depth);
+            const uint64_t w = weight_of(depth_of(r, order_logit(word)), s_powers);
             if (word >= last && w >= r.least) {
                 atomicAdd(&s_sums[order_id(word) / kChunk], static_cast<unsigned long long>(w));
             }
         }
     } else if (n > kList) {
-        for (int64_t id = tid * 8; id < a.vocab; id += kFinish * 8) {
-            float x[8];
-            load8<T>(x, logits, id, a.vocab);
+        for_chunks<T>(logits, a.vocab, 0, chunks, [&](int c, int64_t id, const float(&x)[8]) {
             uint64_t sum = 0;
             for (int i = 0; i < 8; ++i) {
                 const double depth = depth_of(r, x[i]);
                 if (depth < kDepth && bucket_of(depth) >= d.low && order_word(x[i], id + i) >= last) {
-                    const uint64_t w = weight_of(depth);
+                    const uint64_t w = weight_of(depth, s_powers);
                     sum += w >= r.least ? w : 0;
                 }
             }
-            atomicAdd(&s_sums[id / kChunk], static_cast<unsigned long long>(sum));
-        }
+            atomicAdd(&s_sums[c], static_cast<unsigned long long>(sum));
+        });
     }
     __syncthreads();
     // the chunk that u falls on
-    static_assert(kMaxChunks <= kFinish, "one chunk a thread");
-    const uint64_t mine = tid < chunks ? s_sums[tid] : 0;
+    static_assert(kMaxChunks == 2 * kThreads, "two chunks a thread");
+    const uint64_t first = 2 * tid < chunks ? s_sums[2 * tid] : 0;
+    const uint64_t second = 2 * tid + 1 < chunks ? s_sums[2 * tid + 1] : 0;
     uint64_t total;
-    const uint64_t before = block_before<kWaves>(mine, s_part, total);
-    const double u = static_cast<double>(a.random[row]);
-    uint64_t target = u > 0.0 ? static_cast<uint64_t>((u < 1.0 ? u : 1.0) * static_cast<double>(total)) : 0;
+    const uint64_t before = block_before<uint64_t>(first + second, s_part, total);
+    const double share = u > 0.0f ? (u < 1.0f ? static_cast<double>(u) : 1.0) : 0.0;
+    uint64_t target = static_cast<uint64_t>(share * static_cast<double>(total));
     target = target < total ? target : total - 1;
-    if (before <= target && target < before + mine) {
-        s_chunk = tid;
-        s_rest = target - before;
+    if (before <= target && target < before + first + second) {
+        const bool later = target >= before + first;
+        s_chunk = 2 * tid + (later ? 1 : 0);
+        s_rest = target - before - (later ? first : 0);
     }
     __syncthreads();
-    const int64_t id0 = static_cast<int64_t>(s_chunk) * kChunk;
+    const int64_t id = static_cast<int64_t>(s_chunk) * kChunk + tid * 8;
     const uint64_t rest = s_rest;
-    uint64_t w[2] = {0, 0};
-    if (tid < kChunk / 8) {
-        float x[8];
-        load8<T>(x, logits, id0 + tid * 8, a.vocab);
-        uint64_t* const out = s_list;  // [kChunk] weights
+    float x[8];
+    unpack<T>(x, load_piece<T>(logits, id, a.vocab));
+    uint64_t w[8];
+    uint64_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double depth = depth_of(r, x[i]);
-            uint64_t v = 0;
-            if (depth < kDepth && id0 + tid * 8 + i < a.vocab) {
-                v = weight_of(depth);
-                v = v >= r.least && order_word(x[i], id0 + tid * 8 + i) >= last ? v : 0;
-            }
-            out[tid * 8 + i] = v;
-        }
+    for (int i = 0; i < 8; ++i) {
+        const double depth = id + i < a.vocab ? depth_of(r, x[i]) : kDepth;
+        w[i] = depth < kDepth ? weight_of(depth, s_powers) : 0;
+        w[i] = w[i] >= r.least && order_word(x[i], id + i) >= last ? w[i] : 0;
+        mine += w[i];
     }
-    __syncthreads();
-    static_assert(kChunk == 2 * kFinish && kChunk <= kList, "two ids of the chunk a thread");
-    w[0] = s_list[2 * tid];
-    w[1] = s_list[2 * tid + 1];
     uint64_t all;
-    const uint64_t at = block_before<kWaves>(w[0] + w[1], s_part, all);
+    uint64_t from = block_before<uint64_t>(mine, s_part, all);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint64_t from = j == 0 ? at : at + w[0];
-        if (from <= rest && rest < from + w[j]) {
-            a.tokens[row] = static_cast<int32_t>(id0 + 2 * tid + j);
+    for (int i = 0; i < 8; ++i) {
+        if (from <= rest && rest < from + w[i]) {
+            a.tokens[row] = static_cast<int32_t>(id + i);
             if (a.chances != nullptr) {
-                a.chances[row] = static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total));
+                a.chances[row] = static_cast<float>(static_cast<double>(w[i]) / static_cast<double>(total));
             }
         }
+        from += w[i];
     }
 }
 
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
     const int chunks = static_cast<int>((a.vocab + kChunk - 1) / kChunk);
-    // about eight blocks a CU; with few rows a chunk a block
-    const int64_t per = (chunks * a.rows + 2047) / 2048;
+    // about five blocks a CU; with few rows a chunk a block
+    const int64_t per = (chunks * a.rows + kSampleBlocks - 1) / kSampleBlocks;
     const int blocks = static_cast<int>((chunks + per - 1) / per);
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.rows));
     hipLaunchKernelGGL(sample_max_kernel<T>, grid, dim3(kThreads), 0, stream, a, chunks, static_cast<int>(per));
@@ -808,8 +1006,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
         status = hipGetLastError();
     }
     if (status == hipSuccess) {
-        hipLaunchKernelGGL(sample_finish_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(kFinish), 0, stream, a, chunks,
-                           blocks);
+        hipLaunchKernelGGL(sample_finish_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, stream, a, chunks);
         status = hipGetLastError();
     }
     return status;
@@ -817,7 +1014,10 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) { return rows * row_bytes((vocab + kChunk - 1) / kChunk); }
+int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
+    const int64_t bytes = row_bytes((vocab + kChunk - 1) / kChunk);
+    return rows * bytes;
+}
 
 hipError_t launch_sample(int dtype, const SampleArgs& a, hipStream_t stream) {
     if (dtype == 0) {
