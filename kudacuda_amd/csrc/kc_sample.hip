@@ -40,12 +40,14 @@ constexpr int kGroups = kThreads / 16;  // groups of 128 ids of a chunk, 16 lane
 constexpr int kUnits = 64;            // buckets of a factor of two
 constexpr int kDepth = 43 * kUnits;   // buckets of the weights' range
 constexpr int kBuckets = 11 * kThreads;
+constexpr int kPer = kBuckets / kThreads;
 constexpr int kList = 2048;           // most tokens that are ordered in LDS
 constexpr int kWeightBits = 42;
-#ifndef SBL
-#define SBL 1280
-#endif
-constexpr int64_t kSampleBlocks = SBL;
+// Blocks of the first and third launch, and large blocks of the second: more rows than
+// fill these take more chunks a block (128 rows of mixed settings: 2048 and 512 98 us,
+// 1280 and 512 103; 32 rows with top-p: 256 large blocks 55 us, 512 60, 1024 65).
+constexpr int64_t kBlocks = 2048;
+constexpr int64_t kLargeBlocks = 256;
 constexpr int kMaxChunks = static_cast<int>(kSampleMaxVocab / kChunk);
 constexpr int kIdBits = 20;
 constexpr uint64_t kIdMask = (uint64_t{1} << kIdBits) - 1;
@@ -81,7 +83,6 @@ struct Decision {
     int32_t low;          // tokens of buckets below are kept (if min_p lets them)
     int32_t high;         // [low, high]: top-p, or the bucket of the k-th token, decides
     int32_t k_bucket;     // bucket of the k-th token (kBuckets: top-k off or too large)
-    int32_t listed;       // tokens of these buckets
 };
 static_assert(sizeof(Decision) <= 64, "the row's workspace");
 
@@ -176,27 +177,46 @@ __device__ __forceinline__ const typename Raw<T>::type* row_logits(const SampleA
     return static_cast<const typename Raw<T>::type*>(a.logits) + row * a.stride;
 }
 
-// f(chunk, first id, the thread's 8 logits from there) for chunks [begin, end),
-// kAhead of them requested together.
-template <typename T, typename F>
-__device__ __forceinline__ void for_chunks(const typename Raw<T>::type* logits, int64_t vocab, int begin, int end, F f) {
-    for (int c0 = begin; c0 < end; c0 += kAhead) {
-        Piece<T> piece[kAhead];
+// The thread's pieces of chunks c0, c0 + STRIDE, .. that lie before `end`, kAhead of them.
+template <typename T>
+struct Round {
+    Piece<T> piece[kAhead];
+};
+template <typename T, int STRIDE = 1>
+__device__ __forceinline__ Round<T> load_round(const typename Raw<T>::type* logits, int64_t vocab, int c0, int end) {
+    Round<T> r;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (c0 + j < end) {
-                piece[j] = load_piece<T>(logits, static_cast<int64_t>(c0 + j) * kChunk + threadIdx.x * 8, vocab);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (c0 + j < end) {
-                float x[8];
-                unpack<T>(x, piece[j]);
-                f(c0 + j, static_cast<int64_t>(c0 + j) * kChunk + threadIdx.x * 8, x);
-            }
+    for (int j = 0; j < kAhead; ++j) {
+        const int c = c0 + j * STRIDE;
+        if (c < end) {
+            r.piece[j] = load_piece<T>(logits, static_cast<int64_t>(c) * kChunk + threadIdx.x % kThreads * 8, vocab);
         }
     }
+    return r;
+}
+// f(chunk, first id, the thread's 8 logits from there) for every STRIDE-th chunk of
+// [begin, end), a round requested while the one before is worked on; the first is
+// there already.
+template <typename T, int STRIDE = 1, typename F>
+__device__ __forceinline__ void for_chunks(const typename Raw<T>::type* logits, int64_t vocab, int begin, int end,
+                                           Round<T> round, F f) {
+    for (int c0 = begin; c0 < end; c0 += kAhead * STRIDE) {
+        const Round<T> next = load_round<T, STRIDE>(logits, vocab, c0 + kAhead * STRIDE, end);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int c = c0 + j * STRIDE;
+            if (c < end) {
+                float x[8];
+                unpack<T>(x, round.piece[j]);
+                f(c, static_cast<int64_t>(c) * kChunk + threadIdx.x % kThreads * 8, x);
+            }
+        }
+        round = next;
+    }
+}
+template <typename T, typename F>
+__device__ __forceinline__ void for_chunks(const typename Raw<T>::type* logits, int64_t vocab, int begin, int end, F f) {
+    for_chunks<T>(logits, vocab, begin, end, load_round<T>(logits, vocab, begin, end), f);
 }
 
 // Order word of a token: larger comes first in (logit descending, id ascending).
@@ -243,11 +263,9 @@ __device__ __forceinline__ bool decides(const Row& r) { return r.k > 0 || r.p < 
 
 // How far a logit lies below the largest, in buckets; kDepth: it weighs nothing.
 __device__ __forceinline__ double depth_of(const Row& r, float x) {
-    if (x == r.top) {
-        return 0.0;
-    }
     const double d = (static_cast<double>(r.top) - static_cast<double>(x)) * r.scale;
-    return d < kDepth && x > -__builtin_huge_valf() ? d : kDepth;  // (NaN: kDepth)
+    const double within = d < kDepth && x > -__builtin_huge_valf() ? d : kDepth;  // (NaN: kDepth)
+    return x == r.top ? 0.0 : within;
 }
 __device__ __forceinline__ int bucket_of(double depth) { return static_cast<int>(depth); }
 
@@ -268,6 +286,10 @@ __device__ __forceinline__ uint32_t passing(const float (&x)[8], float least) {
     }
     return mask;
 }
+// Tokens before which the weights sum to less than this are in top_p of `total`.
+__device__ __forceinline__ uint64_t top_p_end(const Row& r, uint64_t total) {
+    return static_cast<uint64_t>(ceil(r.p * static_cast<double>(total)));
+}
 // One of 8 values by a running index.
 __device__ __forceinline__ float pick(const float (&x)[8], int i) {
     const float a = (i & 1) != 0 ? x[1] : x[0];
@@ -277,6 +299,24 @@ __device__ __forceinline__ float pick(const float (&x)[8], int i) {
     const float e = (i & 2) != 0 ? b : a;
     const float f = (i & 2) != 0 ? d : c;
     return (i & 4) != 0 ? f : e;
+}
+
+// f(i, x[i]) for the logits that `least` lets pass: one by one where few do, all eight
+// in line (f finds the others out) where some lane of the wave has more than three.
+template <typename F>
+__device__ __forceinline__ void for_passing(const float (&x)[8], float least, F f) {
+    uint32_t mask = passing(x, least);
+    if (__any(__builtin_popcount(mask) > 3)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            f(i, x[i]);
+        }
+        return;
+    }
+    for (; mask != 0; mask &= mask - 1) {
+        const int i = __builtin_ctz(mask);
+        f(i, pick(x, i));
+    }
 }
 
 // 2^(42 - depth / 64) rounded to a whole number, 0 <= depth < kDepth: a table's power
@@ -301,6 +341,7 @@ __device__ __forceinline__ uint64_t weight_of(double depth, const double* powers
 __device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 // Largest of a block's values, in every thread.
+template <int WAVES = kWaves>
 __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s_part) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
@@ -313,14 +354,14 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s_part) {
     __syncthreads();
     v = s_part[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
+    for (int w = 1; w < WAVES; ++w) {
         v = max_u64(v, s_part[w]);
     }
     return v;
 }
 
 // Sum of the values of the threads before this one; total in every thread.
-template <typename V>
+template <typename V, int WAVES = kWaves>
 __device__ __forceinline__ V block_before(V v, uint64_t* s_part, V& total) {
     V sum = v;
 #pragma unroll
@@ -341,7 +382,7 @@ __device__ __forceinline__ V block_before(V v, uint64_t* s_part, V& total) {
     V before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         before += w < static_cast<int>(threadIdx.x >> 6) ? static_cast<V>(s_part[w]) : 0;
         total += static_cast<V>(s_part[w]);
     }
@@ -366,13 +407,13 @@ __device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* s_part) {
     return v;
 }
 
-// The order word of the row's largest logit from the first launch's blocks.
-__device__ __forceinline__ uint64_t row_best(const RowSpace& s, int blocks, uint64_t* s_part) {
+// The thread's largest of the first launch's blocks' order words.
+__device__ __forceinline__ uint64_t load_best(const RowSpace& s, int blocks) {
     uint64_t v = 0;
-    for (int i = threadIdx.x; i < blocks; i += kThreads) {
+    for (int i = threadIdx.x; i < blocks; i += static_cast<int>(blockDim.x)) {
         v = max_u64(v, s.best[i]);
     }
-    return block_max(v, s_part);
+    return v;
 }
 // The block's copy of the powers.
 __device__ __forceinline__ void load_powers(double* s_powers) {
@@ -428,11 +469,16 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int 
     }
 }
 
+// Large blocks: every block adds the buckets that it has filled to the row's, in
+// memory that all XCDs share.
+constexpr int kLarge = 1024;
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_buckets_kernel(SampleArgs a, int chunks, int per) {
+__global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, int chunks, int per, int max_blocks) {
+    constexpr int kStride = kLarge / kThreads;
     __shared__ unsigned long long s_weights[kBuckets];
     __shared__ uint32_t s_counts[kBuckets];
-    __shared__ uint64_t s_part[kWaves];
+    __shared__ uint64_t s_part[kLarge / 64];
     __shared__ double s_powers[kUnits];
     __shared__ int s_limit;
     const int64_t row = blockIdx.y;
@@ -440,160 +486,217 @@ __global__ __launch_bounds__(kThreads) void sample_buckets_kernel(SampleArgs a, 
     if (r.greedy || !decides(r)) {
         return;
     }
-    constexpr int kPer = kBuckets / kThreads;
-    for (int i = threadIdx.x; i < kBuckets; i += kThreads) {
+    const auto* const logits = row_logits<T>(a, row);
+    const int begin = static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / kThreads;
+    const int end = chunks_end(chunks, per);
+    const Round<T> round = load_round<T, kStride>(logits, a.vocab, begin, end);
+    const RowSpace s = row_space(a.workspace, row, chunks);
+    const uint64_t best = load_best(s, max_blocks);
+    const int groups = chunks * kGroups;
+    const bool bounded = r.k > 0 && r.k <= groups;
+    constexpr int kHeld = 2;  // largest logits of a thread that are requested at once
+    float largest[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int at = i * kLarge + static_cast<int>(threadIdx.x);
+        largest[i] = bounded && at < groups ? s.largest[at] : -__builtin_huge_valf();
+    }
+    for (int i = threadIdx.x; i < kBuckets; i += kLarge) {
         s_weights[i] = 0;
         s_counts[i] = 0;
     }
     load_powers(s_powers);
-    const RowSpace s = row_space(a.workspace, row, chunks);
-    r.top = order_logit(row_best(s, static_cast<int>(gridDim.x), s_part));
+    r.top = order_logit(block_max<kLarge / 64>(best, s_part));
     int limit = kDepth;
-    if (r.k > 0 && r.k <= chunks * kGroups) {
+    if (bounded) {
         // k of the groups' largest logits are at least the k-th of them: the k-th token
         // lies no deeper
         if (threadIdx.x == 0) {
             s_limit = kDepth;
         }
-        for (int i = threadIdx.x; i < chunks * kGroups; i += kThreads) {
-            const double d = depth_of(r, s.largest[i]);
+        const auto put = [&](float x) __attribute__((always_inline)) {
+            const double d = depth_of(r, x);
             if (d < kDepth) {
                 atomicAdd(&s_counts[bucket_of(d)], 1u);
             }
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            put(largest[i]);
+        }
+        for (int i = kHeld * kLarge + threadIdx.x; i < groups; i += kLarge) {
+            put(s.largest[i]);
         }
         __syncthreads();
         const int b0 = static_cast<int>(threadIdx.x) * kPer;
+        uint32_t count[kPer];
         uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            mine += s_counts[b0 + i];
+            count[i] = b0 < kBuckets ? s_counts[b0 + i] : 0;
+            mine += count[i];
         }
         uint32_t total;
-        uint32_t c = block_before<uint32_t>(mine, s_part, total);
-        if (c < static_cast<uint32_t>(r.k) && c + mine >= static_cast<uint32_t>(r.k)) {
-            int b = b0;
-            for (; c + s_counts[b] < static_cast<uint32_t>(r.k); ++b) {
-                c += s_counts[b];
+        uint32_t c = block_before<uint32_t, kLarge / 64>(mine, s_part, total);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (c < static_cast<uint32_t>(r.k) && c + count[i] >= static_cast<uint32_t>(r.k)) {
+                s_limit = b0 + i + 1;
             }
-            s_limit = b + 1;
+            c += count[i];
+            if (b0 < kBuckets) {
+                s_counts[b0 + i] = 0;
+            }
         }
         __syncthreads();
         limit = s_limit;
-        for (int i = threadIdx.x; i < kBuckets; i += kThreads) {
-            s_counts[i] = 0;
-        }
-        __syncthreads();
     }
     const float least = least_logit(r, limit);
-    for_chunks<T>(row_logits<T>(a, row), a.vocab, static_cast<int>(blockIdx.x) * per, chunks_end(chunks, per),
-                  [&](int, int64_t, const float(&x)[8]) {
-                      for (uint32_t mask = passing(x, least); mask != 0; mask &= mask - 1) {
-                          const double d = depth_of(r, pick(x, __builtin_ctz(mask)));
-                          if (d < limit) {
-                              atomicAdd(&s_counts[bucket_of(d)], 1u);
-                              if (r.p < 1.0) {
-                                  atomicAdd(&s_weights[bucket_of(d)], static_cast<unsigned long long>(weight_of(d, s_powers)));
-                              }
-                          }
-                      }
-                  });
+    for_chunks<T, kStride>(logits, a.vocab, begin, end, round, [&](int, int64_t, const float(&x)[8]) {
+        for_passing(x, least, [&](int, float v) __attribute__((always_inline)) {
+            const double d = depth_of(r, v);
+            if (d < limit) {
+                if (r.k > 0) {
+                    atomicAdd(&s_counts[bucket_of(d)], 1u);
+                }
+                if (r.p < 1.0) {
+                    atomicAdd(&s_weights[bucket_of(d)], static_cast<unsigned long long>(weight_of(d, s_powers)));
+                }
+            }
+        });
+    });
     __syncthreads();
-    for (int i = threadIdx.x; i < kBuckets; i += kThreads) {
+    for (int i = threadIdx.x; i < kBuckets; i += kLarge) {
         if (s_counts[i] != 0) {
             atomicAdd(&s.counts[i], s_counts[i]);
-            if (r.p < 1.0) {
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.weights[i]), s_weights[i]);
-            }
+        }
+        if (s_weights[i] != 0) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.weights[i]), s_weights[i]);
         }
     }
 }
 
+// A thread's share of the row's buckets as they are loaded, every 256th.
+struct Buckets {
+    uint32_t count[kPer];
+    uint64_t weight[kPer];
+};
+__device__ __forceinline__ Buckets load_buckets(const Row& r, const RowSpace& s) {
+    Buckets b;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        b.count[i] = r.k > 0 ? s.counts[i * kThreads + threadIdx.x] : 0;
+        b.weight[i] = r.p < 1.0 ? s.weights[i * kThreads + threadIdx.x] : 0;
+    }
+    return b;
+}
+
 // The deciding buckets, from the row's counts and weights (all threads of a block).
-__device__ __forceinline__ Decision decide(const Row& r, const RowSpace& s, uint64_t* s_part, Decision* s_decision,
-                                           uint64_t* s_upper) {
-    constexpr int kPer = kBuckets / kThreads;
+struct Found {
+    uint64_t k_weight, upper, low_weight;
+    int32_t k_bucket, k_count, low, high;
+};
+__device__ __forceinline__ Decision decide(const Row& r, const Buckets& loaded, uint64_t* s_weights, uint32_t* s_counts,
+                                           uint64_t* s_part, Found* s_found) {
     const int b0 = static_cast<int>(threadIdx.x) * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        s_counts[i * kThreads + threadIdx.x] = loaded.count[i];
+        s_weights[i * kThreads + threadIdx.x] = loaded.weight[i];
+    }
+    __syncthreads();
     uint32_t count[kPer];
     uint64_t weight[kPer];
     uint32_t counts = 0;
     uint64_t weights = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        count[i] = s.counts[b0 + i];
-        weight[i] = r.p < 1.0 ? s.weights[b0 + i] : 0;
+        count[i] = s_counts[b0 + i];
+        weight[i] = s_weights[b0 + i];
         counts += count[i];
         weights += weight[i];
     }
-    uint32_t all_counts;
-    uint64_t all_weights = 0;
-    const uint32_t counts_before = block_before<uint32_t>(counts, s_part, all_counts);
-    const uint64_t weights_before = r.p < 1.0 ? block_before<uint64_t>(weights, s_part, all_weights) : 0;
-    if (threadIdx.x == 0) {
-        s_decision->k_bucket = kBuckets;
-        s_decision->k_weight = all_weights;
-        s_decision->k_count = static_cast<int32_t>(all_counts);
-        s_decision->low = kBuckets;
-        s_decision->high = kBuckets - 1;
-        s_decision->low_weight = all_weights;
-        *s_upper = all_weights;  // the most that the first top_k tokens can weigh
+    // both sums of the threads before this one
+    uint32_t counts_before = counts;
+    uint64_t weights_before = weights;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t c = __shfl_up(counts_before, o, 64);
+        counts_before += static_cast<int>(threadIdx.x & 63) >= o ? c : 0;
+        if (r.p < 1.0) {
+            const uint64_t w = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(weights_before), o, 64));
+            weights_before += static_cast<int>(threadIdx.x & 63) >= o ? w : 0;
+        }
+    }
+    const int wave = static_cast<int>(threadIdx.x >> 6);
+    if ((threadIdx.x & 63) == 63) {
+        s_part[wave] = weights_before;
+        s_part[kWaves + wave] = counts_before;
     }
     __syncthreads();
-    if (r.k > 0 && counts_before < static_cast<uint32_t>(r.k) && counts_before + counts >= static_cast<uint32_t>(r.k)) {
+    counts_before -= counts;
+    weights_before -= weights;
+    uint32_t all_counts = 0;
+    uint64_t all_weights = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const uint32_t c = static_cast<uint32_t>(s_part[kWaves + w]);
+        counts_before += w < wave ? c : 0;
+        weights_before += w < wave ? s_part[w] : 0;
+        all_counts += c;
+        all_weights += s_part[w];
+    }
+    // the bucket of the k-th token; top-k off or larger than the row: none
+    const uint32_t k = static_cast<uint32_t>(r.k);
+    const bool has_k = r.k > 0 && all_counts >= k;
+    if (has_k && counts_before < k && counts_before + counts >= k) {
         uint32_t c = counts_before;
         uint64_t w = weights_before;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            if (c < static_cast<uint32_t>(r.k) && c + count[i] >= static_cast<uint32_t>(r.k)) {
-                s_decision->k_bucket = b0 + i;
-                s_decision->k_weight = w;
-                s_decision->k_count = static_cast<int32_t>(c);
-                s_decision->low = b0 + i;
-                s_decision->high = b0 + i;
-                s_decision->low_weight = w;
-                *s_upper = w + weight[i];
+            if (c < k && c + count[i] >= k) {
+                s_found->k_bucket = b0 + i;
+                s_found->k_weight = w;
+                s_found->k_count = static_cast<int32_t>(c);
+                s_found->upper = w + weight[i];
             }
             c += count[i];
             w += weight[i];
         }
     }
     __syncthreads();
+    Decision d{};
+    d.k_bucket = has_k ? s_found->k_bucket : kBuckets;
+    d.k_weight = has_k ? s_found->k_weight : all_weights;
+    d.k_count = has_k ? s_found->k_count : static_cast<int32_t>(all_counts);
+    d.low = has_k ? d.k_bucket : kBuckets;
+    d.high = has_k ? d.k_bucket : kBuckets - 1;
+    d.low_weight = d.k_weight;
     if (r.p < 1.0) {
-        // the k-th token's bucket holds some of its weight, at most all of it
-        const double least = r.p * static_cast<double>(s_decision->k_weight);
-        const double most = r.p * static_cast<double>(*s_upper);
+        // of the k-th token's bucket some of the weight counts, at most all of it
+        const uint64_t least = top_p_end(r, d.k_weight);
+        const uint64_t most = top_p_end(r, has_k ? s_found->upper : all_weights);
         uint64_t w = weights_before;
-        int low = -1, high = -1;
-        uint64_t low_weight = 0;
+        if ((w < most || b0 == 0) && w + weights >= least) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const bool first = b0 + i == 0;
-            const double before = static_cast<double>(w);
-            const double after = static_cast<double>(w + weight[i]);
-            const bool is_low = after >= least && (first || before < least);
-            low = is_low ? b0 + i : low;
-            low_weight = is_low ? w : low_weight;
-            high = after >= most && (first || before < most) ? b0 + i : high;
-            w += weight[i];
+            for (int i = 0; i < kPer; ++i) {
+                const uint64_t after = w + weight[i];
+                const bool first = b0 + i == 0;
+                if (after >= least && (first || w < least)) {
+                    s_found->low = b0 + i;
+                    s_found->low_weight = w;
+                }
+                if (after >= most && (first || w < most)) {
+                    s_found->high = b0 + i;
+                }
+                w = after;
+            }
         }
         __syncthreads();
-        if (low >= 0) {
-            s_decision->low = low;
-            s_decision->low_weight = low_weight;
-        }
-        if (high >= 0) {
-            s_decision->high = high;
-        }
-        __syncthreads();
+        d.low = s_found->low;
+        d.high = s_found->high;
+        d.low_weight = s_found->low_weight;
     }
-    uint32_t listed = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int b = b0 + i;
-        listed += (b >= s_decision->low && b <= s_decision->high) || b == s_decision->k_bucket ? count[i] : 0;
-    }
-    const uint32_t all_listed = static_cast<uint32_t>(block_sum(listed, s_part));
-    Decision d = *s_decision;
-    d.listed = static_cast<int32_t>(all_listed);
     return d;
 }
 
@@ -602,13 +705,13 @@ __device__ __forceinline__ bool listed_bucket(const Decision& d, int b) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int chunks, int per) {
-    __shared__ uint64_t s_part[kWaves];
-    __shared__ uint64_t s_list[kList];
+__global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int chunks, int per, int max_blocks) {
+    __shared__ uint64_t s_part[2 * kWaves];
+    __shared__ uint64_t s_list[kBuckets];  // [kBuckets] weights of the buckets, then [kList]
+    __shared__ uint32_t s_counts[kBuckets];
     __shared__ uint64_t s_sums[kWaves * kAhead];
     __shared__ double s_powers[kUnits];
-    __shared__ Decision s_decision;
-    __shared__ uint64_t s_upper;
+    __shared__ Found s_found;
     __shared__ uint32_t s_listed, s_at;
     const int64_t row = blockIdx.y;
     Row r = row_of(a, row);
@@ -616,14 +719,24 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
     if (r.greedy && blockIdx.x != 0) {
         return;
     }
-    const uint64_t best = row_best(s, static_cast<int>(gridDim.x), s_part);
+    // everything that does not wait for the decision is requested first
+    const auto* const logits = row_logits<T>(a, row);
+    const int begin = static_cast<int>(blockIdx.x) * per;
+    const int end = chunks_end(chunks, per);
+    const Round<T> round = load_round<T>(logits, a.vocab, begin, end);
+    const uint64_t mine = load_best(s, max_blocks);
+    Buckets buckets;
+    if (!r.greedy && decides(r)) {
+        buckets = load_buckets(r, s);
+    }
+    const uint64_t best = block_max(mine, s_part);
     r.top = order_logit(best);
     Decision d{};
     d.low = kBuckets;
     d.high = kBuckets - 1;
     d.k_bucket = kBuckets;
     if (!r.greedy && decides(r)) {
-        d = decide(r, s, s_part, &s_decision, &s_upper);
+        d = decide(r, buckets, s_list, s_counts, s_part, &s_found);
     }
     d.best = best;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -637,32 +750,32 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
     }
     load_powers(s_powers);
     __syncthreads();
-    const bool keep_list = d.listed <= kList;
     const int deepest = d.low > kDepth ? kDepth : max(max(d.low, d.high), d.k_bucket < kBuckets ? d.k_bucket : 0) + 1;
     const float least = least_logit(r, deepest);
     int in_round = 0;
-    const int begin = static_cast<int>(blockIdx.x) * per;
-    const int end = chunks_end(chunks, per);
-    for_chunks<T>(row_logits<T>(a, row), a.vocab, begin, end, [&](int c, int64_t id, const float(&x)[8]) {
+    for_chunks<T>(logits, a.vocab, begin, end, round, [&](int c, int64_t id, const float(&x)[8]) {
         uint64_t sum = 0;
-        for (uint32_t mask = passing(x, least); mask != 0; mask &= mask - 1) {
-            const int i = __builtin_ctz(mask);
-            const float v = pick(x, i);
+        for_passing(x, least, [&](int i, float v) __attribute__((always_inline)) {
             const double depth = depth_of(r, v);
             if (depth < kDepth) {
                 const int b = bucket_of(depth);
                 if (b < d.low) {
                     const uint64_t w = weight_of(depth, s_powers);
                     sum += w >= r.least ? w : 0;
-                } else if (keep_list && listed_bucket(d, b)) {
-                    s_list[atomicAdd(&s_listed, 1u) % kList] = order_word(v, id + i);
+                } else if (listed_bucket(d, b)) {
+                    const uint32_t at = atomicAdd(&s_listed, 1u);
+                    if (at < kList) {
+                        s_list[at] = order_word(v, id + i);
+                    }
                 }
             }
-        }
+        });
         // the waves' sums of a round of chunks meet at its end
+        if (__any(sum != 0)) {
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            sum += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(sum), o, 64));
+            for (int o = 32; o >= 1; o >>= 1) {
+                sum += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(sum), o, 64));
+            }
         }
         if ((threadIdx.x & 63) == 0) {
             s_sums[in_round * kWaves + (threadIdx.x >> 6)] = sum;
@@ -682,23 +795,24 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
         }
     });
     __syncthreads();
+    // (tokens past the list are counted: the last launch does without it then)
     if (threadIdx.x == 0 && s_listed != 0) {
         s_at = atomicAdd(s.listed, s_listed);
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < s_listed; i += kThreads) {
-        s.list[(s_at + i) % kList] = s_list[i];
+    for (uint32_t i = threadIdx.x; i < s_listed && i < kList && s_at + i < kList; i += kThreads) {
+        s.list[s_at + i] = s_list[i];
     }
 }
 
 // ------------------------------------------------------------- the last launch
 // Where more tokens than the list holds share the deciding buckets (flat rows):
-// the order word of the first token, in order, up to which count (k > 0) or weight
-// over buckets [low, high] reaches the target, digit by digit over the whole row;
+// the order word of the first token, in order, up to which the count (k > 0) or the
+// weight over buckets [low, high] reaches the target, digit by digit over the whole row;
 // 0: it is never reached.
 template <typename T>
 __device__ __forceinline__ uint64_t select_in_row(const SampleArgs& a, const Row& r, const typename Raw<T>::type* logits,
-                                               int low, int high, uint64_t before, int k, double target,
+                                               int low, int high, uint64_t before, int k, uint64_t target,
                                                unsigned long long* s_bins, uint64_t* s_part, const double* s_powers) {
     static_assert(kThreads == 256, "a thread a digit");
     __shared__ uint64_t s_prefix, s_before;
@@ -734,9 +848,7 @@ __device__ __forceinline__ uint64_t select_in_row(const SampleArgs& a, const Row
         const uint64_t mine = digit >= 0 ? s_bins[digit] : 0;
         uint64_t total;
         const uint64_t until = before + block_before<uint64_t>(mine, s_part, total);
-        const bool short_of = k > 0 ? until < static_cast<uint64_t>(k) : static_cast<double>(until) < target;
-        const bool reaches = k > 0 ? until + mine >= static_cast<uint64_t>(k) : static_cast<double>(until + mine) >= target;
-        if (mine != 0 && short_of && reaches) {
+        if (until < target && until + mine >= target) {
             s_prefix = prefix << bits | static_cast<uint64_t>(digit);
             s_before = until;
             s_found = 1;
@@ -768,6 +880,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     const RowSpace s = row_space(a.workspace, row, chunks);
     const Decision d = *s.decision;
     const float u = a.random[row];
+    const uint64_t listed = s.list[tid];  // (of no use where the list is shorter)
     r.top = order_logit(d.best);
     if (r.greedy || r.top == -__builtin_huge_valf()) {
         if (tid == 0) {
@@ -780,7 +893,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
         return;
     }
     const auto* const logits = row_logits<T>(a, row);
-    const int n = d.listed;
+    const int n = static_cast<int>(*s.listed);
     uint64_t last = 0;  // order word of the last kept token
     load_powers(s_powers);
     for (int c = tid; c < chunks; c += kThreads) {
@@ -791,7 +904,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     }
     if (n > 0 && n <= kThreads) {
         // a token a thread: what comes before it, by comparing it with every other
-        const uint64_t word = tid < n ? s.list[tid] : 0;
+        const uint64_t word = tid < n ? listed : 0;
         __syncthreads();
         const double depth = tid < n ? depth_of(r, order_logit(word)) : 0.0;
         const uint64_t weight = tid < n ? weight_of(depth, s_powers) : 0;
@@ -822,7 +935,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
         last = s_last;
         if (r.p < 1.0) {
             // the last token with less than the target before it: the smallest word
-            const bool under = in_p && static_cast<double>(before) < r.p * static_cast<double>(k_weight);
+            const bool under = in_p && before < top_p_end(r, k_weight);
             last = max_u64(last, ~block_max(under ? ~word : 0, s_part));
         }
     } else if (n > 0 && n <= kList) {
@@ -886,14 +999,14 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
         __syncthreads();
         last = s_last;
         if (r.p < 1.0) {
-            const double target = r.p * static_cast<double>(k_weight);
+            const uint64_t target = top_p_end(r, k_weight);
             uint64_t all;
             uint64_t before = d.low_weight + block_before<uint64_t>(p_mine, s_part, all);
             uint64_t mine = ~uint64_t{0};
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
                 if (in_p[j]) {
-                    mine = static_cast<double>(before) < target ? s_list[kMine * tid + j] : mine;
+                    mine = before < target ? s_list[kMine * tid + j] : mine;
                     before += weight[j];
                 }
             }
@@ -903,8 +1016,8 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
         __syncthreads();
         uint64_t k_weight = d.k_weight;
         if (d.k_bucket < kBuckets) {
-            last = select_in_row<T>(a, r, logits, d.k_bucket, d.k_bucket, static_cast<uint64_t>(d.k_count), r.k, 0.0, s_bins,
-                                    s_part, s_powers);
+            last = select_in_row<T>(a, r, logits, d.k_bucket, d.k_bucket, static_cast<uint64_t>(d.k_count), r.k,
+                                    static_cast<uint64_t>(r.k), s_bins, s_part, s_powers);
             uint64_t mine = 0;
             for_chunks<T>(logits, a.vocab, 0, chunks, [&](int, int64_t id, const float(&x)[8]) {
                 for (int i = 0; i < 8; ++i) {
@@ -918,7 +1031,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
         }
         if (r.p < 1.0) {
             last = max_u64(last, select_in_row<T>(a, r, logits, d.low, d.high, d.low_weight, 0,
-                                                  r.p * static_cast<double>(k_weight), s_bins, s_part, s_powers));
+                                                  top_p_end(r, k_weight), s_bins, s_part, s_powers));
         }
     }
     // the first token stays, whatever the settings
@@ -991,18 +1104,26 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
     const int chunks = static_cast<int>((a.vocab + kChunk - 1) / kChunk);
-    // about five blocks a CU; with few rows a chunk a block
-    const int64_t per = (chunks * a.rows + kSampleBlocks - 1) / kSampleBlocks;
-    const int blocks = static_cast<int>((chunks + per - 1) / per);
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.rows));
-    hipLaunchKernelGGL(sample_max_kernel<T>, grid, dim3(kThreads), 0, stream, a, chunks, static_cast<int>(per));
+    // with few rows a chunk a block (the large blocks: four), at most about the blocks
+    // that the chip holds at a time
+    const auto share = [&](int64_t most, int64_t least) {
+        const int64_t per = (chunks * a.rows + most - 1) / most;
+        return static_cast<int>(per > least ? per : least);
+    };
+    const auto grid = [&](int per) {
+        return dim3(static_cast<unsigned>((chunks + per - 1) / per), static_cast<unsigned>(a.rows));
+    };
+    const int per = share(kBlocks, 1);
+    const int large = share(kLargeBlocks, kLarge / kThreads);
+    const int blocks = static_cast<int>(grid(per).x);
+    hipLaunchKernelGGL(sample_max_kernel<T>, grid(per), dim3(kThreads), 0, stream, a, chunks, per);
     hipError_t status = hipGetLastError();
     if (status == hipSuccess && (a.top_k != nullptr || a.top_p != nullptr)) {
-        hipLaunchKernelGGL(sample_buckets_kernel<T>, grid, dim3(kThreads), 0, stream, a, chunks, static_cast<int>(per));
+        hipLaunchKernelGGL(sample_buckets_kernel<T>, grid(large), dim3(kLarge), 0, stream, a, chunks, large, blocks);
         status = hipGetLastError();
     }
     if (status == hipSuccess) {
-        hipLaunchKernelGGL(sample_sums_kernel<T>, grid, dim3(kThreads), 0, stream, a, chunks, static_cast<int>(per));
+        hipLaunchKernelGGL(sample_sums_kernel<T>, grid(per), dim3(kThreads), 0, stream, a, chunks, per, blocks);
         status = hipGetLastError();
     }
     if (status == hipSuccess) {
