@@ -321,7 +321,7 @@ KUDACUDA_API int kudacuda_rope_paged_append(
 
 /* Causal attention of new tokens over a paged cache.  Sequence i's new tokens are
  * rows query_starts[i] .. query_starts[i + 1] of query (int32 [sequences + 1],
- * ascending); it has kv_lens[i] cached tokens (int32), the new ones the last of
+ * ascending; output must not overlap query); it has kv_lens[i] cached tokens (int32), the new ones the last of
  * them, token j in page page_table[i * table_stride + j / page_size] (int32).  New
  * token t sees the keys up to its own, kv_lens[i] - q_len + t; a row that sees none
  * is zero.  Rows of no sequence are left as they were.  A sequence whose kv_len is
@@ -356,8 +356,10 @@ KUDACUDA_API int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, in
  * (kudacuda_amd/paged_cache.py).  Destinations must differ from each other and
  * from the sources of other pairs; other lists are refused.  Contract: page ids in
  * [0, num_pages), everything in whole 16-byte pieces on 16-byte boundaries,
- * page_stride and (pools > 1) pool_stride >= page_bytes.  A captured call keeps
- * its pairs. */
+ * page_stride and (pools > 1) pool_stride >= page_bytes, and either whole pools
+ * one after the other (pool_stride >= num_pages * page_stride) or a page's pools
+ * side by side (page_stride >= pools * pool_stride).  A captured call keeps its
+ * pairs. */
 KUDACUDA_API int kudacuda_copy_pages(void* handle, uint64_t pool, uint64_t pairs, int64_t count, int64_t pools,
                                      int64_t num_pages, int64_t page_bytes, int64_t page_stride, int64_t pool_stride,
                                      uint64_t stream);

@@ -527,12 +527,15 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
     } else {
         const int run_end = (tid + 1) * per_thread < sequences ? (tid + 1) * per_thread : sequences;
         int longest = 1;
+        bool descending = false;  // (such starts name no rows: their lengths need not fit the line)
         for (int i = tid * per_thread; i < run_end; ++i) {
             own = sequence(a, i);
+            descending |= a.starts[i + 1] < a.starts[i];
             const Line line = line_of(a, own, few_rows, splits);
             mine += length_of(a, line);
             longest = line.tiles > 0 && line.rounds > longest ? line.rounds : longest;
         }
+        longest = descending ? 0x7fffffff : longest;
         int sum = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -548,6 +551,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
         __syncthreads();
         total = __builtin_amdgcn_readfirstlane(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
         most = __builtin_amdgcn_readfirstlane(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
+        if (most == 0x7fffffff) {
+            return;
+        }
         mine_before = sum - mine;
         for (int w = 0; w < (tid >> 6); ++w) {
             mine_before += s_part[w];
@@ -1088,7 +1094,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_merge_kernel(PagedAt
     if (live) {
         const float2* const ml = reinterpret_cast<const float2*>(split_stats(a, D, splits)) + unit * splits;
         const float* const src = a.partials + unit * splits * D + d0;
-        const int made = split_counts(a, D, splits)[unit];
+        const int told = split_counts(a, D, splits)[unit];
+        const int made = told < 0 ? 0 : (told < splits ? told : splits);
         for (int s0 = group; s0 < made; s0 += kAhead * GROUPS) {
             float2 w[kAhead];
             float4 x[kAhead], y[kAhead];
@@ -1226,7 +1233,7 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     const int64_t rows = longest * group;
     const auto cap = [](int64_t v, int64_t most) { return v < 1 ? int64_t{1} : (v < most ? v : most); };
     int64_t few_splits = 0;
-    if (rows <= kFewRows || tokens != sequences * max_query_len) {
+    if (rows <= kFewRows || tokens != sequences * longest) {
         // two blocks a CU; a stretch of at least one round of keys.  The longest sequence
         // may be cut into twice as many stretches as it were in a batch of such ones.
         const int64_t tiles = sequences * kv_heads * (((rows < kFewRows ? rows : kFewRows) + 15) / 16);

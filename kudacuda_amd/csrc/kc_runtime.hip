@@ -1708,10 +1708,12 @@ int kudacuda_rope_paged_append(void* raw, uint64_t query, uint64_t key, uint64_t
 int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences, int64_t max_query_len,
                                                  int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
                                                  int64_t head_dim) {
-    if (tokens < 1 || sequences < 1 || max_query_len < 1 || max_kv_len < 1 || query_heads < 1 || kv_heads < 1 ||
-        head_dim < 1 || query_heads % kv_heads != 0) {
-        return 0;
+    if (!within(query_heads, 1, 1024) || !within(kv_heads, 1, query_heads) || query_heads % kv_heads != 0 ||
+        !within(tokens, 1, (int64_t{1} << 30) / query_heads) || !within(sequences, 1, 65536) || !within(head_dim, 1, 128) ||
+        max_query_len < 1 || max_kv_len < 1) {
+        return 0;  // no call that would be taken
     }
+    max_kv_len = max_kv_len < (int64_t{1} << 30) ? max_kv_len : int64_t{1} << 30;
     return kc::paged_attention_plan(tokens, sequences, max_query_len, max_kv_len, max_kv_len, query_heads, kv_heads, head_dim,
                                     INT64_MAX)
         .workspace_bytes;
@@ -1768,6 +1770,10 @@ int kudacuda_paged_attention(void* raw, uint64_t query, uint64_t key_pages, uint
     }
     if (workspace_bytes < 0) {
         refuse(h, symbol, "workspace_bytes>=0");
+        return 1;
+    }
+    if (output == query) {
+        refuse(h, symbol, "an output apart from the query");
         return 1;
     }
     if (!(scale > 0.0f) || !std::isfinite(scale)) {
@@ -1831,6 +1837,10 @@ int kudacuda_copy_pages(void* raw, uint64_t pool, uint64_t pairs, int64_t count,
         refuse(h, symbol, "whole 16-byte pieces on 16-byte boundaries and strides of at least page_bytes");
         return 1;
     }
+    if (pools > 1 && num_pages > 1 && page_stride / pools < pool_stride && pool_stride / num_pages < page_stride) {
+        refuse(h, symbol, "pools that do not lie in each other's pages (page_stride >= pools * pool_stride or the reverse)");
+        return 1;
+    }
     const int32_t* const list = ptr<const int32_t>(pairs);
     if (!pairs_ok(h, symbol, list, count, num_pages)) {
         return 1;
@@ -1847,7 +1857,7 @@ int kudacuda_copy_pages(void* raw, uint64_t pool, uint64_t pairs, int64_t count,
 }
 
 int64_t kudacuda_sample_workspace_bytes(int64_t rows, int64_t vocab) {
-    return rows < 1 || vocab < 1 ? 0 : kc::sample_workspace_bytes(rows, vocab);
+    return within(rows, 1, 65535) && within(vocab, 1, kc::kSampleMaxVocab) ? kc::sample_workspace_bytes(rows, vocab) : 0;
 }
 
 int kudacuda_sample_tokens(void* raw, uint64_t logits, uint64_t random, uint64_t temperature, uint64_t top_k,

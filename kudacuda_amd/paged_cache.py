@@ -284,10 +284,13 @@ class PagedKvCache:
         nbytes = self.native.lib.kudacuda_paged_attention_workspace_bytes(
             batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads, self.head_dim)
         stream = self._stream()
-        # a workspace a stream: calls on one stream follow one another
-        workspace = self._workspaces.get(stream)
+        # a workspace a stream: calls on one stream follow one another; a captured call
+        # gets its own, from its graph's memory
+        workspace = None if self.torch.cuda.is_current_stream_capturing() else self._workspaces.get(stream)
         if nbytes > 0 and (workspace is None or workspace.numel() < nbytes):
-            workspace = self._workspaces[stream] = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+            workspace = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+            if not self.torch.cuda.is_current_stream_capturing():
+                self._workspaces[stream] = workspace
         self.native.call("kudacuda_paged_attention", query.data_ptr(), keys.data_ptr(), values.data_ptr(),
                          batch.page_table.data_ptr(), batch.query_starts.data_ptr(), batch.kv_lens.data_ptr(),
                          out.data_ptr(), workspace.data_ptr() if nbytes > 0 else 0, nbytes, self._dtype(),

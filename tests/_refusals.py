@@ -4,14 +4,15 @@ from __future__ import annotations
 
 import numpy as np
 
-P = 1 << 20  # a 16-byte aligned address that is never read: every call below is refused
+P = 1 << 20  # 16-byte aligned addresses that are never read: every call below is refused
+Q = P + (1 << 19)
 ROPE = dict(input=P, inv_freq=P, positions=P, output=P, dtype=1, tokens=3, heads=2, head_dim=128, rotary_dim=128,
             interleaved=0, input_stride=256, output_stride=256, amplitude=1.0, stream=0)
 APPEND = dict(query=P, key=P, value=P, inv_freq=P, positions=P, slots=P, query_output=P, key_pages=P, value_pages=P,
               dtype=1, tokens=3, query_heads=4, kv_heads=2, head_dim=128, rotary_dim=64, interleaved=1,
               query_stride=512, key_stride=256, value_stride=256, output_stride=512, num_pages=4, page_size=16,
               page_stride=4096, head_stride=2048, token_stride=128, amplitude=1.0, stream=0)
-ATTEND = dict(query=P, key_pages=P, value_pages=P, page_table=P, query_starts=P, kv_lens=P, output=P, workspace=P,
+ATTEND = dict(query=P, key_pages=P, value_pages=P, page_table=P, query_starts=P, kv_lens=P, output=Q, workspace=P,
               workspace_bytes=1 << 20, dtype=2, tokens=3, sequences=2, max_query_len=2, max_kv_len=50, query_heads=4,
               kv_heads=2, head_dim=64, query_stride=256, output_stride=256, num_pages=4, page_size=16, table_stride=4,
               page_stride=2048, head_stride=1024, token_stride=64, scale=0.125, stream=0)
@@ -45,11 +46,13 @@ CHANGES = {
         (dict(max_kv_len=0), "max_kv_len"), (dict(query_stride=252), "strides"), (dict(token_stride=68), "strides"),
         (dict(head_stride=0), "strides"), (dict(query=P + 8), "16-byte"), (dict(workspace=P + 4), "16-byte"),
         (dict(kv_lens=P + 2), "16-byte"), (dict(workspace_bytes=-1), "workspace_bytes"), (dict(scale=0.0), "scale"),
+        (dict(output=P), "apart"),
         (dict(scale=float("inf")), "scale"), (dict(scale=-1.0), "scale")],
     "kudacuda_copy_pages": [
         (dict(pool=0), "non-null"), (dict(count=1), "non-null"), (dict(count=-1), "count"), (dict(pools=0), "pools"),
         (dict(num_pages=0), "num_pages"), (dict(page_bytes=0), "page_bytes"), (dict(page_bytes=24), "16-byte"),
         (dict(pool=P + 8), "16-byte"), (dict(page_stride=240), "page_bytes"), (dict(pool_stride=128), "page_bytes"),
+        (dict(pool_stride=256), "each other's"), (dict(pool_stride=1024), "each other's"),
         (dict(pairs=[(0, 8)]), "page ids"), (dict(pairs=[(-1, 2)]), "page ids"),
         (dict(pairs=[(0, 2), (1, 2)]), "differ"), (dict(pairs=[(0, 2), (2, 2)]), "differ"),
         (dict(pairs=[(0, 2), (2, 3)]), "source"), (dict(pairs=[(2, 3), (0, 2)]), "source"),

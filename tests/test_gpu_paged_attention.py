@@ -225,3 +225,55 @@ def test_results_do_not_change_from_call_to_call(torch_gpu, native):
     first = batch.call(native, d).clone()
     for _ in range(5):
         assert torch.equal(batch.call(native, d), first)
+
+
+def test_starts_that_descend_stay_inside(torch_gpu, native):
+    """Starts that go back and forth name no batch: whatever the rows become, the sequences' pages and the workspace
+    hold what they held, and the next call is right."""
+
+    for new, kv in (([1] * 6, [400, 30, 70, 2000, 5, 90]), ([70, 1, 40, 3], [300, 20, 100, 50])):
+        batch = Paged(18, new, kv, dim=128)
+        d = batch.device()
+        nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(batch.tokens, len(new), max(new), max(kv), 4, 2, 128)
+        workspace = torch.full((nbytes + 4096,), 0x7f, dtype=torch.uint8, device="cuda:0")
+        pools = d["k"].clone(), d["v"].clone()
+        good = d["starts"].clone()
+        d["starts"].copy_(torch.tensor([0, batch.tokens] * 4, dtype=torch.int32)[:len(new) + 1])
+        batch.call(native, d, workspace=workspace, nbytes=nbytes)
+        torch.cuda.synchronize()
+        assert (workspace[nbytes:] == 0x7f).all()
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(pools, (d["k"], d["v"])))
+        d["starts"].copy_(good)
+        _check(batch, batch.call(native, d, workspace=workspace, nbytes=nbytes))
+
+
+def test_cache_calls_captured_twice_do_not_share_a_workspace(torch_gpu, native):
+    """Two graphs with attention over many splits, replayed at the same time on two streams."""
+
+    from kudacuda_amd.paged_cache import PagedKvCache
+
+    cache = PagedKvCache(native, torch, layers=1, kv_heads=2, head_dim=128, num_pages=400, page_size=16)
+    cache.pool.normal_()
+    batches = []
+    for n in (3000, 2500):
+        s = cache.create()
+        cache.extend([s], [n])
+        batches.append(cache.extend([s], [1]))
+    q = torch.randn((2, 1, 16, 128), device="cuda:0").bfloat16()
+    want = [cache.attend(0, b, x).clone() for b, x in zip(batches, q)]
+    outs = [torch.zeros_like(w) for w in want]
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for b, x, out, s in zip(batches, q, outs, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            cache.attend(0, b, x, out=out)
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        for s in streams:
+            s.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert torch.equal(cache.attend(0, batches[0], q[0]), want[0])
+        torch.cuda.synchronize()

@@ -76,7 +76,7 @@ def test_the_list_may_change_as_soon_as_the_call_returns(torch_gpu, native):
 def test_refusals_leave_a_reason(torch_gpu, native, name):
     buffer = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda:0")
     lib = native.lib
-    stand_in = range(_refusals.P, _refusals.P + 16)
+    stand_in = range(_refusals.P, _refusals.Q + 16)
     for call, args, reason in _refusals.refusals():
         if call == name:
             args = [buffer.data_ptr() + a - _refusals.P if a in stand_in else a for a in args]
