@@ -41,11 +41,13 @@ constexpr int kUnits = 64;            // buckets of a factor of two
 constexpr int kDepth = 43 * kUnits;   // buckets of the weights' range
 constexpr int kBuckets = 11 * kThreads;
 constexpr int kPer = kBuckets / kThreads;
+constexpr int kCoarse = 64;           // buckets that are summed together, a wave's
+static_assert(kBuckets % kCoarse == 0 && kBuckets / kCoarse <= 64, "the sums fit a wave");
 constexpr int kList = 2048;           // most tokens that are ordered in LDS
 constexpr int kWeightBits = 42;
 // Blocks of the first and third launch, and large blocks of the second: more rows than
-// fill these take more chunks a block (128 rows of mixed settings: 2048 and 512 98 us,
-// 1280 and 512 103; 32 rows with top-p: 256 large blocks 55 us, 512 60, 1024 65).
+// fill these take more chunks a block (128 rows of mixed settings: 2048 and 256 87 us,
+// 2048 and 512 90, 1280 and 256 88; 32 rows with top-p: 256 large blocks 50 us, 512 61).
 constexpr int64_t kBlocks = 2048;
 constexpr int64_t kLargeBlocks = 256;
 constexpr int kMaxChunks = static_cast<int>(kSampleMaxVocab / kChunk);
@@ -95,10 +97,12 @@ struct RowSpace {
     Decision* decision;
     uint32_t* listed;
     uint32_t* counts;    // [kBuckets]
+    uint64_t* coarse_weights;  // [64] of kCoarse buckets each
+    uint32_t* coarse_counts;   // [64]
     float* largest;      // [chunks * kGroups] of 128 ids each
 };
 __host__ __device__ inline int64_t row_bytes(int64_t chunks) {
-    return kBuckets * 12 + kList * 8 + chunks * (16 + kGroups * 4) + 64 + 16;
+    return kBuckets * 12 + kList * 8 + chunks * (16 + kGroups * 4) + 64 + 16 + 64 * 12;
 }
 __device__ __forceinline__ RowSpace row_space(uint8_t* base, int64_t row, int chunks) {
     uint8_t* p = base + row * row_bytes(chunks);
@@ -115,6 +119,10 @@ __device__ __forceinline__ RowSpace row_space(uint8_t* base, int64_t row, int ch
     p += 64;
     s.listed = reinterpret_cast<uint32_t*>(p);
     p += 16;
+    s.coarse_weights = reinterpret_cast<uint64_t*>(p);
+    p += 64 * 8;
+    s.coarse_counts = reinterpret_cast<uint32_t*>(p);
+    p += 64 * 4;
     s.counts = reinterpret_cast<uint32_t*>(p);
     p += kBuckets * 4;
     s.largest = reinterpret_cast<float*>(p);
@@ -161,7 +169,7 @@ __device__ __forceinline__ Piece<T> load_piece(const typename Raw<T>::type* row,
     }
     return v;
 }
-// As fp32; NaN counts as -inf, -0 as 0.
+// As fp32, and then: NaN counts as -inf, -0 as 0.
 template <typename T>
 __device__ __forceinline__ void unpack(float (&x)[8], const Piece<T>& v) {
     typename Raw<T>::type raw[8];
@@ -169,8 +177,12 @@ __device__ __forceinline__ void unpack(float (&x)[8], const Piece<T>& v) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         x[i] = T::load(raw[i]);
-        x[i] = x[i] == x[i] ? x[i] + 0.0f : -__builtin_huge_valf();
     }
+}
+__device__ __forceinline__ float settle(float x) { return x == x ? x + 0.0f : -__builtin_huge_valf(); }
+// Their largest (a NaN does not count).
+__device__ __forceinline__ float largest_of(const float (&x)[8]) {
+    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
 }
 template <typename T>
 __device__ __forceinline__ const typename Raw<T>::type* row_logits(const SampleArgs& a, int64_t row) {
@@ -234,6 +246,7 @@ __device__ __forceinline__ int64_t order_id(uint64_t word) { return static_cast<
 // A row's settings.
 struct Row {
     bool greedy;
+    bool plain;      // top and scale are finite
     float top;       // largest logit
     double scale;    // 64 log2(e) / T: buckets of a logit
     int k;           // 0: off
@@ -244,6 +257,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
     Row r;
     const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
     r.greedy = !(t > 0.0f);
+    r.plain = false;
     r.top = 0.0f;
     r.scale = r.greedy ? 0.0 : kUnits * 0x1.71547652b82fep+0 / static_cast<double>(t);
     const int32_t k = a.top_k != nullptr ? a.top_k[row] : 0;
@@ -260,6 +274,11 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
     return r;
 }
 __device__ __forceinline__ bool decides(const Row& r) { return r.k > 0 || r.p < 1.0; }
+
+__device__ __forceinline__ void set_top(Row& r, uint64_t best) {
+    r.top = order_logit(best);
+    r.plain = fabsf(r.top) < __builtin_huge_valf() && r.scale < static_cast<double>(__builtin_huge_val());
+}
 
 // How far a logit lies below the largest, in buckets; kDepth: it weighs nothing.
 __device__ __forceinline__ double depth_of(const Row& r, float x) {
@@ -301,35 +320,46 @@ __device__ __forceinline__ float pick(const float (&x)[8], int i) {
     return (i & 4) != 0 ? f : e;
 }
 
-// f(i, x[i]) for the logits that `least` lets pass: one by one where few do, all eight
-// in line (f finds the others out) where some lane of the wave has more than three.
+// f(i, logit, depth) for the logits that `least` lets pass (f tells the ones that lie
+// too deep): one by one where they are few, all eight in line where half of the
+// wave's lanes have one.
 template <typename F>
-__device__ __forceinline__ void for_passing(const float (&x)[8], float least, F f) {
-    uint32_t mask = passing(x, least);
-    if (__any(__builtin_popcount(mask) > 3)) {
+__device__ __forceinline__ void for_passing(const Row& r, const float (&x)[8], float least, F f) {
+    const uint64_t lanes = __ballot(largest_of(x) >= least);
+    if (lanes == 0) {
+        return;
+    }
+    if (r.plain && __builtin_popcountll(lanes) >= 32) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            f(i, x[i]);
+            // (of a NaN and of -inf no number below any limit)
+            f(i, x[i], (static_cast<double>(r.top) - static_cast<double>(x[i])) * r.scale);
         }
         return;
     }
-    for (; mask != 0; mask &= mask - 1) {
+    float settled[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        settled[i] = settle(x[i]);
+    }
+    for (uint32_t mask = passing(settled, least); mask != 0; mask &= mask - 1) {
         const int i = __builtin_ctz(mask);
-        f(i, pick(x, i));
+        const float v = pick(settled, i);
+        f(i, v, depth_of(r, v));
     }
 }
 
 // 2^(42 - depth / 64) rounded to a whole number, 0 <= depth < kDepth: a table's power
-// for the whole buckets of the fraction, the Taylor polynomial of degree 5 of e^z for
-// the rest (|z| <= ln 2 / 64: off by 2^-49), and the addition of 2^52 that rounds.
+// for the whole buckets of the fraction, the Taylor polynomial of degree 5 of
+// 2^(-z / 64) for the rest (z < 1: off by 2^-49), and the addition of 2^52 that rounds.
 __device__ __forceinline__ uint64_t weight_of(double depth, const double* powers) {
     const int whole = static_cast<int>(depth);
-    const double z = (whole - depth) * (0x1.62e42fefa39efp-1 / kUnits);
-    double e = 1.0 / 120.0;
-    e = fma(e, z, 1.0 / 24.0);
-    e = fma(e, z, 1.0 / 6.0);
-    e = fma(e, z, 0.5);
-    e = fma(e, z, 1.0);
+    const double z = depth - whole;
+    double e = -0x1.5d87fe78a6731p-40;  // (-ln 2 / 64)^n / n!
+    e = fma(e, z, 0x1.3b2ab6fba4e77p-31);
+    e = fma(e, z, -0x1.c6b08d704a0c0p-23);
+    e = fma(e, z, 0x1.ebfbdff82c58fp-15);
+    e = fma(e, z, -0x1.62e42fefa39efp-7);
     e = fma(e, z, 1.0);
     const double y = powers[whole % kUnits] * e;
     const int64_t shift = static_cast<int64_t>(kWeightBits - whole / kUnits) << 52;
@@ -437,33 +467,43 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int 
         s.weights[i] = 0;
         s.counts[i] = 0;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        *s.listed = 0;
+    if (blockIdx.x == 0 && threadIdx.x < 64) {
+        s.coarse_weights[threadIdx.x] = 0;
+        s.coarse_counts[threadIdx.x] = 0;
+        if (threadIdx.x == 0) {
+            *s.listed = 0;
+        }
     }
+    const auto* const logits = row_logits<T>(a, row);
+    const int begin = static_cast<int>(blockIdx.x) * per;
     float best = -__builtin_huge_valf();
-    int64_t best_id = -1;
-    for_chunks<T>(row_logits<T>(a, row), a.vocab, static_cast<int>(blockIdx.x) * per, chunks_end(chunks, per),
-                  [&](int c, int64_t id, const float(&x)[8]) {
-                      float most = x[0];
-                      int at = 0;
+    int chunk = begin;  // the first that holds the thread's largest
+    for_chunks<T>(logits, a.vocab, begin, chunks_end(chunks, per), [&](int c, int64_t, const float(&x)[8]) {
+        float most = largest_of(x);
+        chunk = most > best ? c : chunk;
+        best = fmaxf(best, most);
+        most = fmaxf(most, row_ror<8>(most));
+        most = fmaxf(most, row_ror<4>(most));
+        most = fmaxf(most, row_ror<2>(most));
+        most = fmaxf(most, row_ror<1>(most));
+        if (threadIdx.x % 16 == 0) {
+            s.largest[c * kGroups + threadIdx.x / 16] = settle(most);
+        }
+    });
+    // its place in the chunk's piece
+    const int64_t id = static_cast<int64_t>(chunk) * kChunk + threadIdx.x * 8;
+    uint64_t word = 0;
+    if (id < a.vocab) {
+        float x[8];
+        unpack<T>(x, load_piece<T>(logits, id, a.vocab));
+        int at = 0;
 #pragma unroll
-                      for (int i = 1; i < 8; ++i) {
-                          at = x[i] > most ? i : at;
-                          most = fmaxf(most, x[i]);
-                      }
-                      if (id < a.vocab && (best_id < 0 || most > best)) {
-                          best = most;
-                          best_id = id + at;
-                      }
-                      most = fmaxf(most, row_ror<8>(most));
-                      most = fmaxf(most, row_ror<4>(most));
-                      most = fmaxf(most, row_ror<2>(most));
-                      most = fmaxf(most, row_ror<1>(most));
-                      if (threadIdx.x % 16 == 0) {
-                          s.largest[c * kGroups + threadIdx.x / 16] = most;
-                      }
-                  });
-    const uint64_t word = block_max(best_id < 0 ? 0 : order_word(best, best_id), s_part);
+        for (int i = 7; i >= 0; --i) {
+            at = settle(x[i]) == best ? i : at;
+        }
+        word = order_word(settle(best), id + at);
+    }
+    word = block_max(word, s_part);
     if (threadIdx.x == 0) {
         s.best[blockIdx.x] = word;
     }
@@ -506,7 +546,7 @@ __global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, in
         s_counts[i] = 0;
     }
     load_powers(s_powers);
-    r.top = order_logit(block_max<kLarge / 64>(best, s_part));
+    set_top(r, block_max<kLarge / 64>(best, s_part));
     int limit = kDepth;
     if (bounded) {
         // k of the groups' largest logits are at least the k-th of them: the k-th token
@@ -553,8 +593,7 @@ __global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, in
     }
     const float least = least_logit(r, limit);
     for_chunks<T, kStride>(logits, a.vocab, begin, end, round, [&](int, int64_t, const float(&x)[8]) {
-        for_passing(x, least, [&](int, float v) __attribute__((always_inline)) {
-            const double d = depth_of(r, v);
+        for_passing(r, x, least, [&](int, float, double d) __attribute__((always_inline)) {
             if (d < limit) {
                 if (r.k > 0) {
                     atomicAdd(&s_counts[bucket_of(d)], 1u);
@@ -567,135 +606,100 @@ __global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, in
     });
     __syncthreads();
     for (int i = threadIdx.x; i < kBuckets; i += kLarge) {
-        if (s_counts[i] != 0) {
-            atomicAdd(&s.counts[i], s_counts[i]);
+        uint32_t count = s_counts[i];
+        uint64_t weight = s_weights[i];
+        if (!__any(count != 0 || weight != 0)) {
+            continue;
         }
-        if (s_weights[i] != 0) {
-            atomicAdd(reinterpret_cast<unsigned long long*>(&s.weights[i]), s_weights[i]);
+        if (count != 0) {
+            atomicAdd(&s.counts[i], count);
+        }
+        if (weight != 0) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.weights[i]), static_cast<unsigned long long>(weight));
+        }
+        // the wave's buckets together
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            count += __shfl_xor(count, o, 64);
+            weight += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(weight), o, 64));
+        }
+        if ((threadIdx.x & 63) == 0) {
+            atomicAdd(&s.coarse_counts[i / kCoarse], count);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.coarse_weights[i / kCoarse]),
+                      static_cast<unsigned long long>(weight));
         }
     }
 }
 
-// A thread's share of the row's buckets as they are loaded, every 256th.
-struct Buckets {
-    uint32_t count[kPer];
-    uint64_t weight[kPer];
-};
-__device__ __forceinline__ Buckets load_buckets(const Row& r, const RowSpace& s) {
-    Buckets b;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        b.count[i] = r.k > 0 ? s.counts[i * kThreads + threadIdx.x] : 0;
-        b.weight[i] = r.p < 1.0 ? s.weights[i * kThreads + threadIdx.x] : 0;
-    }
-    return b;
-}
-
-// The deciding buckets, from the row's counts and weights (all threads of a block).
-struct Found {
-    uint64_t k_weight, upper, low_weight;
-    int32_t k_bucket, k_count, low, high;
-};
-__device__ __forceinline__ Decision decide(const Row& r, const Buckets& loaded, uint64_t* s_weights, uint32_t* s_counts,
-                                           uint64_t* s_part, Found* s_found) {
-    const int b0 = static_cast<int>(threadIdx.x) * kPer;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        s_counts[i * kThreads + threadIdx.x] = loaded.count[i];
-        s_weights[i * kThreads + threadIdx.x] = loaded.weight[i];
-    }
-    __syncthreads();
-    uint32_t count[kPer];
-    uint64_t weight[kPer];
-    uint32_t counts = 0;
-    uint64_t weights = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        count[i] = s_counts[b0 + i];
-        weight[i] = s_weights[b0 + i];
-        counts += count[i];
-        weights += weight[i];
-    }
-    // both sums of the threads before this one
-    uint32_t counts_before = counts;
-    uint64_t weights_before = weights;
+// Sum over the wave's lanes up to this one.
+template <typename V>
+__device__ __forceinline__ V wave_until(V v) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t c = __shfl_up(counts_before, o, 64);
-        counts_before += static_cast<int>(threadIdx.x & 63) >= o ? c : 0;
-        if (r.p < 1.0) {
-            const uint64_t w = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(weights_before), o, 64));
-            weights_before += static_cast<int>(threadIdx.x & 63) >= o ? w : 0;
+        V left;
+        if constexpr (sizeof(V) == 8) {
+            left = static_cast<V>(__shfl_up(static_cast<unsigned long long>(v), o, 64));
+        } else {
+            left = __shfl_up(v, o, 64);
         }
+        v += static_cast<int>(threadIdx.x & 63) >= o ? left : 0;
     }
-    const int wave = static_cast<int>(threadIdx.x >> 6);
-    if ((threadIdx.x & 63) == 63) {
-        s_part[wave] = weights_before;
-        s_part[kWaves + wave] = counts_before;
-    }
-    __syncthreads();
-    counts_before -= counts;
-    weights_before -= weights;
-    uint32_t all_counts = 0;
-    uint64_t all_weights = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        const uint32_t c = static_cast<uint32_t>(s_part[kWaves + w]);
-        counts_before += w < wave ? c : 0;
-        weights_before += w < wave ? s_part[w] : 0;
-        all_counts += c;
-        all_weights += s_part[w];
-    }
-    // the bucket of the k-th token; top-k off or larger than the row: none
-    const uint32_t k = static_cast<uint32_t>(r.k);
-    const bool has_k = r.k > 0 && all_counts >= k;
-    if (has_k && counts_before < k && counts_before + counts >= k) {
-        uint32_t c = counts_before;
-        uint64_t w = weights_before;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (c < k && c + count[i] >= k) {
-                s_found->k_bucket = b0 + i;
-                s_found->k_weight = w;
-                s_found->k_count = static_cast<int32_t>(c);
-                s_found->upper = w + weight[i];
-            }
-            c += count[i];
-            w += weight[i];
-        }
-    }
-    __syncthreads();
+    return v;
+}
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) {
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
+    const uint32_t high = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
+    return static_cast<uint64_t>(high) << 32 | low;
+}
+__device__ __forceinline__ int first_lane(bool v) { return __builtin_ctzll(__ballot(v) | uint64_t{1} << 63); }
+
+// The deciding buckets, by every wave for itself: a lane holds the sums of kCoarse
+// buckets, then one of the buckets that the sums point to.
+__device__ __forceinline__ Decision decide(const Row& r, const RowSpace& s, uint32_t count, uint64_t weight) {
+    const int lane = static_cast<int>(threadIdx.x & 63);
     Decision d{};
-    d.k_bucket = has_k ? s_found->k_bucket : kBuckets;
-    d.k_weight = has_k ? s_found->k_weight : all_weights;
-    d.k_count = has_k ? s_found->k_count : static_cast<int32_t>(all_counts);
-    d.low = has_k ? d.k_bucket : kBuckets;
-    d.high = has_k ? d.k_bucket : kBuckets - 1;
+    const uint64_t weights = r.p < 1.0 ? wave_until(weight) : 0;
+    const uint64_t all_weights = from_lane(weights, 63);
+    // the bucket of the k-th token; top-k off or larger than the row: none
+    d.k_bucket = kBuckets;
+    d.k_weight = all_weights;
+    uint64_t upper = all_weights;  // the most that the first top_k tokens can weigh
+    const uint32_t k = static_cast<uint32_t>(r.k);
+    if (r.k > 0) {
+        const uint32_t counts = wave_until(count);
+        if (static_cast<uint32_t>(__builtin_amdgcn_readlane(counts, 63)) >= k) {
+            const int at = first_lane(counts >= k);
+            const uint32_t fine = s.counts[at * kCoarse + lane];
+            const uint64_t fine_weight = r.p < 1.0 ? s.weights[at * kCoarse + lane] : 0;
+            const uint32_t until = static_cast<uint32_t>(__builtin_amdgcn_readlane(counts - count, at)) + wave_until(fine);
+            const int of = first_lane(until >= k);
+            d.k_bucket = at * kCoarse + of;
+            d.k_count = __builtin_amdgcn_readlane(until - fine, of);
+            if (r.p < 1.0) {
+                const uint64_t w = from_lane(weights - weight, at) + wave_until(fine_weight);
+                upper = from_lane(w, of);
+                d.k_weight = from_lane(w - fine_weight, of);
+            }
+        }
+    }
+    d.low = d.k_bucket;
+    d.high = d.k_bucket < kBuckets ? d.k_bucket : kBuckets - 1;
     d.low_weight = d.k_weight;
     if (r.p < 1.0) {
         // of the k-th token's bucket some of the weight counts, at most all of it
+        const auto find = [&](uint64_t target, uint64_t& before) __attribute__((always_inline)) {
+            const int at = first_lane(weights >= target);
+            const uint64_t fine = s.weights[at * kCoarse + (at * kCoarse + lane < kBuckets ? lane : 0)];
+            const uint64_t until = from_lane(weights - weight, at) + wave_until(fine);
+            const int of = first_lane(until >= target);
+            before = from_lane(until - fine, of);
+            return at * kCoarse + of;
+        };
         const uint64_t least = top_p_end(r, d.k_weight);
-        const uint64_t most = top_p_end(r, has_k ? s_found->upper : all_weights);
-        uint64_t w = weights_before;
-        if ((w < most || b0 == 0) && w + weights >= least) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const uint64_t after = w + weight[i];
-                const bool first = b0 + i == 0;
-                if (after >= least && (first || w < least)) {
-                    s_found->low = b0 + i;
-                    s_found->low_weight = w;
-                }
-                if (after >= most && (first || w < most)) {
-                    s_found->high = b0 + i;
-                }
-                w = after;
-            }
-        }
-        __syncthreads();
-        d.low = s_found->low;
-        d.high = s_found->high;
-        d.low_weight = s_found->low_weight;
+        const uint64_t most = top_p_end(r, upper);
+        d.low = find(least, d.low_weight);
+        uint64_t unused;
+        d.high = least == most ? d.low : find(most, unused);
     }
     return d;
 }
@@ -706,12 +710,10 @@ __device__ __forceinline__ bool listed_bucket(const Decision& d, int b) {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int chunks, int per, int max_blocks) {
-    __shared__ uint64_t s_part[2 * kWaves];
-    __shared__ uint64_t s_list[kBuckets];  // [kBuckets] weights of the buckets, then [kList]
-    __shared__ uint32_t s_counts[kBuckets];
+    __shared__ uint64_t s_part[kWaves];
+    __shared__ uint64_t s_list[kList];
     __shared__ uint64_t s_sums[kWaves * kAhead];
     __shared__ double s_powers[kUnits];
-    __shared__ Found s_found;
     __shared__ uint32_t s_listed, s_at;
     const int64_t row = blockIdx.y;
     Row r = row_of(a, row);
@@ -725,18 +727,18 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
     const int end = chunks_end(chunks, per);
     const Round<T> round = load_round<T>(logits, a.vocab, begin, end);
     const uint64_t mine = load_best(s, max_blocks);
-    Buckets buckets;
-    if (!r.greedy && decides(r)) {
-        buckets = load_buckets(r, s);
-    }
+    const bool deciding = !r.greedy && decides(r);
+    const int lane = static_cast<int>(threadIdx.x & 63);
+    const uint32_t count = deciding ? s.coarse_counts[lane] : 0;
+    const uint64_t weight = deciding ? s.coarse_weights[lane] : 0;
     const uint64_t best = block_max(mine, s_part);
-    r.top = order_logit(best);
+    set_top(r, best);
     Decision d{};
     d.low = kBuckets;
     d.high = kBuckets - 1;
     d.k_bucket = kBuckets;
-    if (!r.greedy && decides(r)) {
-        d = decide(r, buckets, s_list, s_counts, s_part, &s_found);
+    if (deciding) {
+        d = decide(r, s, count, weight);
     }
     d.best = best;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -755,8 +757,7 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
     int in_round = 0;
     for_chunks<T>(logits, a.vocab, begin, end, round, [&](int c, int64_t id, const float(&x)[8]) {
         uint64_t sum = 0;
-        for_passing(x, least, [&](int i, float v) __attribute__((always_inline)) {
-            const double depth = depth_of(r, v);
+        for_passing(r, x, least, [&](int i, float v, double depth) __attribute__((always_inline)) {
             if (depth < kDepth) {
                 const int b = bucket_of(depth);
                 if (b < d.low) {
@@ -765,7 +766,7 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
                 } else if (listed_bucket(d, b)) {
                     const uint32_t at = atomicAdd(&s_listed, 1u);
                     if (at < kList) {
-                        s_list[at] = order_word(v, id + i);
+                        s_list[at] = order_word(settle(v), id + i);
                     }
                 }
             }
@@ -831,10 +832,11 @@ __device__ __forceinline__ uint64_t select_in_row(const SampleArgs& a, const Row
         for_chunks<T>(logits, a.vocab, 0, static_cast<int>((a.vocab + kChunk - 1) / kChunk),
                       [&](int, int64_t id, const float(&x)[8]) {
                           for (int i = 0; i < 8; ++i) {
-                              const double depth = depth_of(r, x[i]);
+                              const float v = settle(x[i]);
+                              const double depth = depth_of(r, v);
                               if (depth < kDepth) {
                                   const int b = bucket_of(depth);
-                                  const uint64_t word = order_word(x[i], id + i);
+                                  const uint64_t word = order_word(v, id + i);
                                   if (b >= low && b <= high && (word >> shift) >> bits == prefix) {
                                       atomicAdd(&s_bins[(word >> shift) & ((1u << bits) - 1)],
                                                 static_cast<unsigned long long>(k > 0 ? 1 : weight_of(depth, s_powers)));
@@ -881,7 +883,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     const Decision d = *s.decision;
     const float u = a.random[row];
     const uint64_t listed = s.list[tid];  // (of no use where the list is shorter)
-    r.top = order_logit(d.best);
+    set_top(r, d.best);
     if (r.greedy || r.top == -__builtin_huge_valf()) {
         if (tid == 0) {
             const bool none = r.top == -__builtin_huge_valf();  // no token: no logit above -inf
@@ -1021,8 +1023,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
             uint64_t mine = 0;
             for_chunks<T>(logits, a.vocab, 0, chunks, [&](int, int64_t id, const float(&x)[8]) {
                 for (int i = 0; i < 8; ++i) {
-                    const double depth = depth_of(r, x[i]);
-                    if (depth < kDepth && bucket_of(depth) == d.k_bucket && order_word(x[i], id + i) >= last) {
+                    const float v = settle(x[i]);
+                    const double depth = depth_of(r, v);
+                    if (depth < kDepth && bucket_of(depth) == d.k_bucket && order_word(v, id + i) >= last) {
                         mine += weight_of(depth, s_powers);
                     }
                 }
@@ -1049,8 +1052,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
         for_chunks<T>(logits, a.vocab, 0, chunks, [&](int c, int64_t id, const float(&x)[8]) {
             uint64_t sum = 0;
             for (int i = 0; i < 8; ++i) {
-                const double depth = depth_of(r, x[i]);
-                if (depth < kDepth && bucket_of(depth) >= d.low && order_word(x[i], id + i) >= last) {
+                const float v = settle(x[i]);
+                const double depth = depth_of(r, v);
+                if (depth < kDepth && bucket_of(depth) >= d.low && order_word(v, id + i) >= last) {
                     const uint64_t w = weight_of(depth, s_powers);
                     sum += w >= r.least ? w : 0;
                 }
@@ -1082,9 +1086,10 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     uint64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const double depth = id + i < a.vocab ? depth_of(r, x[i]) : kDepth;
+        const float v = settle(x[i]);
+        const double depth = id + i < a.vocab ? depth_of(r, v) : kDepth;
         w[i] = depth < kDepth ? weight_of(depth, s_powers) : 0;
-        w[i] = w[i] >= r.least && order_word(x[i], id + i) >= last ? w[i] : 0;
+        w[i] = w[i] >= r.least && order_word(v, id + i) >= last ? w[i] : 0;
         mine += w[i];
     }
     uint64_t all;
