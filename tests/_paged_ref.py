@@ -82,23 +82,23 @@ class Paged:
         for x in (self.k, self.v):
             x.transpose(1, 2)[dead] = junk
 
-    def rows(self, i: int, g: int, which: str) -> np.ndarray:
-        x = f64(self.k if which == "k" else self.v)
+    def rows(self, pool: np.ndarray, i: int, g: int) -> np.ndarray:
         j = np.arange(self.kv[i])
-        return x[self.table[i, j // self.page], g, j % self.page]
+        return pool[self.table[i, j // self.page], g, j % self.page]
 
     def want(self):
         """(out, sum of |weight * value|) in fp64; rows of no sequence are NaN."""
 
         out = np.full((self.tokens, self.heads, self.dim), np.nan)
         size = out.copy()
+        queries, keys, values = f64(self.q), f64(self.k), f64(self.v)
         for i, (n, kv) in enumerate(zip(self.new, self.kv)):
             pos = kv - n + np.arange(n)
             hidden = np.arange(kv)[None, :] > pos[:, None]
             for h in range(self.heads):
                 g = h // (self.heads // self.kv_heads)
-                k, v = self.rows(i, g, "k"), self.rows(i, g, "v")
-                q = f64(self.q[self.starts[i]:self.starts[i] + n, h])
+                k, v = self.rows(keys, i, g), self.rows(values, i, g)
+                q = queries[self.starts[i]:self.starts[i] + n, h]
                 with np.errstate(invalid="ignore"):
                     s = np.where(hidden, -np.inf, q @ k.T * self.scale) if kv else np.zeros((n, 0))
                 top = s.max(axis=1, initial=-np.inf, keepdims=True)
@@ -106,6 +106,9 @@ class Paged:
                 total = p.sum(axis=1, keepdims=True)
                 p = np.divide(p, total, out=np.zeros_like(p), where=total > 0)
                 at = slice(self.starts[i], self.starts[i] + n)
+                if np.isfinite(v).all():
+                    out[at, h], size[at, h] = p @ v, p @ np.abs(v)
+                    continue
                 for row in range(n):
                     seen = slice(0, max(0, min(kv, pos[row] + 1)))
                     out[at.start + row, h] = p[row, seen] @ v[seen]

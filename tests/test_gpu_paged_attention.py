@@ -45,6 +45,13 @@ def _check(batch, out, rows=None):
     # sequences without new tokens, without cache rows, and rows that see no key
     ([0, 4, 0, 1, 40], [9, 4, 0, 0, 13], 4, 2, 16, "hnd"),
     ([2, 60], [0, 1], 4, 4, 16, "hnd"),
+    # pages smaller than what a wave loads at once, in tiles
+    ([90, 1, 33], [260, 7, 33], 4, 2, 1, "hnd"),
+    ([150], [390], 2, 1, 2, "nhd"),
+    # tiles enough for two blocks a CU, many sequences
+    ([2048], [2100], 32, 32, 16, "hnd"),
+    ([40, 0, 7, 100] * 70, [41, 5, 30, 100] * 70, 2, 2, 16, "hnd"),
+    ([1] * 300, list(range(1, 301)), 4, 2, 16, "hnd"),
 ])
 def test_matches_fp64(torch_gpu, native, dtype, dim, new, kv, heads, kv_heads, page, layout):
     batch = Paged(len(new) + sum(kv), new, kv, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype,

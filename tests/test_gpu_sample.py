@@ -64,7 +64,7 @@ def _logits(rng, rows, vocab, dtype, std=2.5, pitch=None, shift=0):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,vocab,pitch,shift", [
     (1, 1, None, 0), (3, 2, None, 0), (5, 7, 9, 1), (4, 2047, None, 0), (4, 2048, 2056, 0), (3, 2049, 2051, 3),
-    (6, 32000, None, 0), (2, 151936, None, 0), (40, 5000, 5008, 8),
+    (6, 32000, None, 0), (2, 151936, None, 0), (40, 5000, 5008, 8), (2, 1 << 20, None, 0), (2000, 33, None, 0),
 ])
 def test_settings_row_by_row(torch_gpu, native, dtype, rows, vocab, pitch, shift):
     """Every row its own mix of settings, off and degenerate ones among them."""
@@ -73,7 +73,7 @@ def test_settings_row_by_row(torch_gpu, native, dtype, rows, vocab, pitch, shift
     logits = _logits(rng, rows, vocab, dtype, pitch=pitch, shift=shift)
     for _ in range(3):
         settings = dict(temperature=rng.choice([0.0, -1.0, 0.1, 0.7, 1.0, 1.5], rows),
-                        top_k=rng.choice([-1, 0, 1, 2, 50, 900, 3 * vocab], rows),
+                        top_k=rng.choice([-1, 0, 1, 2, 50, 900, 5000, 3 * vocab], rows),
                         top_p=rng.choice([-1.0, 0.0, 1e-6, 0.3, 0.9, 0.999, 1.0, 2.0], rows),
                         min_p=rng.choice([-1.0, 0.0, 1e-7, 0.05, 0.5, 1.0, 3.0], rows))
         u = rng.random(rows).astype(np.float32)
