@@ -250,11 +250,14 @@ __device__ __forceinline__ void tell_splits(const PagedAttnArgs& a, const Sequen
 // bound by the cache's bytes.  All blocks share the cached rows of all sequences
 // evenly: the work is the line of (sequence, KV head, tile of 16 rows, round of 128
 // keys), cut into one stretch a block, so a batch of unequal lengths ends everywhere
-// at once (a fixed number of splits a sequence: 64 sequences of up to 8192 tokens
-// 88 us instead of 70).  In a round the four waves take 32 keys each, K straight from
-// memory into the first product's operand, V through the wave's own LDS, the next
-// keys requested as soon as the registers of these are free.
-constexpr int kFewRows = 32;
+// at once (64 sequences of up to 8192 tokens, 307 MB: 70 us, 4.4 TB/s; with a fixed
+// number of splits a sequence 88).  In a round the four waves take 32 keys each, K
+// straight from memory into the first product's operand, V through the wave's own LDS,
+// the next keys requested as soon as the registers of these are free.  With more rows
+// the keys were read once a tile of 16, and the row tiles below are faster: 32 rows of
+// 64 sequences of 2000 keys 58 us here and 37 there, of 8192 keys at most 104 and 98, of
+// one with 120000 55 and 34; of 64 with 100 keys 9.9 and 11.7.
+constexpr int kFewRows = 16;
 constexpr int kUnit = 32;
 constexpr int kRound = 4 * kUnit;
 constexpr int64_t kFewBlocks = 512;
@@ -645,8 +648,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 // arithmetic (exp of 32 scores a lane).  Weights enter the second product rounded to
 // 16 bits and their sum adds the rounded ones: half a step of the type a weight, at
 // random, next to the result's own half step (2-norm error of a prompt of 8192 bf16
-// tokens 1.9e-3, of the result's rounding alone 1.6e-3); a second part of each weight
-// would cost half as many products again.  Measured, 8192 tokens of 16 heads over 2
+// tokens 2.1e-3, 1.9e-3 with a maximum that never lags at 284 us for 265, of the
+// result's rounding alone 1.6e-3); a second part of each weight would cost half as many
+// products again.  Measured, 8192 tokens of 16 heads over 2
 // KV heads: 346 us at first, 318 with loads that bypass the compiler's waits, 293
 // with operands read ahead and the maximum allowed to lag, 287 with page bases as
 // scalars, 262 with the waves' priorities and the order of blocks (1050 TFLOP/s; a
@@ -1249,10 +1253,30 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     }
     if (rows > kFewRows) {
         p.slots = tokens * group / kTileRows + sequences;
-        // two blocks of one K-group a CU, or one of two; a split is at least four windows
-        p.tile_groups = p.slots * kv_heads >= 512 ? 1 : 2;
         const int64_t tiles = p.slots * kv_heads;
-        p.tile_splits = cap(tiles > 128 && tiles <= 192 ? 2 : 256 / tiles, cap((max_kv_len + 4 * kWindow - 1) / (4 * kWindow), 32));
+        const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
+        // Splits of at least four windows, while the blocks run side by side: a window of a
+        // block takes about 0.85 us, a merge 3 and 7 more for the partials of 256 full tiles
+        // (600 tokens of 16 heads over 2 KV heads after 4000: 3 splits 39 us, one 67; 1000
+        // after none: one 22.5, 2 splits 27.6; 1300 after 4000: 2 of 164 tiles 76, one 78).
+        const int64_t side_by_side = tiles > 128 && tiles <= 192 ? 384 : 256;
+        const auto cost = [&](int64_t s) { return 85 * windows / s + (s > 1 ? 300 + 700 * tiles * s / 256 : 0); };
+        p.tile_splits = 1;
+        for (int64_t s = 2; s <= (windows + 3) / 4 && s * tiles <= side_by_side; ++s) {
+            p.tile_splits = cost(s) < cost(p.tile_splits) ? s : p.tile_splits;
+        }
+        // Sequences of one tile a KV head, whose partials are small: splits that even out
+        // unequal lengths (64 sequences of 4 tokens and up to 8192 keys: 2 splits 134 us,
+        // 6 98; all of 2000 keys: 2 38.4, 4 37.5; with 8 tokens each: 2 42, 4 50).
+        if (sequences > 1 && rows <= kTileRows) {
+            const int64_t even = cap(1024 / tiles, (windows + 7) / 8);
+            p.tile_splits = p.tile_splits > even ? p.tile_splits : even;
+        }
+        // Blocks of one K-group, two a CU, where they fill the chip; else of two, one a CU
+        // (two of D = 64): 8192 tokens 269 us with one and 298 with two, 6000 166 and 175,
+        // 4000 90 and 80, 3000 64 and 53; splits past 256 blocks 43 and 47 (D = 128), 60
+        // and 56 (D = 64).
+        p.tile_groups = tiles >= 512 || (head_dim == 128 && p.tile_splits > 1 && tiles * p.tile_splits > 256) ? 1 : 2;
     }
     const int64_t unit = tokens * q_heads * (head_dim + 2) * 4;
     const int64_t counts = tokens * q_heads * 4;

@@ -32,9 +32,9 @@ def _check(batch, out, rows=None):
     ([1, 1, 1, 1], [1, 31, 32, 33], 16, 2, 16, "hnd"),
     ([1, 1, 1], [127, 129, 1000], 7, 1, 16, "nhd"),
     ([1] * 9, [5, 700, 1, 64, 65, 333, 16, 17, 2000], 12, 4, 64, "hnd"),
-    ([1, 1], [300, 40], 32, 1, 8, "nhd"),            # 32 heads of a KV head: two rounds of columns
-    ([1, 1], [70, 3], 64, 1, 16, "hnd"),             # 64: past the few-row form
-    # few new tokens: drafts, more columns than 16
+    ([1, 1], [300, 40], 32, 1, 8, "nhd"),            # 32 heads of a KV head: past the few-row form
+    ([1, 1], [70, 3], 64, 1, 16, "hnd"),
+    # few new tokens: drafts, on both sides of 16 columns
     ([3, 2, 4], [3, 100, 260], 8, 2, 16, "hnd"),
     # chunks: first ones (no cache before), later ones, ends inside a tile and a window
     ([17], [17], 4, 2, 16, "hnd"),
@@ -52,6 +52,11 @@ def _check(batch, out, rows=None):
     ([2048], [2100], 32, 32, 16, "hnd"),
     ([40, 0, 7, 100] * 70, [41, 5, 30, 100] * 70, 2, 2, 16, "hnd"),
     ([1] * 300, list(range(1, 301)), 4, 2, 16, "hnd"),
+    # one tile a KV head: more than 64 splits, splits that even out lengths, with empty ones among them
+    ([4], [40000], 16, 2, 16, "hnd"),
+    ([1, 1], [30000, 31], 32, 1, 64, "nhd"),
+    ([4, 0, 3, 4, 2] * 6, [3000, 5, 3, 1999, 64] * 6, 12, 2, 16, "hnd"),
+    ([1] * 10, [2000, 1, 64, 65, 0, 1500, 3, 128, 127, 700], 32, 1, 16, "nhd"),
 ])
 def test_matches_fp64(torch_gpu, native, dtype, dim, new, kv, heads, kv_heads, page, layout):
     batch = Paged(len(new) + sum(kv), new, kv, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype,
