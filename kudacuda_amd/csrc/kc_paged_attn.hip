@@ -1242,19 +1242,14 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     const int64_t longest = max_query_len < tokens ? max_query_len : tokens;
     const int64_t rows = longest * group;
     const auto cap = [](int64_t v, int64_t most) { return v < 1 ? int64_t{1} : (v < most ? v : most); };
-    int64_t few_splits = 0;
-    if (rows <= kFewRows || tokens != sequences * longest) {
-        // two blocks a CU; a stretch of at least one round of keys.  The longest sequence
-        // may be cut into twice as many stretches as it were in a batch of such ones.
-        const int64_t tiles = sequences * kv_heads * (((rows < kFewRows ? rows : kFewRows) + 15) / 16);
-        const int64_t rounds = (max_kv_len + kRound - 1) / kRound;
-        p.few_blocks = rounds < kFewBlocks && tiles * rounds < kFewBlocks ? tiles * rounds : kFewBlocks;
-        few_splits = cap(2 * ((kFewBlocks + tiles - 1) / tiles) + 1, cap(rounds, 256));
-    }
-    if (rows > kFewRows) {
+    const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
+    // Few rows of every sequence go to the kernel for them where all sequences' windows
+    // are at least 28 a CU (64 sequences of up to 8192 keys, 2 KV heads: 70 us, row tiles
+    // 81; 32 36 and 40; 24 35 and 33; 128 of up to 2000 38 and 43, of 1000 31 and 26).
+    const bool few = rows <= kFewRows && sequences * kv_heads * windows >= 7168;
+    if (!few) {
         p.slots = tokens * group / kTileRows + sequences;
         const int64_t tiles = p.slots * kv_heads;
-        const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
         // Splits of at least four windows, while the blocks run side by side: a window of a
         // block takes about 0.85 us, a merge 3 and 7 more for the partials of 256 full tiles
         // (600 tokens of 16 heads over 2 KV heads after 4000: 3 splits 39 us, one 67; 1000
@@ -1277,6 +1272,18 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
         // 4000 90 and 80, 3000 64 and 53; splits past 256 blocks 43 and 47 (D = 128), 60
         // and 56 (D = 64).
         p.tile_groups = tiles >= 512 || (head_dim == 128 && p.tile_splits > 1 && tiles * p.tile_splits > 256) ? 1 : 2;
+    }
+    // Beside longer sequences they go there where a tile would take more than 50 windows (a
+    // chunk of 1000 and a token after 16000: 58 us, with tiles alone 113; 512 and 63 tokens
+    // after up to 4000: 60 and 67; two chunks of 256 and 8 tokens: 40 and 30).
+    int64_t few_splits = 0;
+    if (few || (rows > kFewRows && tokens != sequences * longest && windows > 50 * p.tile_splits)) {
+        // two blocks a CU; a stretch of at least one round of keys.  The longest sequence
+        // may be cut into twice as many stretches as it were in a batch of such ones.
+        const int64_t tiles = sequences * kv_heads * (((rows < kFewRows ? rows : kFewRows) + 15) / 16);
+        const int64_t rounds = (max_kv_len + kRound - 1) / kRound;
+        p.few_blocks = rounds < kFewBlocks && tiles * rounds < kFewBlocks ? tiles * rounds : kFewBlocks;
+        few_splits = cap(2 * ((kFewBlocks + tiles - 1) / tiles) + 1, cap(rounds, 256));
     }
     const int64_t unit = tokens * q_heads * (head_dim + 2) * 4;
     const int64_t counts = tokens * q_heads * 4;

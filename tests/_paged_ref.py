@@ -52,6 +52,7 @@ class Paged:
         rng = np.random.default_rng([77, seed])
         self.new, self.kv, self.page, self.dtype, self.dim = list(new), list(kv), page, dtype, dim
         self.heads, self.kv_heads, self.layout = heads, kv_heads, layout
+        self.hint = None  # the longest length that calls are told; the batch's if None
         self.scale = float(np.float32(dim**-0.5 if scale is None else scale))
         used = [-(-n // page) for n in kv]
         self.num_pages = sum(used) + 3 + spare
@@ -149,7 +150,7 @@ class Paged:
 
     def call(self, native, d, stream=None, workspace=None, max_new=None, max_kv=None, nbytes=None):
         max_new = max(1, max(self.new)) if max_new is None else max_new
-        max_kv = max(1, max(self.kv)) if max_kv is None else max_kv
+        max_kv = (self.hint or max(1, max(self.kv))) if max_kv is None else max_kv
         n = len(self.new)
         if nbytes is None:
             nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(self.tokens, n, max_new, max_kv, self.heads,

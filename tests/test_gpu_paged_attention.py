@@ -12,6 +12,8 @@ from tests._paged_ref import Paged, f64
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
+# A told longest length of 2^20 puts sequences of few rows into the kernel for them, which otherwise takes large batches.
+hints = pytest.mark.parametrize("hint", [None, 1 << 20])
 
 
 def _check(batch, out, rows=None):
@@ -24,6 +26,7 @@ def _check(batch, out, rows=None):
     assert (off <= bound).all(), float((off / np.maximum(bound, 1e-30)).max())
 
 
+@hints
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("new,kv,heads,kv_heads,page,layout", [
@@ -58,9 +61,10 @@ def _check(batch, out, rows=None):
     ([4, 0, 3, 4, 2] * 6, [3000, 5, 3, 1999, 64] * 6, 12, 2, 16, "hnd"),
     ([1] * 10, [2000, 1, 64, 65, 0, 1500, 3, 128, 127, 700], 32, 1, 16, "nhd"),
 ])
-def test_matches_fp64(torch_gpu, native, dtype, dim, new, kv, heads, kv_heads, page, layout):
+def test_matches_fp64(torch_gpu, native, dtype, dim, new, kv, heads, kv_heads, page, layout, hint):
     batch = Paged(len(new) + sum(kv), new, kv, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype,
                   layout=layout, q_extra=1)
+    batch.hint = hint
     print(f"paged attention {new} of {kv}, {heads}/{kv_heads} heads of {dim}, pages of {page}", flush=True)
     _check(batch, batch.call(native, batch.device()))
 
@@ -82,9 +86,11 @@ def test_splits_follow_the_workspace_and_the_hints(torch_gpu, native, new, kv):
         _check(batch, batch.call(native, d, max_new=max_new, max_kv=max_kv))
 
 
+@hints
 @pytest.mark.parametrize("new,kv", [([1, 1, 1], [900, 33, 0]), ([70, 3], [200, 3])])
-def test_rows_behind_the_last_sequence_stay(torch_gpu, native, new, kv):
+def test_rows_behind_the_last_sequence_stay(torch_gpu, native, new, kv, hint):
     batch = Paged(6, new, kv, extra_rows=5)
+    batch.hint = hint
     for nbytes in (None, 0):
         d = batch.device()
         out = batch.call(native, d, nbytes=nbytes)
@@ -92,12 +98,14 @@ def test_rows_behind_the_last_sequence_stay(torch_gpu, native, new, kv):
         assert (f64(out[-5:]) == 7.25).all()
 
 
+@hints
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("new,kv", [([4], [300]), ([150], [400])])
-def test_infinities_and_nan_of_hidden_keys_stay_hidden(torch_gpu, native, dtype, new, kv):
+def test_infinities_and_nan_of_hidden_keys_stay_hidden(torch_gpu, native, dtype, new, kv, hint):
     """The last key's K and V are NaN and infinite: only the row that sees it is not finite."""
 
     batch = Paged(8, new, kv, dtype=dtype, dim=64)
+    batch.hint = hint
     last = kv[0] - 1
     page, at = batch.table[0, last // 16], last % 16
     for value in (float("inf"), float("nan")):
@@ -110,11 +118,13 @@ def test_infinities_and_nan_of_hidden_keys_stay_hidden(torch_gpu, native, dtype,
             assert not np.isfinite(f64(out[-1])).any()
 
 
+@hints
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-def test_large_scores_and_lowest_values(torch_gpu, native, dtype):
+def test_large_scores_and_lowest_values(torch_gpu, native, dtype, hint):
     """Scores of hundreds, keys at the type's lowest value, a first key that outweighs all others by far."""
 
     batch = Paged(9, [1, 40], [600, 300], dtype=dtype, dim=64, junk=float("-inf"))
+    batch.hint = hint
     batch.k *= 12
     page = batch.table[0, 0]
     batch.k[page, :, 3] = 0
@@ -128,12 +138,14 @@ def test_large_scores_and_lowest_values(torch_gpu, native, dtype):
     assert (np.abs(out - want) <= bound).all()
 
 
-def test_pages_outside_the_pool_make_nan_rows(torch_gpu, native):
+@hints
+def test_pages_outside_the_pool_make_nan_rows(torch_gpu, native, hint):
     """A bad page id is not read; the rows that see one of its keys are NaN, the others hold."""
 
     for new, kv in (([1, 1, 1], [500, 90, 33]), ([40, 1], [300, 20])):
         for bad in (-1, 2**31 - 1, None):
             batch = Paged(10, new, kv)
+            batch.hint = hint
             d = batch.device()
             d["table"][0, (kv[0] - 1) // 16 - 1] = batch.num_pages if bad is None else bad
             first = ((kv[0] - 1) // 16 - 1) * 16  # the first key of that page
@@ -146,10 +158,12 @@ def test_pages_outside_the_pool_make_nan_rows(torch_gpu, native):
                 assert np.isfinite(out[new[0]:]).all()
 
 
-def test_lengths_that_do_not_fit_the_table_make_nan_rows(torch_gpu, native):
+@hints
+def test_lengths_that_do_not_fit_the_table_make_nan_rows(torch_gpu, native, hint):
     for new, kv in (([1, 1], [64, 40]), ([50, 3], [64, 40])):
         for bad in (-1, 4 * 16 + 1, 2**31 - 1):
             batch = Paged(11, new, kv)
+            batch.hint = hint
             d = batch.device()
             d["lens"][0] = bad
             for nbytes in (None, 0, 1 << 20):
@@ -158,21 +172,25 @@ def test_lengths_that_do_not_fit_the_table_make_nan_rows(torch_gpu, native):
                 _check(batch, d["out"], rows=np.arange(new[0], batch.tokens))
 
 
-def test_starts_outside_the_rows_stay_inside(torch_gpu, native):
+@hints
+def test_starts_outside_the_rows_stay_inside(torch_gpu, native, hint):
     """Starts past the tokens (and below zero) name no rows."""
 
     batch = Paged(12, [2, 3], [40, 50])
+    batch.hint = hint
     d = batch.device()
     d["starts"].copy_(torch.tensor([-4, 2, 2**31 - 1], dtype=torch.int32))
     out = f64(batch.call(native, d, nbytes=0))
     assert np.isfinite(out).all()
 
 
-def test_offsets_past_32_bits(torch_gpu, native):
+@hints
+def test_offsets_past_32_bits(torch_gpu, native, hint):
     """Pools of more than 2^32 elements: pages 2^25 elements apart, the values half a page behind the keys."""
 
     stride, pages = 1 << 25, 130
     batch = Paged(13, [1, 20], [700, 300], dim=64, kv_heads=2, heads=4, spare=pages - 3 - 44 - 19)
+    batch.hint = hint
     assert batch.num_pages == pages and int(batch.table.max()) > 127
     d = batch.device()
     pool = torch.zeros(pages * stride, dtype=BF16, device="cuda:0")
@@ -205,18 +223,19 @@ def test_two_streams_and_a_second_handle(torch_gpu, native):
     other.close()
 
 
-def test_captured_call_follows_its_tables(torch_gpu, native):
+@hints
+def test_captured_call_follows_its_tables(torch_gpu, native, hint):
     """One capture, replayed while the sequences grow: lengths, tables and starts are read at replay time."""
 
     batch = Paged(16, [1, 1, 1], [900, 600, 40], dim=128)
     d = batch.device()
-    nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(3, 3, 1, 1024, 4, 2, 128)
+    nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(3, 3, 1, hint or 1024, 4, 2, 128)
     workspace = torch.zeros(nbytes, dtype=torch.uint8, device="cuda:0")
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):
-        batch.call(native, d, stream=torch.cuda.current_stream(), workspace=workspace, nbytes=nbytes, max_kv=1024)
+        batch.call(native, d, stream=torch.cuda.current_stream(), workspace=workspace, nbytes=nbytes, max_kv=hint or 1024)
     for kv in ([900, 600, 40], [1, 600, 39], [33, 0, 17], [899, 128, 40]):
         batch.kv = kv
         with torch.cuda.stream(side):
@@ -226,27 +245,32 @@ def test_captured_call_follows_its_tables(torch_gpu, native):
         side.synchronize()
         _check(batch, d["out"])
         replayed = d["out"].clone()
-        batch.call(native, d, workspace=workspace, nbytes=nbytes, max_kv=1024)
+        batch.call(native, d, workspace=workspace, nbytes=nbytes, max_kv=hint or 1024)
         torch.cuda.synchronize()
         assert torch.equal(replayed, d["out"])
 
 
-def test_results_do_not_change_from_call_to_call(torch_gpu, native):
+@hints
+def test_results_do_not_change_from_call_to_call(torch_gpu, native, hint):
     batch = Paged(17, [1, 200, 3], [3000, 900, 60], dim=128, heads=16)
+    batch.hint = hint
     d = batch.device()
     first = batch.call(native, d).clone()
     for _ in range(5):
         assert torch.equal(batch.call(native, d), first)
 
 
-def test_starts_that_descend_stay_inside(torch_gpu, native):
+@hints
+def test_starts_that_descend_stay_inside(torch_gpu, native, hint):
     """Starts that go back and forth name no batch: whatever the rows become, the sequences' pages and the workspace
     hold what they held, and the next call is right."""
 
     for new, kv in (([1] * 6, [400, 30, 70, 2000, 5, 90]), ([70, 1, 40, 3], [300, 20, 100, 50])):
         batch = Paged(18, new, kv, dim=128)
+        batch.hint = hint
         d = batch.device()
-        nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(batch.tokens, len(new), max(new), max(kv), 4, 2, 128)
+        nbytes = native.lib.kudacuda_paged_attention_workspace_bytes(batch.tokens, len(new), max(new), hint or max(kv),
+                                                                          4, 2, 128)
         workspace = torch.full((nbytes + 4096,), 0x7f, dtype=torch.uint8, device="cuda:0")
         pools = d["k"].clone(), d["v"].clone()
         good = d["starts"].clone()
