@@ -297,7 +297,7 @@ KUDACUDA_API int64_t kudacuda_lm_head_workspace_floats(void);
  * far positions and any scaling of the frequencies hold), times amplitude.  Pairs
  * are dims i and i + rotary_dim / 2, or 2 i and 2 i + 1 with interleaved = 1.
  * positions int32.  Strides are elements between tokens; output may be input
- * (same stride), else they must not overlap.  Contract: tokens>=0, heads 1..4096,
+ * (same stride), else they must not overlap.  Contract: tokens 0..2^25, heads 1..4096,
  * head_dim even, 2..256, rotary_dim even, 2..head_dim.  Rows, strides and
  * rotary_dim in whole 16-byte pieces (rotary_dim a multiple of 16) run faster. */
 KUDACUDA_API int kudacuda_rope(void* handle, uint64_t input, uint64_t inv_freq, uint64_t positions, uint64_t output,
@@ -321,9 +321,9 @@ KUDACUDA_API int kudacuda_rope_paged_append(
 
 /* Causal attention of new tokens over a paged cache.  Sequence i's new tokens are
  * rows query_starts[i] .. query_starts[i + 1] of query (int32 [sequences + 1],
- * ascending; output must not overlap query); it has kv_lens[i] cached tokens (int32), the new ones the last of
- * them, token j in page page_table[i * table_stride + j / page_size] (int32).  New
- * token t sees the keys up to its own, kv_lens[i] - q_len + t; a row that sees none
+ * ascending; output must not overlap query); it has kv_lens[i] cached tokens
+ * (int32), the new ones the last of them, token j in page page_table[i *
+ * table_stride + j / page_size] (int32).  New token t sees the keys up to its own, kv_lens[i] - q_len + t; a row that sees none
  * is zero.  Rows of no sequence are left as they were.  A sequence whose kv_len is
  * negative or past its table row, and a row that sees a page id outside the pool,
  * become NaN; such pages are not read.
@@ -333,9 +333,9 @@ KUDACUDA_API int kudacuda_rope_paged_append(
  * kudacuda_paged_attention_workspace_bytes() of the same sizes, or less (fewer
  * splits), or none (0, 0).
  * Contract: head_dim 64 or 128, query_heads a multiple of kv_heads (both 1..1024),
- * 1..65536 sequences, tokens * query_heads <= 2^30, table_stride * page_size <=
- * 2^30, strides multiples of 8, buffers (but the int32 ones) on 16-byte
- * boundaries, positive finite scale. */
+ * 1..65536 sequences, sequences * kv_heads <= 2^22, tokens * query_heads <= 2^27,
+ * table_stride * page_size <= 2^30, strides multiples of 8, buffers (but the int32
+ * ones) on 16-byte boundaries, positive finite scale. */
 KUDACUDA_API int kudacuda_paged_attention(void* handle, uint64_t query, uint64_t key_pages, uint64_t value_pages,
                                           uint64_t page_table, uint64_t query_starts, uint64_t kv_lens, uint64_t output,
                                           uint64_t workspace, int64_t workspace_bytes, int64_t dtype, int64_t tokens,
@@ -355,8 +355,8 @@ KUDACUDA_API int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, in
  * compaction moves high pages to free low ones; the bookkeeping is the caller's
  * (kudacuda_amd/paged_cache.py).  Destinations must differ from each other and
  * from the sources of other pairs; other lists are refused.  Contract: page ids in
- * [0, num_pages), everything in whole 16-byte pieces on 16-byte boundaries,
- * page_stride and (pools > 1) pool_stride >= page_bytes, and either whole pools
+ * [0, num_pages), everything in whole 16-byte pieces on 16-byte boundaries, 1..65536
+ * pools, pools * page_bytes <= 2^37, page_stride and (pools > 1) pool_stride >= page_bytes, and either whole pools
  * one after the other (pool_stride >= num_pages * page_stride) or a page's pools
  * side by side (page_stride >= pools * pool_stride).  A captured call keeps its
  * pairs. */

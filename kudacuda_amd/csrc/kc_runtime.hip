@@ -917,10 +917,11 @@ bool rope_shape_ok(Handle* h, const char* symbol, int64_t dtype, int64_t tokens,
     if (dtype != 1 && dtype != 2) {
         return refuse(h, symbol, "dtype 1 (bf16) or 2 (fp16)");
     }
-    if (!within(tokens, 0, kInt32Max) || !within(heads, 1, 4096) || !within(head_dim, 2, kRopeMaxDim) ||
+    // (a launch has fewer than 2^32 threads)
+    if (!within(tokens, 0, int64_t{1} << 25) || !within(heads, 1, 4096) || !within(head_dim, 2, kRopeMaxDim) ||
         !within(rotary_dim, 2, head_dim) || head_dim % 2 != 0 || rotary_dim % 2 != 0 || !within(interleaved, 0, 1)) {
         return refuse(h, symbol,
-                      "tokens>=0, heads 1..4096, even head_dim 2..256, even rotary_dim 2..head_dim and interleaved 0 or 1");
+                      "2^25>=tokens>=0, heads 1..4096, even head_dim 2..256, even rotary_dim 2..head_dim and interleaved 0 or 1");
     }
     if (!std::isfinite(amplitude)) {
         return refuse(h, symbol, "a finite amplitude");
@@ -1609,6 +1610,10 @@ int kudacuda_rope(void* raw, uint64_t input, uint64_t inv_freq, uint64_t positio
         refuse(h, symbol, "strides of at least heads * head_dim");
         return 1;
     }
+    if (input == output && input_stride != output_stride && tokens > 1) {
+        refuse(h, symbol, "one stride where it works in place");
+        return 1;
+    }
     if (!multiple(input | output, 2) || !multiple(inv_freq, 8) || !multiple(positions, 4)) {
         refuse(h, symbol, "buffers aligned to their elements");
         return 1;
@@ -1663,6 +1668,10 @@ int kudacuda_rope_paged_append(void* raw, uint64_t query, uint64_t key, uint64_t
         refuse(h, symbol, "strides of at least heads * head_dim");
         return 1;
     }
+    if (query == query_output && query_stride != output_stride && tokens > 1) {
+        refuse(h, symbol, "one stride where it works in place");
+        return 1;
+    }
     if (page_stride < head_dim || head_stride < head_dim || token_stride < head_dim) {
         refuse(h, symbol, "pool strides of at least head_dim");
         return 1;
@@ -1709,7 +1718,8 @@ int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, int64_t sequenc
                                                  int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
                                                  int64_t head_dim) {
     if (!within(query_heads, 1, 1024) || !within(kv_heads, 1, query_heads) || query_heads % kv_heads != 0 ||
-        !within(tokens, 1, (int64_t{1} << 30) / query_heads) || !within(sequences, 1, 65536) || !within(head_dim, 1, 128) ||
+        !within(tokens, 1, (int64_t{1} << 27) / query_heads) || !within(sequences, 1, 65536) ||
+        !within(sequences * kv_heads, 1, int64_t{1} << 22) || !within(head_dim, 1, 128) ||
         max_query_len < 1 || max_kv_len < 1) {
         return 0;  // no call that would be taken
     }
@@ -1746,11 +1756,12 @@ int kudacuda_paged_attention(void* raw, uint64_t query, uint64_t key_pages, uint
         return 1;
     }
     const int shift = page_shift_of(page_size);
-    if (!within(tokens, 0, (int64_t{1} << 30) / query_heads) || !within(sequences, 1, 65536) ||
-        !within(num_pages, 1, kInt32Max) || shift < 0 || !within(table_stride, 1, (int64_t{1} << 30) >> shift)) {
+    // (a launch has fewer than 2^32 threads)
+    if (!within(tokens, 0, (int64_t{1} << 27) / query_heads) || !within(sequences, 1, 65536) ||
+        !within(sequences * kv_heads, 1, int64_t{1} << 22) || !within(num_pages, 1, kInt32Max) || shift < 0 || !within(table_stride, 1, (int64_t{1} << 30) >> shift)) {
         refuse(h, symbol,
-               "0 <= tokens * query_heads <= 2^30, 1..65536 sequences, num_pages>=1, page_size a power of two (1..4096) "
-               "and 1 <= table_stride * page_size <= 2^30");
+               "0 <= tokens * query_heads <= 2^27, 1..65536 sequences, sequences * kv_heads <= 2^22, num_pages>=1, "
+               "page_size a power of two (1..4096) and 1 <= table_stride * page_size <= 2^30");
         return 1;
     }
     if (max_query_len < 1 || max_kv_len < 1) {
@@ -1828,8 +1839,8 @@ int kudacuda_copy_pages(void* raw, uint64_t pool, uint64_t pairs, int64_t count,
         return 1;
     }
     if (!within(count, 0, num_pages) || !within(pools, 1, 65536) || !within(num_pages, 1, kInt32Max) ||
-        !within(page_bytes, 16, int64_t{1} << 28)) {
-        refuse(h, symbol, "0 <= count <= num_pages, 1..65536 pools, num_pages>=1 and page_bytes 16..2^28");
+        !within(page_bytes, 16, int64_t{1} << 28) || !within(pools * page_bytes, 16, int64_t{1} << 37)) {
+        refuse(h, symbol, "0 <= count <= num_pages, 1..65536 pools, num_pages>=1, page_bytes 16..2^28 and pools * page_bytes <= 2^37");
         return 1;
     }
     if (!multiple(pool | static_cast<uint64_t>(page_bytes | page_stride | pool_stride), 16) || !multiple(pairs, 4) ||

@@ -12,7 +12,9 @@ pages in use to the lowest ids.  A round of a server is::
         q = cache.append(layer, batch, q, k, v, inv_freq)
         out = cache.attend(layer, batch, q)
 
-Calls run on the torch stream that is current when they are made.
+Calls run on the torch stream that is current when they are made.  The pool is shared
+by all of them: a program with several streams orders them itself (events), and a
+batch whose calls a graph has captured is kept as long as the graph.
 """
 
 from __future__ import annotations
@@ -43,6 +45,7 @@ class Batch:
     query_starts: Any  # int32 [sequences + 1]
     kv_lens: Any       # int32 [sequences]
     page_table: Any    # int32 [sequences, pages of the longest]
+    stream: int = 0    # the stream that they were made on
 
 
 @dataclass
@@ -220,7 +223,7 @@ class PagedKvCache:
             return t.from_numpy(np.ascontiguousarray(a)).to(self.device)
 
         return Batch(tuple(sequences), int(starts[-1]), max(counts), int(lengths.max()), up(np.concatenate(slots)),
-                     up(np.concatenate(positions).astype(np.int32)), up(starts), up(lengths), up(table))
+                     up(np.concatenate(positions).astype(np.int32)), up(starts), up(lengths), up(table), self._stream())
 
     # ------------------------------------------------------------ native calls
     def _stream(self) -> int:
@@ -228,6 +231,15 @@ class PagedKvCache:
 
     def _dtype(self) -> int:
         return 1 if self.pool.dtype == self.torch.bfloat16 else 2
+
+    def _use(self, batch: Batch) -> int:
+        """The current stream; where the batch was made on another one, its memory waits for this one too."""
+
+        stream = self.torch.cuda.current_stream(self.device)
+        if stream.cuda_stream != batch.stream and not self.torch.cuda.is_current_stream_capturing():
+            for x in (batch.slots, batch.positions, batch.query_starts, batch.kv_lens, batch.page_table):
+                x.record_stream(stream)
+        return stream.cuda_stream
 
     def _copy(self, pairs: Sequence[tuple[int, int]]) -> None:
         if not pairs:
@@ -269,7 +281,7 @@ class PagedKvCache:
                          keys.data_ptr(), values.data_ptr(), self._dtype(), batch.tokens, query.shape[1],
                          self.kv_heads, self.head_dim, 2 * inv_freq.numel(), int(interleaved), q_stride, k_stride,
                          v_stride, o_stride, self.num_pages, self.page_size, keys.stride(0), keys.stride(1),
-                         keys.stride(2), float(amplitude), self._stream())
+                         keys.stride(2), float(amplitude), self._use(batch))
         return out
 
     def attend(self, layer: int, batch: Batch, query: Any, *, scale: float | None = None, out: Any = None) -> Any:
@@ -283,7 +295,7 @@ class PagedKvCache:
         n = len(batch.sequences)
         nbytes = self.native.lib.kudacuda_paged_attention_workspace_bytes(
             batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads, self.head_dim)
-        stream = self._stream()
+        stream = self._use(batch)
         # a workspace a stream: calls on one stream follow one another; a captured call
         # gets its own, from its graph's memory
         workspace = None if self.torch.cuda.is_current_stream_capturing() else self._workspaces.get(stream)

@@ -30,12 +30,14 @@ CHANGES = {
         (dict(head_dim=258), "even head_dim"), (dict(rotary_dim=0), "rotary_dim"), (dict(rotary_dim=130), "rotary_dim"),
         (dict(rotary_dim=3), "rotary_dim"), (dict(interleaved=2), "interleaved"), (dict(input_stride=255), "strides"),
         (dict(output_stride=-256), "strides"), (dict(amplitude=float("nan")), "amplitude"),
-        (dict(inv_freq=P + 4), "aligned"), (dict(input=P + 1), "aligned")],
+        (dict(inv_freq=P + 4), "aligned"), (dict(input=P + 1), "aligned"), (dict(tokens=(1 << 25) + 1), "2^25"),
+        (dict(output_stride=512), "in place")],
     "kudacuda_rope_paged_append": [
         (dict(slots=0), "non-null"), (dict(value_pages=0), "non-null"), (dict(kv_heads=0), "kv_heads"),
         (dict(num_pages=0), "num_pages"), (dict(page_size=24), "power of two"), (dict(page_size=8192), "power of two"),
         (dict(key_stride=255), "strides"), (dict(value_stride=0), "strides"), (dict(token_stride=64), "pool strides"),
-        (dict(page_stride=-4096), "pool strides"), (dict(slots=P + 4), "aligned"), (dict(dtype=3), "dtype")],
+        (dict(page_stride=-4096), "pool strides"), (dict(slots=P + 4), "aligned"), (dict(dtype=3), "dtype"),
+        (dict(query_stride=768), "in place"), (dict(tokens=1 << 26), "2^25")],
     "kudacuda_paged_attention": [
         (dict(page_table=0), "non-null"), (dict(output=0), "non-null"), (dict(dtype=0), "dtype"),
         (dict(head_dim=96), "head_dim"), (dict(query_heads=5), "multiple of kv_heads"), (dict(kv_heads=0), "kv_heads"),
@@ -46,7 +48,8 @@ CHANGES = {
         (dict(max_kv_len=0), "max_kv_len"), (dict(query_stride=252), "strides"), (dict(token_stride=68), "strides"),
         (dict(head_stride=0), "strides"), (dict(query=P + 8), "16-byte"), (dict(workspace=P + 4), "16-byte"),
         (dict(kv_lens=P + 2), "16-byte"), (dict(workspace_bytes=-1), "workspace_bytes"), (dict(scale=0.0), "scale"),
-        (dict(output=P), "apart"),
+        (dict(output=P), "apart"), (dict(tokens=(1 << 25) + 1), "2^27"),
+        (dict(sequences=65536, query_heads=128, kv_heads=128), "2^22"),
         (dict(scale=float("inf")), "scale"), (dict(scale=-1.0), "scale")],
     "kudacuda_copy_pages": [
         (dict(pool=0), "non-null"), (dict(count=1), "non-null"), (dict(count=-1), "count"), (dict(pools=0), "pools"),
@@ -57,7 +60,7 @@ CHANGES = {
         (dict(pairs=[(0, 2), (1, 2)]), "differ"), (dict(pairs=[(0, 2), (2, 2)]), "differ"),
         (dict(pairs=[(0, 2), (2, 3)]), "source"), (dict(pairs=[(2, 3), (0, 2)]), "source"),
         (dict(pairs=[(0, 1), (1, 0)]), "source"), (dict(pairs=[(i, (i + 1) % 8) for i in range(8)]), "source"),
-        (dict(pairs=[(0, 1)] * 9), "count")],
+        (dict(pairs=[(0, 1)] * 9), "count"), (dict(pools=65536, page_bytes=1 << 22), "2^37")],
     "kudacuda_sample_tokens": [
         (dict(logits=0), "non-null"), (dict(random=0), "non-null"), (dict(tokens_out=0), "non-null"),
         (dict(workspace=0), "non-null"), (dict(dtype=3), "dtype"), (dict(rows=65536), "rows"), (dict(rows=-1), "rows"),

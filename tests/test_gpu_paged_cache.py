@@ -143,3 +143,32 @@ def test_forks_share_until_they_write_and_compaction_keeps_every_row(torch_gpu, 
     for s in list(truth):
         cache.free(s)
     assert cache.free_pages == 24
+
+
+def test_a_batch_of_another_stream_may_be_dropped_behind_its_calls(torch_gpu, native):
+    """Calls on a side stream with batches made on the first one: memory that takes a dropped batch's place is not theirs."""
+
+    from kudacuda_amd.paged_cache import PagedKvCache
+    from kudacuda_amd.rotary import rope_frequencies
+
+    cache = PagedKvCache(native, torch, layers=1, kv_heads=2, head_dim=64, num_pages=300)
+    freq = torch.from_numpy(rope_frequencies(64, 1e4)[0]).cuda()
+    first, second = cache.create(), cache.create()
+    q, k, v = (torch.randn((2000, h, 64), device="cuda:0").bfloat16() for h in (4, 2, 2))
+    busy = torch.randn((4096, 4096), device="cuda:0")
+    batch = cache.extend([first], [2000])
+    want = cache.attend(0, batch, cache.append(0, batch, q, k, v, freq))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy = (busy @ busy).clamp(-1, 1)  # the calls behind it start late
+    batch = cache.extend([second], [2000])
+    with torch.cuda.stream(side):
+        got = cache.attend(0, batch, cache.append(0, batch, q, k, v, freq))
+    sizes = [x.numel() * x.element_size() for x in (batch.slots, batch.positions, batch.kv_lens, batch.page_table)]
+    del batch
+    filled = [torch.full((n,), 0x7f, dtype=torch.uint8, device="cuda:0") for n in sizes for _ in range(8)]
+    side.synchronize()
+    assert torch.equal(got, want)
+    del filled
