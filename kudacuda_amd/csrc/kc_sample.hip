@@ -21,7 +21,7 @@
 //      largest of 128, below which no kept token lies);
 //   3. tokens of the deciding buckets to a list, sums of the surely kept tokens of
 //      each chunk of 2048 ids;
-//   4. one block a row: the list ordered, the last kept token, the chunk and in it
+//   4. one block a row: the last kept token of the list, the chunk and in it
 //      the token that u falls on.
 // The row is read by the first three (once from memory, then from the caches) and
 // one chunk of it by the last.  A logit is first compared with the least one that
@@ -807,6 +807,75 @@ __global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int
 }
 
 // ------------------------------------------------------------- the last launch
+// The order word of the first of the block's tokens (those of `in`), in order, up to
+// which their values reach the target, digit by digit from the first in which they
+// differ, until one is left; 0: it is never reached.
+template <int MINE>
+__device__ __forceinline__ uint64_t select_in_list(const uint64_t (&word)[MINE], const uint64_t (&value)[MINE], uint32_t in,
+                                                uint64_t before, uint64_t target, unsigned long long* s_bins,
+                                                uint32_t* s_counts, uint64_t* s_part) {
+    static_assert(kThreads == 256, "a thread a digit");
+    __shared__ uint64_t s_prefix, s_before;
+    __shared__ int s_found;  // tokens of the digit
+    uint64_t largest = 0;
+    uint64_t smallest = 0;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        largest = (in >> j & 1) != 0 ? max_u64(largest, word[j]) : largest;
+        smallest = (in >> j & 1) != 0 ? max_u64(smallest, ~word[j]) : smallest;
+    }
+    largest = block_max(largest, s_part);
+    smallest = ~block_max(smallest, s_part);
+    if (largest < smallest) {
+        return 0;  // none
+    }
+    int shift = largest == smallest ? 0 : 64 - __builtin_clzll(largest ^ smallest);
+    uint64_t prefix = largest >> shift;
+    do {
+        const int bits = shift >= 8 ? 8 : shift;
+        shift -= bits;
+        __syncthreads();
+        s_bins[threadIdx.x] = 0;
+        s_counts[threadIdx.x] = 0;
+        if (threadIdx.x == 0) {
+            s_found = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+            if ((in >> j & 1) != 0 && (word[j] >> shift) >> bits == prefix) {
+                const int digit = static_cast<int>(word[j] >> shift) & ((1 << bits) - 1);
+                atomicAdd(&s_bins[digit], static_cast<unsigned long long>(value[j]));
+                atomicAdd(&s_counts[digit], 1u);
+            }
+        }
+        __syncthreads();
+        // bins from the highest digit down: thread i holds digit last - i
+        const int digit = (1 << bits) - 1 - static_cast<int>(threadIdx.x);
+        const uint64_t mine = digit >= 0 ? s_bins[digit] : 0;
+        uint64_t total;
+        const uint64_t until = before + block_before<uint64_t>(mine, s_part, total);
+        if (until < target && until + mine >= target) {
+            s_prefix = prefix << bits | static_cast<uint64_t>(digit);
+            s_before = until;
+            s_found = static_cast<int>(s_counts[digit]);
+        }
+        __syncthreads();
+        if (s_found == 0) {
+            return 0;
+        }
+        prefix = s_prefix;
+        before = s_before;
+    } while (shift > 0 && s_found > 1);
+    // the one that has these digits
+    uint64_t found = 0;
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        found = (in >> j & 1) != 0 && word[j] >> shift == prefix ? word[j] : found;
+    }
+    return block_max(found, s_part);
+}
+
 // Where more tokens than the list holds share the deciding buckets (flat rows):
 // the order word of the first token, in order, up to which the count (k > 0) or the
 // weight over buckets [low, high] reaches the target, digit by digit over the whole row;
@@ -872,7 +941,8 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     __shared__ uint64_t s_list[kList];
     __shared__ uint64_t s_weights[kThreads];
     __shared__ unsigned long long s_sums[kMaxChunks];
-    __shared__ unsigned long long s_bins[256];
+    __shared__ unsigned long long s_bins[kThreads];
+    __shared__ uint32_t s_counts[kThreads];
     __shared__ double s_powers[kUnits];
     __shared__ uint64_t s_last, s_rest;
     __shared__ int s_chunk;
@@ -941,78 +1011,40 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
             last = max_u64(last, ~block_max(under ? ~word : 0, s_part));
         }
     } else if (n > 0 && n <= kList) {
-        // the list in order: a bitonic network over the next power of two
-        int size = 2 * kThreads;
-        while (size < n) {
-            size *= 2;
-        }
-        for (int i = tid; i < kList; i += kThreads) {
-            s_list[i] = i < n ? s.list[i] : 0;
-        }
-        for (int width = 2; width <= size; width *= 2) {
-            for (int step = width / 2; step >= 1; step /= 2) {
-                __syncthreads();
-                for (int i = tid; i < size / 2; i += kThreads) {
-                    const int x = 2 * i - (i & (step - 1));
-                    const int y = x + step;
-                    const bool down = (x & width) == 0;
-                    const uint64_t v = s_list[x];
-                    const uint64_t w = s_list[y];
-                    if ((v < w) == down) {
-                        s_list[x] = w;
-                        s_list[y] = v;
-                    }
-                }
-            }
-        }
+        uint64_t word[kMine], weight[kMine];
+        uint32_t in_k = 0;
+        uint32_t in_p = 0;
         __syncthreads();
-        uint64_t weight[kMine];
-        bool in_k[kMine], in_p[kMine];
-        uint32_t k_mine = 0;
-        uint64_t p_mine = 0;
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-            const int i = kMine * tid + j;
-            const double depth = i < n ? depth_of(r, order_logit(s_list[i])) : 0.0;
+            const int i = j * kThreads + tid;
+            word[j] = i < n ? s.list[i] : 0;
+            s_list[i] = word[j];
+            const double depth = i < n ? depth_of(r, order_logit(word[j])) : 0.0;
             weight[j] = i < n ? weight_of(depth, s_powers) : 0;
             const int b = i < n ? bucket_of(depth) : -1;
-            in_k[j] = b == d.k_bucket;
-            in_p[j] = b >= d.low && b <= d.high;
-            k_mine += in_k[j] ? 1 : 0;
-            p_mine += in_p[j] ? weight[j] : 0;
+            in_k |= b == d.k_bucket ? 1u << j : 0u;
+            in_p |= b >= d.low && b <= d.high ? 1u << j : 0u;
         }
         uint64_t k_weight = d.k_weight;
         if (d.k_bucket < kBuckets) {
-            uint32_t all;
-            int place = d.k_count + static_cast<int>(block_before<uint32_t>(k_mine, s_part, all));
+            uint64_t one[kMine];
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                one[j] = 1;
+            }
+            last = select_in_list<kMine>(word, one, in_k, static_cast<uint64_t>(d.k_count), static_cast<uint64_t>(r.k), s_bins,
+                                         s_counts, s_part);
             uint64_t mine = 0;
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
-                if (in_k[j]) {
-                    mine += place < r.k ? weight[j] : 0;
-                    if (place + 1 == r.k) {
-                        s_last = s_list[kMine * tid + j];
-                    }
-                    ++place;
-                }
+                mine += (in_k >> j & 1) != 0 && word[j] >= last ? weight[j] : 0;
             }
             k_weight += block_sum(mine, s_part);
         }
-        __syncthreads();
-        last = s_last;
         if (r.p < 1.0) {
-            const uint64_t target = top_p_end(r, k_weight);
-            uint64_t all;
-            uint64_t before = d.low_weight + block_before<uint64_t>(p_mine, s_part, all);
-            uint64_t mine = ~uint64_t{0};
-#pragma unroll
-            for (int j = 0; j < kMine; ++j) {
-                if (in_p[j]) {
-                    mine = before < target ? s_list[kMine * tid + j] : mine;
-                    before += weight[j];
-                }
-            }
-            last = max_u64(last, ~block_max(~mine, s_part));
+            last = max_u64(last, select_in_list<kMine>(word, weight, in_p, d.low_weight, top_p_end(r, k_weight), s_bins,
+                                                       s_counts, s_part));
         }
     } else if (n > kList) {
         __syncthreads();
