@@ -46,10 +46,16 @@ static_assert(kBuckets % kCoarse == 0 && kBuckets / kCoarse <= 64, "the sums fit
 constexpr int kList = 2048;           // most tokens that are ordered in LDS
 constexpr int kWeightBits = 42;
 // Blocks of the first and third launch, and large blocks of the second: more rows than
-// fill these take more chunks a block (128 rows of mixed settings: 2048 and 256 87 us,
-// 2048 and 512 90, 1280 and 256 88; 32 rows with top-p: 256 large blocks 50 us, 512 61).
+// fill these take more chunks a block (128 rows of mixed settings in their own order: 2048 and
+// 256 87 us, 2048 and 512 90, 1280 and 256 88; 32 rows with top-p: 256 large blocks 50 us, 512 61).
 constexpr int64_t kBlocks = 2048;
 constexpr int64_t kLargeBlocks = 256;
+// From so many rows on the rows with the most work start first, and the second launch's
+// blocks go to the rows that have work there, two to a row of which all logits count for
+// one to a row of few (128 rows of mixed settings: in their own order 82 us, so 74, three
+// to one 79; 256 133 and 109; 32 42.9 and 43.4; 64 rows of one setting alone 64 and 65).
+constexpr int64_t kOrderedRows = 64;
+constexpr int kDenseShare = 2;
 constexpr int kMaxChunks = static_cast<int>(kSampleMaxVocab / kChunk);
 constexpr int kIdBits = 20;
 constexpr uint64_t kIdMask = (uint64_t{1} << kIdBits) - 1;
@@ -274,6 +280,21 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
     return r;
 }
 __device__ __forceinline__ bool decides(const Row& r) { return r.k > 0 || r.p < 1.0; }
+// Top-k that the largest logits of 128 ids each bound.
+__device__ __forceinline__ bool bounded(const Row& r, int chunks) { return r.k > 0 && r.k <= chunks * kGroups; }
+
+// Rows by the work that the second and third launch have with them, behind all rows'
+// workspaces: where each class ends, then the rows class by class.
+constexpr int kClasses = 4;  // all logits in both; all in the third alone; few; none
+__device__ __forceinline__ int32_t* row_order(const SampleArgs& a, int chunks) {
+    return reinterpret_cast<int32_t*>(a.workspace + a.rows * row_bytes(chunks));
+}
+__device__ __forceinline__ int class_of(const Row& r, int chunks) {
+    if (r.greedy) {
+        return 3;
+    }
+    return bounded(r, chunks) ? 2 : (decides(r) ? 0 : 1);
+}
 
 __device__ __forceinline__ void set_top(Row& r, uint64_t best) {
     r.top = order_logit(best);
@@ -457,9 +478,64 @@ __device__ __forceinline__ int chunks_end(int chunks, int per) {
 }
 
 // ---------------------------------------------------------------- launches
+// By the first launch's first block.
+__device__ __forceinline__ void write_order(const SampleArgs& a, int chunks) {
+    __shared__ int s_total[kClasses];
+    __shared__ int s_count[kWaves][kClasses];
+    const int rows = static_cast<int>(a.rows);
+    const int tid = static_cast<int>(threadIdx.x);
+    int32_t* const order = row_order(a, chunks);
+    if (tid < kClasses) {
+        s_total[tid] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < rows; i += kThreads) {
+        atomicAdd(&s_total[class_of(row_of(a, i), chunks)], 1);
+    }
+    __syncthreads();
+    int at[kClasses];
+    int end = 0;
+#pragma unroll
+    for (int c = 0; c < kClasses; ++c) {
+        at[c] = end;
+        end += s_total[c];
+        if (tid == 0) {
+            order[c] = end;
+        }
+    }
+    for (int i0 = 0; i0 < rows; i0 += kThreads) {
+        const int mine = i0 + tid < rows ? class_of(row_of(a, i0 + tid), chunks) : -1;
+        int place = 0;
+#pragma unroll
+        for (int c = 0; c < kClasses; ++c) {
+            const uint64_t same = __ballot(mine == c);
+            if ((tid & 63) == 0) {
+                s_count[tid >> 6][c] = __builtin_popcountll(same);
+            }
+            place = mine == c ? at[c] + __builtin_popcountll(same & ((uint64_t{1} << (tid & 63)) - 1)) : place;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kClasses; ++c) {
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                place += mine == c && w < (tid >> 6) ? s_count[w][c] : 0;
+                at[c] += s_count[w][c];
+            }
+        }
+        if (mine >= 0) {
+            order[kClasses + place] = i0 + tid;
+        }
+        __syncthreads();
+    }
+}
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int chunks, int per) {
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int chunks, int per, bool ordered) {
     __shared__ uint64_t s_part[kWaves];
+    if (ordered && blockIdx.x == 0 && blockIdx.y == 0) {
+        write_order(a, chunks);
+    }
     const int64_t row = blockIdx.y;
     const RowSpace s = row_space(a.workspace, row, chunks);
     const int blocks = static_cast<int>(gridDim.x);
@@ -514,32 +590,60 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, int 
 constexpr int kLarge = 1024;
 
 template <typename T>
-__global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, int chunks, int per, int max_blocks) {
+__global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, int chunks, int per, int max_blocks,
+                                                                bool ordered) {
     constexpr int kStride = kLarge / kThreads;
     __shared__ unsigned long long s_weights[kBuckets];
     __shared__ uint32_t s_counts[kBuckets];
     __shared__ uint64_t s_part[kLarge / 64];
     __shared__ double s_powers[kUnits];
     __shared__ int s_limit;
-    const int64_t row = blockIdx.y;
+    int64_t row = blockIdx.y;
+    int part = static_cast<int>(blockIdx.x);
+    if (ordered) {
+        // (no more parts than blocks and, of one part each, rows: the grid has both)
+        const int32_t* const order = row_order(a, chunks);
+        const int dense = order[0];
+        const int sparse = order[2] - order[1];
+        const int total = kDenseShare * dense + sparse;
+        const int blocks = static_cast<int>(gridDim.x - a.rows);
+        const int most = (chunks + kStride - 1) / kStride;
+        const auto parts_of = [&](int n) {
+            const int v = total > 0 ? blocks * n / total : 1;
+            return v < 1 ? 1 : (v < most ? v : most);
+        };
+        const int dense_parts = parts_of(kDenseShare);
+        const bool is_dense = part < dense * dense_parts;
+        const int parts = is_dense ? dense_parts : parts_of(1);
+        const int place = is_dense ? part : part - dense * dense_parts;
+        if (!is_dense && place >= sparse * parts) {
+            return;
+        }
+        row = order[kClasses + (is_dense ? 0 : order[1]) + place / parts];
+        part = place % parts;
+        per = ((chunks + parts - 1) / parts + kStride - 1) / kStride * kStride;
+        if (part * per >= chunks) {
+            return;
+        }
+    }
     Row r = row_of(a, row);
     if (r.greedy || !decides(r)) {
         return;
     }
     const auto* const logits = row_logits<T>(a, row);
-    const int begin = static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / kThreads;
-    const int end = chunks_end(chunks, per);
+    const int begin = part * per + static_cast<int>(threadIdx.x) / kThreads;
+    const int end = (part + 1) * per < chunks ? (part + 1) * per : chunks;
     const Round<T> round = load_round<T, kStride>(logits, a.vocab, begin, end);
     const RowSpace s = row_space(a.workspace, row, chunks);
     const uint64_t best = load_best(s, max_blocks);
     const int groups = chunks * kGroups;
-    const bool bounded = r.k > 0 && r.k <= groups;
+    const bool by_groups = bounded(r, chunks);
     constexpr int kHeld = 2;  // largest logits of a thread that are requested at once
     float largest[kHeld];
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int at = i * kLarge + static_cast<int>(threadIdx.x);
-        largest[i] = bounded && at < groups ? s.largest[at] : -__builtin_huge_valf();
+        largest[i] = by_groups && at < groups ? s.largest[at] : -__builtin_huge_valf();
     }
     for (int i = threadIdx.x; i < kBuckets; i += kLarge) {
         s_weights[i] = 0;
@@ -548,7 +652,7 @@ __global__ __launch_bounds__(kLarge) void sample_buckets_kernel(SampleArgs a, in
     load_powers(s_powers);
     set_top(r, block_max<kLarge / 64>(best, s_part));
     int limit = kDepth;
-    if (bounded) {
+    if (by_groups) {
         // k of the groups' largest logits are at least the k-th of them: the k-th token
         // lies no deeper
         if (threadIdx.x == 0) {
@@ -709,13 +813,14 @@ __device__ __forceinline__ bool listed_bucket(const Decision& d, int b) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int chunks, int per, int max_blocks) {
+__global__ __launch_bounds__(kThreads) void sample_sums_kernel(SampleArgs a, int chunks, int per, int max_blocks, bool ordered) {
     __shared__ uint64_t s_part[kWaves];
     __shared__ uint64_t s_list[kList];
     __shared__ uint64_t s_sums[kWaves * kAhead];
     __shared__ double s_powers[kUnits];
     __shared__ uint32_t s_listed, s_at;
-    const int64_t row = blockIdx.y;
+    // rows with the most work start first
+    const int64_t row = ordered ? row_order(a, chunks)[kClasses + blockIdx.y] : static_cast<int64_t>(blockIdx.y);
     Row r = row_of(a, row);
     const RowSpace s = row_space(a.workspace, row, chunks);
     if (r.greedy && blockIdx.x != 0) {
@@ -1153,14 +1258,17 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
     const int per = share(kBlocks, 1);
     const int large = share(kLargeBlocks, kLarge / kThreads);
     const int blocks = static_cast<int>(grid(per).x);
-    hipLaunchKernelGGL(sample_max_kernel<T>, grid(per), dim3(kThreads), 0, stream, a, chunks, per);
+    const bool ordered = a.rows >= kOrderedRows;
+    hipLaunchKernelGGL(sample_max_kernel<T>, grid(per), dim3(kThreads), 0, stream, a, chunks, per, ordered);
     hipError_t status = hipGetLastError();
     if (status == hipSuccess && (a.top_k != nullptr || a.top_p != nullptr)) {
-        hipLaunchKernelGGL(sample_buckets_kernel<T>, grid(large), dim3(kLarge), 0, stream, a, chunks, large, blocks);
+        const dim3 shared(static_cast<unsigned>(kLargeBlocks + a.rows));
+        hipLaunchKernelGGL(sample_buckets_kernel<T>, ordered ? shared : grid(large), dim3(kLarge), 0, stream, a, chunks, large,
+                           blocks, ordered);
         status = hipGetLastError();
     }
     if (status == hipSuccess) {
-        hipLaunchKernelGGL(sample_sums_kernel<T>, grid(per), dim3(kThreads), 0, stream, a, chunks, per, blocks);
+        hipLaunchKernelGGL(sample_sums_kernel<T>, grid(per), dim3(kThreads), 0, stream, a, chunks, per, blocks, ordered);
         status = hipGetLastError();
     }
     if (status == hipSuccess) {
@@ -1174,7 +1282,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
 
 int64_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
     const int64_t bytes = row_bytes((vocab + kChunk - 1) / kChunk);
-    return rows * bytes;
+    return rows * bytes + (kClasses + rows + 3) / 4 * 16;
 }
 
 hipError_t launch_sample(int dtype, const SampleArgs& a, hipStream_t stream) {

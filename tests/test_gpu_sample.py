@@ -65,6 +65,7 @@ def _logits(rng, rows, vocab, dtype, std=2.5, pitch=None, shift=0):
 @pytest.mark.parametrize("rows,vocab,pitch,shift", [
     (1, 1, None, 0), (3, 2, None, 0), (5, 7, 9, 1), (4, 2047, None, 0), (4, 2048, 2056, 0), (3, 2049, 2051, 3),
     (6, 32000, None, 0), (2, 151936, None, 0), (40, 5000, 5008, 8), (2, 1 << 20, None, 0), (2000, 33, None, 0),
+    (63, 4100, None, 0), (64, 9000, None, 0), (300, 5000, 5003, 3),
 ])
 def test_settings_row_by_row(torch_gpu, native, dtype, rows, vocab, pitch, shift):
     """Every row its own mix of settings, off and degenerate ones among them."""
