@@ -650,8 +650,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 // random, next to the result's own half step (2-norm error of a prompt of 8192 bf16
 // tokens 2.1e-3, 1.9e-3 with a maximum that never lags at 284 us for 265, of the
 // result's rounding alone 1.6e-3); a second part of each weight would cost half as many
-// products again.  Measured, 8192 tokens of 16 heads over 2
-// KV heads: 346 us at first, 318 with loads that bypass the compiler's waits, 293
+// products again.  Measured, 8192 tokens of 16 heads over 2 KV heads: 346 us at first, 318 with loads that bypass the compiler's waits, 293
 // with operands read ahead and the maximum allowed to lag, 287 with page bases as
 // scalars, 262 with the waves' priorities and the order of blocks (1050 TFLOP/s; a
 // library product of 8192^3 1405).  Forming the next window's scores between this
