@@ -313,3 +313,20 @@ def test_cache_calls_captured_twice_do_not_share_a_workspace(torch_gpu, native):
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
         assert torch.equal(cache.attend(0, batches[0], q[0]), want[0])
         torch.cuda.synchronize()
+
+
+@hints
+@pytest.mark.parametrize("new,kv,heads", [
+    ([1], [5000], 16), ([1] * 40, [900, 3, 64, 0, 2000] * 8, 8), ([3, 4, 1] * 20, [700, 30, 2500] * 20, 8), ([700], [900], 4),
+    ([90, 1, 1], [1200, 7000, 40], 16)])
+def test_calls_stay_inside_their_workspace(torch_gpu, native, new, kv, heads, hint):
+    """Of the told size and of less."""
+
+    batch = Paged(19, new, kv, heads=heads, dim=128)
+    batch.hint = hint
+    d = batch.device()
+    full = native.lib.kudacuda_paged_attention_workspace_bytes(batch.tokens, len(new), max(new), hint or max(kv), heads, 2, 128)
+    for nbytes in (full, full // 2 // 16 * 16, full // 5 // 16 * 16):
+        workspace = torch.full((nbytes + 4096,), 0x7f, dtype=torch.uint8, device="cuda:0")
+        _check(batch, batch.call(native, d, workspace=workspace, nbytes=nbytes))
+        assert (workspace[nbytes:] == 0x7f).all()

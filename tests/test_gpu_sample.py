@@ -165,11 +165,12 @@ def test_draws_follow_the_distribution(torch_gpu, native):
     assert np.abs(chances - share[tokens]).max() <= 1e-6
 
 
-def test_captured_call_without_chances_on_another_stream(torch_gpu, native):
+@pytest.mark.parametrize("rows", [6, 70])
+def test_captured_call_without_chances_on_another_stream(torch_gpu, native, rows):
     """Replays read new logits, numbers and settings; the workspace is not cleared between them."""
 
     rng = np.random.default_rng(14)
-    rows, vocab = 6, 30000
+    vocab = 30000
     logits = _logits(rng, rows, vocab, torch.bfloat16)
     u, temperature, top_p, min_p = (torch.zeros(rows, device="cuda:0") for _ in range(4))
     top_k = torch.zeros(rows, dtype=torch.int32, device="cuda:0")
@@ -197,3 +198,22 @@ def test_captured_call_without_chances_on_another_stream(torch_gpu, native):
         eager, chances = _call(native, logits, numbers, **values)
         assert np.array_equal(tokens.cpu().numpy(), eager)
         _check(logits, (eager, chances), numbers, **values, least=0.6)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 64, 301])
+@pytest.mark.parametrize("vocab", [1, 2049, 40000])
+def test_calls_stay_inside_their_workspace(torch_gpu, native, rows, vocab):
+    rng = np.random.default_rng([15, rows, vocab])
+    logits = _logits(rng, rows, vocab, torch.float16, std=0.5)
+    u = torch.from_numpy(rng.random(rows).astype(np.float32)).cuda()
+    top_k = torch.from_numpy(rng.choice([0, 3, 500, 30000], rows).astype(np.int32)).cuda()
+    top_p = torch.from_numpy(rng.choice([0.4, 0.97, 1.0], rows).astype(np.float32)).cuda()
+    tokens = torch.full((rows + 1,), -5, dtype=torch.int32, device="cuda:0")
+    nbytes = native.lib.kudacuda_sample_workspace_bytes(rows, vocab)
+    workspace = torch.full((nbytes + 4096,), 0x7f, dtype=torch.uint8, device="cuda:0")
+    native.call("kudacuda_sample_tokens", logits.data_ptr(), u.data_ptr(), 0, top_k.data_ptr(), top_p.data_ptr(), 0,
+                tokens.data_ptr(), 0, workspace.data_ptr(), nbytes, 2, rows, vocab, vocab,
+                torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert (workspace[nbytes:] == 0x7f).all()
+    assert (tokens[:-1] >= 0).all() and (tokens[:-1] < vocab).all() and int(tokens[-1]) == -5
