@@ -113,7 +113,8 @@ class Native:
 
     def __init__(self, device_id: int = 0, lib: ctypes.CDLL | None = None) -> None:
         self.lib = lib or load_library()
-        self.handle = self.lib.kudacuda_create(int(device_id))
+        self.device_id = int(device_id)
+        self.handle = self.lib.kudacuda_create(self.device_id)
         if not self.handle:
             raise NativeError("kudacuda_create returned a null handle")
         self.check(self.lib.kudacuda_freeze(self.handle), "kudacuda_freeze")

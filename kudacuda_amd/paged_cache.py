@@ -66,6 +66,11 @@ class PagedKvCache:
             raise ValueError("page_size must be a power of two, 1..4096")
         if min(layers, kv_heads, head_dim, num_pages) < 1 or head_dim % 8 != 0:
             raise ValueError("layers, kv_heads and num_pages must be positive, head_dim a multiple of 8")
+        place = torch.device(device)
+        if isinstance(native, Native):
+            index = torch.cuda.current_device() if place.type == "cuda" and place.index is None else place.index
+            if place.type != "cuda" or index != native.device_id:
+                raise ValueError(f"a cache on {place} needs a handle of that GPU, not of cuda:{native.device_id}")
         self.native = native
         self.torch = torch
         self.layers = int(layers)

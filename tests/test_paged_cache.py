@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+from kudacuda_amd._native import Native
 from kudacuda_amd.paged_cache import OutOfPages, PagedKvCache
 from kudacuda_amd.rotary import rope_frequencies
 
@@ -206,3 +207,11 @@ def test_rotary_frequencies():
 def test_rotary_refusals(bad):
     with pytest.raises(ValueError):
         rope_frequencies(**(dict(rotary_dim=64) | bad))
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda:1"])
+def test_a_cache_lies_on_its_handles_device(device):
+    native = Native.__new__(Native)
+    native.handle, native.device_id = None, 0
+    with pytest.raises(ValueError, match="cuda:0"):
+        PagedKvCache(native, torch, layers=1, kv_heads=1, head_dim=8, num_pages=1, device=device)
