@@ -246,15 +246,15 @@ __device__ __forceinline__ void tell_splits(const PagedAttnArgs& a, const Sequen
 }
 
 // ------------------------------------------------------------------ few rows
-// Sequences of which a KV head has at most kFewRows rows, the form of single tokens:
-// bound by the cache's bytes.  All blocks share the cached rows of all sequences
+// Sequences of which a KV head has at most kFewRows rows, many and long ones (the plan
+// says which): single tokens, bound by the cache's bytes.  All blocks share the cached rows of all sequences
 // evenly: the work is the line of (sequence, KV head, tile of 16 rows, round of 128
 // keys), cut into one stretch a block, so a batch of unequal lengths ends everywhere
 // at once (64 sequences of up to 8192 tokens, 307 MB: 70 us, 4.4 TB/s; with a fixed
 // number of splits a sequence 88).  In a round the four waves take 32 keys each, K
 // straight from memory into the first product's operand, V through the wave's own LDS,
 // the next keys requested as soon as the registers of these are free.  With more rows
-// the keys were read once a tile of 16, and the row tiles below are faster: 32 rows of
+// the keys would be read once a tile of 16, and the row tiles below are faster: 32 rows of
 // 64 sequences of 2000 keys 58 us here and 37 there, of 8192 keys at most 104 and 98, of
 // one with 120000 55 and 34; of 64 with 100 keys 9.9 and 11.7.
 constexpr int kFewRows = 16;
