@@ -15,6 +15,8 @@
 // the same order: the weights never leave their lane.  V's rows go to LDS as they
 // are and are read transposed (ds_read_b64_tr_b16: a group of 16 lanes reads 4
 // keys x 16 dims and each lane receives the 4 keys of one dim).
+#include <type_traits>
+
 #include "kc_device.h"
 #include "kc_kernels.h"
 
@@ -650,12 +652,20 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 // random, next to the result's own half step (2-norm error of a prompt of 8192 bf16
 // tokens 2.1e-3, 1.9e-3 with a maximum that never lags at 284 us for 265, of the
 // result's rounding alone 1.6e-3); a second part of each weight would cost half as many
-// products again.  Measured, 8192 tokens of 16 heads over 2 KV heads: 346 us at first, 318 with loads that bypass the compiler's waits, 293
-// with operands read ahead and the maximum allowed to lag, 287 with page bases as
-// scalars, 262 with the waves' priorities and the order of blocks (1050 TFLOP/s; a
-// library product of 8192^3 1405).  Forming the next window's scores between this
+// products again.  Measured, 8192 tokens of 16 heads over 2 KV heads: 346 us at first,
+// 318 with loads that bypass the compiler's waits, 293 with operands read ahead and the
+// maximum allowed to lag, 287 with page bases as scalars, 262 with the waves' priorities
+// and the order of blocks (1050 TFLOP/s; a library product of 8192^3 1405).  Forming the next window's scores between this
 // window's weights (250 VGPRs) took 293.
+//
+// Sequences of at most kFineRows rows a KV head (single tokens, drafts) are one wave's
+// columns: their products have room, and their weights keep both 16-bit parts, as in the
+// kernel for few rows (16 bits of the fp32 weight in bf16, 22 in fp16); their sum adds
+// them as they are.  What that costs is forming the second parts, fp32 arithmetic of one
+// wave: a token over 2000 keys 14.2 us (one part: 13.4), over 120000 33.4 (32.1), 16
+// over up to 4000 20.8 (18.8), two chunks of 256 beside 8 tokens 35 (30).
 constexpr int kTileRows = 128;
+constexpr int kFineRows = 32;
 constexpr int kWindow = 64;
 
 // 16 bytes a lane from base + offset straight into LDS, lane after lane from `lds`.
@@ -848,136 +858,153 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
         fetch(w_begin + group, 0);
         look(w_begin + group + GROUPS);
     }
-    int buffer = 0;
-    for (int w0 = w_begin; w0 < w_end; w0 += GROUPS, buffer ^= 1) {
-        const int w = w0 + group;
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the window is in LDS
-        __syncthreads();
-        if (w + GROUPS < w_end) {
-            fetch(w + GROUPS, buffer ^ 1);
-            look(w + 2 * GROUPS);
-        }
-        const int key0 = w * kWindow;
-        if (w >= w_end || key0 > last_pos) {
-            continue;  // no window for this group, or no column of this wave sees it
-        }
-        const uint8_t* const s_k = s_mem[group][buffer];
-        const uint8_t* const s_v = s_k + kTileBytes;
-        const auto read_k = [&](uint4 (&k)[2], int i) __attribute__((always_inline)) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int row = 32 * t + r;
-                const int piece = (2 * i + q) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
-                k[t] = *reinterpret_cast<const uint4*>(s_k + row * kRowBytes + piece * 16);
+    const auto sweep = [&](auto parts) __attribute__((always_inline)) {
+        constexpr bool kFine = decltype(parts)::value == 2;
+        int buffer = 0;
+        for (int w0 = w_begin; w0 < w_end; w0 += GROUPS, buffer ^= 1) {
+            const int w = w0 + group;
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the window is in LDS
+            __syncthreads();
+            if (w + GROUPS < w_end) {
+                fetch(w + GROUPS, buffer ^ 1);
+                look(w + 2 * GROUPS);
             }
-        };
-        const auto read_v = [&](uint4& v, int n, int i) __attribute__((always_inline)) {
-            uint2 part[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                // 16 lanes: keys 16 n + 8 t + 4 q .. + 3, dims 32 i + 16 (lane / 16 % 2) .. + 15
-                const int row = 16 * n + 8 * t + 4 * q + (lane & 15) / 4;
-                const int piece = (4 * i + 2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^
-                                  (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
-                part[t] = read_transposed(s_v + row * kRowBytes + piece * 16 + (lane & 1) * 8);
+            const int key0 = w * kWindow;
+            if (w >= w_end || key0 > last_pos) {
+                continue;  // no window for this group, or no column of this wave sees it
             }
-            v = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
-        };
-        // operands are read ahead of their products, held there by the scheduling
-        // barriers; a wave that multiplies goes before one that does arithmetic
-        floatx16 sc[2] = {floatx16{}, floatx16{}};
-        constexpr int kAhead = D == 128 ? 2 : 1;
-        uint4 kf[kAhead + 1][2], vf[D / 32];
+            const uint8_t* const s_k = s_mem[group][buffer];
+            const uint8_t* const s_v = s_k + kTileBytes;
+            const auto read_k = [&](uint4 (&k)[2], int i) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            read_k(kf[i], i);
-        }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            if (i + kAhead < kSteps) {
-                read_k(kf[(i + kAhead) % (kAhead + 1)], i + kAhead);
-            }
-            if (i + 2 >= kSteps) {
-#pragma unroll
-                for (int d = 0; d < D / 64; ++d) {
-                    read_v(vf[(i + 2 - kSteps) * (D / 64) + d], 0, (i + 2 - kSteps) * (D / 64) + d);
+                for (int t = 0; t < 2; ++t) {
+                    const int row = 32 * t + r;
+                    const int piece = (2 * i + q) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
+                    k[t] = *reinterpret_cast<const uint4*>(s_k + row * kRowBytes + piece * 16);
                 }
-            }
+            };
+            const auto read_v = [&](uint4& v, int n, int i) __attribute__((always_inline)) {
+                uint2 part[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                sc[t] = mfma32(T{}, kf[i % (kAhead + 1)][t], qf[i], sc[t]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        __builtin_amdgcn_s_setprio(0);
-        // sc[t][e]: key 32 t + 8 (e / 4) + 4 q + e % 4 of the window
-        if (__builtin_amdgcn_readfirstlane(static_cast<int>(key0 + kWindow > first_pos + 1)) != 0) {
-            const int rel = pos - key0 - 4 * q;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    sc[t][e] = 32 * t + 8 * (e / 4) + e % 4 <= rel ? sc[t][e] : kNegInf;
+                for (int t = 0; t < 2; ++t) {
+                    // 16 lanes: keys 16 n + 8 t + 4 q .. + 3, dims 32 i + 16 (lane / 16 % 2) .. + 15
+                    const int row = 16 * n + 8 * t + 4 * q + (lane & 15) / 4;
+                    const int piece = (4 * i + 2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^
+                                      (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
+                    part[t] = read_transposed(s_v + row * kRowBytes + piece * 16 + (lane & 1) * 8);
                 }
+                v = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+            };
+            // operands are read ahead of their products, held there by the scheduling
+            // barriers; a wave that multiplies goes before one that does arithmetic
+            floatx16 sc[2] = {floatx16{}, floatx16{}};
+            constexpr int kAhead = D == 128 ? 2 : 1;
+            uint4 kf[kAhead + 1][2], vf[D / 32];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                read_k(kf[i], i);
             }
-        }
-        float mx = kNegInf;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                mx = fmaxf(mx, sc[t][e]);
-            }
-        }
-        // the maximum may lag behind by 2^8 (weights up to 256 are as exact): sums are
-        // rescaled a few times a row, not in every window
-        const float m_new = fmaxf(m_run, halves_max(mx) * a.scale_log2);
-        if (__any(m_new > m_run + 8.0f)) {
-            const float corr = __builtin_amdgcn_exp2f(m_run - (m_new == kNegInf ? 0.0f : m_new));
-            l_run *= corr;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    acc[i][e] *= corr;
+            for (int i = 0; i < kSteps; ++i) {
+                if (i + kAhead < kSteps) {
+                    read_k(kf[(i + kAhead) % (kAhead + 1)], i + kAhead);
                 }
-            }
-            m_run = m_new;
-        }
-        const float m_sub = m_run == kNegInf ? 0.0f : m_run;
-        // steps of 16 keys: the lane's weights of scores 8 (n % 2) .. + 7 of half n / 2;
-        // between the products of a step the next step's weights are formed and its V read
-        uint32_t p[2][4];
-        const auto weights = [&](int n, int e) __attribute__((always_inline)) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e], a.scale_log2, -m_sub));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e + 1], a.scale_log2, -m_sub));
-            p[n & 1][e] = pack(T{}, p0, p1);
-            l_run = add_pair(T{}, p[n & 1][e], l_run);
-        };
+                if (i + 2 >= kSteps) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            weights(0, e);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const uint4 pf = make_uint4(p[n & 1][0], p[n & 1][1], p[n & 1][2], p[n & 1][3]);
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                acc[i] = mfma32(T{}, vf[i], pf, acc[i]);
-                if (n < 3) {
-#pragma unroll
-                    for (int e = 0; e < 128 / D; ++e) {
-                        weights(n + 1, i * (128 / D) + e);
+                    for (int d = 0; d < D / 64; ++d) {
+                        read_v(vf[(i + 2 - kSteps) * (D / 64) + d], 0, (i + 2 - kSteps) * (D / 64) + d);
                     }
-                    read_v(vf[i], n + 1, i);
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    sc[t] = mfma32(T{}, kf[i % (kAhead + 1)][t], qf[i], sc[t]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
+            // sc[t][e]: key 32 t + 8 (e / 4) + 4 q + e % 4 of the window
+            if (__builtin_amdgcn_readfirstlane(static_cast<int>(key0 + kWindow > first_pos + 1)) != 0) {
+                const int rel = pos - key0 - 4 * q;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        sc[t][e] = 32 * t + 8 * (e / 4) + e % 4 <= rel ? sc[t][e] : kNegInf;
+                    }
+                }
+            }
+            float mx = kNegInf;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    mx = fmaxf(mx, sc[t][e]);
+                }
+            }
+            // the maximum may lag behind by 2^8 (weights up to 256 are as exact): sums are
+            // rescaled a few times a row, not in every window
+            const float m_new = fmaxf(m_run, halves_max(mx) * a.scale_log2);
+            if (__any(m_new > m_run + 8.0f)) {
+                const float corr = __builtin_amdgcn_exp2f(m_run - (m_new == kNegInf ? 0.0f : m_new));
+                l_run *= corr;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        acc[i][e] *= corr;
+                    }
+                }
+                m_run = m_new;
+            }
+            const float m_sub = m_run == kNegInf ? 0.0f : m_run;
+            // steps of 16 keys: the lane's weights of scores 8 (n % 2) .. + 7 of half n / 2;
+            // between the products of a step the next step's weights are formed and its V read
+            uint32_t p[2][4], rest[2][kFine ? 4 : 1];
+            const auto weights = [&](int n, int e) __attribute__((always_inline)) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e], a.scale_log2, -m_sub));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[n / 2][8 * (n % 2) + 2 * e + 1], a.scale_log2, -m_sub));
+                p[n & 1][e] = pack(T{}, p0, p1);
+                if constexpr (kFine) {
+                    rest[n & 1][e] = pack(T{}, p0 - low<T>(p[n & 1][e]), p1 - high<T>(p[n & 1][e]));
+                    l_run += p0 + p1;
+                } else {
+                    l_run = add_pair(T{}, p[n & 1][e], l_run);
+                }
+            };
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                weights(0, e);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint4 pf = make_uint4(p[n & 1][0], p[n & 1][1], p[n & 1][2], p[n & 1][3]);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    acc[i] = mfma32(T{}, vf[i], pf, acc[i]);
+                    if constexpr (kFine) {
+                        const uint32_t(&x)[4] = rest[n & 1];
+                        acc[i] = mfma32(T{}, vf[i], make_uint4(x[0], x[1], x[2], x[3]), acc[i]);
+                    }
+                    if (n < 3) {
+#pragma unroll
+                        for (int e = 0; e < 128 / D; ++e) {
+                            weights(n + 1, i * (128 / D) + e);
+                        }
+                        read_v(vf[i], n + 1, i);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            __builtin_amdgcn_s_setprio(0);
         }
-        __builtin_amdgcn_s_setprio(0);
+    };
+    if (total > kFineRows) {
+        sweep(std::integral_constant<int, 1>{});
+    } else {
+        sweep(std::integral_constant<int, 2>{});
     }
     l_run = halves_sum(l_run);
     {
