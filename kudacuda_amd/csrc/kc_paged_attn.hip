@@ -61,6 +61,23 @@ __device__ __forceinline__ float add_pair(F16, uint32_t v, float sum) {
     typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, v), __builtin_bit_cast(halfx2, 0x3c003c00u), sum, false);
 }
+// Weights are 2^(score - maximum + kUp): in fp16 they use the type's upper range, up to
+// 2^15, so that the many small ones of a long cache keep their bits (an fp16 number loses
+// the first below 2^-14 and the last below 2^-25: 2^-36 of the largest weight).  The row
+// tiles' maximum may lag by kLag powers of two.  The sums of weights and of values have
+// the factor alike, it cancels in their quotient; partials tell the maximum less kUp.
+template <typename T>
+struct Weights {
+    static constexpr float kUp = 0.0f;
+    static constexpr float kLag = 8.0f;
+    static constexpr float kFewUp = 0.0f;
+};
+template <>
+struct Weights<F16> {
+    static constexpr float kUp = 11.0f;
+    static constexpr float kLag = 4.0f;
+    static constexpr float kFewUp = 14.0f;
+};
 template <typename T>
 __device__ __forceinline__ float low(uint32_t v) {
     return T::load(static_cast<uint16_t>(v & 0xffffu));
@@ -404,13 +421,16 @@ __device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequ
         const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
         m_run = m_new;
         l_run *= corr;
-        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16, 22
-        // in fp16): this form waits for memory, the second product is free
+        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16; 22 in fp16,
+        // fewer below 2^-28 of the largest, none below 2^-39, which 2^20 keys would
+        // have to have for 2^-19 of it): this form waits for memory, the second product
+        // is free
+        const float m_w = m_sub - Weights<T>::kFewUp;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_sub);
-            const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_sub);
+            const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_w);
+            const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_w);
             l_run += p0 + p1;
             hi[e] = pack(T{}, p0, p1);
             lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
@@ -444,7 +464,7 @@ __device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequ
     }
     float* const s_acc = reinterpret_cast<float*>(s_mem);  // [wave][16][D / 2]: half of the dims a round
     if (q == 0) {
-        s_ml[wave][r][0] = m_run;
+        s_ml[wave][r][0] = m_run - Weights<T>::kFewUp;
         s_ml[wave][r][1] = l_run;
     }
     bool redo = bad;
@@ -942,10 +962,10 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
                     mx = fmaxf(mx, sc[t][e]);
                 }
             }
-            // the maximum may lag behind by 2^8 (weights up to 256 are as exact): sums are
-            // rescaled a few times a row, not in every window
+            // the maximum may lag behind (larger weights are as exact): sums are rescaled a
+            // few times a row, not in every window
             const float m_new = fmaxf(m_run, halves_max(mx) * a.scale_log2);
-            if (__any(m_new > m_run + 8.0f)) {
+            if (__any(m_new > m_run + Weights<T>::kLag)) {
                 const float corr = __builtin_amdgcn_exp2f(m_run - (m_new == kNegInf ? 0.0f : m_new));
                 l_run *= corr;
 #pragma unroll
@@ -957,7 +977,7 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
                 }
                 m_run = m_new;
             }
-            const float m_sub = m_run == kNegInf ? 0.0f : m_run;
+            const float m_sub = (m_run == kNegInf ? 0.0f : m_run) - Weights<T>::kUp;
             // steps of 16 keys: the lane's weights of scores 8 (n % 2) .. + 7 of half n / 2;
             // between the products of a step the next step's weights are formed and its V read
             uint32_t p[2][4], rest[2][kFine ? 4 : 1];
@@ -1094,7 +1114,7 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
         }
     }
     if (q == 0) {
-        *reinterpret_cast<float2*>(split_stats(a, D, splits) + 2 * at) = make_float2(m_run, l_run);
+        *reinterpret_cast<float2*>(split_stats(a, D, splits) + 2 * at) = make_float2(m_run - Weights<T>::kUp, l_run);
     }
 }
 

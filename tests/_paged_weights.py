@@ -38,12 +38,20 @@ def weight_bound(batch: Paged, want: np.ndarray, size: np.ndarray) -> np.ndarray
         of the matrix instructions, 2^-24 each at worst, below 2^-13;
       * the weights' own rounding: half a step of the type, or, in two parts, the second part's half step of a half
         step, 2^-16 (bf16) or less;
-    """
+    and in fp16, whose weights are scaled into the type's upper range, half of its smallest step, 2^-25, of 2^11 at
+    least: 2^-36 a key of the largest weight, which is 1, times the largest value."""
 
     half = HALF[batch.dtype]
     coarse = np.where(fine_rows(batch), 2.0**-16, half)[:, None, None]
     bound = half * np.abs(want) + (2.0**-13 + coarse) * size
-    return bound + (2.0**-25 if batch.dtype == torch.float16 else 0.0)
+    if batch.dtype == torch.float16:
+        top = float(batch.v[~torch.isnan(batch.v)].abs().max())
+        bound += 2.0**-25 + max(batch.kv) * 2.0**-36 * top
+    return bound
+
+
+def _place(batch: Paged, i: int, key: int) -> tuple[int, int]:
+    return int(batch.table[i, key // batch.page]), key % batch.page
 
 
 def _clear(batch: Paged, value: float) -> None:
@@ -54,6 +62,19 @@ def _clear(batch: Paged, value: float) -> None:
     nan = torch.isnan(batch.k)
     batch.k = torch.where(nan, batch.k, torch.zeros_like(batch.k))
     batch.v = torch.where(nan, batch.v, torch.full_like(batch.v, value))
+
+
+def one_above_a_tail(new, kv, key: int, gap: float, **kwargs) -> Paged:
+    """Key `key` of every sequence has 2^gap times the weight of each other one and no value, the others have 1: the
+    result is the tail's share."""
+
+    batch = Paged(31, new, kv, scale=LN2, **kwargs)
+    _clear(batch, 1.0)
+    for i, n in enumerate(kv):
+        page, at = _place(batch, i, min(key, n - 1))
+        batch.k[page, :, at, 0] = gap
+        batch.v[page, :, at] = 0.0
+    return batch
 
 
 def opposite_roundings(new, kv, **kwargs) -> Paged:

@@ -1,5 +1,5 @@
-"""GPU: what attention over a paged cache does with single weights: their rounding, and that no key of a long
-cache is left out.  Against softmax in 64 bits."""
+"""GPU: what attention over a paged cache does with single weights: small ones beside a large one, their rounding,
+and that no key of a long cache is left out.  Against softmax in 64 bits."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tests._paged_ref import f64
-from tests._paged_weights import marked, opposite_roundings, told, weight_bound
+from tests._paged_weights import marked, one_above_a_tail, opposite_roundings, told, weight_bound
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -25,6 +25,17 @@ def _check(native, batch, hint):
         d["out"].fill_(7.25)
         off = np.abs(f64(batch.call(native, d, nbytes=nbytes)) - want)
         assert (off <= bound).all(), (nbytes, float((off / np.maximum(bound, 1e-30)).max()))
+
+
+@hints
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [[1], [40]])
+@pytest.mark.parametrize("gap", [16.0, 20.0, 24.5, 25.0, 28.25])
+def test_a_long_tail_beside_one_large_weight_counts(torch_gpu, native, dtype, dim, new, gap, hint):
+    for key in (5, 20011, 39950):
+        print(f"tail of 40000 keys 2^-{gap} below key {key}, {new} new", flush=True)
+        _check(native, one_above_a_tail(new, [40000], key, gap, heads=4, kv_heads=2, dim=dim, dtype=dtype), hint)
 
 
 @hints

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests._paged_ref import f64
-from tests._paged_weights import marked, opposite_roundings, weight_bound
+from tests._paged_weights import marked, one_above_a_tail, opposite_roundings, weight_bound
 
 
 def _weights(batch):
@@ -44,6 +44,19 @@ def test_one_window_left_out_is_rejected(dtype, dim, edges, new, kv):
             q = p.copy()
             q[lost] = 0.0
             assert (np.abs(q @ v / q.sum() - want[row, 0]) > bound).any(), lost
+
+
+def test_weights_below_the_smallest_step_are_rejected():
+    """The tail in fp16 weights of at most 1, the sum of the same rounded weights."""
+
+    for gap in (24.5, 25.0, 28.25):
+        for new in ([1], [40]):
+            batch = one_above_a_tail(new, [40000], 5, gap, heads=1, kv_heads=1, dim=64, dtype=torch.float16)
+            row, p, v = _weights(batch)
+            rounded = f64(torch.from_numpy(p).half())
+            assert _rejected(batch, rounded @ v / rounded.sum(), row)
+            scaled = f64(torch.from_numpy(p * 2.0**11).half())
+            assert new == [1] or not _rejected(batch, scaled @ v / scaled.sum(), row)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
