@@ -142,7 +142,8 @@ class PagedKvCache:
         """Room for ``counts[i]`` new tokens behind sequence ``sequences[i]`` each.
 
         A last page that is shared and has room is copied first.  Raises
-        ``OutOfPages``, and changes nothing, where the pool is too small."""
+        ``OutOfPages`` where the pool is too small.  Where it raises, that or what the
+        copy or the batch's upload meets, nothing is changed."""
 
         sequences = [int(s) for s in sequences]
         counts = [int(c) for c in counts]
@@ -165,18 +166,32 @@ class PagedKvCache:
             wanted += -(-(entry.length + count) // size) - len(entry.pages) + copy
         if wanted > len(self._free):
             raise OutOfPages(f"{wanted} pages wanted, {len(self._free)} free")
+        before = [(entry.length, len(entry.pages), entry.pages[-1:]) for entry in entries]
+        shared = {page: self._users[page] for page in users}
+        left = len(self._free) - wanted
+        fresh = self._free[left:]
         pairs = []
-        for entry, count, copy in zip(entries, counts, copied):
-            if copy:
-                page = self._take()
-                pairs.append((entry.pages[-1], page))
-                self._users[entry.pages[-1]] -= 1
-                entry.pages[-1] = page
-            entry.length += count
-            while len(entry.pages) * size < entry.length:
-                entry.pages.append(self._take())
-        self._copy(pairs)
-        return self._batch(sequences, entries, counts)
+        try:
+            for entry, count, copy in zip(entries, counts, copied):
+                if copy:
+                    page = self._take()
+                    pairs.append((entry.pages[-1], page))
+                    self._users[entry.pages[-1]] -= 1
+                    entry.pages[-1] = page
+                entry.length += count
+                while len(entry.pages) * size < entry.length:
+                    entry.pages.append(self._take())
+            batch = self._batch(sequences, entries, counts)
+            self._copy(pairs)
+            return batch
+        except BaseException:
+            for entry, (length, n, last) in zip(entries, before):
+                entry.length = length
+                entry.pages[max(0, n - 1):] = last
+            for page, n in [*shared.items(), *((page, 0) for page in fresh)]:
+                self._users[page] = n
+            self._free[left:] = fresh
+            raise
 
     def compact(self) -> int:
         """Move the pages in use to the lowest ids (the pool could then be cut); returns how many moved.

@@ -215,3 +215,30 @@ def test_a_cache_lies_on_its_handles_device(device):
     native.handle, native.device_id = None, 0
     with pytest.raises(ValueError, match="cuda:0"):
         PagedKvCache(native, torch, layers=1, kv_heads=1, head_dim=8, num_pages=1, device=device)
+
+
+@pytest.mark.parametrize("fault", ["copy", "upload"])
+def test_an_extension_that_fails_changes_nothing(cache, monkeypatch, fault):
+    """A refused page copy, or a batch that finds no device memory: the books are as before, and a retry is right."""
+
+    a, b = cache.create(), cache.create()
+    _write(cache, cache.extend([a, b], [6, 3]), list(range(9)))
+    c = cache.fork(a)
+
+    def state():
+        return [(cache.pages(s), cache.length(s)) for s in (a, b, c)], list(cache._free), list(cache._users)
+
+    before = state()
+    with monkeypatch.context() as m:
+        def fail(*_args):
+            raise RuntimeError("out of device memory")
+
+        if fault == "copy":
+            m.setattr(cache.native, "call", fail)
+        else:
+            m.setattr(cache.torch, "from_numpy", fail)
+        with pytest.raises(RuntimeError, match="memory"):
+            cache.extend([b, a], [2, 3])
+    assert state() == before
+    _write(cache, cache.extend([b, a], [2, 3]), [20, 21, 10, 11, 12])
+    assert [_read(cache, s) for s in (a, b, c)] == [[*range(6), 10, 11, 12], [6, 7, 8, 20, 21], list(range(6))]
