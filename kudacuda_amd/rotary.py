@@ -25,7 +25,9 @@ def rope_frequencies(rotary_dim: int, theta: float = 1.0e6, *, scaling: str = "n
     divided by it and the fastest is kept.  ``yarn`` (Peng et al., 2023) keeps the
     pairs that turn more than ``fast`` times over ``original_positions``, divides
     those that turn less than ``slow`` times, goes from one to the other linearly in
-    between, and multiplies the rows by 0.1 ln(factor) + 1."""
+    the pair's number between (from the last whole number before the one limit to the
+    first behind the other: what models of that configuration run, where the paper's
+    text goes linearly in the turns), and multiplies the rows by 0.1 ln(factor) + 1."""
 
     if rotary_dim < 2 or rotary_dim % 2 != 0:
         raise ValueError("rotary_dim must be even and at least 2")
@@ -42,7 +44,16 @@ def rope_frequencies(rotary_dim: int, theta: float = 1.0e6, *, scaling: str = "n
         last = exponent[-1]
         return inv_freq if last == 0 else (theta * factor ** (1.0 / last)) ** -exponent, 1.0
     if scaling == "yarn":
-        turns = original_positions * inv_freq / (2.0 * math.pi)
-        kept = np.clip((turns - slow) / (fast - slow), 0.0, 1.0)
-        return inv_freq * (kept + (1.0 - kept) / factor), 0.1 * math.log(factor) + 1.0
+        if not (0.0 < slow < fast and original_positions > 0 and theta > 1.0):
+            raise ValueError("yarn needs 0 < slow < fast, original_positions and theta > 1")
+
+        def pair(turns: float) -> float:
+            # theta ^ (-2 i / rotary_dim) * original_positions = 2 pi turns
+            return rotary_dim * math.log(original_positions / (2.0 * math.pi * turns)) / (2.0 * math.log(theta))
+
+        first = max(math.floor(pair(fast)), 0)
+        last = min(math.ceil(pair(slow)), rotary_dim - 1)
+        # (nothing between the limits: the pairs up to the first are kept)
+        ramp = np.clip((np.arange(rotary_dim // 2) - first) / max(last - first, 0.001), 0.0, 1.0)
+        return inv_freq * (1.0 - ramp + ramp / factor), 0.1 * math.log(factor) + 1.0
     return inv_freq, 1.0

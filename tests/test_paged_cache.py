@@ -242,3 +242,37 @@ def test_an_extension_that_fails_changes_nothing(cache, monkeypatch, fault):
     assert state() == before
     _write(cache, cache.extend([b, a], [2, 3]), [20, 21, 10, 11, 12])
     assert [_read(cache, s) for s in (a, b, c)] == [[*range(6), 10, 11, 12], [6, 7, 8, 20, 21], list(range(6))]
+
+
+@pytest.mark.parametrize("dim,theta,factor,positions,slow,fast", [
+    (128, 1.0e6, 4.0, 32768, 1.0, 32.0), (64, 1.0e4, 16.0, 4096, 1.0, 32.0), (96, 5.0e5, 8.0, 8192, 1.0, 32.0),
+    (32, 1.0e4, 40.0, 4096, 1.0, 32.0), (128, 1.0e6, 2.0, 32768, 2.0, 8.0), (64, 1.0e4, 4.0, 100, 1.0, 32.0),
+    (8, 1.0e4, 4.0, 1 << 20, 1.0, 1.5), (128, 1.0e4, 1.0, 4096, 1.0, 32.0)])
+def test_yarn_frequencies_are_those_that_models_run(dim, theta, factor, positions, slow, fast):
+    """Transformers' table, which is made in fp32: powers and exponents off by 2^-21 (14 of them at 2^-25), sums by a
+    few roundings, and 1 - ramp by 2^-24 of the plain frequency, up to `factor` times the sum."""
+
+    transformers = pytest.importorskip("transformers")
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+
+    scaling = dict(rope_type="yarn", rope_theta=theta, factor=factor, original_max_position_embeddings=positions,
+                   beta_slow=slow, beta_fast=fast)
+    config = transformers.Qwen2Config(hidden_size=4 * dim, num_attention_heads=4, num_key_value_heads=4,
+                                      max_position_embeddings=int(positions * factor), rope_parameters=scaling)
+    want, scale = ROPE_INIT_FUNCTIONS["yarn"](config, "cpu")
+    got, amplitude = rope_frequencies(dim, theta, scaling="yarn", factor=factor, original_positions=positions, slow=slow,
+                                      fast=fast)
+    assert amplitude == pytest.approx(scale, rel=1e-6)
+    want = want.double().numpy()
+    assert (np.abs(got - want) <= (2.0**-20 + factor * 2.0**-23) * want).all(), (got / want).tolist()
+
+
+def test_yarn_keeps_pairs_that_all_turn_often():
+    plain = rope_frequencies(8, 1.0e4)[0]
+    assert np.array_equal(rope_frequencies(8, 1.0e4, scaling="yarn", factor=4.0, original_positions=1 << 40)[0], plain)
+
+
+@pytest.mark.parametrize("bad", [dict(slow=32.0, fast=1.0), dict(slow=0.0), dict(original_positions=0), dict(theta=1.0)])
+def test_yarn_refusals(bad):
+    with pytest.raises(ValueError):
+        rope_frequencies(**(dict(rotary_dim=64, scaling="yarn", factor=4.0) | bad))
