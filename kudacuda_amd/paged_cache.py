@@ -78,8 +78,8 @@ class PagedKvCache:
         self.head_dim = int(head_dim)
         self.num_pages = int(num_pages)
         self.page_size = int(page_size)
-        self.device = torch.device(device)
         self.pool = torch.zeros((2 * layers, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.device = self.pool.device  # with its number, whichever device is current later
         self._free = list(range(num_pages - 1, -1, -1))  # taken from the end: lowest first
         self._users = [0] * num_pages
         self._entries: dict[int, _Entry] = {}
@@ -252,14 +252,24 @@ class PagedKvCache:
     def _dtype(self) -> int:
         return 1 if self.pool.dtype == self.torch.bfloat16 else 2
 
-    def _use(self, batch: Batch) -> int:
-        """The current stream; where the batch was made on another one, its memory waits for this one too."""
+    def _capturing(self) -> bool:
+        """Whether a graph captures the current stream of the cache's device."""
 
-        stream = self.torch.cuda.current_stream(self.device)
-        if stream.cuda_stream != batch.stream and not self.torch.cuda.is_current_stream_capturing():
+        cuda = self.torch.cuda
+        if cuda.current_device() == self.device.index:
+            return cuda.is_current_stream_capturing()
+        with cuda.device(self.device):
+            return cuda.is_current_stream_capturing()
+
+    def _use(self, batch: Batch) -> tuple[int, bool]:
+        """The current stream, and whether it is captured; where the batch was made on another one, its memory waits
+        for this one too."""
+
+        stream, capturing = self.torch.cuda.current_stream(self.device), self._capturing()
+        if stream.cuda_stream != batch.stream and not capturing:
             for x in (batch.slots, batch.positions, batch.query_starts, batch.kv_lens, batch.page_table):
                 x.record_stream(stream)
-        return stream.cuda_stream
+        return stream.cuda_stream, capturing
 
     def _copy(self, pairs: Sequence[tuple[int, int]]) -> None:
         if not pairs:
@@ -296,12 +306,13 @@ class PagedKvCache:
         out = self.torch.empty_like(query, memory_format=self.torch.contiguous_format) if out is None else out
         o_stride = self._rows("out", out, batch.tokens, query.shape[1])
         keys, values = self.keys(layer), self.values(layer)
+        stream, _ = self._use(batch)
         self.native.call("kudacuda_rope_paged_append", query.data_ptr(), key.data_ptr(), value.data_ptr(),
                          inv_freq.data_ptr(), batch.positions.data_ptr(), batch.slots.data_ptr(), out.data_ptr(),
                          keys.data_ptr(), values.data_ptr(), self._dtype(), batch.tokens, query.shape[1],
                          self.kv_heads, self.head_dim, 2 * inv_freq.numel(), int(interleaved), q_stride, k_stride,
                          v_stride, o_stride, self.num_pages, self.page_size, keys.stride(0), keys.stride(1),
-                         keys.stride(2), float(amplitude), self._use(batch))
+                         keys.stride(2), float(amplitude), stream)
         return out
 
     def attend(self, layer: int, batch: Batch, query: Any, *, scale: float | None = None, out: Any = None) -> Any:
@@ -315,13 +326,13 @@ class PagedKvCache:
         n = len(batch.sequences)
         nbytes = self.native.lib.kudacuda_paged_attention_workspace_bytes(
             batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads, self.head_dim)
-        stream = self._use(batch)
+        stream, capturing = self._use(batch)
         # a workspace a stream: calls on one stream follow one another; a captured call
         # gets its own, from its graph's memory
-        workspace = None if self.torch.cuda.is_current_stream_capturing() else self._workspaces.get(stream)
+        workspace = None if capturing else self._workspaces.get(stream)
         if nbytes > 0 and (workspace is None or workspace.numel() < nbytes):
             workspace = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
-            if not self.torch.cuda.is_current_stream_capturing():
+            if not capturing:
                 self._workspaces[stream] = workspace
         self.native.call("kudacuda_paged_attention", query.data_ptr(), keys.data_ptr(), values.data_ptr(),
                          batch.page_table.data_ptr(), batch.query_starts.data_ptr(), batch.kv_lens.data_ptr(),

@@ -172,3 +172,12 @@ def test_a_batch_of_another_stream_may_be_dropped_behind_its_calls(torch_gpu, na
     side.synchronize()
     assert torch.equal(got, want)
     del filled
+
+
+def test_a_cache_keeps_the_number_of_its_device(torch_gpu, native):
+    """"cuda" is the device that is current when the cache is made, not when it is used."""
+
+    from kudacuda_amd.paged_cache import PagedKvCache
+
+    cache = PagedKvCache(native, torch, layers=1, kv_heads=1, head_dim=64, num_pages=2, device="cuda")
+    assert cache.device == torch.device("cuda:0") == cache.pool.device

@@ -2,8 +2,10 @@
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -276,3 +278,62 @@ def test_yarn_keeps_pairs_that_all_turn_often():
 def test_yarn_refusals(bad):
     with pytest.raises(ValueError):
         rope_frequencies(**(dict(rotary_dim=64, scaling="yarn", factor=4.0) | bad))
+
+
+# -------------------------------------------------- streams and devices of the calls
+class FakeCuda:
+    """torch.cuda with two devices of one stream each; `capturing` are those whose stream a graph captures."""
+
+    def __init__(self):
+        self.current = 0
+        self.capturing = set()
+
+    def current_device(self):
+        return self.current
+
+    def current_stream(self, device):
+        return SimpleNamespace(cuda_stream=100 + torch.device(device).index)
+
+    def is_current_stream_capturing(self):
+        return self.current in self.capturing
+
+    @contextlib.contextmanager
+    def device(self, device):
+        before, self.current = self.current, torch.device(device).index
+        yield
+        self.current = before
+
+
+@pytest.fixture
+def second(monkeypatch):
+    """A cache on cuda:1 (its tensors stay on the CPU) and its torch; calls are kept."""
+
+    calls = []
+    native = SimpleNamespace(call=lambda name, *args: calls.append((name, args)),
+                             lib=SimpleNamespace(kudacuda_paged_attention_workspace_bytes=lambda *_: 64))
+    c = PagedKvCache(native, torch, layers=1, kv_heads=1, head_dim=8, num_pages=4, page_size=4, device="cpu")
+    cuda = FakeCuda()
+    c.torch = SimpleNamespace(cuda=cuda, empty=lambda n, dtype, device: torch.empty(n, dtype=dtype), uint8=torch.uint8,
+                              empty_like=torch.empty_like, contiguous_format=torch.contiguous_format,
+                              from_numpy=torch.from_numpy, float64=torch.float64, bfloat16=torch.bfloat16)
+    monkeypatch.setattr(c, "_stream", lambda: 101)
+    batch = c.extend([c.create()], [1])
+    c.device = torch.device("cuda:1")
+    return c, cuda, batch, calls
+
+
+def test_a_captured_call_has_its_own_workspace_whichever_device_is_current(second):
+    cache, cuda, batch, calls = second
+    q = torch.zeros((1, 1, 8), dtype=torch.bfloat16)
+    cuda.capturing = {1}
+    for current in (0, 1):
+        cuda.current = current
+        cache.attend(0, batch, q)
+        assert cache._workspaces == {} and cuda.current == current
+    cuda.capturing = {0}  # another device's graph: an ordinary call here
+    for current in (0, 1):
+        cuda.current = current
+        cache.attend(0, batch, q)
+    assert list(cache._workspaces) == [101]
+    kept = cache._workspaces[101].data_ptr()
+    assert [args[7] == kept for _, args in calls][-2:] == [True, True]
