@@ -290,7 +290,7 @@ class PagedKvCache:
                              f"on {self.pool.device}")
         if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != self.head_dim):
             raise ValueError(f"the heads of a token of {name} must be contiguous")
-        return x.stride(0) if tokens > 1 else max(x.stride(0), x.shape[1] * self.head_dim)
+        return x.stride(0) if tokens > 1 else x.shape[1] * self.head_dim
 
     def append(self, layer: int, batch: Batch, query: Any, key: Any, value: Any, inv_freq: Any, *,
                amplitude: float = 1.0, interleaved: bool = False, out: Any = None) -> Any:

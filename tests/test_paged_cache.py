@@ -337,3 +337,16 @@ def test_a_captured_call_has_its_own_workspace_whichever_device_is_current(secon
     assert list(cache._workspaces) == [101]
     kept = cache._workspaces[101].data_ptr()
     assert [args[7] == kept for _, args in calls][-2:] == [True, True]
+
+
+def test_one_token_has_no_stride(second):
+    """The row of a single token may lie anywhere on its boundary: its distance to a next one is never used."""
+
+    cache, _, batch, calls = second
+    rows = torch.zeros(3 * 17, dtype=torch.bfloat16)
+    q = torch.as_strided(rows, (1, 2, 8), (17, 8, 1))
+    k = torch.as_strided(rows, (1, 1, 8), (3, 8, 1))
+    cache.append(0, batch, q, k, k, torch.zeros(4, dtype=torch.float64), out=q)
+    cache.attend(0, batch, q)
+    append, attend = (args for _, args in calls)
+    assert append[16:20] == (16, 8, 8, 16) and attend[17:19] == (16, 16)
