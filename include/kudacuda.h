@@ -327,6 +327,10 @@ KUDACUDA_API int kudacuda_rope_paged_append(
  * is zero.  Rows of no sequence are left as they were.  A sequence whose kv_len is
  * negative or past its table row, and a row that sees a page id outside the pool,
  * become NaN; such pages are not read.
+ * Sums, maxima and products are fp32.  Softmax weights meet the values with 16 bits
+ * (bf16) or 22 (fp16) in sequences whose new tokens, times the query heads of a KV head,
+ * are at most 32; rounded once to the type, and summed so, in longer ones.  An fp16
+ * weight below 2^-36 of its row's largest may count as zero.
  * max_query_len and max_kv_len say how long the longest sequence may be; they
  * choose kernels and key splits, results hold whatever they are.  Long caches with
  * few rows are split over the chip through the workspace:
@@ -372,7 +376,10 @@ KUDACUDA_API int kudacuda_copy_pages(void* handle, uint64_t pool, uint64_t pairs
  * (p >= 1: all), min_p of these the ones with w >= min_p; the first token is always
  * kept.  tokens_out (int32) is the lowest id whose kept weights, summed by id, pass
  * u times their sum; chances (fp32, may be 0) its share of that sum.  Weights are
- * formed in 64 bits and summed exactly, so equal inputs give equal tokens.
+ * formed in 64 bits, rounded to whole multiples of 2^-42 of the largest (one below
+ * 2^-43 of it weighs nothing: that token is never drawn) and summed exactly, so equal
+ * inputs give equal tokens; a small chance is as exact as its weight, off by up to 2^-43
+ * of the largest one's.
  * temperature <= 0 takes the first token (chance 1).  temperature, top_k (int32),
  * top_p and min_p are arrays of one value a row, each may be 0 (off).  NaN logits
  * count as -inf; a row of nothing else gives token 0 with chance 0.

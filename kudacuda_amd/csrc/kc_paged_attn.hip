@@ -266,16 +266,17 @@ __device__ __forceinline__ void tell_splits(const PagedAttnArgs& a, const Sequen
 
 // ------------------------------------------------------------------ few rows
 // Sequences of which a KV head has at most kFewRows rows, many and long ones (the plan
-// says which): single tokens, bound by the cache's bytes.  All blocks share the cached rows of all sequences
-// evenly: the work is the line of (sequence, KV head, tile of 16 rows, round of 128
-// keys), cut into one stretch a block, so a batch of unequal lengths ends everywhere
-// at once (64 sequences of up to 8192 tokens, 307 MB: 70 us, 4.4 TB/s; with a fixed
-// number of splits a sequence 88).  In a round the four waves take 32 keys each, K
+// says which): single tokens, bound by the cache's bytes.  All blocks share the cached
+// rows of all sequences evenly: the work is the line of (sequence, KV head, tile of 16
+// rows, round of 128 keys), cut into one stretch a block, so a batch of unequal lengths
+// ends everywhere at once (64 sequences of up to 8192 tokens, 307 MB: 70 us, 4.4 TB/s;
+// with a fixed number of splits a sequence 88).  A stretch is whole rounds: 9.25 of them
+// a block, as there, are 10 for 474 blocks and none for 38.  In a round the four waves take 32 keys each, K
 // straight from memory into the first product's operand, V through the wave's own LDS,
 // the next keys requested as soon as the registers of these are free.  With more rows
 // the keys would be read once a tile of 16, and the row tiles below are faster: 32 rows of
-// 64 sequences of 2000 keys 58 us here and 37 there, of 8192 keys at most 104 and 98, of
-// one with 120000 55 and 34; of 64 with 100 keys 9.9 and 11.7.
+// 64 sequences of 2000 keys 58 us here and 38 there, of up to 8192 keys 104 and 82, of
+// one with 120000 55 and 35; of 64 with 100 keys 9.9 and 12.
 constexpr int kFewRows = 16;
 constexpr int kUnit = 32;
 constexpr int kRound = 4 * kUnit;
@@ -671,12 +672,14 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 // 16 bits and their sum adds the rounded ones: half a step of the type a weight, at
 // random, next to the result's own half step (2-norm error of a prompt of 8192 bf16
 // tokens 2.1e-3, 1.9e-3 with a maximum that never lags at 284 us for 265, of the
-// result's rounding alone 1.6e-3); a second part of each weight would cost half as many
-// products again.  Measured, 8192 tokens of 16 heads over 2 KV heads: 346 us at first,
-// 318 with loads that bypass the compiler's waits, 293 with operands read ahead and the
-// maximum allowed to lag, 287 with page bases as scalars, 262 with the waves' priorities
-// and the order of blocks (1050 TFLOP/s; a library product of 8192^3 1405).  Forming the next window's scores between this
-// window's weights (250 VGPRs) took 293.
+// result's rounding alone 1.6e-3).  A second part of each weight costs half as many
+// products again and its forming: that prompt 354 us for 266, six mixed fp16
+// chunks with heads of 64 63 for 49.  Measured, 8192 tokens of 16 heads over 2 KV heads:
+// 346 us at first, 318 with loads that bypass the compiler's waits, 293 with operands
+// read ahead and the maximum allowed to lag, 287 with page bases as scalars, 262 with the
+// waves' priorities and the order of blocks, 266 with the second loop that follows here
+// in one kernel (1035 TFLOP/s; a library product of 8192^3 1405).  Forming the next
+// window's scores between this window's weights (250 VGPRs) took 293.
 //
 // Sequences of at most kFineRows rows a KV head (single tokens, drafts) are one wave's
 // columns: their products have room, and their weights keep both 16-bit parts, as in the
@@ -1290,8 +1293,9 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     const auto cap = [](int64_t v, int64_t most) { return v < 1 ? int64_t{1} : (v < most ? v : most); };
     const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
     // Few rows of every sequence go to the kernel for them where all sequences' windows
-    // are at least 28 a CU (64 sequences of up to 8192 keys, 2 KV heads: 70 us, row tiles
-    // 81; 32 36 and 40; 24 35 and 33; 128 of up to 2000 38 and 43, of 1000 31 and 26).
+    // are at least 28 a CU (64 sequences of up to 8192 keys, 2 KV heads: 71 us, row tiles
+    // 84; 32 36 and 43; 24 35 and 35; 16 23.6 and 22.9; 128 of up to 2000 38 and 45, of
+    // 1000 30 and 27).
     const bool few = rows <= kFewRows && sequences * kv_heads * windows >= 7168;
     if (!few) {
         p.slots = tokens * group / kTileRows + sequences;
@@ -1307,8 +1311,9 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
             p.tile_splits = cost(s) < cost(p.tile_splits) ? s : p.tile_splits;
         }
         // Sequences of one tile a KV head, whose partials are small: splits that even out
-        // unequal lengths (64 sequences of 4 tokens and up to 8192 keys: 2 splits 134 us,
-        // 6 98; all of 2000 keys: 2 38.4, 4 37.5; with 8 tokens each: 2 42, 4 50).
+        // unequal lengths (64 sequences of 4 tokens and up to 8192 keys: 150 us without, 82
+        // with; all of 2000 keys 39.7 and 37.8; of 1 to 5 tokens and up to 4000 keys 56 and
+        // 48; but 8 tokens each after 2000 43 and 49).
         if (sequences > 1 && rows <= kTileRows) {
             const int64_t even = cap(1024 / tiles, (windows + 7) / 8);
             p.tile_splits = p.tile_splits > even ? p.tile_splits : even;
@@ -1321,7 +1326,7 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     }
     // Beside longer sequences they go there where a tile would take more than 50 windows (a
     // chunk of 1000 and a token after 16000: 58 us, with tiles alone 113; 512 and 63 tokens
-    // after up to 4000: 60 and 67; two chunks of 256 and 8 tokens: 40 and 30).
+    // after up to 4000: 60 and 67; two chunks of 256 and 8 tokens: 40 and 35).
     int64_t few_splits = 0;
     if (few || (rows > kFewRows && tokens != sequences * longest && windows > 50 * p.tile_splits)) {
         // two blocks a CU; a stretch of at least one round of keys.  The longest sequence

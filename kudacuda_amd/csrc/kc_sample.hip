@@ -372,7 +372,7 @@ __device__ __forceinline__ void for_passing(const Row& r, const float (&x)[8], f
 
 // 2^(42 - depth / 64) rounded to a whole number, 0 <= depth < kDepth: a table's power
 // for the whole buckets of the fraction, the Taylor polynomial of degree 5 of
-// 2^(-z / 64) for the rest (z < 1: off by 2^-49), and the addition of 2^52 that rounds.
+// 2^(-z / 64) for the rest (z < 1: off by 2^-48.6), and the addition of 2^52 that rounds.
 __device__ __forceinline__ uint64_t weight_of(double depth, const double* powers) {
     const int whole = static_cast<int>(depth);
     const double z = depth - whole;
@@ -981,10 +981,14 @@ __device__ __forceinline__ uint64_t select_in_list(const uint64_t (&word)[MINE],
     return block_max(found, s_part);
 }
 
-// Where more tokens than the list holds share the deciding buckets (flat rows):
+// Where more tokens than the list holds share the deciding buckets (flat rows: high
+// temperatures, or 16-bit logits so far from zero that thousands are equal):
 // the order word of the first token, in order, up to which the count (k > 0) or the
 // weight over buckets [low, high] reaches the target, digit by digit over the whole row;
-// 0: it is never reached.
+// 0: it is never reached.  One block reads its row up to seven times: a call with such
+// rows takes about a millisecond (151936 logits, top-p 0.95, bf16 normal logits around 16
+// or at temperature 60: one row 1.0 ms, 128 1.1; with a top-k of 20000 1.5 and 1.7), where
+// others take 26 to 110 us.
 template <typename T>
 __device__ __forceinline__ uint64_t select_in_row(const SampleArgs& a, const Row& r, const typename Raw<T>::type* logits,
                                                int low, int high, uint64_t before, int k, uint64_t target,
