@@ -685,8 +685,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 // columns: their products have room, and their weights keep both 16-bit parts, as in the
 // kernel for few rows (16 bits of the fp32 weight in bf16, 22 in fp16); their sum adds
 // them as they are.  What that costs is forming the second parts, fp32 arithmetic of one
-// wave: a token over 2000 keys 14.2 us (one part: 13.4), over 120000 33.4 (32.1), 16
-// over up to 4000 20.8 (18.8), two chunks of 256 beside 8 tokens 35 (30).
+// wave: a token over 2000 keys 14.2 us (one part: 14.0), over 120000 33.4 (32.7), 16
+// over up to 4000 20.5 (18.1), two chunks of 256 beside 8 tokens 30.4 (30.1; with the
+// waves of both K-groups on one SIMD 35).
 constexpr int kTileRows = 128;
 constexpr int kFineRows = 32;
 constexpr int kWindow = 64;
@@ -789,14 +790,16 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
     const int w_begin = split * per_split;
     const int w_end = w_begin + per_split < windows ? w_begin + per_split : windows;
 
-    const int local = wave * 32 + r;
+    // the K-groups' waves of the same columns on different SIMDs, for tiles of few columns
+    const int strip = (wave + 2 * group) & 3;
+    const int local = strip * 32 + r;
     const int column = static_cast<int>(c0) + (local < count ? local : count - 1);
     const int head = g * G + column % G;
     const int pos = before + column / G;
-    const int wave_column = static_cast<int>(c0) + (wave * 32 < count ? wave * 32 : count - 1);
+    const int wave_column = static_cast<int>(c0) + (strip * 32 < count ? strip * 32 : count - 1);
     const int first_pos = before + wave_column / G;  // lowest and highest positions of the wave's columns
-    const int wave_last = wave * 32 + 31 < count ? wave * 32 + 31 : count - 1;
-    const int last_pos = wave * 32 < count ? before + (static_cast<int>(c0) + wave_last) / G : -1;
+    const int wave_last = strip * 32 + 31 < count ? strip * 32 + 31 : count - 1;
+    const int last_pos = strip * 32 < count ? before + (static_cast<int>(c0) + wave_last) / G : -1;
 
     uint4 qf[kSteps];
     {
@@ -1057,7 +1060,7 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
             for (int i = 0; i < D / 32; ++i) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    s_acc[(wave * (D / 8) + i * 4 + j) * 64 + lane] =
+                    s_acc[(strip * (D / 8) + i * 4 + j) * 64 + lane] =
                         make_float4(acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]);
                 }
             }
@@ -1079,7 +1082,7 @@ __global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) 
         for (int i = 0; i < D / 32; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float4 v = s_acc[(wave * (D / 8) + i * 4 + j) * 64 + lane];
+                const float4 v = s_acc[(strip * (D / 8) + i * 4 + j) * 64 + lane];
                 acc[i][4 * j] = acc[i][4 * j] * f0 + v.x * f1;
                 acc[i][4 * j + 1] = acc[i][4 * j + 1] * f0 + v.y * f1;
                 acc[i][4 * j + 2] = acc[i][4 * j + 2] * f0 + v.z * f1;
@@ -1326,7 +1329,7 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     }
     // Beside longer sequences they go there where a tile would take more than 50 windows (a
     // chunk of 1000 and a token after 16000: 58 us, with tiles alone 113; 512 and 63 tokens
-    // after up to 4000: 60 and 67; two chunks of 256 and 8 tokens: 40 and 35).
+    // after up to 4000: 60 and 67; two chunks of 256 and 8 tokens: 40 and 30).
     int64_t few_splits = 0;
     if (few || (rows > kFewRows && tokens != sequences * longest && windows > 50 * p.tile_splits)) {
         // two blocks a CU; a stretch of at least one round of keys.  The longest sequence
