@@ -329,8 +329,8 @@ KUDACUDA_API int kudacuda_rope_paged_append(
  * become NaN; such pages are not read.
  * Sums, maxima and products are fp32.  Softmax weights meet the values with 16 bits
  * (bf16) or 22 (fp16) in sequences whose new tokens, times the query heads of a KV head,
- * are at most 32; rounded once to the type, and summed so, in longer ones.  An fp16
- * weight below 2^-36 of its row's largest may count as zero.
+ * are at most 32; rounded once to the type, and summed so, in longer ones.  In fp16 a
+ * weight below 2^-14 of its row's largest has fewer bits, one below 2^-36 may have none.
  * max_query_len and max_kv_len say how long the longest sequence may be; they
  * choose kernels and key splits, results hold whatever they are.  Long caches with
  * few rows are split over the chip through the workspace:

@@ -271,12 +271,12 @@ __device__ __forceinline__ void tell_splits(const PagedAttnArgs& a, const Sequen
 // rows, round of 128 keys), cut into one stretch a block, so a batch of unequal lengths
 // ends everywhere at once (64 sequences of up to 8192 tokens, 307 MB: 70 us, 4.4 TB/s;
 // with a fixed number of splits a sequence 88).  A stretch is whole rounds: 9.25 of them
-// a block, as there, are 10 for 474 blocks and none for 38.  In a round the four waves take 32 keys each, K
-// straight from memory into the first product's operand, V through the wave's own LDS,
-// the next keys requested as soon as the registers of these are free.  With more rows
-// the keys would be read once a tile of 16, and the row tiles below are faster: 32 rows of
-// 64 sequences of 2000 keys 58 us here and 38 there, of up to 8192 keys 104 and 82, of
-// one with 120000 55 and 35; of 64 with 100 keys 9.9 and 12.
+// a block, as there, are 10 for 474 blocks and none for 38.  In a round the four waves
+// take 32 keys each, K straight from memory into the first product's operand, V through
+// the wave's own LDS, the next keys requested as soon as the registers of these are free.
+// With more rows the keys would be read once a tile of 16, and the row tiles below are
+// faster: 32 rows of 64 sequences of 2000 keys 58 us here and 38 there, of up to 8192
+// keys 104 and 82, of one with 120000 55 and 35; of 64 with 100 keys 9.9 and 12.
 constexpr int kFewRows = 16;
 constexpr int kUnit = 32;
 constexpr int kRound = 4 * kUnit;
@@ -422,10 +422,10 @@ __device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequ
         const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
         m_run = m_new;
         l_run *= corr;
-        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16; 22 in fp16,
-        // fewer below 2^-28 of the largest, none below 2^-39, which 2^20 keys would
-        // have to have for 2^-19 of it): this form waits for memory, the second product
-        // is free
+        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16; in fp16 22,
+        // one fewer for each power of two below 2^-17 of the largest, none below 2^-39:
+        // 2^20 such keys would be 2^-19 of it, in l_run alone): this form waits for
+        // memory, the second product is free
         const float m_w = m_sub - Weights<T>::kFewUp;
         uint32_t hi[4], lo[4];
 #pragma unroll
@@ -673,8 +673,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 // random, next to the result's own half step (2-norm error of a prompt of 8192 bf16
 // tokens 2.1e-3, 1.9e-3 with a maximum that never lags at 284 us for 265, of the
 // result's rounding alone 1.6e-3).  A second part of each weight costs half as many
-// products again and its forming: that prompt 354 us for 266, six mixed fp16
-// chunks with heads of 64 63 for 49.  Measured, 8192 tokens of 16 heads over 2 KV heads:
+// products again and its forming: that prompt 354 us for 266, six mixed fp16 chunks with
+// heads of 64 63 for 49.  Measured, 8192 tokens of 16 heads over 2 KV heads:
 // 346 us at first, 318 with loads that bypass the compiler's waits, 293 with operands
 // read ahead and the maximum allowed to lag, 287 with page bases as scalars, 262 with the
 // waves' priorities and the order of blocks, 266 with the second loop that follows here
@@ -683,8 +683,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 //
 // Sequences of at most kFineRows rows a KV head (single tokens, drafts) are one wave's
 // columns: their products have room, and their weights keep both 16-bit parts, as in the
-// kernel for few rows (16 bits of the fp32 weight in bf16, 22 in fp16); their sum adds
-// them as they are.  What that costs is forming the second parts, fp32 arithmetic of one
+// kernel for few rows (16 bits of the fp32 weight in bf16, up to 22 in fp16); their sum
+// adds them as they are.  What that costs is forming the second parts, fp32 arithmetic of one
 // wave: a token over 2000 keys 14.2 us (one part: 14.0), over 120000 33.4 (32.7), 16
 // over up to 4000 20.5 (18.1), two chunks of 256 beside 8 tokens 30.4 (30.1; with the
 // waves of both K-groups on one SIMD 35).
