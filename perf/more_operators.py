@@ -39,6 +39,7 @@ CODES = {"bf16": 1, "fp16": 2}
 # the lowest power of two that a block of 4 or 8 bits has: its elements are numbers of the type
 LOWEST = {("bf16", 4): -110, ("bf16", 8): -110, ("fp16", 4): -23, ("fp16", 8): -15}
 TILE = 64  # rows of an adapter's tile
+FACTOR = float(np.float32(1.1386))  # an amplitude that scaled frequencies bring, as calls take it: in 32 bits
 
 
 # ------------------------------------------------------------------ cases
@@ -47,7 +48,7 @@ def listed() -> list[dict]:
         # one decode round of a small batch: the smallest call, once a layer and token
         _append("append 8 tokens", "bf16", 4, 8),
         # a round of prompt chunks, a model that rotates half of each head in pairs, stretched fourfold
-        _append("append 19999 fp16 pairs 8 bits", "fp16", 8, 19999, rotary=DIM // 2, pairs=True, stretch=4.0, factor=1.1386),
+        _append("append 19999 fp16 pairs 8 bits", "fp16", 8, 19999, rotary=DIM // 2, pairs=True, stretch=4.0, factor=FACTOR),
         # a short sequence that moves to another cache
         _read("read 2000 tokens", "bf16", 4, 2000),
         # a long one
@@ -112,7 +113,7 @@ def draw(rng) -> dict:
     if kind == "append":
         case = _append("", dtype, bits, _spread(rng, 1, 16000), heads, kv_heads, dim,
                        rng.choice([dim, dim, dim // 2, dim // 4]), rng.random() < 0.4, rng.choice([1.0, 1.0, 4.0, 32.0]),
-                       rng.choice([1.0, 1.0, 1.1386]), page)
+                       rng.choice([1.0, 1.0, FACTOR]), page)
     elif kind == "read":
         case = _read("", dtype, bits, _spread(rng, 1, 60000 // kv_heads), kv_heads, dim, page)
     elif kind == "attention":
