@@ -352,6 +352,80 @@ KUDACUDA_API int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, in
                                                               int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
                                                               int64_t head_dim);
 
+/* The same cache in 4 or 8 bits (bits): blocks of 32 dims of a row share a power of
+ * two, their elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign; dim 2 i in the
+ * low half of byte i) or e4m3 (up to 448).  A page holds the elements [kv_heads,
+ * page_size, head_dim] and behind them the blocks' bytes [kv_heads, page_size,
+ * head_dim / 32], 127 + the exponent, 255 for NaN; page p begins page_stride * p BYTES
+ * into the pool.  What a page of zero bytes holds is zeros.  copy_pages copies such pages.
+ * Contract: head_dim 64 or 128, page_size a power of two, 16..4096, kv_heads 1..1024,
+ * pools and page_stride on 16-byte boundaries.
+ *
+ * kudacuda_rope_paged_append_mx is kudacuda_rope_paged_append into such pages: a key row is
+ * turned (in 64 bits) and rounded to the type, then it and the value row are rounded to
+ * their blocks' steps, nearest, ties to even.  A block's exponent is the least e for which
+ * no magnitude reaches 7 * 2^e (bits 8: 464 * 2^e), so no element is off by more than half
+ * a step, and at least -110 in bf16, -23 (bits 4) or -15 (bits 8) in fp16; past 125 (119)
+ * in bf16 and 13 (7) in fp16, where elements would pass the type's largest number, they
+ * saturate at 6 * 2^e (448 * 2^e).  A block with an infinity or NaN is all NaN. */
+KUDACUDA_API int kudacuda_rope_paged_append_mx(
+    void* handle, uint64_t query, uint64_t key, uint64_t value, uint64_t inv_freq, uint64_t positions, uint64_t slots,
+    uint64_t query_output, uint64_t key_pages, uint64_t value_pages, int64_t dtype, int64_t bits, int64_t tokens,
+    int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t interleaved,
+    int64_t query_stride, int64_t key_stride, int64_t value_stride, int64_t output_stride, int64_t num_pages,
+    int64_t page_size, int64_t page_stride, float amplitude, uint64_t stream);
+
+/* Rows of such a cache as numbers of the type (what append wrote with that dtype comes back
+ * exactly): key_output and value_output [tokens, kv_heads, head_dim] are the rows at
+ * slots[token] (int64).  A slot that is negative or past the pool is padding: nothing is
+ * written for it.  Contract: tokens 0..2^30, strides (elements between tokens) multiples of
+ * 8, outputs on 16-byte boundaries and apart. */
+KUDACUDA_API int kudacuda_paged_read_mx(void* handle, uint64_t key_pages, uint64_t value_pages, uint64_t slots,
+                                        uint64_t key_output, uint64_t value_output, int64_t dtype, int64_t bits,
+                                        int64_t tokens, int64_t kv_heads, int64_t head_dim, int64_t key_stride,
+                                        int64_t value_stride, int64_t num_pages, int64_t page_size, int64_t page_stride,
+                                        uint64_t stream);
+
+/* kudacuda_paged_attention over such a cache: the same rows, masks, sums and workspace
+ * rules, on the numbers that the cache holds (kudacuda_paged_read_mx with the same dtype);
+ * a row that sees a NaN block is NaN where that block weighs in. */
+KUDACUDA_API int kudacuda_paged_attention_mx(void* handle, uint64_t query, uint64_t key_pages, uint64_t value_pages,
+                                             uint64_t page_table, uint64_t query_starts, uint64_t kv_lens,
+                                             uint64_t output, uint64_t workspace, int64_t workspace_bytes, int64_t dtype,
+                                             int64_t bits, int64_t tokens, int64_t sequences, int64_t max_query_len,
+                                             int64_t max_kv_len, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                                             int64_t query_stride, int64_t output_stride, int64_t num_pages,
+                                             int64_t page_size, int64_t table_stride, int64_t page_stride, float scale,
+                                             uint64_t stream);
+KUDACUDA_API int64_t kudacuda_paged_attention_mx_workspace_bytes(int64_t bits, int64_t tokens, int64_t sequences,
+                                                                 int64_t max_query_len, int64_t max_kv_len,
+                                                                 int64_t query_heads, int64_t kv_heads,
+                                                                 int64_t head_dim);
+
+/* Low-rank adapters of many requests beside a shared projection: for the rows x of adapter
+ * a, output = base + scales[a] * (x A_a^T) B_a^T, in fp32 but for x A^T's way into the second
+ * product (two 16-bit parts: 16 bits of the row's largest in bf16, 22 in fp16), rounded once.
+ * a_factors [adapters, max_rank, in_features] holds A_a's ranks[a] rows (int32), b_factors
+ * [adapters, out_features * max_rank] B_a's out_features rows one after the other, each of
+ * ranks[a] rounded up to a multiple of 8, zeros at the end; scales fp32.  The plan groups
+ * the rows: order (int32 [tokens]) lists rows of input, base and output, tiles (int32
+ * [tile_count][3]) are (adapter, first, count <= 64): rows order[first] .. of one adapter.
+ * An adapter outside [0, adapters), or of rank 0, adds nothing: its rows are base's.  Rows
+ * of no tile are left as they were; no row may be in two.  base may be output, or 0 (zeros).
+ * Contract: tokens 0..2^20, max_rank 8..128, in_features up to 2^17 and out_features up to
+ * 2^20, all multiples of 8, as strides are; tile_count <= 2^20, tile_count * out_features <=
+ * 2^31; buffers (but the 4-byte ones) on 16-byte boundaries; workspace of
+ * kudacuda_lora_workspace_bytes(tokens, tile_count, max_rank, in_features) bytes.
+ * (kudacuda_amd/lora.py keeps such factors and plans.) */
+KUDACUDA_API int kudacuda_lora_add(void* handle, uint64_t input, uint64_t a_factors, uint64_t b_factors, uint64_t ranks,
+                                   uint64_t scales, uint64_t order, uint64_t tiles, uint64_t base, uint64_t output,
+                                   uint64_t workspace, int64_t workspace_bytes, int64_t dtype, int64_t tokens,
+                                   int64_t tile_count, int64_t adapters, int64_t max_rank, int64_t in_features,
+                                   int64_t out_features, int64_t input_stride, int64_t base_stride,
+                                   int64_t output_stride, uint64_t stream);
+KUDACUDA_API int64_t kudacuda_lora_workspace_bytes(int64_t tokens, int64_t tile_count, int64_t max_rank,
+                                                   int64_t in_features);
+
 /* Copies pages inside a cache: for every pair (source, destination) of `pairs`
  * (int32 [count][2] in HOST memory, read before the call returns) and each of
  * `pools` pools (layers' keys and values) page_bytes bytes at pool + i *

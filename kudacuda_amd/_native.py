@@ -67,6 +67,12 @@ SIGNATURES: dict[str, tuple[list[Any], Any]] = {
     "kudacuda_rope_paged_append": ([_vp] + [_u64] * 9 + [_i64] * 16 + [_f, _u64], _i),
     "kudacuda_paged_attention": ([_vp] + [_u64] * 8 + [_i64] * 17 + [_f, _u64], _i),
     "kudacuda_paged_attention_workspace_bytes": ([_i64] * 7, _i64),
+    "kudacuda_rope_paged_append_mx": ([_vp] + [_u64] * 9 + [_i64] * 15 + [_f, _u64], _i),
+    "kudacuda_paged_read_mx": ([_vp] + [_u64] * 5 + [_i64] * 10 + [_u64], _i),
+    "kudacuda_paged_attention_mx": ([_vp] + [_u64] * 8 + [_i64] * 16 + [_f, _u64], _i),
+    "kudacuda_paged_attention_mx_workspace_bytes": ([_i64] * 8, _i64),
+    "kudacuda_lora_add": ([_vp] + [_u64] * 10 + [_i64] * 11 + [_u64], _i),
+    "kudacuda_lora_workspace_bytes": ([_i64] * 4, _i64),
     "kudacuda_copy_pages": ([_vp, _u64, _u64] + [_i64] * 6 + [_u64], _i),
     "kudacuda_sample_tokens": ([_vp] + [_u64] * 9 + [_i64] * 5 + [_u64], _i),
     "kudacuda_sample_workspace_bytes": ([_i64] * 2, _i64),

@@ -354,6 +354,7 @@ struct PagedAttnArgs {
     int64_t page_stride = 0, head_stride = 0, token_stride = 0;
     int page_shift = 0;
     float scale_log2 = 0.0f;  // scale * log2(e)
+    int64_t block_offset = 0;  // microscaled pages: bytes before the blocks' powers of two
 };
 // Which kernels a call takes (0: not launched), the few-row kernel for sequences with
 // few rows, the tile kernel for the others, and over how many key splits.
@@ -370,6 +371,60 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
                                    int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                    int64_t workspace_bytes);
 hipError_t launch_paged_attention(Act act, const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t stream);
+// The splits' partials to the output.
+hipError_t launch_paged_merge(Act act, const PagedAttnArgs& args, int64_t splits, hipStream_t stream);
+
+// A paged cache of microscaled numbers (kc_mx.h): a page of a pool begins at page *
+// page_stride bytes and holds the elements [kv_heads, page_size, head_dim] of `bits` bits,
+// at block_offset behind them the blocks' bytes [kv_heads, page_size, head_dim / 32].
+struct MxAppendArgs {
+    const uint16_t* q = nullptr;
+    const uint16_t* k = nullptr;
+    const uint16_t* v = nullptr;
+    const double* inv_freq = nullptr;  // [rotary_dim / 2]
+    const int32_t* positions = nullptr;
+    const int64_t* slots = nullptr;
+    uint16_t* q_out = nullptr;
+    uint8_t* k_pages = nullptr;
+    uint8_t* v_pages = nullptr;
+    int64_t tokens = 0;
+    int bits = 0;
+    int q_heads = 0;
+    int kv_heads = 0;
+    int head_dim = 0;  // 64 or 128
+    int rotary_dim = 0;
+    bool interleaved = false;
+    int page_shift = 0;
+    int64_t q_stride = 0, k_stride = 0, v_stride = 0, out_stride = 0;  // elements between tokens
+    int64_t num_pages = 0;
+    int64_t page_stride = 0, block_offset = 0;
+    float amplitude = 1.0f;
+};
+hipError_t launch_mx_append(Act act, const MxAppendArgs& args, hipStream_t stream);
+
+struct MxReadArgs {
+    const uint8_t* k_pages = nullptr;
+    const uint8_t* v_pages = nullptr;
+    const int64_t* slots = nullptr;
+    uint16_t* k_out = nullptr;
+    uint16_t* v_out = nullptr;
+    int64_t tokens = 0;
+    int bits = 0;
+    int kv_heads = 0;
+    int head_dim = 0;
+    int page_shift = 0;
+    int64_t k_stride = 0, v_stride = 0;  // elements between tokens
+    int64_t num_pages = 0;
+    int64_t page_stride = 0, block_offset = 0;
+};
+hipError_t launch_mx_read(Act act, const MxReadArgs& args, hipStream_t stream);
+
+// Attention over such a cache: of the arguments, k and v are its pools, page_stride,
+// head_stride and token_stride the bytes between pages, heads and tokens of elements.
+PagedAttnPlan mx_attention_plan(int bits, int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
+                                int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                int64_t workspace_bytes);
+hipError_t launch_mx_attention(Act act, int bits, const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t stream);
 
 constexpr int kPagePairs = 448;  // pairs of a launch: 3584 bytes of kernel arguments
 struct CopyPagesArgs {
@@ -400,6 +455,32 @@ constexpr int64_t kSampleMaxVocab = int64_t{1} << 20;
 int64_t sample_workspace_bytes(int64_t rows, int64_t vocab);
 // dtype: 0 = fp32, 1 = bf16, 2 = fp16
 hipError_t launch_sample(int dtype, const SampleArgs& args, hipStream_t stream);
+
+// -------------------------------------------------- adapters beside a projection
+constexpr int kLoraTile = 64;      // rows of a tile at most
+constexpr int kLoraMaxRank = 128;
+struct LoraArgs {
+    const uint16_t* x = nullptr;       // [tokens, in]
+    const uint16_t* a = nullptr;       // [adapters, max_rank, in]
+    const uint16_t* b = nullptr;       // [adapters, out * max_rank]: rows of the rank rounded up to 8
+    const int32_t* ranks = nullptr;    // [adapters]
+    const float* scales = nullptr;     // [adapters]
+    const int32_t* order = nullptr;    // [tokens] rows, an adapter's side by side
+    const int32_t* tiles = nullptr;    // [tile_count][3]: adapter, first of order, how many
+    const uint16_t* base = nullptr;    // [tokens, out] or null
+    uint16_t* out = nullptr;
+    float* partials = nullptr;         // [splits, tokens, pitch]
+    int64_t tokens = 0, tile_count = 0, adapters = 0, max_rank = 0, in_features = 0, out_features = 0;
+    int64_t x_stride = 0, base_stride = 0, out_stride = 0;
+    int64_t pitch = 0;
+};
+struct LoraPlan {
+    int64_t splits = 1;  // of the first product's inner axis
+    int64_t pitch = 0;   // ranks of a partial's row
+    int64_t workspace_bytes = 0;
+};
+LoraPlan lora_plan(int64_t tokens, int64_t tile_count, int64_t max_rank, int64_t in_features);
+hipError_t launch_lora(Act act, const LoraArgs& args, const LoraPlan& plan, hipStream_t stream);
 
 // ------------------------------------------------------------------ misc ops
 hipError_t launch_vector_add(const float* a, const float* b, float* out, int64_t n, hipStream_t stream);

@@ -1,0 +1,416 @@
+// Low-rank adapters of many requests beside a shared projection:
+//     out = base + s_a (x A_a^T) B_a^T
+// for the rows of adapter a; A_a is [rank, in], B_a [out, rank].  The caller's plan groups
+// the rows: a tile is up to 64 rows of one adapter.
+//
+// Two launches.  The first forms u = x A^T, a tile's 64 rows by up to 64 ranks a block,
+// over a share of `in` (few tiles are split so that the adapters' bytes come through all
+// CUs); the four waves take alternate steps of 32 and meet in LDS.  The second sums the
+// shares in order, splits u into two 16-bit parts (normalised by a power of two a row, so
+// that fp16 keeps 22 bits of it and bf16 16) and takes tiles of 64 rows by 64 outputs a
+// wave: both parts lie along the product's inner axis, so rank 16 is one matrix
+// instruction of depth 32.  Operands come straight from memory: both factors' rows are
+// contiguous along the inner axis.
+#include <type_traits>
+
+#include "kc_device.h"
+#include "kc_kernels.h"
+
+namespace kc {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kStep = 32;            // of the inner axis, a matrix instruction
+constexpr int kBlockStep = 4 * kStep;  // of the four waves
+constexpr int64_t kBlocks = 512;
+
+__device__ __forceinline__ floatx4 mfma16(Bf16, uint4 a, uint4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mfma16(F16, uint4 a, uint4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pair(Bf16, float lo, float hi) { return pack2(lo, hi); }
+__device__ __forceinline__ uint32_t pair(F16, float lo, float hi) {
+    typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+    const halfx2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// A tile of the plan; whatever it holds, rows stay inside the order and the adapter inside
+// the pools (adapter -1: none).
+struct Tile {
+    int adapter;
+    int rank;
+    int first;
+    int count;
+};
+__device__ __forceinline__ Tile tile_of(const LoraArgs& a, int index) {
+    const int32_t* const p = a.tiles + 3 * static_cast<int64_t>(index);
+    Tile t;
+    const int tokens = static_cast<int>(a.tokens);
+    t.adapter = __builtin_amdgcn_readfirstlane(p[0]);
+    t.first = __builtin_amdgcn_readfirstlane(p[1]);
+    t.count = __builtin_amdgcn_readfirstlane(p[2]);
+    t.count = t.first < 0 || t.first >= tokens || t.count < 0 ? 0 : t.count;
+    t.count = t.count < kLoraTile ? t.count : kLoraTile;
+    t.count = t.count < tokens - t.first ? t.count : tokens - t.first;
+    t.rank = 0;
+    if (t.adapter >= 0 && t.adapter < a.adapters) {
+        const int rank = __builtin_amdgcn_readfirstlane(a.ranks[t.adapter]);
+        t.rank = rank < 0 ? 0 : (rank < a.max_rank ? rank : static_cast<int>(a.max_rank));
+    }
+    return t;
+}
+// Row `i` of a tile in the inputs and outputs, -1 if there is none.
+__device__ __forceinline__ int row_of(const LoraArgs& a, const Tile& t, int i) {
+    const int row = i < t.count ? a.order[t.first + i] : -1;
+    return row < a.tokens ? row : -1;
+}
+
+// ------------------------------------------------------------------- x A^T
+// RT tiles of 16 ranks from rank0 on, SUBS of 16 rows.
+template <typename T, int RT, int SUBS>
+__device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int rank0, int k_begin, int k_end,
+                                           float* partials, float (*s_u)[16][RT * 16 + 4]) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int r = lane & 15;
+    const int q = lane >> 4;
+    const uint16_t* const factor = a.a + static_cast<int64_t>(t.adapter) * a.max_rank * a.in_features;
+    const uint16_t* arow[RT];
+    const uint16_t* xrow[SUBS];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int rank = rank0 + 16 * i + r;
+        arow[i] = factor + static_cast<int64_t>(rank < t.rank ? rank : t.rank - 1) * a.in_features;
+    }
+#pragma unroll
+    for (int i = 0; i < SUBS; ++i) {
+        const int row = row_of(a, t, 16 * i + r);
+        xrow[i] = a.x + static_cast<int64_t>(row < 0 ? 0 : row) * a.x_stride;
+    }
+    floatx4 acc[SUBS][RT];
+#pragma unroll
+    for (int s = 0; s < SUBS; ++s) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            acc[s][i] = floatx4{};
+        }
+    }
+    const int tiles = (t.rank - rank0 + 15) / 16;
+    constexpr int kAhead = RT * SUBS <= 2 ? 4 : (RT + SUBS <= 5 ? 2 : 1);
+    for (int k0 = k_begin + wave * kStep; k0 < k_end; k0 += kAhead * kBlockStep) {
+        uint4 av[kAhead][RT], xv[kAhead][SUBS];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int k = k0 + n * kBlockStep + 8 * q;
+            const bool in = k < k_end;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                av[n][i] = make_uint4(0, 0, 0, 0);
+                if (in && i < tiles) {
+                    av[n][i] = load_stream(reinterpret_cast<const uint4*>(arow[i] + k));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s) {
+                xv[n][s] = make_uint4(0, 0, 0, 0);
+                if (in && 16 * s < t.count) {
+                    xv[n][s] = *reinterpret_cast<const uint4*>(xrow[s] + k);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+#pragma unroll
+                for (int s = 0; s < SUBS; ++s) {
+                    acc[s][i] = mfma16(T{}, av[n][i], xv[n][s], acc[s][i]);
+                }
+            }
+        }
+    }
+    // acc[s][i][e]: rank 16 i + 4 q + e of row 16 s + r; the waves' shares meet in LDS
+#pragma unroll
+    for (int s = 0; s < SUBS; ++s) {
+        if (16 * s >= t.count) {
+            break;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            *reinterpret_cast<float4*>(&s_u[wave][r][16 * i + 4 * q]) =
+                make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * RT * 4; i += kThreads) {
+            const int row = i / (RT * 4);
+            const int rank = i % (RT * 4) * 4;
+            if (16 * s + row < t.count && rank0 + rank < t.rank) {
+                float4 sum = *reinterpret_cast<const float4*>(&s_u[0][row][rank]);
+#pragma unroll
+                for (int w = 1; w < 4; ++w) {
+                    const float4 v = *reinterpret_cast<const float4*>(&s_u[w][row][rank]);
+                    sum.x += v.x;
+                    sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
+                }
+                *reinterpret_cast<float4*>(partials + static_cast<int64_t>(t.first + 16 * s + row) * a.pitch + rank0 + rank) = sum;
+            }
+        }
+    }
+}
+
+template <typename T, int RT>
+__global__ __launch_bounds__(kThreads) void lora_inner_kernel(LoraArgs a, int splits, int chunks) {
+    __shared__ __attribute__((aligned(16))) float s_u[4][16][RT * 16 + 4];
+    const int chunk = static_cast<int>(blockIdx.x) % chunks;
+    const int split = static_cast<int>(blockIdx.x) / chunks % splits;
+    const Tile t = tile_of(a, static_cast<int>(blockIdx.x) / chunks / splits);
+    const int rank0 = chunk * RT * 16;
+    if (t.count == 0 || rank0 >= t.rank) {
+        return;
+    }
+    const int in = static_cast<int>(a.in_features);
+    const int steps = (in + kBlockStep - 1) / kBlockStep;
+    const int per_split = (steps + splits - 1) / splits * kBlockStep;
+    const int begin = split * per_split < in ? split * per_split : in;
+    const int end = begin + per_split < in ? begin + per_split : in;
+    float* const partials = a.partials + static_cast<int64_t>(split) * a.tokens * a.pitch;
+    if (t.count <= 16) {
+        inner_tile<T, RT, 1>(a, t, rank0, begin, end, partials, s_u);
+    } else {
+        inner_tile<T, RT, kLoraTile / 16>(a, t, rank0, begin, end, partials, s_u);
+    }
+}
+
+// ------------------------------------------------------------------- u B^T
+// A block: a tile's rows by `groups` groups of 64 outputs a wave.  LDS holds a row's u first
+// in fp32, then as pieces of 8: the first parts of the ranks, the second parts, zeros.
+template <typename T, int RT, int SUBS>
+__device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int splits, int column0, int groups,
+                                           uint8_t* s_row, float* s_factor) {
+    constexpr int kRowBytes = RT * 64 + 16;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15;
+    const int q = lane >> 4;
+    const int pieces = (t.rank + 7) / 8;
+    const int steps = (pieces + 1) / 2;
+    if (t.rank > 0) {
+        for (int i = tid; i < 16 * SUBS * RT * 4; i += kThreads) {
+            const int row = i / (RT * 4);
+            const int rank = i % (RT * 4) * 4;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (row < t.count && rank < t.rank) {
+                const float* const p = a.partials + static_cast<int64_t>(t.first + row) * a.pitch + rank;
+                const int64_t share = a.tokens * a.pitch;
+#pragma unroll 4
+                for (int s = 0; s < splits; ++s) {
+                    const float4 v = *reinterpret_cast<const float4*>(p + s * share);
+                    sum.x += v.x;
+                    sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
+                }
+                sum.y = rank + 1 < t.rank ? sum.y : 0.0f;
+                sum.z = rank + 2 < t.rank ? sum.z : 0.0f;
+                sum.w = rank + 3 < t.rank ? sum.w : 0.0f;
+            }
+            *reinterpret_cast<float4*>(s_row + row * kRowBytes + rank * 4) = sum;
+        }
+        __syncthreads();
+        const int row = tid / 4;
+        const int part = tid % 4;
+        float4 u[RT];
+        float most = 0.0f;
+        if (row < 16 * SUBS) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                u[i] = *reinterpret_cast<const float4*>(s_row + row * kRowBytes + (16 * i + 4 * part) * 4);
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(u[i].x), fabsf(u[i].y)), fmaxf(fabsf(u[i].z), fabsf(u[i].w))));
+            }
+        }
+        most = fmaxf(most, __shfl_xor(most, 1, 4));
+        most = fmaxf(most, __shfl_xor(most, 2, 4));
+        __syncthreads();
+        if (row < 16 * SUBS) {
+            // u 2^-e lies below 1: its parts fit fp16 (e kept where 2^-e and 2^e are normal)
+            int e = static_cast<int>(__float_as_uint(most) >> 23) - 126;
+            e = e > -120 ? (e < 120 ? e : 120) : -120;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            if (part == 0) {
+                s_factor[row] = a.scales[t.adapter] * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                if (i < steps) {
+                    const float v[4] = {u[i].x * down, u[i].y * down, u[i].z * down, u[i].w * down};
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        hi[j] = pair(T{}, v[2 * j], v[2 * j + 1]);
+                        const float x = v[2 * j] - T::load(static_cast<uint16_t>(hi[j] & 0xffffu));
+                        const float y = v[2 * j + 1] - T::load(static_cast<uint16_t>(hi[j] >> 16));
+                        lo[j] = pair(T{}, x == x ? x : 0.0f, y == y ? y : 0.0f);  // (infinities have no rest)
+                    }
+                    const int piece = 2 * i + part / 2;
+                    // (an odd number of pieces: the one behind the last is zero, both parts at the end)
+                    const int first = piece < pieces ? piece : 2 * pieces;
+                    const int second = piece < pieces ? pieces + piece : 2 * pieces + 1;
+                    uint8_t* const at = s_row + row * kRowBytes + part % 2 * 8;
+                    *reinterpret_cast<uint2*>(at + first * 16) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(at + second * 16) = make_uint2(lo[0], lo[1]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const int pitch = 8 * pieces;
+    const uint16_t* const factor = a.b + static_cast<int64_t>(t.adapter < 0 ? 0 : t.adapter) * a.max_rank * a.out_features;
+    const int out = static_cast<int>(a.out_features);
+    int rows[SUBS];
+#pragma unroll
+    for (int s = 0; s < SUBS; ++s) {
+        rows[s] = row_of(a, t, 16 * s + r);
+    }
+    for (int n = 0; n < groups; ++n) {
+        const int o0 = column0 + (n * 4 + wave) * 64;
+        if (o0 >= out) {
+            break;
+        }
+        // the outputs of row r of operand t: lane (r, q) of a result then has outputs
+        // 32 h + 8 q .. + 7 of its token, from operands 2 h and 2 h + 1
+        floatx4 acc[SUBS][4];
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[s][i] = floatx4{};
+            }
+        }
+        const uint16_t* brow[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int o = o0 + 32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3);
+            brow[i] = factor + static_cast<int64_t>(o < out ? o : out - 1) * pitch;
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int slot = 4 * step + q;
+            const bool some = slot < 2 * pieces;
+            const int piece = slot < pieces ? slot : slot - pieces;
+            uint4 bv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bv[i] = make_uint4(0, 0, 0, 0);
+                if (some) {
+                    bv[i] = *reinterpret_cast<const uint4*>(brow[i] + 8 * piece);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s) {
+                const uint4 uv = *reinterpret_cast<const uint4*>(s_row + (16 * s + r) * kRowBytes + slot * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[s][i] = mfma16(T{}, bv[i], uv, acc[s][i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+            if (rows[s] < 0) {
+                continue;
+            }
+            const float f = t.rank > 0 ? s_factor[16 * s + r] : 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int o = o0 + 32 * h + 8 * q;
+                if (o < out) {
+                    float v[8] = {};
+                    if (a.base != nullptr) {
+                        unpack8<T>(*reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(rows[s]) * a.base_stride + o), v);
+                    }
+                    if (t.rank > 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            v[e] = fmaf(acc[s][2 * h + e / 4][e % 4], f, v[e]);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(rows[s]) * a.out_stride + o) =
+                        make_uint4(pair(T{}, v[0], v[1]), pair(T{}, v[2], v[3]), pair(T{}, v[4], v[5]), pair(T{}, v[6], v[7]));
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int RT>
+__global__ __launch_bounds__(kThreads) void lora_outer_kernel(LoraArgs a, int splits, int blocks, int groups) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_row[kLoraTile * (RT * 64 + 16)];
+    __shared__ float s_factor[kLoraTile];
+    const Tile t = tile_of(a, static_cast<int>(blockIdx.x) / blocks);
+    const int column0 = static_cast<int>(blockIdx.x) % blocks * groups * 256;
+    if (t.count == 0 || (t.rank == 0 && a.out == a.base)) {
+        return;
+    }
+    if (t.count <= 16) {
+        outer_tile<T, RT, 1>(a, t, splits, column0, groups, s_row, s_factor);
+    } else {
+        outer_tile<T, RT, kLoraTile / 16>(a, t, splits, column0, groups, s_row, s_factor);
+    }
+}
+
+template <typename T, int RT>
+hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
+    constexpr int kChunk = RT < 4 ? RT : 4;  // ranks of 16 that a block of the first product takes
+    const int64_t chunks = (a.pitch / 16 + kChunk - 1) / kChunk;
+    hipLaunchKernelGGL((lora_inner_kernel<T, kChunk>), dim3(static_cast<unsigned>(a.tile_count * plan.splits * chunks)),
+                       dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits), static_cast<int>(chunks));
+    const hipError_t status = hipGetLastError();
+    if (status != hipSuccess) {
+        return status;
+    }
+    // one group of 64 outputs a wave, more where there are blocks enough without
+    const int64_t columns = (a.out_features + 255) / 256;
+    int64_t groups = a.tile_count * columns / (2 * kBlocks);
+    groups = groups < 1 ? 1 : (groups < 8 ? groups : 8);
+    const int64_t blocks = (columns + groups - 1) / groups;
+    hipLaunchKernelGGL((lora_outer_kernel<T, RT>), dim3(static_cast<unsigned>(a.tile_count * blocks)), dim3(kThreads), 0, stream,
+                       a, static_cast<int>(plan.splits), static_cast<int>(blocks), static_cast<int>(groups));
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
+    const int64_t tiles = a.pitch / 16;
+    return tiles <= 1 ? launch<T, 1>(a, plan, stream)
+                      : (tiles <= 2 ? launch<T, 2>(a, plan, stream)
+                                    : (tiles <= 4 ? launch<T, 4>(a, plan, stream) : launch<T, 8>(a, plan, stream)));
+}
+
+}  // namespace
+
+LoraPlan lora_plan(int64_t tokens, int64_t tile_count, int64_t max_rank, int64_t in_features) {
+    LoraPlan p;
+    p.pitch = (max_rank + 15) / 16 * 16;
+    const int64_t steps = (in_features + kBlockStep - 1) / kBlockStep;
+    const int64_t wanted = tile_count > 0 ? kBlocks / tile_count : 1;
+    p.splits = wanted < 1 ? 1 : (wanted < steps ? wanted : steps);
+    p.splits = p.splits < 32 ? p.splits : 32;
+    p.workspace_bytes = p.splits * tokens * p.pitch * 4;
+    return p;
+}
+
+hipError_t launch_lora(Act act, const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
+    return act == Act::kBf16 ? launch<Bf16>(a, plan, stream) : launch<F16>(a, plan, stream);
+}
+
+}  // namespace kc

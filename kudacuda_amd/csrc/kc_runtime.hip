@@ -908,9 +908,36 @@ int page_shift_of(int64_t page_size) {
     return -1;
 }
 
-bool within(int64_t v, int64_t low, int64_t high) { return v >= low && v <= high; }
-bool multiple(uint64_t v, uint64_t n) { return v % n == 0; }
 constexpr int64_t kInt32Max = 0x7fffffff;
+
+bool within(int64_t v, int64_t low, int64_t high) { return v >= low && v <= high; }
+
+// The pages of a microscaled cache: bytes of a page's elements, or -1 with a reason.
+int64_t mx_elements(Handle* h, const char* symbol, int64_t bits, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                    int64_t page_size, int64_t page_stride, uint64_t key_pages, uint64_t value_pages) {
+    const auto no = [&](const char* reason) {
+        h->set_error(std::string(symbol) + " requires " + reason);
+        return int64_t{-1};
+    };
+    if (bits != 4 && bits != 8) {
+        return no("bits 4 or 8");
+    }
+    if (head_dim != 64 && head_dim != 128) {
+        return no("head_dim 64 or 128");
+    }
+    if (!within(kv_heads, 1, 1024) || !within(num_pages, 1, kInt32Max) || page_size < 16 || page_shift_of(page_size) < 0) {
+        return no("kv_heads 1..1024, num_pages>=1 and a page_size that is a power of two, 16..4096");
+    }
+    const int64_t elements = kv_heads * page_size * head_dim * bits / 8;
+    if (page_stride < elements + kv_heads * page_size * (head_dim / 32) || page_stride % 16 != 0 ||
+        page_stride > kInt32Max || ((key_pages | value_pages) & 15) != 0) {
+        return no("pages on 16-byte boundaries and a page_stride of at least kv_heads * page_size * "
+                  "(head_dim * bits / 8 + head_dim / 32) bytes");
+    }
+    return elements;
+}
+
+bool multiple(uint64_t v, uint64_t n) { return v % n == 0; }
 
 bool rope_shape_ok(Handle* h, const char* symbol, int64_t dtype, int64_t tokens, int64_t heads, int64_t head_dim,
                    int64_t rotary_dim, int64_t interleaved, float amplitude) {
@@ -992,6 +1019,7 @@ using kc::ready;
 using kc::claim_scratch;
 using kc::scratch_launched;
 using kc::kInt32Max;
+using kc::mx_elements;
 using kc::launch_on;
 using kc::multiple;
 using kc::page_shift_of;
@@ -1825,6 +1853,345 @@ int kudacuda_paged_attention(void* raw, uint64_t query, uint64_t key_pages, uint
     return launch_on(h, symbol, [&] {
         return kc::launch_paged_attention(dtype == 1 ? Act::kBf16 : Act::kF16, a, plan, as_stream(stream));
     });
+}
+
+// ----------------------------------------- a paged cache of microscaled numbers
+int kudacuda_rope_paged_append_mx(void* raw, uint64_t query, uint64_t key, uint64_t value, uint64_t inv_freq,
+                                  uint64_t positions, uint64_t slots, uint64_t query_output, uint64_t key_pages,
+                                  uint64_t value_pages, int64_t dtype, int64_t bits, int64_t tokens, int64_t query_heads,
+                                  int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t interleaved,
+                                  int64_t query_stride, int64_t key_stride, int64_t value_stride, int64_t output_stride,
+                                  int64_t num_pages, int64_t page_size, int64_t page_stride, float amplitude,
+                                  uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "rope_paged_append_mx";
+    if (!ready(h, "kudacuda_rope_paged_append_mx")) {
+        return 1;
+    }
+    if (query == 0 || key == 0 || value == 0 || inv_freq == 0 || positions == 0 || slots == 0 || query_output == 0 ||
+        key_pages == 0 || value_pages == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (!rope_shape_ok(h, symbol, dtype, tokens, query_heads, head_dim, rotary_dim, interleaved, amplitude)) {
+        return 1;
+    }
+    const int64_t elements =
+        mx_elements(h, symbol, bits, kv_heads, head_dim, num_pages, page_size, page_stride, key_pages, value_pages);
+    if (elements < 0) {
+        return 1;
+    }
+    if (query_stride < query_heads * head_dim || output_stride < query_heads * head_dim ||
+        key_stride < kv_heads * head_dim || value_stride < kv_heads * head_dim) {
+        refuse(h, symbol, "strides of at least heads * head_dim");
+        return 1;
+    }
+    if (query == query_output && query_stride != output_stride && tokens > 1) {
+        refuse(h, symbol, "one stride where it works in place");
+        return 1;
+    }
+    if (!multiple(query | key | value | query_output, 2) || !multiple(inv_freq | slots, 8) || !multiple(positions, 4)) {
+        refuse(h, symbol, "buffers aligned to their elements");
+        return 1;
+    }
+    if (tokens == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::MxAppendArgs a;
+    a.q = ptr<const uint16_t>(query);
+    a.k = ptr<const uint16_t>(key);
+    a.v = ptr<const uint16_t>(value);
+    a.inv_freq = ptr<const double>(inv_freq);
+    a.positions = ptr<const int32_t>(positions);
+    a.slots = ptr<const int64_t>(slots);
+    a.q_out = ptr<uint16_t>(query_output);
+    a.k_pages = ptr<uint8_t>(key_pages);
+    a.v_pages = ptr<uint8_t>(value_pages);
+    a.tokens = tokens;
+    a.bits = static_cast<int>(bits);
+    a.q_heads = static_cast<int>(query_heads);
+    a.kv_heads = static_cast<int>(kv_heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.rotary_dim = static_cast<int>(rotary_dim);
+    a.interleaved = interleaved != 0;
+    a.page_shift = page_shift_of(page_size);
+    a.q_stride = query_stride;
+    a.k_stride = key_stride;
+    a.v_stride = value_stride;
+    a.out_stride = output_stride;
+    a.num_pages = num_pages;
+    a.page_stride = page_stride;
+    a.block_offset = elements;
+    a.amplitude = amplitude;
+    return launch_on(h, symbol,
+                     [&] { return kc::launch_mx_append(dtype == 1 ? Act::kBf16 : Act::kF16, a, as_stream(stream)); });
+}
+
+int kudacuda_paged_read_mx(void* raw, uint64_t key_pages, uint64_t value_pages, uint64_t slots, uint64_t key_output,
+                           uint64_t value_output, int64_t dtype, int64_t bits, int64_t tokens, int64_t kv_heads,
+                           int64_t head_dim, int64_t key_stride, int64_t value_stride, int64_t num_pages,
+                           int64_t page_size, int64_t page_stride, uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "paged_read_mx";
+    if (!ready(h, "kudacuda_paged_read_mx")) {
+        return 1;
+    }
+    if (key_pages == 0 || value_pages == 0 || slots == 0 || key_output == 0 || value_output == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (dtype != 1 && dtype != 2) {
+        refuse(h, symbol, "dtype 1 (bf16) or 2 (fp16)");
+        return 1;
+    }
+    const int64_t elements =
+        mx_elements(h, symbol, bits, kv_heads, head_dim, num_pages, page_size, page_stride, key_pages, value_pages);
+    if (elements < 0) {
+        return 1;
+    }
+    if (!within(tokens, 0, int64_t{1} << 30)) {
+        refuse(h, symbol, "0 <= tokens <= 2^30");
+        return 1;
+    }
+    if (key_stride < kv_heads * head_dim || value_stride < kv_heads * head_dim || (key_stride | value_stride) % 8 != 0 ||
+        !multiple(key_output | value_output, 16) || !multiple(slots, 8)) {
+        refuse(h, symbol, "outputs on 16-byte boundaries and strides of at least kv_heads * head_dim, multiples of 8");
+        return 1;
+    }
+    if (key_output == value_output) {
+        refuse(h, symbol, "two outputs");
+        return 1;
+    }
+    if (tokens == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::MxReadArgs a;
+    a.k_pages = ptr<const uint8_t>(key_pages);
+    a.v_pages = ptr<const uint8_t>(value_pages);
+    a.slots = ptr<const int64_t>(slots);
+    a.k_out = ptr<uint16_t>(key_output);
+    a.v_out = ptr<uint16_t>(value_output);
+    a.tokens = tokens;
+    a.bits = static_cast<int>(bits);
+    a.kv_heads = static_cast<int>(kv_heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.page_shift = page_shift_of(page_size);
+    a.k_stride = key_stride;
+    a.v_stride = value_stride;
+    a.num_pages = num_pages;
+    a.page_stride = page_stride;
+    a.block_offset = elements;
+    return launch_on(h, symbol,
+                     [&] { return kc::launch_mx_read(dtype == 1 ? Act::kBf16 : Act::kF16, a, as_stream(stream)); });
+}
+
+int64_t kudacuda_paged_attention_mx_workspace_bytes(int64_t bits, int64_t tokens, int64_t sequences, int64_t max_query_len,
+                                                    int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
+                                                    int64_t head_dim) {
+    if ((bits != 4 && bits != 8) || !within(query_heads, 1, 1024) || !within(kv_heads, 1, query_heads) ||
+        query_heads % kv_heads != 0 || !within(tokens, 1, (int64_t{1} << 27) / query_heads) ||
+        !within(sequences, 1, 65536) || !within(sequences * kv_heads, 1, int64_t{1} << 22) ||
+        (head_dim != 64 && head_dim != 128) || max_query_len < 1 || max_kv_len < 1) {
+        return 0;  // no call that would be taken
+    }
+    max_kv_len = max_kv_len < (int64_t{1} << 30) ? max_kv_len : int64_t{1} << 30;
+    return kc::mx_attention_plan(static_cast<int>(bits), tokens, sequences, max_query_len, max_kv_len, max_kv_len,
+                                 query_heads, kv_heads, head_dim, INT64_MAX)
+        .workspace_bytes;
+}
+
+int kudacuda_paged_attention_mx(void* raw, uint64_t query, uint64_t key_pages, uint64_t value_pages, uint64_t page_table,
+                                uint64_t query_starts, uint64_t kv_lens, uint64_t output, uint64_t workspace,
+                                int64_t workspace_bytes, int64_t dtype, int64_t bits, int64_t tokens, int64_t sequences,
+                                int64_t max_query_len, int64_t max_kv_len, int64_t query_heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t query_stride, int64_t output_stride, int64_t num_pages,
+                                int64_t page_size, int64_t table_stride, int64_t page_stride, float scale,
+                                uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "paged_attention_mx";
+    if (!ready(h, "kudacuda_paged_attention_mx")) {
+        return 1;
+    }
+    if (query == 0 || key_pages == 0 || value_pages == 0 || page_table == 0 || query_starts == 0 || kv_lens == 0 ||
+        output == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (dtype != 1 && dtype != 2) {
+        refuse(h, symbol, "dtype 1 (bf16) or 2 (fp16)");
+        return 1;
+    }
+    const int64_t elements =
+        mx_elements(h, symbol, bits, kv_heads, head_dim, num_pages, page_size, page_stride, key_pages, value_pages);
+    if (elements < 0) {
+        return 1;
+    }
+    if (!within(query_heads, kv_heads, 1024) || query_heads % kv_heads != 0) {
+        refuse(h, symbol, "query_heads (1..1024) a multiple of kv_heads");
+        return 1;
+    }
+    const int shift = page_shift_of(page_size);
+    if (!within(tokens, 0, (int64_t{1} << 27) / query_heads) || !within(sequences, 1, 65536) ||
+        !within(sequences * kv_heads, 1, int64_t{1} << 22) || !within(table_stride, 1, (int64_t{1} << 30) >> shift)) {
+        refuse(h, symbol,
+               "0 <= tokens * query_heads <= 2^27, 1..65536 sequences, sequences * kv_heads <= 2^22 and "
+               "1 <= table_stride * page_size <= 2^30");
+        return 1;
+    }
+    if (max_query_len < 1 || max_kv_len < 1) {
+        refuse(h, symbol, "max_query_len>=1 and max_kv_len>=1");
+        return 1;
+    }
+    if (query_stride < query_heads * head_dim || output_stride < query_heads * head_dim ||
+        (query_stride | output_stride) % 8 != 0) {
+        refuse(h, symbol, "strides of at least a row, multiples of 8");
+        return 1;
+    }
+    if (!multiple(query | output | workspace, 16) || !multiple(page_table | query_starts | kv_lens, 4)) {
+        refuse(h, symbol, "buffers on 16-byte boundaries");
+        return 1;
+    }
+    if (workspace_bytes < 0) {
+        refuse(h, symbol, "workspace_bytes>=0");
+        return 1;
+    }
+    if (output == query) {
+        refuse(h, symbol, "an output apart from the query");
+        return 1;
+    }
+    if (!(scale > 0.0f) || !std::isfinite(scale)) {
+        refuse(h, symbol, "a positive finite scale");
+        return 1;
+    }
+    if (tokens == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    kc::PagedAttnArgs a;
+    a.q = ptr<const uint16_t>(query);
+    a.k = ptr<const uint16_t>(key_pages);
+    a.v = ptr<const uint16_t>(value_pages);
+    a.table = ptr<const int32_t>(page_table);
+    a.starts = ptr<const int32_t>(query_starts);
+    a.kv_lens = ptr<const int32_t>(kv_lens);
+    a.out = ptr<uint16_t>(output);
+    a.partials = ptr<float>(workspace);
+    a.tokens = tokens;
+    a.sequences = sequences;
+    a.q_heads = query_heads;
+    a.kv_heads = kv_heads;
+    a.group = query_heads / kv_heads;
+    a.head_dim = head_dim;
+    a.q_stride = query_stride;
+    a.out_stride = output_stride;
+    a.num_pages = num_pages;
+    a.table_stride = table_stride;
+    a.page_stride = page_stride;
+    a.token_stride = head_dim * bits / 8;
+    a.head_stride = page_size * a.token_stride;
+    a.block_offset = elements;
+    a.page_shift = shift;
+    a.scale_log2 = scale * kc::kLog2e;
+    const int64_t longest = table_stride << shift;
+    const kc::PagedAttnPlan plan = kc::mx_attention_plan(
+        static_cast<int>(bits), tokens, sequences, max_query_len, max_kv_len < longest ? max_kv_len : longest, longest,
+        query_heads, kv_heads, head_dim, workspace != 0 ? workspace_bytes : 0);
+    return launch_on(h, symbol, [&] {
+        return kc::launch_mx_attention(dtype == 1 ? Act::kBf16 : Act::kF16, static_cast<int>(bits), a, plan,
+                                       as_stream(stream));
+    });
+}
+
+// ------------------------------------------------- adapters beside a projection
+int64_t kudacuda_lora_workspace_bytes(int64_t tokens, int64_t tile_count, int64_t max_rank, int64_t in_features) {
+    if (!within(tokens, 1, int64_t{1} << 20) || !within(tile_count, 0, int64_t{1} << 20) ||
+        !within(max_rank, 8, kc::kLoraMaxRank) || max_rank % 8 != 0 || !within(in_features, 8, int64_t{1} << 17)) {
+        return 0;  // no call that would be taken
+    }
+    return kc::lora_plan(tokens, tile_count, max_rank, in_features).workspace_bytes;
+}
+
+int kudacuda_lora_add(void* raw, uint64_t input, uint64_t a_factors, uint64_t b_factors, uint64_t ranks, uint64_t scales,
+                      uint64_t order, uint64_t tiles, uint64_t base, uint64_t output, uint64_t workspace,
+                      int64_t workspace_bytes, int64_t dtype, int64_t tokens, int64_t tile_count, int64_t adapters,
+                      int64_t max_rank, int64_t in_features, int64_t out_features, int64_t input_stride,
+                      int64_t base_stride, int64_t output_stride, uint64_t stream) {
+    Handle* h = as_handle(raw);
+    const char* symbol = "lora_add";
+    if (!ready(h, "kudacuda_lora_add")) {
+        return 1;
+    }
+    if (input == 0 || a_factors == 0 || b_factors == 0 || ranks == 0 || scales == 0 || order == 0 || tiles == 0 ||
+        output == 0) {
+        h->set_error(std::string(symbol) + " requires non-null device pointers");
+        return 1;
+    }
+    if (dtype != 1 && dtype != 2) {
+        refuse(h, symbol, "dtype 1 (bf16) or 2 (fp16)");
+        return 1;
+    }
+    if (!within(tokens, 0, int64_t{1} << 20) || !within(adapters, 1, 65536) || !within(max_rank, 8, kc::kLoraMaxRank) ||
+        max_rank % 8 != 0) {
+        refuse(h, symbol, "0..2^20 tokens, 1..65536 adapters and a max_rank of 8..128, a multiple of 8");
+        return 1;
+    }
+    if (!within(in_features, 8, int64_t{1} << 17) || !within(out_features, 8, int64_t{1} << 20) ||
+        (in_features | out_features) % 8 != 0) {
+        refuse(h, symbol, "in_features 8..2^17 and out_features 8..2^20, multiples of 8");
+        return 1;
+    }
+    if (!within(tile_count, 0, (int64_t{1} << 31) / (out_features < 2048 ? 2048 : out_features))) {
+        refuse(h, symbol, "tile_count>=0 and tile_count * out_features <= 2^31, tile_count <= 2^20");
+        return 1;
+    }
+    if (input_stride < in_features || output_stride < out_features || (base != 0 && base_stride < out_features) ||
+        (input_stride | output_stride | (base != 0 ? base_stride : 0)) % 8 != 0) {
+        refuse(h, symbol, "strides of at least a row, multiples of 8");
+        return 1;
+    }
+    if (!multiple(input | a_factors | b_factors | base | output | workspace, 16) ||
+        !multiple(ranks | scales | order | tiles, 4)) {
+        refuse(h, symbol, "buffers on 16-byte boundaries");
+        return 1;
+    }
+    if (output == input) {
+        refuse(h, symbol, "an output apart from the input");
+        return 1;
+    }
+    if (output == base && output_stride != base_stride && tokens > 1) {
+        refuse(h, symbol, "one stride where it works in place");
+        return 1;
+    }
+    if (tokens == 0 || tile_count == 0) {
+        return finish(h, symbol, hipSuccess);
+    }
+    const kc::LoraPlan plan = kc::lora_plan(tokens, tile_count, max_rank, in_features);
+    if (workspace == 0 || workspace_bytes < plan.workspace_bytes) {
+        refuse(h, symbol, "a workspace of kudacuda_lora_workspace_bytes() bytes");
+        return 1;
+    }
+    kc::LoraArgs a;
+    a.x = ptr<const uint16_t>(input);
+    a.a = ptr<const uint16_t>(a_factors);
+    a.b = ptr<const uint16_t>(b_factors);
+    a.ranks = ptr<const int32_t>(ranks);
+    a.scales = ptr<const float>(scales);
+    a.order = ptr<const int32_t>(order);
+    a.tiles = ptr<const int32_t>(tiles);
+    a.base = ptr<const uint16_t>(base);
+    a.out = ptr<uint16_t>(output);
+    a.partials = ptr<float>(workspace);
+    a.tokens = tokens;
+    a.tile_count = tile_count;
+    a.adapters = adapters;
+    a.max_rank = max_rank;
+    a.in_features = in_features;
+    a.out_features = out_features;
+    a.x_stride = input_stride;
+    a.base_stride = base_stride;
+    a.out_stride = output_stride;
+    a.pitch = plan.pitch;
+    return launch_on(h, symbol,
+                     [&] { return kc::launch_lora(dtype == 1 ? Act::kBf16 : Act::kF16, a, plan, as_stream(stream)); });
 }
 
 int kudacuda_copy_pages(void* raw, uint64_t pool, uint64_t pairs, int64_t count, int64_t pools, int64_t num_pages,

@@ -12,6 +12,11 @@ pages in use to the lowest ids.  A round of a server is::
         q = cache.append(layer, batch, q, k, v, inv_freq)
         out = cache.attend(layer, batch, q)
 
+With ``bits`` 8 or 4 the pool holds bytes instead, ``[2 * layers, num_pages, page_bytes]``:
+rows in blocks of 32 dims that share a power of two (``include/kudacuda.h``), 1.94 or 3.76
+times as many tokens in the same memory.  ``append`` rounds to them, ``attend`` works on
+what they hold, and ``read`` gives that back.
+
 Calls run on the torch stream that is current when they are made.  The pool is shared
 by all of them: a program with several streams orders them itself (events), and a
 batch whose calls a graph has captured is kept as long as the graph.
@@ -58,7 +63,7 @@ class PagedKvCache:
     """Pages of several sequences in one pool, and the native calls on them."""
 
     def __init__(self, native: Native, torch: Any, *, layers: int, kv_heads: int, head_dim: int, num_pages: int,
-                 page_size: int = 16, dtype: Any = None, device: Any = "cuda:0") -> None:
+                 page_size: int = 16, dtype: Any = None, bits: int = 16, device: Any = "cuda:0") -> None:
         dtype = torch.bfloat16 if dtype is None else dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("a cache holds bfloat16 or float16")
@@ -66,6 +71,10 @@ class PagedKvCache:
             raise ValueError("page_size must be a power of two, 1..4096")
         if min(layers, kv_heads, head_dim, num_pages) < 1 or head_dim % 8 != 0:
             raise ValueError("layers, kv_heads and num_pages must be positive, head_dim a multiple of 8")
+        if bits not in (16, 8, 4):
+            raise ValueError("a cache holds numbers of 16, 8 or 4 bits")
+        if bits < 16 and (head_dim not in (64, 128) or page_size < 16 or kv_heads > 1024):
+            raise ValueError("a cache of 8 or 4 bits takes heads of 64 or 128, up to 1024, and pages of 16 tokens or more")
         place = torch.device(device)
         if isinstance(native, Native):
             index = torch.cuda.current_device() if place.type == "cuda" and place.index is None else place.index
@@ -78,7 +87,13 @@ class PagedKvCache:
         self.head_dim = int(head_dim)
         self.num_pages = int(num_pages)
         self.page_size = int(page_size)
-        self.pool = torch.zeros((2 * layers, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.dtype = dtype  # of the rows that come and go
+        self.bits = int(bits)
+        if bits == 16:
+            self.pool = torch.zeros((2 * layers, num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        else:
+            page_bytes = kv_heads * page_size * (head_dim * bits // 8 + head_dim // 32)
+            self.pool = torch.zeros((2 * layers, num_pages, page_bytes), dtype=torch.uint8, device=device)
         self.device = self.pool.device  # with its number, whichever device is current later
         self._free = list(range(num_pages - 1, -1, -1))  # taken from the end: lowest first
         self._users = [0] * num_pages
@@ -98,6 +113,8 @@ class PagedKvCache:
         return list(self._entry(sequence).pages)
 
     def keys(self, layer: int) -> Any:
+        """A layer's pages of keys, as the pool holds them."""
+
         return self.pool[2 * layer]
 
     def values(self, layer: int) -> Any:
@@ -250,7 +267,7 @@ class PagedKvCache:
         return self.torch.cuda.current_stream(self.device).cuda_stream
 
     def _dtype(self) -> int:
-        return 1 if self.pool.dtype == self.torch.bfloat16 else 2
+        return 1 if self.dtype == self.torch.bfloat16 else 2
 
     def _capturing(self) -> bool:
         """Whether a graph captures the current stream of the cache's device."""
@@ -285,8 +302,8 @@ class PagedKvCache:
         """Check [tokens, heads, head_dim] rows with packed heads; returns the stride between tokens."""
 
         if (x.dim() != 3 or x.shape[0] != tokens or (heads is not None and x.shape[1] != heads)
-                or x.shape[2] != self.head_dim or x.dtype != self.pool.dtype or x.device != self.pool.device):
-            raise ValueError(f"{name} must be [{tokens}, {heads or 'heads'}, {self.head_dim}] {self.pool.dtype} "
+                or x.shape[2] != self.head_dim or x.dtype != self.dtype or x.device != self.pool.device):
+            raise ValueError(f"{name} must be [{tokens}, {heads or 'heads'}, {self.head_dim}] {self.dtype} "
                              f"on {self.pool.device}")
         if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != self.head_dim):
             raise ValueError(f"the heads of a token of {name} must be contiguous")
@@ -307,6 +324,13 @@ class PagedKvCache:
         o_stride = self._rows("out", out, batch.tokens, query.shape[1])
         keys, values = self.keys(layer), self.values(layer)
         stream, _ = self._use(batch)
+        if self.bits < 16:
+            self.native.call("kudacuda_rope_paged_append_mx", query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                             inv_freq.data_ptr(), batch.positions.data_ptr(), batch.slots.data_ptr(), out.data_ptr(),
+                             keys.data_ptr(), values.data_ptr(), self._dtype(), self.bits, batch.tokens, query.shape[1],
+                             self.kv_heads, self.head_dim, 2 * inv_freq.numel(), int(interleaved), q_stride, k_stride,
+                             v_stride, o_stride, self.num_pages, self.page_size, keys.stride(0), float(amplitude), stream)
+            return out
         self.native.call("kudacuda_rope_paged_append", query.data_ptr(), key.data_ptr(), value.data_ptr(),
                          inv_freq.data_ptr(), batch.positions.data_ptr(), batch.slots.data_ptr(), out.data_ptr(),
                          keys.data_ptr(), values.data_ptr(), self._dtype(), batch.tokens, query.shape[1],
@@ -324,8 +348,10 @@ class PagedKvCache:
         o_stride = self._rows("out", out, batch.tokens, heads)
         keys, values = self.keys(layer), self.values(layer)
         n = len(batch.sequences)
-        nbytes = self.native.lib.kudacuda_paged_attention_workspace_bytes(
-            batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads, self.head_dim)
+        lib, sizes = self.native.lib, (batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads,
+                                       self.head_dim)
+        nbytes = (lib.kudacuda_paged_attention_workspace_bytes(*sizes) if self.bits == 16 else
+                  lib.kudacuda_paged_attention_mx_workspace_bytes(self.bits, *sizes))
         stream, capturing = self._use(batch)
         # a workspace a stream: calls on one stream follow one another; a captured call
         # gets its own, from its graph's memory
@@ -334,11 +360,42 @@ class PagedKvCache:
             workspace = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
             if not capturing:
                 self._workspaces[stream] = workspace
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+        if self.bits < 16:
+            self.native.call("kudacuda_paged_attention_mx", query.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                             batch.page_table.data_ptr(), batch.query_starts.data_ptr(), batch.kv_lens.data_ptr(),
+                             out.data_ptr(), workspace.data_ptr() if nbytes > 0 else 0, nbytes, self._dtype(), self.bits,
+                             batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads, self.head_dim,
+                             q_stride, o_stride, self.num_pages, self.page_size, batch.page_table.shape[1],
+                             keys.stride(0), scale, stream)
+            return out
         self.native.call("kudacuda_paged_attention", query.data_ptr(), keys.data_ptr(), values.data_ptr(),
                          batch.page_table.data_ptr(), batch.query_starts.data_ptr(), batch.kv_lens.data_ptr(),
                          out.data_ptr(), workspace.data_ptr() if nbytes > 0 else 0, nbytes, self._dtype(),
                          batch.tokens, n, batch.max_query_len, batch.max_kv_len, heads, self.kv_heads, self.head_dim,
                          q_stride, o_stride, self.num_pages, self.page_size, batch.page_table.shape[1],
-                         keys.stride(0), keys.stride(1), keys.stride(2),
-                         1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), stream)
+                         keys.stride(0), keys.stride(1), keys.stride(2), scale, stream)
         return out
+
+    def read(self, layer: int, sequence: int, start: int = 0, stop: int | None = None) -> tuple[Any, Any]:
+        """What the cache holds for tokens ``start`` .. ``stop`` of a sequence: keys (turned) and values, [tokens,
+        kv_heads, head_dim] in the cache's type."""
+
+        entry = self._entry(sequence)
+        stop = entry.length if stop is None else stop
+        if not 0 <= start <= stop <= entry.length:
+            raise ValueError(f"tokens {start}..{stop} of a sequence of {entry.length}")
+        t, at = self.torch, np.arange(start, stop)
+        slots = np.asarray(entry.pages, dtype=np.int64)[at // self.page_size] * self.page_size + at % self.page_size
+        slots = t.from_numpy(slots).to(self.device)
+        keys, values = self.keys(layer), self.values(layer)
+        if self.bits == 16:
+            page, offset = slots // self.page_size, slots % self.page_size
+            return keys[page, :, offset], values[page, :, offset]
+        rows = t.empty((2, len(at), self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        if len(at) > 0:
+            self.native.call("kudacuda_paged_read_mx", keys.data_ptr(), values.data_ptr(), slots.data_ptr(),
+                             rows[0].data_ptr(), rows[1].data_ptr(), self._dtype(), self.bits, len(at), self.kv_heads,
+                             self.head_dim, rows.stride(1), rows.stride(1), self.num_pages, self.page_size,
+                             keys.stride(0), self._stream())
+        return rows[0], rows[1]
