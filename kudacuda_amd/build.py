@@ -54,6 +54,7 @@ PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=6"]
 # files inside the GEMM's window loop).
 SOURCE_FLAGS = {
     "kc_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kc_mx_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     **{name: PRELOAD for name in ("kc_nf4.hip", "kc_gqa.hip", "kc_lmhead.hip")},
 }
 

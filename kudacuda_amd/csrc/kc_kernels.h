@@ -371,8 +371,8 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
                                    int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                    int64_t workspace_bytes);
 hipError_t launch_paged_attention(Act act, const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t stream);
-// The splits' partials to the output.
-hipError_t launch_paged_merge(Act act, const PagedAttnArgs& args, int64_t splits, hipStream_t stream);
+// The splits' partials to the output; fours: up to 16 splits in groups of four.
+hipError_t launch_paged_merge(Act act, const PagedAttnArgs& args, int64_t splits, bool fours, hipStream_t stream);
 
 // A paged cache of microscaled numbers (kc_mx.h): a page of a pool begins at page *
 // page_stride bytes and holds the elements [kv_heads, page_size, head_dim] of `bits` bits,
@@ -421,7 +421,7 @@ hipError_t launch_mx_read(Act act, const MxReadArgs& args, hipStream_t stream);
 
 // Attention over such a cache: of the arguments, k and v are its pools, page_stride,
 // head_stride and token_stride the bytes between pages, heads and tokens of elements.
-PagedAttnPlan mx_attention_plan(int bits, int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
+PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
                                 int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                 int64_t workspace_bytes);
 hipError_t launch_mx_attention(Act act, int bits, const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t stream);

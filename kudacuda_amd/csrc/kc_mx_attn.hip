@@ -37,157 +37,666 @@ struct MxRow {
     }
 };
 
-// A wave's 32 keys: lane (r, q) holds dims D / 4 * q .. of keys r and 16 + r, which share
-// a power of two; the 16 keys' rows lie in one page.
-template <typename T, int D, int BITS>
-struct MxFewRows : MxRow<T, D, BITS> {
-    static constexpr int kSteps = D / 32;
-    static constexpr int kBytes = D * BITS / 32;  // of a lane
-    static constexpr int kWords = kBytes / 4;
-    const PagedAttnArgs& a;
-    const int32_t* const table;
-    const uint8_t* const kpool;
-    const uint8_t* const vpool;
-    const int g, keys, r, q;
-    bool bad = false;
-    int page[2];
-    MxPlace at[2];
-    uint32_t kw[2][kWords], vw[2][kWords];
-    uint32_t kb[2], vb[2];
+// ------------------------------------------------------------------ few rows
+// The two tiles of 16 keys that a wave takes next: their rows lie in one page each, whose
+// place is the wave's; K straight into the first product's operand, V through LDS.
+//
+// Heads of 128 meet K as it is stored: the scaled matrix instruction takes a row of 128
+// elements with its four blocks' bytes, and the query as e4m3 numbers in PARTS parts with a
+// power of two a block -- 4 bits each, so that two parts are a bf16 query exactly and
+// three an fp16 one, down to 2^-21 and 2^-25 of the largest of a block's 32 dims.  Unpacking
+// K costs more than that in vector instructions, and these are what bounds the kernel
+// beside memory.  Heads of 64 would leave half of the instruction empty: they unpack K.
+typedef int intx8 __attribute__((ext_vector_type(8)));
 
-    static __device__ __forceinline__ int first_dim(int q, int i) { return D / 4 * q + 8 * i; }
-    __device__ __forceinline__ MxFewRows(const PagedAttnArgs& args, const int32_t* table_row, int head, int n, int lane_r,
-                                         int lane_q)
-        : a(args), table(table_row), kpool(reinterpret_cast<const uint8_t*>(args.k)),
-          vpool(reinterpret_cast<const uint8_t*>(args.v)), g(head), keys(n), r(lane_r), q(lane_q) {}
-    __device__ __forceinline__ void pages(int u) {
+// The exponent that makes the largest of a block 128 .. 255.
+__device__ __forceinline__ int query_exponent(float most) {
+    const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127 - 7;
+    return e > -110 ? (e < 120 ? e : 120) : -110;
+}
+// Four numbers' e4m3 parts of this exponent; what is left of the numbers stays.
+__device__ __forceinline__ int query_part(float* x, int exponent) {
+    typedef short shortx2 __attribute__((ext_vector_type(2)));
+    typedef float floatx2 __attribute__((ext_vector_type(2)));
+    const float power = __uint_as_float(static_cast<uint32_t>(exponent + 127) << 23);
+    shortx2 w = {0, 0};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[0], x[1], power, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[2], x[3], power, true);
+    const int word = __builtin_bit_cast(int, w);
+    const floatx2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, power, false);
+    const floatx2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, power, true);
+    x[0] -= lo[0];
+    x[1] -= lo[1];
+    x[2] -= hi[0];
+    x[3] -= hi[1];
+    return word;
+}
+
+template <typename T, int D, int BITS>
+struct MxQuery {  // heads of 64
+    static constexpr int kSteps = D / 32;
+    uint4 part[kSteps];
+    static __device__ __forceinline__ int key_offset(int q, int i) { return (D / 4 * q + 16 * i) * BITS / 8; }
+    __device__ __forceinline__ void load(const uint16_t* row, int q) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int key = u * kUnit + 16 * t;
-            page[t] = table[(key < keys ? key : keys - 1) >> a.page_shift];
+        for (int i = 0; i < kSteps; ++i) {
+            part[i] = *reinterpret_cast<const uint4*>(row + D / 4 * q + 8 * i);
         }
     }
-    __device__ __forceinline__ void place(int u) {
+    __device__ __forceinline__ void form(int) {}
+    template <int WORDS>
+    __device__ __forceinline__ floatx4 scores(const uint32_t (&key)[WORDS], uint32_t byte) const {
+        floatx4 sc = floatx4{};
+        const float power = mx_power(byte);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int key = u * kUnit + 16 * t + r;
-            // (a key past the end reads the last one, in the page of the 16 or before it)
-            at[t] = MxRow<T, D, BITS>::place_of(a, page[t], key < keys ? key : keys - 1, g, bad);
-            at[t].elements += q * kBytes;
-            at[t].blocks += q * (D / 4) / kMxBlock;
+        for (int i = 0; i < kSteps; ++i) {
+            sc = mfma16(T{}, mx_unpack8<T, BITS>(key + i * (BITS / 4), power), part[i], sc);
         }
-    }
-    __device__ __forceinline__ void fetch(uint32_t (&w)[2][kWords], uint32_t (&b)[2], const uint8_t* pool) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            get_words(w[t], pool + at[t].elements);
-            b[t] = pool[at[t].blocks];
-        }
-    }
-    __device__ __forceinline__ void fetch_k() { fetch(kw, kb, kpool); }
-    __device__ __forceinline__ void fetch_v() { fetch(vw, vb, vpool); }
-    template <typename At>
-    __device__ __forceinline__ void store_v(uint8_t* s_v, At at_piece) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const float power = mx_power(vb[t]);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                *reinterpret_cast<uint4*>(s_v + at_piece(16 * t + r, kSteps * q + i)) =
-                    mx_unpack8<T, BITS>(vw[t] + i * (BITS / 4), power);
-            }
-        }
-    }
-    __device__ __forceinline__ uint4 k(int t, int i) const {
-        return mx_unpack8<T, BITS>(kw[t] + i * (BITS / 4), mx_power(kb[t]));
+        return sc;
     }
 };
 
-// A window's rows through registers: a lane takes a block of a row, of K and of V (D =
-// 64: of one of them).  V's rows are dealt so that 16 lanes' stores, and the transposed
-// reads of 4 rows, lie in different banks.
+template <typename T, int BITS>
+struct MxQuery<T, 128, BITS> {
+    static constexpr int kParts = std::is_same<T, Bf16>::value ? 2 : 3;
+    intx8 part[kParts];
+    int byte[kParts];
+    // 8 bits: the instruction's lane q has dims 16 q .. and 64 + 16 q .., 4 bits: 32 q ..
+    static __device__ __forceinline__ int key_offset(int q, int i) { return BITS == 4 ? 16 * q : 16 * q + 64 * i; }
+    uint4 raw[4];
+    __device__ __forceinline__ void load(const uint16_t* row, int q) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            raw[i] = *reinterpret_cast<const uint4*>(row + 64 * (i / 2) + 16 * q + 8 * (i % 2));
+        }
+    }
+    __device__ __forceinline__ void form(int q) {
+        float x[2][16];
+        int e[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float half[8];
+            unpack8<T>(raw[2 * h], half);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[h][i] = half[i];
+            }
+            unpack8<T>(raw[2 * h + 1], half);
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[h][8 + i] = half[i];
+                most = fmaxf(most, fmaxf(fabsf(x[h][i]), fabsf(half[i])));
+            }
+            most = fmaxf(most, __shfl_xor(most, 16, 64));  // a block is two lanes' halves
+            e[h] = query_exponent(most);
+        }
+        const int lane = static_cast<int>(threadIdx.x) & 15;
+        const int low_block = __shfl(e[0], lane + (q == 1 ? 32 : 0), 64);
+        const int high_block = __shfl(e[1], lane + (q == 3 ? 48 : 0), 64);
+        const int block = q < 2 ? low_block : high_block;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+            byte[p] = block - 4 * p + 127;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    part[p][4 * h + i] = query_part(x[h] + 4 * i, e[h] - 4 * p);
+                }
+            }
+        }
+    }
+    template <int WORDS>
+    __device__ __forceinline__ floatx4 scores(const uint32_t (&key)[WORDS], uint32_t power) const {
+        intx8 k;  // (of 4 bits the first half is read)
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            k[i] = static_cast<int>(key[i]);
+        }
+        floatx4 sc = floatx4{};
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+            sc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, part[p], sc, BITS == 4 ? 4 : 0, 0, 0,
+                                                                  static_cast<int>(power), 0, byte[p]);
+        }
+        return sc;
+    }
+};
+
+template <typename T, int D, int BITS>
+struct MxFewTile {
+    static constexpr int kRowBytes = D * BITS / 8;
+    static constexpr int kWords = kRowBytes / 16;  // of a lane's quarter of a row
+    static constexpr int kSteps = D / 32;
+    static constexpr int kDepth = 2;  // units that are on their way
+
+    struct Raw {
+        uint32_t k[2][kWords], v[2][kWords];
+        uint32_t k_byte[2], v_byte[2];
+    };
+
+    static __device__ __forceinline__ void run(const PagedAttnArgs& a, const Sequence& s, int index, int g, int c0, int begin,
+                                               int end, int split, int splits, uint8_t* s_mem, float (*s_ml)[16][2],
+                                               int* s_redo) {
+        constexpr int kPieces = D / 8;  // 16-byte pieces of an unpacked row
+        const int tid = threadIdx.x;
+        const int lane = tid & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int r = lane & 15;
+        const int q = lane >> 4;
+        const int G = static_cast<int>(a.group);
+        const int rows = s.q_len * G;
+        const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
+        uint8_t* const s_v = s_mem + wave * (kUnit * D * 2);
+
+        const int count = rows - c0 < 16 ? rows - c0 : 16;
+        const int column = c0 + (r < count ? r : count - 1);
+        const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
+        const int first_pos = s.kv_len - s.q_len + c0 / G;
+        const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
+        const int keys = ends > 0 ? ends : 0;
+        const int units = (keys + kUnit - 1) / kUnit;
+        const int u_end = end * 4 < units ? end * 4 : units;
+        int unit = begin * 4 + wave;
+
+        // Pages of the wave's next 64 tiles, one a lane: read in the loop, their ids would come
+        // behind the rows that are on their way, since loads return in order.
+        const int last_tile = (keys > 0 ? keys - 1 : 0) & ~15;
+        const int page_mask = (1 << a.page_shift) - 1;
+        int pages = 0;
+        int pages_from = unit;
+        bool bad = false;
+        const auto look = [&](int u) __attribute__((always_inline)) {
+            const int key = (u + lane / 2 * 4) * kUnit + lane % 2 * 16;
+            pages = table[(key < last_tile ? key : last_tile) >> a.page_shift];
+            asm volatile("" : "+v"(pages));  // (waited for here, once in 32 units, not wherever it is read)
+            pages_from = u;
+        };
+        const int k_lane0 = MxQuery<T, D, BITS>::key_offset(q, 0);
+        const int v_lane = q * (kRowBytes / 4);
+        const int b_lane = q * (D / 4) / kMxBlock;
+        const uint8_t* const kpool = reinterpret_cast<const uint8_t*>(a.k);
+        const uint8_t* const vpool = reinterpret_cast<const uint8_t*>(a.v);
+        const auto fetch = [&](int u, Raw& raw) __attribute__((always_inline)) {
+            if (u == pages_from + 4 * 32) {
+                look(u);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int id = __builtin_amdgcn_readlane(pages, (u - pages_from) / 2 + t);
+                const bool out = static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.num_pages);
+                bad |= out;
+                int key = u * kUnit + 16 * t;
+                key = key < last_tile ? key : last_tile;
+                // (rows past the end read the last one)
+                const int row = r < keys - 1 - key ? r : keys - 1 - key;
+                const int64_t at = static_cast<int64_t>(out ? 0 : id) * a.page_stride;
+                const int64_t first = (static_cast<int64_t>(g) << a.page_shift) + (key & page_mask);
+                const uint8_t* const k_at = kpool + at + first * kRowBytes;
+                const uint8_t* const v_at = vpool + at + first * kRowBytes;
+                const int64_t blocks = at + a.block_offset + first * (D / kMxBlock);
+                const uint32_t offset = static_cast<uint32_t>(row * kRowBytes);
+                const uint32_t block = static_cast<uint32_t>(row * (D / kMxBlock) + b_lane);
+                if constexpr (D == 128 && BITS == 8) {
+                    const uint4 x = load_stream(reinterpret_cast<const uint4*>(k_at + (offset + k_lane0)));
+                    const uint4 y = load_stream(reinterpret_cast<const uint4*>(k_at + (offset + k_lane0 + 64)));
+                    raw.k[t][0] = x.x;
+                    raw.k[t][1] = x.y;
+                    raw.k[t][2] = x.z;
+                    raw.k[t][3] = x.w;
+                    raw.k[t][4] = y.x;
+                    raw.k[t][5] = y.y;
+                    raw.k[t][6] = y.z;
+                    raw.k[t][7] = y.w;
+                } else {
+                    get_words(raw.k[t], k_at + (offset + k_lane0));
+                }
+                get_words(raw.v[t], v_at + (offset + v_lane));
+                raw.k_byte[t] = (kpool + blocks)[block];
+                raw.v_byte[t] = (vpool + blocks)[block];
+            }
+        };
+
+        // (the query is requested first: loads return in order)
+        MxQuery<T, D, BITS> query;
+        query.load(a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + (g * G + column % G) * D, q);
+        Raw raw[kDepth];
+        if (unit < u_end) {
+            look(unit);
+            fetch(unit, raw[0]);
+            if (unit + 4 < u_end) {
+                fetch(unit + 4, raw[1]);
+            }
+        }
+        query.form(q);
+        floatx4 acc[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            acc[i] = floatx4{};
+        }
+        float m_run = kNegInf;
+        float l_run = 0.0f;
+        const auto step = [&](Raw& now) __attribute__((always_inline)) {
+            floatx4 sc[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                sc[t] = query.scores(now.k[t], now.k_byte[t]);
+            }
+            // V's rows, their 16-byte pieces swizzled so that the 8 rows of a
+            // transposed half-wave read lie in different banks
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float power = mx_power(now.v_byte[t]);
+                const int row = 16 * t + r;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int piece = (kSteps * q + i) ^ (((row & 7) << 1) % kPieces);
+                    *reinterpret_cast<uint4*>(s_v + row * (D * 2) + piece * 16) =
+                        mx_unpack8<T, BITS>(now.v[t] + i * (BITS / 4), power);
+                }
+            }
+            if (unit + 4 * kDepth < u_end) {
+                fetch(unit + 4 * kDepth, now);
+            }
+            // sc[t][i]: key 16 t + 4 q + i of the unit
+            if (unit * kUnit + kUnit > first_pos + 1) {
+                const int rel = pos - unit * kUnit - 4 * q;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sc[t][i] = 16 * t + i <= rel ? sc[t][i] : kNegInf;
+                    }
+                }
+            }
+            float mx = kNegInf;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    mx = fmaxf(mx, sc[t][i]);
+                }
+            }
+            const auto p16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = halves_max(fmaxf(__uint_as_float(p16[0]), __uint_as_float(p16[1])));
+            const float m_new = fmaxf(m_run, mx * a.scale_log2);
+            if (__any(m_new > m_run)) {
+                const float corr = __builtin_amdgcn_exp2f(m_run - (m_new == kNegInf ? 0.0f : m_new));
+                l_run *= corr;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc[i][e] *= corr;
+                    }
+                }
+                m_run = m_new;
+            }
+            // weights as two 16-bit parts, as over 16-bit rows
+            const float m_w = (m_run == kNegInf ? 0.0f : m_run) - Weights<T>::kFewUp;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[e / 2][2 * (e % 2)], a.scale_log2, -m_w));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[e / 2][2 * (e % 2) + 1], a.scale_log2, -m_w));
+                l_run += p0 + p1;
+                hi[e] = pack(T{}, p0, p1);
+                lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
+            }
+            const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint2 part[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int row = 16 * t + 4 * q + r / 4;
+                    const int piece = (2 * i + (r & 3) / 2) ^ (((row & 7) << 1) % kPieces);
+                    part[t] = read_transposed(s_v + row * (D * 2) + piece * 16 + (r & 1) * 8);
+                }
+                const uint4 vt = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+                acc[i] = mfma16(T{}, vt, ph, acc[i]);
+                acc[i] = mfma16(T{}, vt, pl, acc[i]);
+            }
+        };
+        while (unit < u_end) {
+            step(raw[0]);
+            unit += 4;
+            if (unit >= u_end) {
+                break;
+            }
+            step(raw[1]);
+            unit += 4;
+        }
+        join_waves<T, D, MxRow<T, D, BITS>>(a, s, table, g, c0, count, begin * kRound, u_end * kUnit, split, splits, acc, m_run,
+                                            l_run, bad, s_mem, s_ml, s_redo);
+    }
+};
+
+// A block takes one piece: a share of the rounds of 128 keys of one (sequence, KV head,
+// tile of 16 rows).  Sequences are shared evenly into pieces of at most `longest` rounds,
+// the least number for which the pieces of the batch fit on the chip at once.  (Blocks of
+// equal stretches of all sequences' rounds, as over 16-bit rows, end together, but most of
+// them then begin and end two pieces, and what a piece costs beside its rows -- places
+// found one after the other, a query's parts, the waves' meeting -- is as long as two or
+// three rounds here.)
+constexpr int64_t kFewAtOnce = 512;  // two blocks a CU
+constexpr int kMxFewRows = 32;
+
+// Sums over the block's threads up to and with this one, a wave at a time: the waves' sums
+// are in s_part behind the barrier.
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (*s_part)[N]) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = wave_scan(v[i], [](int x, int y) { return x + y; });
+    }
+    if ((threadIdx.x & 63) == 63) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s_part[wave][i] = v[i];
+        }
+    }
+    __syncthreads();
+}
+template <int N>
+__device__ __forceinline__ int block_sum(int (*s_part)[N], int i) {
+    return __builtin_amdgcn_readfirstlane(s_part[0][i] + s_part[1][i] + s_part[2][i] + s_part[3][i]);
+}
+
+// ceil(n / d) for n < 2^23: the quotient of the nearest floats is at most one off.
+__device__ __forceinline__ int parts_of(int n, int d) {
+    const int up = n + d - 1;
+    int q = static_cast<int>(static_cast<float>(up) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+    q -= q * d > up ? 1 : 0;
+    return q + ((q + 1) * d <= up ? 1 : 0);
+}
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, int splits, int few_rows) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
+    __shared__ float s_ml[4][16][2];
+    constexpr int kTries = 4;
+    __shared__ int s_total[4][2], s_most[4], s_tries[4][kTries];
+    __shared__ int s_found[6];
+    __shared__ int s_redo;
+    const int tid = threadIdx.x;
+    const int sequences = static_cast<int>(a.sequences);
+    const int kv_heads = static_cast<int>(a.kv_heads);
+    const auto pieces_of = [&](const Line& line, int longest) __attribute__((always_inline)) {
+        return kv_heads * line.tiles * parts_of(line.rounds, longest);
+    };
+    int pieces;   // of the batch
+    int longest;  // rounds of a piece
+    int before = 0;      // pieces before this thread's run of sequences (one of up to 256)
+    int own_pieces = 0;  // and in it
+    const int per_thread = (sequences + kThreads - 1) / kThreads;
+    const int run = tid * per_thread;
+    Sequence own = {};
+    if (sequences == 1) {
+        own = wave_sequence(a, 0);
+        const Line line = line_of(a, own, few_rows, splits);
+        const int heads = kv_heads * line.tiles;
+        const int share = heads > 0 ? static_cast<int>(kFewAtOnce) / heads : 1;  // pieces of a tile
+        const int parts = share < 1 ? 1 : (share < splits ? share : splits);
+        longest = (line.rounds + parts - 1) / parts;
+        pieces = pieces_of(line, longest);
+    } else {
+        const int run_end = run + per_thread < sequences ? run + per_thread : sequences;
+        Line line = {};
+        int total[2] = {};  // rounds, tiles
+        int most = 1;
+        bool descending = false;  // (such starts name no rows: their lengths need not fit the line)
+        for (int i = run; i < run_end; ++i) {
+            own = sequence(a, i);
+            descending |= a.starts[i + 1] < a.starts[i];
+            line = line_of(a, own, few_rows, splits);
+            total[0] += length_of(a, line);
+            total[1] += kv_heads * line.tiles;
+            most = line.tiles > 0 && line.rounds > most ? line.rounds : most;
+        }
+        most = wave_scan(descending ? 0x7fffffff : most, [](int x, int y) { return x > y ? x : y; });
+        if ((tid & 63) == 63) {
+            s_most[tid >> 6] = most;
+        }
+        block_scan(total, s_total);
+        total[0] = block_sum(s_total, 0);
+        total[1] = block_sum(s_total, 1);
+        most = __builtin_amdgcn_readfirstlane(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
+        if (most == 0x7fffffff || total[0] == 0) {
+            return;
+        }
+        // candidates from an even share of the rounds on, to where every tile may have a
+        // short last piece
+        const int at_once = static_cast<int>(kFewAtOnce);
+        const int spare = at_once - total[1] > at_once / 4 ? at_once - total[1] : at_once / 4;
+        int least = (total[0] + at_once - 1) / at_once;
+        const int allowed = (most + splits - 1) / splits;
+        least = least > allowed ? least : allowed;
+        const int enough = (total[0] + spare - 1) / spare;
+        const int step = enough > least ? (enough - least + kTries - 2) / (kTries - 1) : 1;
+        int tries[kTries] = {};
+        for (int i = run; i < run_end; ++i) {
+            if (per_thread > 1) {
+                line = line_of(a, sequence(a, i), few_rows, splits);
+            }
+#pragma unroll
+            for (int t = 0; t < kTries; ++t) {
+                tries[t] += pieces_of(line, least + t * step);
+            }
+        }
+        int mine[kTries];
+#pragma unroll
+        for (int t = 0; t < kTries; ++t) {
+            mine[t] = tries[t];
+        }
+        block_scan(tries, s_tries);
+        longest = 0;
+        pieces = 0;
+#pragma unroll
+        for (int t = kTries - 1; t >= 0; --t) {
+            const int sum = block_sum(s_tries, t);
+            if (sum <= at_once || t == kTries - 1) {  // (more tiles than fit at once: the last)
+                longest = least + t * step;
+                pieces = sum;
+                own_pieces = mine[t];
+                before = tries[t] - mine[t];
+                for (int w = 0; w < (tid >> 6); ++w) {
+                    before += s_tries[w][t];
+                }
+            }
+        }
+    }
+    const int piece = static_cast<int>(blockIdx.x);
+    if (piece >= pieces) {
+        return;
+    }
+    int index = 0;
+    int first = 0;  // the first piece of the sequence
+    Sequence s = own;
+    if (sequences > 1) {
+        // the thread whose sequences the piece is of tells which
+        if (before <= piece && piece < before + own_pieces) {
+            int i = run;
+            for (; per_thread > 1; ++i) {
+                own = sequence(a, i);
+                const int next = before + pieces_of(line_of(a, own, few_rows, splits), longest);
+                if (piece < next) {
+                    break;
+                }
+                before = next;
+            }
+            s_found[0] = i;
+            s_found[1] = before;
+            s_found[2] = own.first;
+            s_found[3] = own.q_len;
+            s_found[4] = own.kv_len;
+            s_found[5] = own.bad;
+        }
+        __syncthreads();
+        index = __builtin_amdgcn_readfirstlane(s_found[0]);
+        first = __builtin_amdgcn_readfirstlane(s_found[1]);
+        s.first = __builtin_amdgcn_readfirstlane(s_found[2]);
+        s.q_len = __builtin_amdgcn_readfirstlane(s_found[3]);
+        s.kv_len = __builtin_amdgcn_readfirstlane(s_found[4]);
+        s.bad = __builtin_amdgcn_readfirstlane(s_found[5]) != 0;
+    }
+    const Line line = line_of(a, s, few_rows, splits);
+    const int parts = parts_of(line.rounds, longest);
+    const int split = (piece - first) % parts;
+    const int tile = (piece - first) / parts;
+    const int g = tile / line.tiles;
+    const int c0 = tile % line.tiles * 16;
+    const int rest = s.q_len * static_cast<int>(a.group) - c0;
+    const int count = rest < 16 ? rest : 16;
+    if (s.bad) {
+        if (split == 0) {
+            nan_columns<T, D>(a, s, g, c0, count, splits);
+        }
+        return;
+    }
+    if (split == 0 && splits > 1) {
+        tell_splits<D>(a, s, g, c0, count, parts, splits);
+    }
+    const int share = (line.rounds + parts - 1) / parts;
+    const int end = share * (split + 1) < line.rounds ? share * (split + 1) : line.rounds;
+    MxFewTile<T, D, BITS>::run(a, s, index, g, c0, split * share, splits > 1 ? end : 0x7fffffff / kRound, split, splits, s_mem,
+                               s_ml, &s_redo);
+}
+
+// ----------------------------------------------------------------- row tiles
+// A window's rows through registers, unpacked into what the tiles over 16-bit rows have in
+// LDS: a wave takes 16 rows of K and of V, which lie in one page, a lane a block of a row of
+// both (D = 64: lanes 0 .. 31 K's, the others V's).  V's rows are dealt so that 16 lanes'
+// stores, and the transposed reads of 4 rows, lie in different banks.  The products, the
+// arithmetic and LDS are each about as busy there, and unpacking adds to two of them: a
+// prompt of 8192 tokens takes 7 % longer than over 16-bit rows.  (Measured instead: the
+// same behind the barrier, a window later, 5 % slower; K kept packed, its products by scaled
+// instructions with the query in parts, as above for few rows, 1 % faster in bf16 heads of
+// 128 in 4 bits, 2 % slower in 8, 9 % in fp16, with three parts, and 18 % in heads of 64.)
 template <typename T, int D, int BITS>
 struct MxWindow {
     using Rows = MxRow<T, D, BITS>;
+    static constexpr bool kTwoBlocks = false;
     static constexpr int kParts = D / 64;
+    static constexpr int kRowBytes = D * BITS / 8;
     static constexpr int kWords = kMxBlock * BITS / 32;
     static constexpr int kTileBytes = kWindow * D * 2;
+    static constexpr int kKeyBytes = kTileBytes;
+    static constexpr int kBufferBytes = 2 * kTileBytes;
     const PagedAttnArgs& a;
     const int32_t* const table;
-    const int g, keys;
+    const int keys, lane, wave;
+    const int64_t head_row;  // the head's first row in a page
+    const int last_tile;
     uint8_t* const lds;
-    int row[kParts];
+    const uint8_t* pool[kParts];
+    int row[kParts];  // of the wave's 16
     int block[kParts];
-    bool value[kParts];
-    int page[kParts];
+    int place[kParts];  // in LDS
+    int page = 0;
     uint32_t words[kParts][kWords];
     uint32_t bytes[kParts];
+    uint4 qf[D / 16];
     bool bad = false;
 
     static __device__ __forceinline__ int k_place(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
     static __device__ __forceinline__ int v_place(int row) {
         return (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2) | ((row >> 2) & 3);
     }
-    __device__ __forceinline__ MxWindow(const PagedAttnArgs& args, const int32_t* table_row, int head, int n, int lane, int wave,
+    __device__ __forceinline__ MxWindow(const PagedAttnArgs& args, const int32_t* table_row, int head, int n, int lane_id, int wave_id,
                                         uint8_t* buffers)
-        : a(args), table(table_row), g(head), keys(n), lds(buffers) {
+        : a(args), table(table_row), keys(n), lane(lane_id), wave(wave_id), head_row(static_cast<int64_t>(head) << args.page_shift),
+          last_tile((n > 0 ? n - 1 : 0) & ~15), lds(buffers) {
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
+            const bool value = D == 128 ? p == 1 : lane >= 32;
             if constexpr (D == 128) {
-                value[p] = p == 1;
                 block[p] = lane & 3;
-                row[p] = 16 * wave + (value[p] ? (lane >> 4) + 4 * ((lane >> 2) & 3) : lane >> 2);
+                row[p] = value ? (lane >> 4) + 4 * ((lane >> 2) & 3) : lane >> 2;
             } else {
-                value[p] = wave >= 2;
                 block[p] = lane & 1;
-                row[p] = 32 * (wave & 1) + (value[p] ? ((lane >> 1) & 1) + 4 * ((lane >> 2) & 3) + 2 * ((lane >> 4) & 1) +
-                                                           16 * (lane >> 5)
-                                                     : lane >> 1);
+                row[p] = value ? ((lane >> 1) & 1) + 4 * ((lane >> 2) & 3) + 2 * ((lane >> 4) & 1) : lane >> 1;
             }
-            page[p] = 0;
+            pool[p] = reinterpret_cast<const uint8_t*>(value ? a.v : a.k);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                words[p][i] = 0;
+            }
+            place[p] = (value ? kTileBytes : 0) + (16 * wave + row[p]) * (D * 2) +
+                       16 * ((4 * block[p]) ^ (value ? v_place(row[p]) : k_place(row[p])));
             bytes[p] = 0;
         }
     }
-    __device__ __forceinline__ int key_of(int w, int p) const {
-        const int key = w * kWindow + row[p];
-        return key < keys ? key : keys - 1;
+    __device__ __forceinline__ int tile_of(int w) const {
+        const int key = w * kWindow + 16 * wave;
+        return key < last_tile ? key : last_tile;
     }
-    __device__ __forceinline__ void look(int w) {
+    __device__ __forceinline__ void look(int w) { page = table[tile_of(w) >> a.page_shift]; }
+    __device__ __forceinline__ void fetch(int w) {
+        const int key = tile_of(w);
+        const int id = __builtin_amdgcn_readfirstlane(page);
+        const bool out = static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.num_pages);
+        bad |= out;
+        const int64_t first = head_row + (key & ((1 << a.page_shift) - 1));
+        const int64_t at = static_cast<int64_t>(out ? 0 : id) * a.page_stride;
+        const int64_t elements = at + first * kRowBytes;
+        const int64_t blocks = at + a.block_offset + first * (D / kMxBlock);
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
-            page[p] = table[key_of(w, p) >> a.page_shift];
+            // (rows past the end read the last one)
+            const int mine = row[p] < keys - 1 - key ? row[p] : keys - 1 - key;
+            get_words(words[p], pool[p] + elements + static_cast<uint32_t>(mine * kRowBytes + block[p] * (4 * kWords)));
+            bytes[p] = (pool[p] + blocks)[static_cast<uint32_t>(mine * (D / kMxBlock) + block[p])];
         }
     }
-    __device__ __forceinline__ void fetch(int w, int) {
+    // The rows that have come, unpacked into LDS.  (Where there is no such window it is the last
+    // rows again, and nobody reads them.)
+    __device__ __forceinline__ void arrive(int buffer) {
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
-            const MxPlace at = Rows::place_of(a, page[p], key_of(w, p), g, bad);
-            const uint8_t* const pool = reinterpret_cast<const uint8_t*>(value[p] ? a.v : a.k);
-            get_words(words[p], pool + at.elements + block[p] * (4 * kWords));
-            bytes[p] = pool[at.blocks + block[p]];
-        }
-    }
-    __device__ __forceinline__ void arrive(bool live, int buffer) {
-        if (!live) {
-            return;
-        }
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-            uint8_t* const at = lds + buffer * (2 * kTileBytes) + (value[p] ? kTileBytes : 0) + row[p] * (D * 2);
-            const int place = value[p] ? v_place(row[p]) : k_place(row[p]);
             const float power = mx_power(bytes[p]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                *reinterpret_cast<uint4*>(at + ((4 * block[p] + j) ^ place) * 16) =
+                *reinterpret_cast<uint4*>(lds + buffer * kBufferBytes + (place[p] ^ (16 * j))) =
                     mx_unpack8<T, BITS>(words[p] + j * (BITS / 4), power);
             }
         }
+    }
+    __device__ __forceinline__ void start(int w, int step, int) {
+        look(w);
+        fetch(w);
+        look(w + step);
+    }
+    __device__ __forceinline__ void next(int w, int step, int, int) {
+        fetch(w);
+        look(w + step);
+    }
+    __device__ __forceinline__ void query(const uint16_t* row) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            qf[i] = *reinterpret_cast<const uint4*>(row + 8 * (lane >> 5) + 16 * i);
+        }
+    }
+    template <typename Late>
+    __device__ __forceinline__ void scores(floatx16 (&sc)[2], int buffer, Late late) {
+        tile_scores<T, D, MxWindow>(sc, qf, lds + buffer * kBufferBytes, lane, late);
     }
 };
 
 template <typename T, int D, int BITS>
 hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
-    return launch_kernels<T, D, MxFewRows<T, D, BITS>, MxWindow<T, D, BITS>>(a, plan, stream);
+    if (plan.few_blocks > 0) {
+        hipLaunchKernelGGL((mx_few_kernel<T, D, BITS>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(kThreads), 0, stream,
+                           a, static_cast<int>(plan.splits), plan.tile_splits > 0 ? kMxFewRows : 0x7fffffff);
+        const hipError_t status = hipGetLastError();
+        if (status != hipSuccess) {
+            return status;
+        }
+    }
+    return launch_tiles<T, D, MxWindow<T, D, BITS>>(a, plan, kMxFewRows, true, stream);
 }
 template <typename T>
 hipError_t launch(int bits, const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
@@ -199,11 +708,44 @@ hipError_t launch(int bits, const PagedAttnArgs& a, const PagedAttnPlan& plan, h
 
 }  // namespace
 
-PagedAttnPlan mx_attention_plan(int, int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
+PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
                                 int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                 int64_t workspace_bytes) {
-    return paged_attention_plan(tokens, sequences, max_query_len, max_kv_len, max_keys, q_heads, kv_heads, head_dim,
-                                workspace_bytes);
+    const int64_t group = q_heads / kv_heads;
+    PagedAttnPlan p;
+    const int64_t longest = max_query_len < tokens ? max_query_len : tokens;
+    const int64_t rows = longest * group;
+    const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
+    const int64_t rounds = (max_kv_len + kRound - 1) / kRound;
+    const bool few = rows <= kMxFewRows;
+    if (!few) {
+        plan_tiles(p, tokens, sequences, group, rows, windows, kv_heads, head_dim);
+    }
+    int64_t few_splits = 0;
+    if (few || (tokens != sequences * longest && windows > 50 * p.tile_splits)) {
+        // Where no other sequence is split: up to 5 rounds in one piece (a token over 512
+        // keys 9.1 us so, 10.7 split and merged; over 768 11.2 and 10.7).
+        const int64_t tiles = sequences * kv_heads * ((cap(rows, kMxFewRows) + 15) / 16);
+        few_splits = p.tile_splits <= 1 && rounds <= 5 ? 1 : cap(2 * ((kFewAtOnce + tiles - 1) / tiles) + 1, cap(rounds, 256));
+    }
+    const int64_t unit = tokens * q_heads * (head_dim + 2) * 4;
+    const int64_t counts = tokens * q_heads * 4;
+    const int64_t room = unit > 0 ? (workspace_bytes - counts) / unit : 0;
+    // the pieces of few rows are counted in 31 bits
+    const int64_t all_tiles = kv_heads * (few ? tokens * group / 16 + sequences : sequences * (kMxFewRows / 16));
+    const bool countable = all_tiles * ((max_keys + kRound - 1) / kRound) < (int64_t{1} << 31);
+    const int64_t most = room > 1 && countable ? room : 1;
+    few_splits = few_splits < most ? few_splits : most;
+    p.tile_splits = p.tile_splits < most ? p.tile_splits : most;
+    p.splits = few_splits > p.tile_splits ? few_splits : p.tile_splits;
+    p.workspace_bytes = p.splits > 1 ? unit * p.splits + counts : 0;
+    if (few_splits > 0) {
+        // a block a piece, whatever the lengths are: at most a quarter of those at once and
+        // one more a tile where the tiles alone are more than fit
+        const int64_t pieces = all_tiles + kFewAtOnce / 4 > kFewAtOnce ? all_tiles + kFewAtOnce / 4 : kFewAtOnce;
+        p.few_blocks = pieces < all_tiles * p.splits ? pieces : all_tiles * p.splits;
+    }
+    return p;
 }
 
 hipError_t launch_mx_attention(Act act, int bits, const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {

@@ -289,193 +289,75 @@ __device__ __forceinline__ int length_of(const PagedAttnArgs& a, const Line& lin
     return static_cast<int>(a.kv_heads) * line.tiles * line.rounds;
 }
 
-//
-// Rows reads 32 keys of a wave: pages(u) and place(u) find unit u's keys, fetch_k() and
-// fetch_v() request them, store_v() puts V's rows in LDS, 8 elements a piece, and k(t, i)
-// is the lane's part of the product i of key 16 t + r: dims first_dim(q, i) .. + 7.
+// The four waves' columns meet in LDS (s_mem: 64 * D floats, each wave's part in its own
+// quarter) and go out: a lane (r, q) holds dims 16 i + 4 q .. + 3 of column r in acc[i], its
+// maximum m_run and its part of the sum.  Keys [begin, end) are summed again with care
+// where anything is not finite.
 template <typename T, int D, typename Rows>
-__device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequence& s, int index, int g, int c0,
-                                              int begin, int end, int split, int splits, uint8_t* s_mem,
-                                              float (*s_ml)[16][2], int* s_redo) {
-    constexpr int kSteps = D / 32;   // products of 32 dims a score
-    constexpr int kPieces = D / 8;   // 16-byte pieces of a row
+__device__ __forceinline__ void join_waves(const PagedAttnArgs& a, const Sequence& s, const int32_t* table, int g, int c0,
+                                           int count, int begin, int end, int split, int splits,
+                                           const floatx4 (&acc)[D / 16], float m_run, float l_run, bool bad,
+                                           uint8_t* s_mem, float (*s_ml)[16][2], int* s_redo) {
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15;
     const int q = lane >> 4;
     const int G = static_cast<int>(a.group);
-    const int rows = s.q_len * G;
-    const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
-    uint8_t* const s_v = s_mem + wave * (kUnit * D * 2);
-
-    const int count = rows - c0 < 16 ? rows - c0 : 16;
-    const int column = c0 + (r < count ? r : count - 1);
-    const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
-    const int head = g * G + column % G;
-    const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
-    const int keys = ends > 0 ? ends : 0;
-    const int units = (keys + kUnit - 1) / kUnit;
-    const int u_end = end * 4 < units ? end * 4 : units;
-    int unit = begin * 4 + wave;
-
-    uint4 qf[kSteps];
-    {
-        const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            qf[i] = *reinterpret_cast<const uint4*>(src + Rows::first_dim(q, i));
-        }
-    }
-    Rows cached(a, table, g, keys, r, q);
-    floatx4 acc[D / 16];
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        acc[i] = floatx4{};
-    }
-    float m_run = kNegInf;
-    float l_run = 0.0f;
-    if (unit < u_end) {
-        cached.pages(unit);
-        cached.place(unit);
-        cached.fetch_k();
-        cached.fetch_v();
-        cached.pages(unit + 4);
-    }
-    for (; unit < u_end; unit += 4) {
-        // V's rows, their 16-byte pieces swizzled so that the 8 rows of a
-        // transposed half-wave read lie in different banks
-        cached.store_v(s_v, [&](int row, int piece) __attribute__((always_inline)) {
-            return row * (D * 2) + (piece ^ (((row & 7) << 1) % kPieces)) * 16;
-        });
-        const bool more = unit + 4 < u_end;
-        if (more) {
-            cached.place(unit + 4);
-            cached.fetch_v();
-            cached.pages(unit + 8);
-        }
-        floatx4 sc[2] = {floatx4{}, floatx4{}};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            sc[0] = mfma16(T{}, cached.k(0, i), qf[i], sc[0]);
-            sc[1] = mfma16(T{}, cached.k(1, i), qf[i], sc[1]);
-        }
-        if (more) {
-            cached.fetch_k();
-        }
-        // sc[t][i]: key 16 t + 4 q + i of the unit
-        const int rel = pos - unit * kUnit - 4 * q;
-        float mx = kNegInf;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[t][i] = 16 * t + i <= rel ? sc[t][i] * a.scale_log2 : kNegInf;
-                mx = fmaxf(mx, sc[t][i]);
-            }
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float m_new = fmaxf(m_run, mx);
-        const float m_sub = m_new == kNegInf ? 0.0f : m_new;
-        const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
-        m_run = m_new;
-        l_run *= corr;
-        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16; in fp16 22,
-        // one fewer for each power of two below 2^-17 of the largest, none below 2^-39:
-        // 2^20 such keys would be 2^-19 of it, in l_run alone): this form waits for
-        // memory, the second product is free
-        const float m_w = m_sub - Weights<T>::kFewUp;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_w);
-            const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_w);
-            l_run += p0 + p1;
-            hi[e] = pack(T{}, p0, p1);
-            lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
-        }
-        const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            uint2 part[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int row = 16 * t + 4 * q + r / 4;
-                const int piece = (2 * i + (r & 3) / 2) ^ (((row & 7) << 1) % kPieces);
-                part[t] = read_transposed(s_v + row * (D * 2) + piece * 16 + (r & 1) * 8);
-            }
-            const uint4 vt = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[i][e] *= corr;
-            }
-            acc[i] = mfma16(T{}, vt, ph, acc[i]);
-            acc[i] = mfma16(T{}, vt, pl, acc[i]);
-        }
-    }
     l_run += __shfl_xor(l_run, 16, 64);
     l_run += __shfl_xor(l_run, 32, 64);
-    // the waves' columns meet in LDS, each in the wave's own part: [column][dim]
-    __syncthreads();
+    // the waves' columns meet in LDS, each in the wave's own part, which no other wave reads
+    // before: [column][dim], rotated so that the 16 columns of a store start in different banks
     if (tid == 0) {
         *s_redo = 0;
     }
-    float* const s_acc = reinterpret_cast<float*>(s_mem);  // [wave][16][D / 2]: half of the dims a round
+    float* const s_acc = reinterpret_cast<float*>(s_mem);  // [wave][16][D]
     if (q == 0) {
         s_ml[wave][r][0] = m_run - Weights<T>::kFewUp;
         s_ml[wave][r][1] = l_run;
     }
-    bool redo = cached.bad;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        __syncthreads();
-        // a padded, rotated row: the 16 columns of a store start in different banks
+    for (int i = 0; i < D / 16; ++i) {
+        const int dim = 16 * i + 4 * q;
+        *reinterpret_cast<float4*>(s_acc + (wave * 16 + r) * D + (dim ^ ((r & 7) * 4))) =
+            make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    }
+    __syncthreads();
+    bool redo = bad;
+    constexpr int kChunks = D / 8;  // 8 dims of a row
+    if (tid < 16 * kChunks) {
+        const int c = tid / kChunks;
+        const int d = tid % kChunks * 8;
+        float m = s_ml[0][c][0];
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int dim = 16 * i + 4 * q;
-            *reinterpret_cast<float4*>(s_acc + (wave * 16 + r) * (D / 2) + (dim ^ ((r & 7) * 4))) =
-                make_float4(acc[half * (D / 32) + i][0], acc[half * (D / 32) + i][1], acc[half * (D / 32) + i][2],
-                            acc[half * (D / 32) + i][3]);
+        for (int w = 1; w < 4; ++w) {
+            m = fmaxf(m, s_ml[w][c][0]);
         }
-        __syncthreads();
-        constexpr int kChunks = D / 16;  // 8 dims of a half row
-        if (tid < 16 * kChunks) {
-            const int c = tid / kChunks;
-            const int d = tid % kChunks * 8;
-            float m = s_ml[0][c][0];
+        const float m_sub = m == kNegInf ? 0.0f : m;
+        float l = 0.0f;
+        float v[8] = {};
 #pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                m = fmaxf(m, s_ml[w][c][0]);
-            }
-            const float m_sub = m == kNegInf ? 0.0f : m;
-            float l = 0.0f;
-            float v[8] = {};
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[w][c][0] - m_sub);
+            l = fmaf(s_ml[w][c][1], f, l);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(s_ml[w][c][0] - m_sub);
-                l = fmaf(s_ml[w][c][1], f, l);
+            for (int j = 0; j < 2; ++j) {
+                const float4 p = *reinterpret_cast<const float4*>(s_acc + (w * 16 + c) * D + ((d + 4 * j) ^ ((c & 7) * 4)));
+                v[4 * j] = fmaf(p.x, f, v[4 * j]);
+                v[4 * j + 1] = fmaf(p.y, f, v[4 * j + 1]);
+                v[4 * j + 2] = fmaf(p.z, f, v[4 * j + 2]);
+                v[4 * j + 3] = fmaf(p.w, f, v[4 * j + 3]);
+            }
+        }
+        float zero = l * 0.0f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float4 p = *reinterpret_cast<const float4*>(s_acc + (w * 16 + c) * (D / 2) +
-                                                                     ((d + 4 * j) ^ ((c & 7) * 4)));
-                    v[4 * j] = fmaf(p.x, f, v[4 * j]);
-                    v[4 * j + 1] = fmaf(p.y, f, v[4 * j + 1]);
-                    v[4 * j + 2] = fmaf(p.z, f, v[4 * j + 2]);
-                    v[4 * j + 3] = fmaf(p.w, f, v[4 * j + 3]);
-                }
-            }
-            float zero = l * 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                zero = fmaf(v[j], 0.0f, zero);
-            }
-            redo |= zero != zero;
-            if (c < count) {
-                const int col = c0 + c;
-                put_column<T, D>(a, s.first + col / G, g * G + col % G, half * (D / 2) + d, v, m, l, split, splits);
-            }
+        for (int j = 0; j < 8; ++j) {
+            zero = fmaf(v[j], 0.0f, zero);
+        }
+        redo |= zero != zero;
+        if (c < count) {
+            const int col = c0 + c;
+            put_column<T, D>(a, s.first + col / G, g * G + col % G, d, v, m, l, split, splits);
         }
     }
     if (redo) {
@@ -483,141 +365,23 @@ __device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequ
     }
     __syncthreads();
     if (*s_redo != 0) {
-        careful_columns<T, D, Rows>(a, s, table, g, c0, count, begin * kRound, u_end * kUnit, split, splits);
+        careful_columns<T, D, Rows>(a, s, table, g, c0, count, begin, end, split, splits);
     }
     __syncthreads();
 }
 
-template <typename T, int D, typename Rows>
-__device__ __forceinline__ void few_rows_stretch(const PagedAttnArgs& a, int splits, int few_rows) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
-    __shared__ float s_ml[4][16][2];
-    __shared__ int s_part[4], s_most[4];
-    __shared__ int s_found[6];
-    __shared__ int s_redo;
-    const int tid = threadIdx.x;
-    const int sequences = static_cast<int>(a.sequences);
-    // (the line's length fits in 31 bits: the plan splits nothing where it might not)
-    // a thread's run of sequences (one of up to 256): the run's part of the line, where
-    // it begins, and its first sequence
-    const int per_thread = (sequences + kThreads - 1) / kThreads;
-    int mine = 0;
-    int mine_before = 0;
-    Sequence own = {};
-    int total, most;
-    if (sequences == 1) {
-        const Line line = line_of(a, wave_sequence(a, 0), few_rows, splits);
-        total = length_of(a, line);
-        most = line.rounds;
-    } else {
-        const int run_end = (tid + 1) * per_thread < sequences ? (tid + 1) * per_thread : sequences;
-        int longest = 1;
-        bool descending = false;  // (such starts name no rows: their lengths need not fit the line)
-        for (int i = tid * per_thread; i < run_end; ++i) {
-            own = sequence(a, i);
-            descending |= a.starts[i + 1] < a.starts[i];
-            const Line line = line_of(a, own, few_rows, splits);
-            mine += length_of(a, line);
-            longest = line.tiles > 0 && line.rounds > longest ? line.rounds : longest;
-        }
-        longest = descending ? 0x7fffffff : longest;
-        int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int left = __shfl_up(sum, o, 64);
-            const int other = __shfl_xor(longest, o, 64);
-            sum += (tid & 63) >= o ? left : 0;
-            longest = other > longest ? other : longest;
-        }
-        if ((tid & 63) == 63) {
-            s_part[tid >> 6] = sum;
-            s_most[tid >> 6] = longest;
-        }
-        __syncthreads();
-        total = __builtin_amdgcn_readfirstlane(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
-        most = __builtin_amdgcn_readfirstlane(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
-        if (most == 0x7fffffff) {
-            return;
-        }
-        mine_before = sum - mine;
-        for (int w = 0; w < (tid >> 6); ++w) {
-            mine_before += s_part[w];
-        }
-    }
-    // a stretch: an even share, and long enough that no tile lies in more than `splits`
-    const int blocks = static_cast<int>(gridDim.x);
-    int stretch = (total + blocks - 1) / blocks;
-    const int least = splits > 1 ? (most + splits - 2) / (splits - 1) : 1;
-    stretch = stretch > least ? stretch : least;
-    const int64_t begin = static_cast<int64_t>(blockIdx.x) * stretch;
-    if (begin >= total) {
-        return;
-    }
-    int at = static_cast<int>(begin);
-    const int stop = at + stretch < total ? at + stretch : total;
-    int index, before;
-    Sequence s;
-    if (sequences == 1) {
-        index = 0;
-        before = 0;
-        s = wave_sequence(a, 0);
-    } else {
-        // the thread whose sequences the stretch begins in tells which
-        if (mine_before <= at && at < mine_before + mine) {
-            int i = tid * per_thread;
-            for (; per_thread > 1; ++i) {
-                own = sequence(a, i);
-                const int next = mine_before + length_of(a, line_of(a, own, few_rows, splits));
-                if (at < next) {
-                    break;
-                }
-                mine_before = next;
-            }
-            s_found[0] = i;
-            s_found[1] = mine_before;
-            s_found[2] = own.first;
-            s_found[3] = own.q_len;
-            s_found[4] = own.kv_len;
-            s_found[5] = own.bad;
-        }
-        __syncthreads();
-        index = __builtin_amdgcn_readfirstlane(s_found[0]);
-        before = __builtin_amdgcn_readfirstlane(s_found[1]);
-        s.first = __builtin_amdgcn_readfirstlane(s_found[2]);
-        s.q_len = __builtin_amdgcn_readfirstlane(s_found[3]);
-        s.kv_len = __builtin_amdgcn_readfirstlane(s_found[4]);
-        s.bad = __builtin_amdgcn_readfirstlane(s_found[5]) != 0;
-    }
-    for (;;) {
-        const Line line = line_of(a, s, few_rows, splits);
-        const int next = before + length_of(a, line);
-        while (at < stop && at < next) {
-            const int piece = (at - before) / line.rounds;
-            const int first = before + piece * line.rounds;
-            const int to = stop - first < line.rounds ? stop - first : line.rounds;
-            const int g = piece / line.tiles;
-            const int c0 = piece % line.tiles * 16;
-            const int rest = s.q_len * static_cast<int>(a.group) - c0;
-            const int count = rest < 16 ? rest : 16;
-            const int split = splits > 1 ? static_cast<int>(blockIdx.x) - first / stretch : 0;
-            if (s.bad) {
-                nan_columns<T, D>(a, s, g, c0, count, splits);
-            } else {
-                if (to == line.rounds && splits > 1) {
-                    tell_splits<D>(a, s, g, c0, count, split + 1, splits);
-                }
-                few_rows_tile<T, D, Rows>(a, s, index, g, c0, at - first, splits > 1 ? to : 0x7fffffff / kRound, split,
-                                          splits, s_mem, s_ml, &s_redo);
-            }
-            at = first + to;
-        }
-        if (at >= stop) {
-            return;
-        }
-        before = next;
-        s = wave_sequence(a, ++index);
-    }
+// Lanes 0 .. own of the wave joined, by shifts in rows of 16 and broadcasts of their last
+// lanes; 0 joins in nothing.
+template <typename Join>
+__device__ __forceinline__ int wave_scan(int v, Join join) {
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+    v = join(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+    return join(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
 }
+
 // ----------------------------------------------------------------- row tiles
 // 128 columns of a (sequence, KV head): four waves of 32 over the same 64 keys,
 // whose K and V rows go straight to LDS, one window ahead.  Two waves a SIMD hide
@@ -650,6 +414,19 @@ constexpr int kTileRows = 128;
 constexpr int kFineRows = 32;
 constexpr int kWindow = 64;
 
+// 16 bytes a lane from base + offset straight into LDS, lane after lane from `lds`.
+// (As an instruction of its own: behind the builtin the compiler waits for the load
+// before the next LDS read, whatever that reads.  It writes no register; the wait is
+// the window's own.  Nothing else in these kernels keeps a value in m0.)
+__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void load_lds16(const uint16_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
+}
 __device__ __forceinline__ float halves_max(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
@@ -659,19 +436,66 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// A window's products with K's rows of 16-bit numbers, 8 a piece, piece i of row j at place
+// i ^ k_place(j): operands are read ahead, held there by the scheduling barriers; a wave
+// that multiplies goes before one that does arithmetic.
+template <typename T, int D, typename Window, typename Late>
+__device__ __forceinline__ void tile_scores(floatx16 (&sc)[2], const uint4 (&qf)[D / 16], const uint8_t* s_k, int lane,
+                                            Late late) {
+    constexpr int kSteps = D / 16;
+    const int r = lane & 31;
+    const int q = lane >> 5;
+    const auto read_k = [&](uint4 (&k)[2], int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int row = 32 * t + r;
+            const int piece = (2 * i + q) ^ Window::k_place(row);
+            k[t] = *reinterpret_cast<const uint4*>(s_k + row * (D * 2) + piece * 16);
+        }
+    };
+    constexpr int kAhead = D == 128 ? 2 : 1;
+    uint4 kf[kAhead + 1][2];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        read_k(kf[i], i);
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        if (i + kAhead < kSteps) {
+            read_k(kf[(i + kAhead) % (kAhead + 1)], i + kAhead);
+        }
+        if (i + 2 >= kSteps) {
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d) {
+                late((i + 2 - kSteps) * (D / 64) + d);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            sc[t] = mfma32(T{}, kf[i % (kAhead + 1)][t], qf[i], sc[t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+}
+
 // Tile slots: sequence i owns slots from floor(starts[i] G / 128) + i on, at least
 // as many as it has tiles, so the grid follows from the token count alone.
 //
-// Window brings windows of 64 keys to LDS: look(w) finds window w's pages, fetch(w,
-// buffer) requests its rows, arrive(live, buffer) sees this wave's part of them into LDS,
-// row by row of 8 elements a piece, piece i of row j of K at place i ^ k_place(j), of V at
-// i ^ v_place(j).
+// Window brings windows of 64 keys to LDS, a buffer of kBufferBytes each: K as its own
+// products take it, and kKeyBytes behind it V's rows of 16-bit numbers, 8 a piece, piece i
+// of row j at place i ^ v_place(j).  start(w, ...) requests the first window.  Before the
+// barrier of a window arrive() sees to it that this wave's part of it is there, behind it
+// next() requests the window after it (w, if it is before w_end).  scores() forms a window's
+// products with the lane's query (query()) and calls `late`, which reads the first values,
+// between the last of them.
 template <typename T, int D, int GROUPS, typename Window>
 __device__ __forceinline__ void tile_columns(const PagedAttnArgs& a, int slots, int tile_splits, int splits, int few_rows) {
-    constexpr int kSteps = D / 16;
     constexpr int kRowBytes = D * 2;
-    constexpr int kTileBytes = kWindow * kRowBytes;
-    __shared__ __attribute__((aligned(16))) uint8_t s_mem[GROUPS][2][2 * kTileBytes];
+    // (the K-groups' sums meet there, too)
+    static_assert(GROUPS == 1 || GROUPS * 2 * Window::kBufferBytes >= kTileRows * D * 4, "room for a group's sums");
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[GROUPS][2][Window::kBufferBytes];
     __shared__ float s_stats[GROUPS > 1 ? kTileRows : 1][2];
     __shared__ int s_index;
     __shared__ int s_redo;
@@ -744,15 +568,8 @@ __device__ __forceinline__ void tile_columns(const PagedAttnArgs& a, int slots, 
     const int wave_last = strip * 32 + 31 < count ? strip * 32 + 31 : count - 1;
     const int last_pos = strip * 32 < count ? before + (static_cast<int>(c0) + wave_last) / G : -1;
 
-    uint4 qf[kSteps];
-    {
-        const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D + 8 * q;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            qf[i] = *reinterpret_cast<const uint4*>(src + 16 * i);
-        }
-    }
     Window cached(a, table, g, keys, lane, wave, s_mem[group][0]);
+    cached.query(a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D);
     floatx16 acc[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
@@ -761,35 +578,21 @@ __device__ __forceinline__ void tile_columns(const PagedAttnArgs& a, int slots, 
     float m_run = kNegInf;
     float l_run = 0.0f;
     if (w_begin + group < w_end) {
-        cached.look(w_begin + group);
-        cached.fetch(w_begin + group, 0);
-        cached.look(w_begin + group + GROUPS);
+        cached.start(w_begin + group, GROUPS, w_end);
     }
     const auto sweep = [&](auto parts) __attribute__((always_inline)) {
         constexpr bool kFine = decltype(parts)::value == 2;
         int buffer = 0;
         for (int w0 = w_begin; w0 < w_end; w0 += GROUPS, buffer ^= 1) {
             const int w = w0 + group;
-            cached.arrive(w < w_end, buffer);
+            cached.arrive(buffer);
             __syncthreads();
-            if (w + GROUPS < w_end) {
-                cached.fetch(w + GROUPS, buffer ^ 1);
-                cached.look(w + 2 * GROUPS);
-            }
+            cached.next(w + GROUPS, GROUPS, w_end, buffer ^ 1);
             const int key0 = w * kWindow;
             if (w >= w_end || key0 > last_pos) {
                 continue;  // no window for this group, or no column of this wave sees it
             }
-            const uint8_t* const s_k = s_mem[group][buffer];
-            const uint8_t* const s_v = s_k + kTileBytes;
-            const auto read_k = [&](uint4 (&k)[2], int i) __attribute__((always_inline)) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int row = 32 * t + r;
-                    const int piece = (2 * i + q) ^ Window::k_place(row);
-                    k[t] = *reinterpret_cast<const uint4*>(s_k + row * kRowBytes + piece * 16);
-                }
-            };
+            const uint8_t* const s_v = s_mem[group][buffer] + Window::kKeyBytes;
             const auto read_v = [&](uint4& v, int n, int i) __attribute__((always_inline)) {
                 uint2 part[2];
 #pragma unroll
@@ -801,34 +604,9 @@ __device__ __forceinline__ void tile_columns(const PagedAttnArgs& a, int slots, 
                 }
                 v = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
             };
-            // operands are read ahead of their products, held there by the scheduling
-            // barriers; a wave that multiplies goes before one that does arithmetic
             floatx16 sc[2] = {floatx16{}, floatx16{}};
-            constexpr int kAhead = D == 128 ? 2 : 1;
-            uint4 kf[kAhead + 1][2], vf[D / 32];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                read_k(kf[i], i);
-            }
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                if (i + kAhead < kSteps) {
-                    read_k(kf[(i + kAhead) % (kAhead + 1)], i + kAhead);
-                }
-                if (i + 2 >= kSteps) {
-#pragma unroll
-                    for (int d = 0; d < D / 64; ++d) {
-                        read_v(vf[(i + 2 - kSteps) * (D / 64) + d], 0, (i + 2 - kSteps) * (D / 64) + d);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    sc[t] = mfma32(T{}, kf[i % (kAhead + 1)][t], qf[i], sc[t]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            __builtin_amdgcn_s_setprio(0);
+            uint4 vf[D / 32];
+            cached.scores(sc, buffer, [&](int i) __attribute__((always_inline)) { read_v(vf[i], 0, i); });
             // sc[t][e]: key 32 t + 8 (e / 4) + 4 q + e % 4 of the window
             if (__builtin_amdgcn_readfirstlane(static_cast<int>(key0 + kWindow > first_pos + 1)) != 0) {
                 const int rel = pos - key0 - 4 * q;
@@ -1004,31 +782,54 @@ __device__ __forceinline__ void tile_columns(const PagedAttnArgs& a, int slots, 
     }
 }
 
-// ------------------------------------------------------------------- launches
-template <typename T, int D, typename Rows>
-__global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttnArgs a, int splits, int few_rows) {
-    few_rows_stretch<T, D, Rows>(a, splits, few_rows);
+// --------------------------------------------------------------------- plan
+inline int64_t cap(int64_t v, int64_t most) { return v < 1 ? 1 : (v < most ? v : most); }
+
+// The tile kernel's part of a plan: sequences of up to `rows` rows a KV head over `windows`
+// windows of keys.
+inline void plan_tiles(PagedAttnPlan& p, int64_t tokens, int64_t sequences, int64_t group, int64_t rows, int64_t windows,
+                       int64_t kv_heads, int64_t head_dim) {
+    p.slots = tokens * group / kTileRows + sequences;
+    const int64_t tiles = p.slots * kv_heads;
+    // Splits of at least four windows, while the blocks run side by side: a window of a
+    // block takes about 0.85 us, a merge 3 and 7 more for the partials of 256 full tiles
+    // (600 tokens of 16 heads over 2 KV heads after 4000: 3 splits 39 us, one 67; 1000
+    // after none: one 22.5, 2 splits 27.6; 1300 after 4000: 2 of 164 tiles 76, one 78).
+    const int64_t side_by_side = tiles > 128 && tiles <= 192 ? 384 : 256;
+    const auto cost = [&](int64_t s) { return 85 * windows / s + (s > 1 ? 300 + 700 * tiles * s / 256 : 0); };
+    p.tile_splits = 1;
+    for (int64_t s = 2; s <= (windows + 3) / 4 && s * tiles <= side_by_side; ++s) {
+        p.tile_splits = cost(s) < cost(p.tile_splits) ? s : p.tile_splits;
+    }
+    // Sequences of one tile a KV head, whose partials are small: splits that even out
+    // unequal lengths (64 sequences of 4 tokens and up to 8192 keys: 150 us without, 82
+    // with; all of 2000 keys 39.7 and 37.8; of 1 to 5 tokens and up to 4000 keys 56 and
+    // 48; but 8 tokens each after 2000 43 and 49).
+    if (sequences > 1 && rows <= kTileRows) {
+        const int64_t even = cap(1024 / tiles, (windows + 7) / 8);
+        p.tile_splits = p.tile_splits > even ? p.tile_splits : even;
+    }
+    // Blocks of one K-group, two a CU, where they fill the chip; else of two, one a CU
+    // (two of D = 64): 8192 tokens 269 us with one and 298 with two, 6000 166 and 175,
+    // 4000 90 and 80, 3000 64 and 53; splits past 256 blocks 43 and 47 (D = 128), 60
+    // and 56 (D = 64).
+    p.tile_groups = tiles >= 512 || (head_dim == 128 && p.tile_splits > 1 && tiles * p.tile_splits > 256) ? 1 : 2;
 }
 
+// ------------------------------------------------------------------- launches
 template <typename T, int D, int GROUPS, typename Window>
-__global__ __launch_bounds__(kThreads * GROUPS, D == 64 && GROUPS == 2 ? 4 : 2) void paged_attention_tile_kernel(
+__global__ __launch_bounds__(kThreads * GROUPS, Window::kTwoBlocks && D == 64 && GROUPS == 2 ? 4 : 2) void paged_attention_tile_kernel(
     PagedAttnArgs a, int slots, int tile_splits, int splits, int few_rows) {
     tile_columns<T, D, GROUPS, Window>(a, slots, tile_splits, splits, few_rows);
 }
 
-template <typename T, int D, typename Rows, typename Window>
-hipError_t launch_kernels(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
-    if (plan.few_blocks > 0) {
-        hipLaunchKernelGGL((paged_attention_few_kernel<T, D, Rows>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(kThreads), 0,
-                           stream, a, static_cast<int>(plan.splits), plan.tile_splits > 0 ? kFewRows : 0x7fffffff);
-        const hipError_t status = hipGetLastError();
-        if (status != hipSuccess) {
-            return status;
-        }
-    }
+// The row tiles of a call, for sequences of more than `few` rows a KV head where the
+// others have a kernel, and the merge of its splits.
+template <typename T, int D, typename Window>
+hipError_t launch_tiles(const PagedAttnArgs& a, const PagedAttnPlan& plan, int few, bool fours, hipStream_t stream) {
     if (plan.tile_splits > 0) {
         const dim3 grid(static_cast<unsigned>(plan.slots * a.kv_heads * plan.tile_splits));
-        const int few_rows = plan.few_blocks > 0 ? kFewRows : 0;
+        const int few_rows = plan.few_blocks > 0 ? few : 0;
         if (plan.tile_groups == 1) {
             hipLaunchKernelGGL((paged_attention_tile_kernel<T, D, 1, Window>), grid, dim3(kThreads), 0, stream, a,
                                static_cast<int>(plan.slots), static_cast<int>(plan.tile_splits),
@@ -1043,7 +844,7 @@ hipError_t launch_kernels(const PagedAttnArgs& a, const PagedAttnPlan& plan, hip
             return status;
         }
     }
-    return plan.splits > 1 ? launch_paged_merge(std::is_same<T, Bf16>::value ? Act::kBf16 : Act::kF16, a, plan.splits, stream)
+    return plan.splits > 1 ? launch_paged_merge(std::is_same<T, Bf16>::value ? Act::kBf16 : Act::kF16, a, plan.splits, fours, stream)
                            : hipSuccess;
 }
 

@@ -86,29 +86,270 @@ struct FewRows : CachedRow<T> {
     __device__ __forceinline__ uint4 k(int t, int i) const { return kf[t][i]; }
 };
 
-// 16 bytes a lane from base + offset straight into LDS, lane after lane from `lds`.
-// (As an instruction of its own: behind the builtin the compiler waits for the load
-// before the next LDS read, whatever that reads.  It writes no register; the wait is
-// the window's own.  Nothing else in these kernels keeps a value in m0.)
-__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "memory");
+template <typename T, int D>
+__device__ __forceinline__ void few_rows_tile(const PagedAttnArgs& a, const Sequence& s, int index, int g, int c0,
+                                              int begin, int end, int split, int splits, uint8_t* s_mem,
+                                              float (*s_ml)[16][2], int* s_redo) {
+    constexpr int kSteps = D / 32;   // products of 32 dims a score
+    constexpr int kPieces = D / 8;   // 16-byte pieces of a row
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15;
+    const int q = lane >> 4;
+    const int G = static_cast<int>(a.group);
+    const int rows = s.q_len * G;
+    const int32_t* const table = a.table + static_cast<int64_t>(index) * a.table_stride;
+    uint8_t* const s_v = s_mem + wave * (kUnit * D * 2);
+
+    const int count = rows - c0 < 16 ? rows - c0 : 16;
+    const int column = c0 + (r < count ? r : count - 1);
+    const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
+    const int head = g * G + column % G;
+    const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
+    const int keys = ends > 0 ? ends : 0;
+    const int units = (keys + kUnit - 1) / kUnit;
+    const int u_end = end * 4 < units ? end * 4 : units;
+    int unit = begin * 4 + wave;
+
+    uint4 qf[kSteps];
+    {
+        const uint16_t* const src = a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + head * D;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            qf[i] = *reinterpret_cast<const uint4*>(src + FewRows<T, D>::first_dim(q, i));
+        }
+    }
+    FewRows<T, D> cached(a, table, g, keys, r, q);
+    floatx4 acc[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        acc[i] = floatx4{};
+    }
+    float m_run = kNegInf;
+    float l_run = 0.0f;
+    if (unit < u_end) {
+        cached.pages(unit);
+        cached.place(unit);
+        cached.fetch_k();
+        cached.fetch_v();
+        cached.pages(unit + 4);
+    }
+    for (; unit < u_end; unit += 4) {
+        // V's rows, their 16-byte pieces swizzled so that the 8 rows of a
+        // transposed half-wave read lie in different banks
+        cached.store_v(s_v, [&](int row, int piece) __attribute__((always_inline)) {
+            return row * (D * 2) + (piece ^ (((row & 7) << 1) % kPieces)) * 16;
+        });
+        const bool more = unit + 4 < u_end;
+        if (more) {
+            cached.place(unit + 4);
+            cached.fetch_v();
+            cached.pages(unit + 8);
+        }
+        floatx4 sc[2] = {floatx4{}, floatx4{}};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            sc[0] = mfma16(T{}, cached.k(0, i), qf[i], sc[0]);
+            sc[1] = mfma16(T{}, cached.k(1, i), qf[i], sc[1]);
+        }
+        if (more) {
+            cached.fetch_k();
+        }
+        // sc[t][i]: key 16 t + 4 q + i of the unit
+        const int rel = pos - unit * kUnit - 4 * q;
+        float mx = kNegInf;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[t][i] = 16 * t + i <= rel ? sc[t][i] * a.scale_log2 : kNegInf;
+                mx = fmaxf(mx, sc[t][i]);
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_run, mx);
+        const float m_sub = m_new == kNegInf ? 0.0f : m_new;
+        const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+        m_run = m_new;
+        l_run *= corr;
+        // weights as two 16-bit parts (16 bits of the fp32 weight in bf16; in fp16 22,
+        // one fewer for each power of two below 2^-17 of the largest, none below 2^-39:
+        // 2^20 such keys would be 2^-19 of it, in l_run alone): this form waits for
+        // memory, the second product is free
+        const float m_w = m_sub - Weights<T>::kFewUp;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2)] - m_w);
+            const float p1 = __builtin_amdgcn_exp2f(sc[e / 2][2 * (e % 2) + 1] - m_w);
+            l_run += p0 + p1;
+            hi[e] = pack(T{}, p0, p1);
+            lo[e] = pack(T{}, p0 - low<T>(hi[e]), p1 - high<T>(hi[e]));
+        }
+        const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        const uint4 pl = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            uint2 part[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int row = 16 * t + 4 * q + r / 4;
+                const int piece = (2 * i + (r & 3) / 2) ^ (((row & 7) << 1) % kPieces);
+                part[t] = read_transposed(s_v + row * (D * 2) + piece * 16 + (r & 1) * 8);
+            }
+            const uint4 vt = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[i][e] *= corr;
+            }
+            acc[i] = mfma16(T{}, vt, ph, acc[i]);
+            acc[i] = mfma16(T{}, vt, pl, acc[i]);
+        }
+    }
+    join_waves<T, D, CachedRow<T>>(a, s, table, g, c0, count, begin * kRound, u_end * kUnit, split, splits, acc, m_run, l_run,
+                           cached.bad, s_mem, s_ml, s_redo);
 }
-__device__ __forceinline__ void load_lds16(const uint16_t* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory");
-}
-__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttnArgs a, int splits, int few_rows) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
+    __shared__ float s_ml[4][16][2];
+    __shared__ int s_part[4], s_most[4];
+    __shared__ int s_found[6];
+    __shared__ int s_redo;
+    const int tid = threadIdx.x;
+    const int sequences = static_cast<int>(a.sequences);
+    // (the line's length fits in 31 bits: the plan splits nothing where it might not)
+    // a thread's run of sequences (one of up to 256): the run's part of the line, where
+    // it begins, and its first sequence
+    const int per_thread = (sequences + kThreads - 1) / kThreads;
+    int mine = 0;
+    int mine_before = 0;
+    Sequence own = {};
+    int total, most;
+    if (sequences == 1) {
+        const Line line = line_of(a, wave_sequence(a, 0), few_rows, splits);
+        total = length_of(a, line);
+        most = line.rounds;
+    } else {
+        const int run_end = (tid + 1) * per_thread < sequences ? (tid + 1) * per_thread : sequences;
+        int longest = 1;
+        bool descending = false;  // (such starts name no rows: their lengths need not fit the line)
+        for (int i = tid * per_thread; i < run_end; ++i) {
+            own = sequence(a, i);
+            descending |= a.starts[i + 1] < a.starts[i];
+            const Line line = line_of(a, own, few_rows, splits);
+            mine += length_of(a, line);
+            longest = line.tiles > 0 && line.rounds > longest ? line.rounds : longest;
+        }
+        longest = descending ? 0x7fffffff : longest;
+        const int sum = wave_scan(mine, [](int x, int y) { return x + y; });
+        longest = wave_scan(longest, [](int x, int y) { return x > y ? x : y; });
+        if ((tid & 63) == 63) {
+            s_part[tid >> 6] = sum;
+            s_most[tid >> 6] = longest;
+        }
+        __syncthreads();
+        total = __builtin_amdgcn_readfirstlane(s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+        most = __builtin_amdgcn_readfirstlane(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
+        if (most == 0x7fffffff) {
+            return;
+        }
+        mine_before = sum - mine;
+        for (int w = 0; w < (tid >> 6); ++w) {
+            mine_before += s_part[w];
+        }
+    }
+    // a stretch: an even share, and long enough that no tile lies in more than `splits`
+    const int blocks = static_cast<int>(gridDim.x);
+    int stretch = (total + blocks - 1) / blocks;
+    const int least = splits > 1 ? (most + splits - 2) / (splits - 1) : 1;
+    stretch = stretch > least ? stretch : least;
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * stretch;
+    if (begin >= total) {
+        return;
+    }
+    int at = static_cast<int>(begin);
+    const int stop = at + stretch < total ? at + stretch : total;
+    int index, before;
+    Sequence s;
+    if (sequences == 1) {
+        index = 0;
+        before = 0;
+        s = wave_sequence(a, 0);
+    } else {
+        // the thread whose sequences the stretch begins in tells which
+        if (mine_before <= at && at < mine_before + mine) {
+            int i = tid * per_thread;
+            for (; per_thread > 1; ++i) {
+                own = sequence(a, i);
+                const int next = mine_before + length_of(a, line_of(a, own, few_rows, splits));
+                if (at < next) {
+                    break;
+                }
+                mine_before = next;
+            }
+            s_found[0] = i;
+            s_found[1] = mine_before;
+            s_found[2] = own.first;
+            s_found[3] = own.q_len;
+            s_found[4] = own.kv_len;
+            s_found[5] = own.bad;
+        }
+        __syncthreads();
+        index = __builtin_amdgcn_readfirstlane(s_found[0]);
+        before = __builtin_amdgcn_readfirstlane(s_found[1]);
+        s.first = __builtin_amdgcn_readfirstlane(s_found[2]);
+        s.q_len = __builtin_amdgcn_readfirstlane(s_found[3]);
+        s.kv_len = __builtin_amdgcn_readfirstlane(s_found[4]);
+        s.bad = __builtin_amdgcn_readfirstlane(s_found[5]) != 0;
+    }
+    for (;;) {
+        const Line line = line_of(a, s, few_rows, splits);
+        const int next = before + length_of(a, line);
+        while (at < stop && at < next) {
+            const int piece = (at - before) / line.rounds;
+            const int first = before + piece * line.rounds;
+            const int to = stop - first < line.rounds ? stop - first : line.rounds;
+            const int g = piece / line.tiles;
+            const int c0 = piece % line.tiles * 16;
+            const int rest = s.q_len * static_cast<int>(a.group) - c0;
+            const int count = rest < 16 ? rest : 16;
+            const int split = splits > 1 ? static_cast<int>(blockIdx.x) - first / stretch : 0;
+            if (s.bad) {
+                nan_columns<T, D>(a, s, g, c0, count, splits);
+            } else {
+                if (to == line.rounds && splits > 1) {
+                    tell_splits<D>(a, s, g, c0, count, split + 1, splits);
+                }
+                few_rows_tile<T, D>(a, s, index, g, c0, at - first, splits > 1 ? to : 0x7fffffff / kRound, split, splits, s_mem, s_ml,
+                          &s_redo);
+            }
+            at = first + to;
+        }
+        if (at >= stop) {
+            return;
+        }
+        before = next;
+        s = wave_sequence(a, ++index);
+    }
 }
 
+// --------------------------------------------------------------- windows of 16 bits
 // A window's rows straight to LDS.  K's pieces are swizzled by row against the 16 (D = 64:
 // 8) rows that a read takes together, V's so that the 4 rows of a transposed half-wave
 // read lie in different banks; the lane fetches the piece that belongs in its place.
 template <typename T, int D>
 struct AsyncWindow {
     using Rows = CachedRow<T>;
+    static constexpr bool kTwoBlocks = true;
     static constexpr int kRowBytes = D * 2;
     static constexpr int kPieces = D / 8;
     static constexpr int kTileBytes = kWindow * kRowBytes;
+    static constexpr int kKeyBytes = kTileBytes;
+    static constexpr int kBufferBytes = 2 * kTileBytes;
+    static constexpr int kSteps = D / 16;
     static constexpr int kLoadRows = 1024 / kRowBytes;        // rows of a wave's load
     static constexpr int kLoads = kWindow / (4 * kLoadRows);  // loads of a wave for a tile of K (and of V)
     const PagedAttnArgs& a;
@@ -117,7 +358,9 @@ struct AsyncWindow {
     const uint16_t* const vbase;
     const int keys, lane, wave;
     const int lane_row;  // of a load's kLoadRows rows, which begin at a multiple of that
+    const uint8_t* const buffers;
     const uint32_t lds0;
+    uint4 qf[kSteps];
     // Whole windows of pages that hold a load's rows together (and begin within 4 GB
     // of a pool's beginning times a page id): a load's base is the wave's, its lanes'
     // offsets are the same in every window.  Bytes from here on.
@@ -139,7 +382,7 @@ struct AsyncWindow {
     __device__ __forceinline__ AsyncWindow(const PagedAttnArgs& args, const int32_t* table_row, int g, int n, int lane_id,
                                            int wave_id, const uint8_t* lds)
         : a(args), table(table_row), kbase(args.k + g * args.head_stride), vbase(args.v + g * args.head_stride), keys(n),
-          lane(lane_id), wave(wave_id), lane_row(lane_id / kPieces),
+          lane(lane_id), wave(wave_id), lane_row(lane_id / kPieces), buffers(lds),
           lds0(__builtin_amdgcn_readfirstlane(lds_address(lds) + wave_id * 1024)), page_mask((1 << args.page_shift) - 1),
           together(page_mask + 1 >= kLoadRows && args.token_stride < (1 << 26) && args.page_stride < (1 << 30)),
           page_bytes(static_cast<uint32_t>(2 * args.page_stride)), token_bytes(static_cast<uint32_t>(2 * args.token_stride)) {
@@ -183,8 +426,29 @@ struct AsyncWindow {
             }
         }
     }
-    __device__ __forceinline__ void arrive(bool, int) {
+    __device__ __forceinline__ void start(int w, int step, int) {
+        look(w);
+        fetch(w, 0);
+        look(w + step);
+    }
+    __device__ __forceinline__ void arrive(int) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the window is in LDS
+    }
+    __device__ __forceinline__ void next(int w, int step, int w_end, int buffer) {
+        if (w < w_end) {
+            fetch(w, buffer);
+            look(w + step);
+        }
+    }
+    __device__ __forceinline__ void query(const uint16_t* row) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            qf[i] = *reinterpret_cast<const uint4*>(row + 8 * (lane >> 5) + 16 * i);
+        }
+    }
+    template <typename Late>
+    __device__ __forceinline__ void scores(floatx16 (&sc)[2], int buffer, Late late) {
+        tile_scores<T, D, AsyncWindow>(sc, qf, buffers + buffer * kBufferBytes, lane, late);
     }
 };
 
@@ -206,24 +470,41 @@ __global__ __launch_bounds__(kThreads / PARTS) void paged_attention_merge_kernel
     const int64_t unit = static_cast<int64_t>(blockIdx.x / PARTS) * kUnits + mine;
     const int64_t row = unit / a.q_heads;
     const int head = static_cast<int>(unit % a.q_heads);
-    const bool live = row < a.tokens && row >= a.starts[0] && row < a.starts[a.sequences];
     const int l0 = static_cast<int>(threadIdx.x) % kLanes * 8;  // of the part's dims
     const int d0 = static_cast<int>(blockIdx.x) % PARTS * (kLanes * 8) + l0;
+    const float2* const ml = reinterpret_cast<const float2*>(split_stats(a, D, splits)) + unit * splits;
+    const float* const src = a.partials + unit * splits * D + d0;
+    float2 w[kAhead];
+    float4 x[kAhead], y[kAhead];
+    // Groups of few splits ask for their first ones before they know how many there are (the
+    // partials have room for `splits`): otherwise four loads wait for one another.  64 rows
+    // of 16 heads over up to 9 splits 6.3 us so and 5.4 now.
+    if (GROUPS > 1 && row < a.tokens) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int s = group + j * GROUPS;
+            if (s < splits) {
+                w[j] = ml[s];
+                x[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D);
+                y[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * D + 4);
+            }
+        }
+    }
+    const bool live = row < a.tokens && row >= a.starts[0] && row < a.starts[a.sequences];
     float m = kNegInf;
     float l = 0.0f;
     float v[8] = {};
     if (live) {
-        const float2* const ml = reinterpret_cast<const float2*>(split_stats(a, D, splits)) + unit * splits;
-        const float* const src = a.partials + unit * splits * D + d0;
         const int told = split_counts(a, D, splits)[unit];
         const int made = told < 0 ? 0 : (told < splits ? told : splits);
         for (int s0 = group; s0 < made; s0 += kAhead * GROUPS) {
-            float2 w[kAhead];
-            float4 x[kAhead], y[kAhead];
+            const bool ahead = GROUPS > 1 && s0 == group;
+            if (!ahead) {
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int s = s0 + j * GROUPS < made ? s0 + j * GROUPS : made - 1;
-                w[j] = ml[s];
+                for (int j = 0; j < kAhead; ++j) {
+                    const int s = s0 + j * GROUPS < made ? s0 + j * GROUPS : made - 1;
+                    w[j] = ml[s];
+                }
             }
             float m_new = m;
 #pragma unroll
@@ -231,7 +512,7 @@ __global__ __launch_bounds__(kThreads / PARTS) void paged_attention_merge_kernel
                 // (sum 0: no key of the row in this split)
                 w[j].y = s0 + j * GROUPS < made ? w[j].y : 0.0f;
                 m_new = fmaxf(m_new, w[j].y != 0.0f ? w[j].x : kNegInf);
-                if (w[j].y != 0.0f) {
+                if (!ahead && w[j].y != 0.0f) {
                     x[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s0 + j * GROUPS) * D);
                     y[j] = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s0 + j * GROUPS) * D + 4);
                 }
@@ -309,7 +590,12 @@ hipError_t launch_merge(const PagedAttnArgs& a, int64_t splits, hipStream_t stre
 }
 
 template <typename T, int D>
-hipError_t launch_merges(const PagedAttnArgs& a, int64_t splits, hipStream_t stream) {
+hipError_t launch_merges(const PagedAttnArgs& a, int64_t splits, bool fours, hipStream_t stream) {
+    // (groups of four for up to 16 splits: those 64 rows 4.4 us, with 16 groups 5.4; the
+    // attention over 16-bit rows keeps its order of sums)
+    if (fours && splits <= 16 && a.tokens * a.q_heads < 2048) {
+        return launch_merge<T, D, 4, 1>(a, splits, stream);
+    }
     // many splits of few rows: groups work on them side by side, the parts of a row's
     // dims on as many CUs (16 splits of 16 rows 4.1 us with groups, 11.8 without; 256
     // splits 6.4 with parts, 8.2 without)
@@ -322,16 +608,24 @@ hipError_t launch_merges(const PagedAttnArgs& a, int64_t splits, hipStream_t str
 
 template <typename T, int D>
 hipError_t launch(const PagedAttnArgs& a, const PagedAttnPlan& plan, hipStream_t stream) {
-    return launch_kernels<T, D, FewRows<T, D>, AsyncWindow<T, D>>(a, plan, stream);
+    if (plan.few_blocks > 0) {
+        hipLaunchKernelGGL((paged_attention_few_kernel<T, D>), dim3(static_cast<unsigned>(plan.few_blocks)), dim3(kThreads), 0,
+                           stream, a, static_cast<int>(plan.splits), plan.tile_splits > 0 ? kFewRows : 0x7fffffff);
+        const hipError_t status = hipGetLastError();
+        if (status != hipSuccess) {
+            return status;
+        }
+    }
+    return launch_tiles<T, D, AsyncWindow<T, D>>(a, plan, kFewRows, false, stream);
 }
 
 }  // namespace
 
-hipError_t launch_paged_merge(Act act, const PagedAttnArgs& a, int64_t splits, hipStream_t stream) {
+hipError_t launch_paged_merge(Act act, const PagedAttnArgs& a, int64_t splits, bool fours, hipStream_t stream) {
     if (a.head_dim == 64) {
-        return act == Act::kBf16 ? launch_merges<Bf16, 64>(a, splits, stream) : launch_merges<F16, 64>(a, splits, stream);
+        return act == Act::kBf16 ? launch_merges<Bf16, 64>(a, splits, fours, stream) : launch_merges<F16, 64>(a, splits, fours, stream);
     }
-    return act == Act::kBf16 ? launch_merges<Bf16, 128>(a, splits, stream) : launch_merges<F16, 128>(a, splits, stream);
+    return act == Act::kBf16 ? launch_merges<Bf16, 128>(a, splits, fours, stream) : launch_merges<F16, 128>(a, splits, fours, stream);
 }
 
 PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
@@ -341,7 +635,6 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     PagedAttnPlan p;
     const int64_t longest = max_query_len < tokens ? max_query_len : tokens;
     const int64_t rows = longest * group;
-    const auto cap = [](int64_t v, int64_t most) { return v < 1 ? int64_t{1} : (v < most ? v : most); };
     const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
     // Few rows of every sequence go to the kernel for them where all sequences' windows
     // are at least 28 a CU (64 sequences of up to 8192 keys, 2 KV heads: 71 us, row tiles
@@ -349,31 +642,7 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int64_t sequences, int64_t ma
     // 1000 30 and 27).
     const bool few = rows <= kFewRows && sequences * kv_heads * windows >= 7168;
     if (!few) {
-        p.slots = tokens * group / kTileRows + sequences;
-        const int64_t tiles = p.slots * kv_heads;
-        // Splits of at least four windows, while the blocks run side by side: a window of a
-        // block takes about 0.85 us, a merge 3 and 7 more for the partials of 256 full tiles
-        // (600 tokens of 16 heads over 2 KV heads after 4000: 3 splits 39 us, one 67; 1000
-        // after none: one 22.5, 2 splits 27.6; 1300 after 4000: 2 of 164 tiles 76, one 78).
-        const int64_t side_by_side = tiles > 128 && tiles <= 192 ? 384 : 256;
-        const auto cost = [&](int64_t s) { return 85 * windows / s + (s > 1 ? 300 + 700 * tiles * s / 256 : 0); };
-        p.tile_splits = 1;
-        for (int64_t s = 2; s <= (windows + 3) / 4 && s * tiles <= side_by_side; ++s) {
-            p.tile_splits = cost(s) < cost(p.tile_splits) ? s : p.tile_splits;
-        }
-        // Sequences of one tile a KV head, whose partials are small: splits that even out
-        // unequal lengths (64 sequences of 4 tokens and up to 8192 keys: 150 us without, 82
-        // with; all of 2000 keys 39.7 and 37.8; of 1 to 5 tokens and up to 4000 keys 56 and
-        // 48; but 8 tokens each after 2000 43 and 49).
-        if (sequences > 1 && rows <= kTileRows) {
-            const int64_t even = cap(1024 / tiles, (windows + 7) / 8);
-            p.tile_splits = p.tile_splits > even ? p.tile_splits : even;
-        }
-        // Blocks of one K-group, two a CU, where they fill the chip; else of two, one a CU
-        // (two of D = 64): 8192 tokens 269 us with one and 298 with two, 6000 166 and 175,
-        // 4000 90 and 80, 3000 64 and 53; splits past 256 blocks 43 and 47 (D = 128), 60
-        // and 56 (D = 64).
-        p.tile_groups = tiles >= 512 || (head_dim == 128 && p.tile_splits > 1 && tiles * p.tile_splits > 256) ? 1 : 2;
+        plan_tiles(p, tokens, sequences, group, rows, windows, kv_heads, head_dim);
     }
     // Beside longer sequences they go there where a tile would take more than 50 windows (a
     // chunk of 1000 and a token after 16000: 58 us, with tiles alone 113; 512 and 63 tokens

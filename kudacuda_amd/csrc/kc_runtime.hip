@@ -1995,8 +1995,8 @@ int64_t kudacuda_paged_attention_mx_workspace_bytes(int64_t bits, int64_t tokens
         return 0;  // no call that would be taken
     }
     max_kv_len = max_kv_len < (int64_t{1} << 30) ? max_kv_len : int64_t{1} << 30;
-    return kc::mx_attention_plan(static_cast<int>(bits), tokens, sequences, max_query_len, max_kv_len, max_kv_len,
-                                 query_heads, kv_heads, head_dim, INT64_MAX)
+    return kc::mx_attention_plan(tokens, sequences, max_query_len, max_kv_len, max_kv_len, query_heads, kv_heads, head_dim,
+                                 INT64_MAX)
         .workspace_bytes;
 }
 
@@ -2092,9 +2092,9 @@ int kudacuda_paged_attention_mx(void* raw, uint64_t query, uint64_t key_pages, u
     a.page_shift = shift;
     a.scale_log2 = scale * kc::kLog2e;
     const int64_t longest = table_stride << shift;
-    const kc::PagedAttnPlan plan = kc::mx_attention_plan(
-        static_cast<int>(bits), tokens, sequences, max_query_len, max_kv_len < longest ? max_kv_len : longest, longest,
-        query_heads, kv_heads, head_dim, workspace != 0 ? workspace_bytes : 0);
+    const kc::PagedAttnPlan plan =
+        kc::mx_attention_plan(tokens, sequences, max_query_len, max_kv_len < longest ? max_kv_len : longest, longest,
+                              query_heads, kv_heads, head_dim, workspace != 0 ? workspace_bytes : 0);
     return launch_on(h, symbol, [&] {
         return kc::launch_mx_attention(dtype == 1 ? Act::kBf16 : Act::kF16, static_cast<int>(bits), a, plan,
                                        as_stream(stream));
