@@ -51,10 +51,11 @@ PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=6"]
 
 # Per-source additions.  kc_prefill.hip: MFMA accumulators in VGPRs (the
 # default AGPR form makes the compiler shuffle accumulators between register
-# files inside the GEMM's window loop).
+# files inside the GEMM's window loop); kc_mx_attn.hip and kc_lora.hip likewise.
 SOURCE_FLAGS = {
     "kc_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "kc_mx_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kc_lora.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     **{name: PRELOAD for name in ("kc_nf4.hip", "kc_gqa.hip", "kc_lmhead.hip")},
 }
 

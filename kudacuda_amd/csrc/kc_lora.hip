@@ -3,14 +3,20 @@
 // for the rows of adapter a; A_a is [rank, in], B_a [out, rank].  The caller's plan groups
 // the rows: a tile is up to 64 rows of one adapter.
 //
-// Two launches.  The first forms u = x A^T, a tile's 64 rows by up to 64 ranks a block,
-// over a share of `in` (few tiles are split so that the adapters' bytes come through all
-// CUs); the four waves take alternate steps of 32 and meet in LDS.  The second sums the
-// shares in order, splits u into two 16-bit parts (normalised by a power of two a row, so
-// that fp16 keeps 22 bits of it and bf16 16) and takes tiles of 64 rows by 64 outputs a
-// wave: both parts lie along the product's inner axis, so rank 16 is one matrix
-// instruction of depth 32.  Operands come straight from memory: both factors' rows are
-// contiguous along the inner axis.
+// Two launches, bound by bytes: the adapters' factors where rows are few (64 adapters of 64
+// rows, 2048 -> 11008, ranks 8 to 64, 53 MB: 5.4 + 17 us, 2.4 TB/s), else the base rows and
+// the results (2000 rows of one adapter, 8.2 + 88 MB: 7.4 + 25.9 us, 2.9 TB/s); one row is
+// the latency of two launches (3.5 + 4.7 us).
+//
+// The first forms u = x A^T, a tile's rows by up to 64 ranks a block, over a share of `in`
+// (few tiles are split so that the adapters' bytes come through all CUs); the four waves
+// take alternate steps of 32 and meet in LDS.  The second sums the shares in order, splits
+// u into two 16-bit parts (normalised by a power of two a row, so that fp16 keeps 22 bits
+// of it and bf16 16) and takes 64 outputs a wave: up to rank 16 both parts lie along one
+// product's inner axis of 32, above the factor meets one after the other.  Operands come
+// straight from memory: both factors' rows are contiguous along the inner axis.  Nothing
+// is stored through or kept past the caches: streamed (nontemporal) factors cost 22 %,
+// since several loads touch a line.
 #include <type_traits>
 
 #include "kc_device.h"
@@ -103,28 +109,33 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
         }
     }
     const int tiles = (t.rank - rank0 + 15) / 16;
-    constexpr int kAhead = RT * SUBS <= 2 ? 4 : (RT + SUBS <= 5 ? 2 : 1);
-    for (int k0 = k_begin + wave * kStep; k0 < k_end; k0 += kAhead * kBlockStep) {
-        uint4 av[kAhead][RT], xv[kAhead][SUBS];
+    // steps on their way while others are multiplied
+    constexpr int kAhead = RT * SUBS <= 2 ? 4 : 2;
+    uint4 av[kAhead][RT], xv[kAhead][SUBS];
+    const auto request = [&](int n, int k0) __attribute__((always_inline)) {
+        const int k = k0 + 8 * q;
+        const bool in = k < k_end;
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n) {
-            const int k = k0 + n * kBlockStep + 8 * q;
-            const bool in = k < k_end;
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                av[n][i] = make_uint4(0, 0, 0, 0);
-                if (in && i < tiles) {
-                    av[n][i] = load_stream(reinterpret_cast<const uint4*>(arow[i] + k));
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < SUBS; ++s) {
-                xv[n][s] = make_uint4(0, 0, 0, 0);
-                if (in && 16 * s < t.count) {
-                    xv[n][s] = *reinterpret_cast<const uint4*>(xrow[s] + k);
-                }
+        for (int i = 0; i < RT; ++i) {
+            av[n][i] = make_uint4(0, 0, 0, 0);
+            if (in && i < tiles) {
+                av[n][i] = *reinterpret_cast<const uint4*>(arow[i] + k);
             }
         }
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+            xv[n][s] = make_uint4(0, 0, 0, 0);
+            if (in && 16 * s < t.count) {
+                xv[n][s] = *reinterpret_cast<const uint4*>(xrow[s] + k);
+            }
+        }
+    };
+    int k0 = k_begin + wave * kStep;
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+        request(n, k0 + n * kBlockStep);
+    }
+    for (; k0 < k_end; k0 += kAhead * kBlockStep) {
 #pragma unroll
         for (int n = 0; n < kAhead; ++n) {
 #pragma unroll
@@ -134,6 +145,7 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
                     acc[s][i] = mfma16(T{}, av[n][i], xv[n][s], acc[s][i]);
                 }
             }
+            request(n, k0 + (n + kAhead) * kBlockStep);
         }
     }
     // acc[s][i][e]: rank 16 i + 4 q + e of row 16 s + r; the waves' shares meet in LDS
@@ -168,7 +180,21 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
     }
 }
 
-template <typename T, int RT>
+// Sixteen rows after sixteen of a tile, or (SUBS 4) a whole one together.
+template <typename Work>
+__device__ __forceinline__ void rows_of_tile(const Tile& t, int step, Work work) {
+    for (int row = 0; row < t.count; row += step) {
+        Tile part = t;
+        part.first += row;
+        part.count = t.count - row < step ? t.count - row : step;
+        if (row > 0) {
+            __syncthreads();
+        }
+        work(part);
+    }
+}
+
+template <typename T, int RT, int SUBS>
 __global__ __launch_bounds__(kThreads) void lora_inner_kernel(LoraArgs a, int splits, int chunks) {
     __shared__ __attribute__((aligned(16))) float s_u[4][16][RT * 16 + 4];
     const int chunk = static_cast<int>(blockIdx.x) % chunks;
@@ -184,27 +210,72 @@ __global__ __launch_bounds__(kThreads) void lora_inner_kernel(LoraArgs a, int sp
     const int begin = split * per_split < in ? split * per_split : in;
     const int end = begin + per_split < in ? begin + per_split : in;
     float* const partials = a.partials + static_cast<int64_t>(split) * a.tokens * a.pitch;
-    if (t.count <= 16) {
-        inner_tile<T, RT, 1>(a, t, rank0, begin, end, partials, s_u);
-    } else {
-        inner_tile<T, RT, kLoraTile / 16>(a, t, rank0, begin, end, partials, s_u);
-    }
+    rows_of_tile(t, 16 * SUBS, [&](const Tile& part) __attribute__((always_inline)) {
+        inner_tile<T, RT, SUBS>(a, part, rank0, begin, end, partials, s_u);
+    });
 }
 
 // ------------------------------------------------------------------- u B^T
-// A block: a tile's rows by `groups` groups of 64 outputs a wave.  LDS holds a row's u first
-// in fp32, then as pieces of 8: the first parts of the ranks, the second parts, zeros.
+// A block: a tile's rows by `groups` groups of 64 outputs a wave; the first group's factors
+// and base rows are requested before anything else.  LDS holds a row's u first in fp32, then
+// as pieces of 8 ranks: `half` first parts, then as many second ones.  Up to 16 ranks both
+// parts are one instruction's (pieces 0, 1 of each), else a factor's 32 ranks meet the
+// first and then the second parts.
+constexpr int outer_sets(int rank_tiles, int subs) { return subs == 1 && rank_tiles <= 4 ? 2 : 1; }
+
 template <typename T, int RT, int SUBS>
 __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int splits, int column0, int groups,
                                            uint8_t* s_row, float* s_factor) {
     constexpr int kRowBytes = RT * 64 + 16;
+    constexpr int kFactors = (RT + 1) / 2;  // of 32 ranks
+    constexpr int kSets = outer_sets(RT, SUBS);
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15;
     const int q = lane >> 4;
     const int pieces = (t.rank + 7) / 8;
-    const int steps = (pieces + 1) / 2;
+    const bool one = pieces <= 2;
+    const int half = one ? 2 : (pieces + 3) / 4 * 4;
+    const int factors = t.rank > 0 ? (pieces + 3) / 4 : 0;
+    const uint16_t* const factor = a.b + static_cast<int64_t>(t.adapter < 0 ? 0 : t.adapter) * a.max_rank * a.out_features;
+    const int out = static_cast<int>(a.out_features);
+    const float scale = t.rank > 0 ? a.scales[t.adapter] : 0.0f;
+    int rows[SUBS];
+#pragma unroll
+    for (int s = 0; s < SUBS; ++s) {
+        rows[s] = row_of(a, t, 16 * s + r);
+    }
+    // The outputs of row r of operand i: lane (r, q) of a result then has outputs 32 h + 8 q
+    // .. + 7 of its token, from operands 2 h and 2 h + 1.
+    uint4 bv[kSets][kFactors][4], base[kSets][SUBS][2];
+    const auto request = [&](int set, int o0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int o = o0 + 32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3);
+            const uint16_t* const brow = factor + static_cast<int64_t>(o < out ? o : out - 1) * (8 * pieces);
+#pragma unroll
+            for (int f = 0; f < kFactors; ++f) {
+                const int piece = one ? q & 1 : 4 * f + q;
+                bv[set][f][i] = make_uint4(0, 0, 0, 0);
+                if (piece < pieces) {
+                    bv[set][f][i] = *reinterpret_cast<const uint4*>(brow + 8 * piece);
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < SUBS; ++s) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int o = o0 + 32 * h + 8 * q;
+                base[set][s][h] = make_uint4(0, 0, 0, 0);
+                if (a.base != nullptr && rows[s] >= 0 && o < out) {
+                    base[set][s][h] = *reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(rows[s]) * a.base_stride + o);
+                }
+            }
+        }
+    };
+    request(0, column0 + wave * 64);
     if (t.rank > 0) {
         for (int i = tid; i < 16 * SUBS * RT * 4; i += kThreads) {
             const int row = i / (RT * 4);
@@ -213,7 +284,7 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
             if (row < t.count && rank < t.rank) {
                 const float* const p = a.partials + static_cast<int64_t>(t.first + row) * a.pitch + rank;
                 const int64_t share = a.tokens * a.pitch;
-#pragma unroll 4
+#pragma unroll 8
                 for (int s = 0; s < splits; ++s) {
                     const float4 v = *reinterpret_cast<const float4*>(p + s * share);
                     sum.x += v.x;
@@ -248,11 +319,12 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
             e = e > -120 ? (e < 120 ? e : 120) : -120;
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
             if (part == 0) {
-                s_factor[row] = a.scales[t.adapter] * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                s_factor[row] = scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                if (i < steps) {
+                const int piece = 2 * i + part / 2;
+                if (piece < half) {
                     const float v[4] = {u[i].x * down, u[i].y * down, u[i].z * down, u[i].w * down};
                     uint32_t hi[2], lo[2];
 #pragma unroll
@@ -262,33 +334,15 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
                         const float y = v[2 * j + 1] - T::load(static_cast<uint16_t>(hi[j] >> 16));
                         lo[j] = pair(T{}, x == x ? x : 0.0f, y == y ? y : 0.0f);  // (infinities have no rest)
                     }
-                    const int piece = 2 * i + part / 2;
-                    // (an odd number of pieces: the one behind the last is zero, both parts at the end)
-                    const int first = piece < pieces ? piece : 2 * pieces;
-                    const int second = piece < pieces ? pieces + piece : 2 * pieces + 1;
                     uint8_t* const at = s_row + row * kRowBytes + part % 2 * 8;
-                    *reinterpret_cast<uint2*>(at + first * 16) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2*>(at + second * 16) = make_uint2(lo[0], lo[1]);
+                    *reinterpret_cast<uint2*>(at + piece * 16) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(at + (half + piece) * 16) = make_uint2(lo[0], lo[1]);
                 }
             }
         }
         __syncthreads();
     }
-    const int pitch = 8 * pieces;
-    const uint16_t* const factor = a.b + static_cast<int64_t>(t.adapter < 0 ? 0 : t.adapter) * a.max_rank * a.out_features;
-    const int out = static_cast<int>(a.out_features);
-    int rows[SUBS];
-#pragma unroll
-    for (int s = 0; s < SUBS; ++s) {
-        rows[s] = row_of(a, t, 16 * s + r);
-    }
-    for (int n = 0; n < groups; ++n) {
-        const int o0 = column0 + (n * 4 + wave) * 64;
-        if (o0 >= out) {
-            break;
-        }
-        // the outputs of row r of operand t: lane (r, q) of a result then has outputs
-        // 32 h + 8 q .. + 7 of its token, from operands 2 h and 2 h + 1
+    const auto multiply = [&](int set, int o0) __attribute__((always_inline)) {
         floatx4 acc[SUBS][4];
 #pragma unroll
         for (int s = 0; s < SUBS; ++s) {
@@ -297,30 +351,24 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
                 acc[s][i] = floatx4{};
             }
         }
-        const uint16_t* brow[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int o = o0 + 32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3);
-            brow[i] = factor + static_cast<int64_t>(o < out ? o : out - 1) * pitch;
-        }
-        for (int step = 0; step < steps; ++step) {
-            const int slot = 4 * step + q;
-            const bool some = slot < 2 * pieces;
-            const int piece = slot < pieces ? slot : slot - pieces;
-            uint4 bv[4];
+        for (int f = 0; f < kFactors; ++f) {
+            if (f < factors) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bv[i] = make_uint4(0, 0, 0, 0);
-                if (some) {
-                    bv[i] = *reinterpret_cast<const uint4*>(brow[i] + 8 * piece);
-                }
-            }
+                for (int s = 0; s < SUBS; ++s) {
+                    const uint8_t* const at = s_row + (16 * s + r) * kRowBytes + (4 * f + q) * 16;
+                    const uint4 hi = *reinterpret_cast<const uint4*>(at);
 #pragma unroll
-            for (int s = 0; s < SUBS; ++s) {
-                const uint4 uv = *reinterpret_cast<const uint4*>(s_row + (16 * s + r) * kRowBytes + slot * 16);
+                    for (int i = 0; i < 4; ++i) {
+                        acc[s][i] = mfma16(T{}, bv[set][f][i], hi, acc[s][i]);
+                    }
+                    if (!one) {
+                        const uint4 lo = *reinterpret_cast<const uint4*>(at + half * 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[s][i] = mfma16(T{}, bv[i], uv, acc[s][i]);
+                        for (int i = 0; i < 4; ++i) {
+                            acc[s][i] = mfma16(T{}, bv[set][f][i], lo, acc[s][i]);
+                        }
+                    }
                 }
             }
         }
@@ -334,10 +382,8 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
             for (int h = 0; h < 2; ++h) {
                 const int o = o0 + 32 * h + 8 * q;
                 if (o < out) {
-                    float v[8] = {};
-                    if (a.base != nullptr) {
-                        unpack8<T>(*reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(rows[s]) * a.base_stride + o), v);
-                    }
+                    float v[8];
+                    unpack8<T>(base[set][s][h], v);
                     if (t.rank > 0) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
@@ -349,51 +395,81 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
                 }
             }
         }
+    };
+    // (a group past the end requests the last factors again)
+    int o0 = column0 + wave * 64;
+    for (int n = 0; n < groups; n += kSets) {
+        if constexpr (kSets == 2) {
+            request(1, o0 + 256);
+        }
+        multiply(0, o0);
+        o0 += 256;
+        if (n + 1 >= groups) {
+            break;
+        }
+        if constexpr (kSets == 2) {
+            request(0, o0 + 256);
+            multiply(1, o0);
+            o0 += 256;
+        } else {
+            request(0, o0);
+        }
     }
 }
 
-template <typename T, int RT>
+template <typename T, int RT, int SUBS>
 __global__ __launch_bounds__(kThreads) void lora_outer_kernel(LoraArgs a, int splits, int blocks, int groups) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_row[kLoraTile * (RT * 64 + 16)];
-    __shared__ float s_factor[kLoraTile];
+    __shared__ __attribute__((aligned(16))) uint8_t s_row[16 * SUBS * (RT * 64 + 16)];
+    __shared__ float s_factor[16 * SUBS];
     const Tile t = tile_of(a, static_cast<int>(blockIdx.x) / blocks);
     const int column0 = static_cast<int>(blockIdx.x) % blocks * groups * 256;
     if (t.count == 0 || (t.rank == 0 && a.out == a.base)) {
         return;
     }
-    if (t.count <= 16) {
-        outer_tile<T, RT, 1>(a, t, splits, column0, groups, s_row, s_factor);
-    } else {
-        outer_tile<T, RT, kLoraTile / 16>(a, t, splits, column0, groups, s_row, s_factor);
-    }
+    rows_of_tile(t, 16 * SUBS, [&](const Tile& part) __attribute__((always_inline)) {
+        outer_tile<T, RT, SUBS>(a, part, splits, column0, groups, s_row, s_factor);
+    });
 }
 
-template <typename T, int RT>
+template <typename T, int RT, int SUBS>
 hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
     constexpr int kChunk = RT < 4 ? RT : 4;  // ranks of 16 that a block of the first product takes
     const int64_t chunks = (a.pitch / 16 + kChunk - 1) / kChunk;
-    hipLaunchKernelGGL((lora_inner_kernel<T, kChunk>), dim3(static_cast<unsigned>(a.tile_count * plan.splits * chunks)),
+    hipLaunchKernelGGL((lora_inner_kernel<T, kChunk, SUBS>), dim3(static_cast<unsigned>(a.tile_count * plan.splits * chunks)),
                        dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits), static_cast<int>(chunks));
     const hipError_t status = hipGetLastError();
     if (status != hipSuccess) {
         return status;
     }
-    // one group of 64 outputs a wave, more where there are blocks enough without
+    // One group of 64 outputs a wave, more where there are blocks enough without.  Few rows a
+    // tile are bound by what a block does before its first product, and the groups after the
+    // first come while others are multiplied: 64 adapters, 64 rows of 11008 outputs, ranks 8
+    // to 64 -- one group 27.5 us, two 21.7, four 17.2, six 20.5; one adapter and row 4.7 with
+    // one.  Tiles of 64 rows are bound by their rows: 2000 rows of 11008 outputs -- one
+    // group 25.9 us, four 29.
+    constexpr int kSets = outer_sets(RT, SUBS);
     const int64_t columns = (a.out_features + 255) / 256;
-    int64_t groups = a.tile_count * columns / (2 * kBlocks);
-    groups = groups < 1 ? 1 : (groups < 8 ? groups : 8);
+    int64_t groups = a.tile_count * columns / (kSets == 2 ? 640 : 4 * kBlocks);
+    groups = groups < 2 ? 1 : (groups < 16 ? groups / kSets * kSets : 16);
     const int64_t blocks = (columns + groups - 1) / groups;
-    hipLaunchKernelGGL((lora_outer_kernel<T, RT>), dim3(static_cast<unsigned>(a.tile_count * blocks)), dim3(kThreads), 0, stream,
-                       a, static_cast<int>(plan.splits), static_cast<int>(blocks), static_cast<int>(groups));
+    hipLaunchKernelGGL((lora_outer_kernel<T, RT, SUBS>), dim3(static_cast<unsigned>(a.tile_count * blocks)), dim3(kThreads), 0,
+                       stream, a, static_cast<int>(plan.splits), static_cast<int>(blocks), static_cast<int>(groups));
     return hipGetLastError();
+}
+
+template <typename T, int SUBS>
+hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
+    const int64_t tiles = a.pitch / 16;
+    return tiles <= 1 ? launch<T, 1, SUBS>(a, plan, stream)
+                      : (tiles <= 2 ? launch<T, 2, SUBS>(a, plan, stream)
+                                    : (tiles <= 4 ? launch<T, 4, SUBS>(a, plan, stream) : launch<T, 8, SUBS>(a, plan, stream)));
 }
 
 template <typename T>
 hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
-    const int64_t tiles = a.pitch / 16;
-    return tiles <= 1 ? launch<T, 1>(a, plan, stream)
-                      : (tiles <= 2 ? launch<T, 2>(a, plan, stream)
-                                    : (tiles <= 4 ? launch<T, 4>(a, plan, stream) : launch<T, 8>(a, plan, stream)));
+    // tiles of 16 rows on average or fewer: kernels for 16 rows at a time (64 adapters of one
+    // row each 17 us in the second kernel; with room for 64 rows 28)
+    return a.tokens <= 16 * a.tile_count ? launch<T, 1>(a, plan, stream) : launch<T, kLoraTile / 16>(a, plan, stream);
 }
 
 }  // namespace
@@ -403,8 +479,9 @@ LoraPlan lora_plan(int64_t tokens, int64_t tile_count, int64_t max_rank, int64_t
     p.pitch = (max_rank + 15) / 16 * 16;
     const int64_t steps = (in_features + kBlockStep - 1) / kBlockStep;
     const int64_t wanted = tile_count > 0 ? kBlocks / tile_count : 1;
-    p.splits = wanted < 1 ? 1 : (wanted < steps ? wanted : steps);
-    p.splits = p.splits < 32 ? p.splits : 32;
+    // (at least four steps a split: their loads are on their way together)
+    const int64_t most = (steps + 3) / 4;
+    p.splits = wanted < 1 ? 1 : (wanted < most ? wanted : most);
     p.workspace_bytes = p.splits * tokens * p.pitch * 4;
     return p;
 }
