@@ -7,9 +7,10 @@
 // apart a number on the border of two codes lands in the other one, 2^7 (8 bits: 2^4) bf16
 // steps away; the queries' are fp32 as there.
 //
-// Bound by the bytes of the projections' rows.  Four lanes share a block, 8 dims each:
-// 16 bytes in, 4 or 8 out, the largest magnitude by two exchanges.  A key's lane also
-// loads the 8 dims that its own are paired with.
+// Bound by the bytes of the projections' rows: 19999 tokens of 16 and 2 heads of 128 into
+// 8 bits, 216 MB, 41 us, 5.2 TB/s; 8 tokens 4.4 us, a launch and the angles.  Four lanes
+// share a block, 8 dims each: 16 bytes in, 4 or 8 out, the largest magnitude by two
+// exchanges.  A key's lane also loads the 8 dims that its own are paired with.
 #include <type_traits>
 
 #include "kc_kernels.h"
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(MxAppendArgs a) {
 
 template <typename T, int BITS, bool WIDE>
 hipError_t launch(const MxAppendArgs& a, hipStream_t stream) {
-    // few tokens: one a block, to spread them over the chip
+    // few tokens: one a block, to spread them over the chip, as in kc_rope.hip
     if (a.tokens < 2048) {
         hipLaunchKernelGGL((append_kernel<T, BITS, WIDE, 1>), dim3(static_cast<unsigned>(a.tokens)), dim3(kThreads), 0, stream, a);
     } else {
@@ -211,39 +212,83 @@ hipError_t launch(const MxAppendArgs& a, hipStream_t stream) {
 }
 
 // ---------------------------------------------------------------- reading back
-// A lane unpacks 8 dims: 4 or 8 bytes in, 16 out, so that a wave writes whole lines.
-template <typename T, int BITS>
-__global__ __launch_bounds__(kThreads) void read_kernel(MxReadArgs a) {
+// A lane unpacks 8 dims at a time: 4 or 8 bytes in, 16 out, so that a wave writes whole
+// lines; UNITS of them, whose slots and then whose bytes are asked for together.
+template <typename T, int BITS, int UNITS>
+__device__ __forceinline__ void read_units(const MxReadArgs& a, int64_t first) {
     const int chunks = a.head_dim / 8;
     const int row_units = 2 * a.kv_heads * chunks;  // of a token
-    const int64_t total = a.tokens * row_units;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < total;
-         u += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t token = u / row_units;
-        const int i = static_cast<int>(u % row_units);
-        const int64_t slot = a.slots[token];
-        if (slot < 0 || slot >= (a.num_pages << a.page_shift)) {
-            continue;  // padding
-        }
-        const bool value = i >= row_units / 2;
-        const int head = (value ? i - row_units / 2 : i) / chunks;
-        const int d0 = i % chunks * 8;
-        const uint8_t* const page = (value ? a.v_pages : a.k_pages) + (slot >> a.page_shift) * a.page_stride;
-        const int64_t row = static_cast<int64_t>(head << a.page_shift) + (slot & ((int64_t{1} << a.page_shift) - 1));
-        uint32_t words[BITS / 4];
-        get_words(words, page + (row * a.head_dim + d0) * BITS / 8);
-        const uint32_t byte = page[a.block_offset + (row * a.head_dim + d0) / kMxBlock];
-        uint16_t* const out = value ? a.v_out + token * a.v_stride : a.k_out + token * a.k_stride;
-        *reinterpret_cast<uint4*>(out + head * a.head_dim + d0) = mx_unpack8<T, BITS>(words, mx_power(byte));
+    const int64_t token0 = first / row_units;
+    const int rest = static_cast<int>(first - token0 * row_units);
+    const uint8_t* page[UNITS];
+    int64_t row[UNITS], token[UNITS];
+    int unit[UNITS];
+#pragma unroll
+    for (int n = 0; n < UNITS; ++n) {
+        const unsigned i = static_cast<unsigned>(rest + n * kThreads) + threadIdx.x;
+        const unsigned ahead = i / static_cast<unsigned>(row_units);
+        unit[n] = static_cast<int>(i - ahead * row_units);
+        token[n] = token0 + ahead;
+        row[n] = token[n] < a.tokens ? a.slots[token[n]] : -1;
     }
+#pragma unroll
+    for (int n = 0; n < UNITS; ++n) {
+        const int64_t slot = row[n];
+        const bool value = unit[n] >= row_units / 2;
+        page[n] = nullptr;  // padding, or behind the last row
+        if (slot >= 0 && slot < (a.num_pages << a.page_shift)) {
+            const int head = (value ? unit[n] - row_units / 2 : unit[n]) / chunks;
+            page[n] = (value ? a.v_pages : a.k_pages) + (slot >> a.page_shift) * a.page_stride;
+            row[n] = static_cast<int64_t>(head << a.page_shift) + (slot & ((int64_t{1} << a.page_shift) - 1));
+        }
+    }
+    uint32_t words[UNITS][BITS / 4];
+    uint32_t byte[UNITS];
+#pragma unroll
+    for (int n = 0; n < UNITS; ++n) {
+        byte[n] = 0;
+        if (page[n] != nullptr) {
+            const int64_t at = row[n] * a.head_dim + unit[n] % chunks * 8;
+            get_words(words[n], page[n] + at * BITS / 8);
+            byte[n] = page[n][a.block_offset + at / kMxBlock];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < UNITS; ++n) {
+        if (page[n] != nullptr) {
+            const bool value = unit[n] >= row_units / 2;
+            uint16_t* const out = value ? a.v_out + token[n] * a.v_stride : a.k_out + token[n] * a.k_stride;
+            *reinterpret_cast<uint4*>(out + (value ? unit[n] - row_units / 2 : unit[n]) * 8) =
+                mx_unpack8<T, BITS>(words[n], mx_power(byte[n]));
+        }
+    }
+}
+
+template <typename T, int BITS, int UNITS>
+__global__ __launch_bounds__(kThreads) void read_kernel(MxReadArgs a, int64_t units) {
+    constexpr int kBlockUnits = UNITS * kThreads;
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * kBlockUnits; first < units;
+         first += static_cast<int64_t>(gridDim.x) * kBlockUnits) {
+        read_units<T, BITS, UNITS>(a, first);
+    }
+}
+
+template <typename T, int BITS, int UNITS>
+hipError_t launch(const MxReadArgs& a, int64_t units, hipStream_t stream) {
+    constexpr int64_t kMostBlocks = int64_t{1} << 20;
+    const int64_t blocks = (units + UNITS * kThreads - 1) / (UNITS * kThreads);
+    hipLaunchKernelGGL((read_kernel<T, BITS, UNITS>), dim3(static_cast<unsigned>(blocks < kMostBlocks ? blocks : kMostBlocks)),
+                       dim3(kThreads), 0, stream, a, units);
+    return hipGetLastError();
 }
 
 template <typename T, int BITS>
 hipError_t launch(const MxReadArgs& a, hipStream_t stream) {
-    const int64_t blocks = (a.tokens * 2 * a.kv_heads * (a.head_dim / 8) + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL((read_kernel<T, BITS>), dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(kThreads), 0,
-                       stream, a);
-    return hipGetLastError();
+    const int64_t units = a.tokens * 2 * a.kv_heads * (a.head_dim / 8);
+    // few rows: a unit a lane, to spread them (the kernel alone, 2 heads of 128 in 8 bits: 2000
+    // rows 3.4 us by one and 4.8 by four, 8192 5.8 and 6.2, 32000 13.7 and 13.1, 120000 51 and
+    // 41 -- 187 MB, 4.6 TB/s)
+    return units <= int64_t{1} << 20 ? launch<T, BITS, 1>(a, units, stream) : launch<T, BITS, 4>(a, units, stream);
 }
 
 }  // namespace
