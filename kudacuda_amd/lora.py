@@ -35,6 +35,7 @@ class LoraBatch:
     order: Any       # int32 [tokens]
     tiles: Any       # int32 [tiles, 3]: adapter (-1: none), first of order, how many
     stream: int = 0  # the stream that they were made on
+    most: int = -1   # the largest adapter
 
 
 def lora_batch(torch: Any, adapters: Sequence[int | None], counts: Sequence[int], device: Any = "cuda:0") -> LoraBatch:
@@ -51,7 +52,8 @@ def lora_batch(torch: Any, adapters: Sequence[int | None], counts: Sequence[int]
     table = np.asarray(tiles, dtype=np.int32)
     device = torch.device(device)
     stream = torch.cuda.current_stream(device).cuda_stream if device.type == "cuda" else 0
-    return LoraBatch(len(rows), len(table), torch.from_numpy(order).to(device), torch.from_numpy(table).to(device), stream)
+    return LoraBatch(len(rows), len(table), torch.from_numpy(order).to(device), torch.from_numpy(table).to(device), stream,
+                     max(of))
 
 
 class LoraAdapters:
@@ -98,6 +100,7 @@ class LoraAdapters:
                 or tuple(b.shape) != (self.out_features, rank)):
             raise ValueError(f"factors must be [rank, {self.in_features}] and [{self.out_features}, rank], rank 1.."
                              f"{self.max_rank}")
+        a, b = a.detach(), b.detach()
         pitch = -(-rank // 8) * 8
         rows = self.torch.zeros((self.out_features, pitch), dtype=self.dtype, device=self.device)
         rows[:, :rank] = b
@@ -130,6 +133,8 @@ class LoraAdapters:
         """``out`` = ``base`` + what every row's adapter makes of ``x``; ``out`` is ``base`` unless given."""
 
         out = base if out is None else out
+        if batch.most >= self.count:
+            raise IndexError(f"adapter {batch.most} of {self.count}")
         x_stride = self._rows("x", x, batch.tokens, self.in_features)
         base_stride = self._rows("base", base, batch.tokens, self.out_features)
         out_stride = self._rows("out", out, batch.tokens, self.out_features)

@@ -232,3 +232,18 @@ def test_the_class_refuses_rows_that_do_not_fit(torch_gpu, native):
     for bad in ((x[:2], base), (x, base[:, :24]), (x.half(), base), (x.cpu(), base), (x, base, base.t().contiguous().t())):
         with pytest.raises(ValueError):
             r.pool.add(r.batch, *bad)
+
+
+def test_trained_factors_and_adapters_that_are_not_there(torch_gpu, native):
+    """Parameters are loaded as they are, without a graph behind them; a plan may not name more than there are."""
+
+    pool = LoraAdapters(native, torch, in_features=64, out_features=32, adapters=2, max_rank=8)
+    a, b = (torch.randn(s, device="cuda:0").bfloat16().requires_grad_() for s in ((4, 64), (32, 4)))
+    pool.load(1, a, b, scale=2.0)
+    x, y = torch.randn((3, 64), device="cuda:0").bfloat16(), torch.zeros((3, 32), dtype=BF16, device="cuda:0")
+    pool.add(lora_batch(torch, [1], [3]), x, y)
+    assert not (pool.a.requires_grad or pool.b.requires_grad) and int(y.count_nonzero()) > 0
+    before = y.clone()
+    with pytest.raises(IndexError):
+        pool.add(lora_batch(torch, [0, 2], [1, 2]), x, y)
+    assert torch.equal(y, before)

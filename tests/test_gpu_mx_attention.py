@@ -336,3 +336,25 @@ def test_cache_calls_captured_twice_do_not_share_a_workspace(torch_gpu, native, 
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
         assert torch.equal(step(batches[0], news[0], None), want[0])
         torch.cuda.synchronize()
+
+
+@hints
+@all_bits
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [40, 300, 7]), ([3, 1], [200, 50]), ([20, 15], [90, 15])])
+def test_queries_without_a_number_spoil_their_own_rows_only(torch_gpu, native, dtype, bits, dim, new, kv, hint):
+    """A query with a NaN, or with an infinity at a dim where its keys are positive: NaN rows, and no others."""
+
+    batch = MxPaged(3, new, kv, bits=bits, heads=4, kv_heads=2, dim=dim, dtype=dtype)
+    batch.hint = hint
+    batch.k[..., dim - 1] = batch.k[..., dim - 1].abs() + 1.0
+    batch.repack()
+    want, size = batch.want()
+    spoilt = np.zeros((batch.tokens, 4), dtype=bool)
+    for row, head, d, value in ((0, 1, 0, "nan"), (1, 3, dim - 1, "inf"), (batch.tokens - 1, 0, dim - 1, "inf")):
+        batch.q[row, head, d] = float(value)
+        spoilt[row, head] = True
+    got = f64(batch.call(native, batch.device()))
+    assert np.isnan(got[spoilt]).all()
+    assert (np.abs(got - want) <= batch.bound(want, size))[~spoilt].all()
