@@ -579,7 +579,7 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
 template <typename T, int D, int BITS>
 struct MxWindow {
     using Rows = MxRow<T, D, BITS>;
-    static constexpr bool kTwoBlocks = false;
+    static constexpr int waves(int groups) { return D == 64 && groups == 1 ? 3 : 2; }  // a SIMD
     static constexpr int kParts = D / 64;
     static constexpr int kRowBytes = D * BITS / 8;
     static constexpr int kWords = kMxBlock * BITS / 32;
@@ -720,6 +720,24 @@ PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_q
     const bool few = rows <= kMxFewRows;
     if (!few) {
         plan_tiles(p, tokens, sequences, group, rows, windows, kv_heads, head_dim);
+        // Tiles of one K-group here are two blocks a CU (heads of 64: three), of two K-groups one
+        // (kc_paged_attn.hip's are two of heads of 64).  So sequences of one tile each, whose
+        // lengths splits even out, take one group where there are blocks enough for it (heads of
+        // 64, 64 sequences of 30 tokens after 3000: 71 us with two groups, 57 with one; 32 of 25
+        // after 1000 32 and 23), and so do chunks behind a past at least as long, with splits that
+        // fill the chip (1500 tokens of 12 heads of 64 over 4 KV heads after 3000: 53 and 45;
+        // heads of 128, 16 over 2: 1200 after 2000 62 and 51, 2500 after 3000 138 and 129).
+        // Shorter and fewer ones would lose by the merge what they gain: 3 chunks of 800 after
+        // 1000 27 (heads of 128 60) and 36 (64), 1200 of heads of 64 after 2000 31 and 34, whole
+        // prompts likewise.
+        const int64_t tiles = p.slots * kv_heads;
+        if (sequences > 1 && rows <= kTileRows) {
+            p.tile_groups = tiles * p.tile_splits > 256 ? 1 : p.tile_groups;
+        } else if (max_kv_len >= 2 * longest && windows >= 40 && tiles > (head_dim == 64 ? 128 : 96) &&
+                   tiles < (head_dim == 64 ? 512 : 342)) {
+            p.tile_groups = 1;
+            p.tile_splits = head_dim == 64 ? (511 + tiles) / tiles : (tiles <= 256 ? 512 : 1024) / tiles;
+        }
     }
     int64_t few_splits = 0;
     if (few || (tokens != sequences * longest && windows > 50 * p.tile_splits)) {

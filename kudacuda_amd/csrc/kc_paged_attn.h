@@ -818,7 +818,7 @@ inline void plan_tiles(PagedAttnPlan& p, int64_t tokens, int64_t sequences, int6
 
 // ------------------------------------------------------------------- launches
 template <typename T, int D, int GROUPS, typename Window>
-__global__ __launch_bounds__(kThreads * GROUPS, Window::kTwoBlocks && D == 64 && GROUPS == 2 ? 4 : 2) void paged_attention_tile_kernel(
+__global__ __launch_bounds__(kThreads * GROUPS, Window::waves(GROUPS)) void paged_attention_tile_kernel(
     PagedAttnArgs a, int slots, int tile_splits, int splits, int few_rows) {
     tile_columns<T, D, GROUPS, Window>(a, slots, tile_splits, splits, few_rows);
 }

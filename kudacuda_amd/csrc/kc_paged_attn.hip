@@ -343,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_few_kernel(PagedAttn
 template <typename T, int D>
 struct AsyncWindow {
     using Rows = CachedRow<T>;
-    static constexpr bool kTwoBlocks = true;
+    static constexpr int waves(int groups) { return D == 64 && groups == 2 ? 4 : 2; }  // a SIMD
     static constexpr int kRowBytes = D * 2;
     static constexpr int kPieces = D / 8;
     static constexpr int kTileBytes = kWindow * kRowBytes;
