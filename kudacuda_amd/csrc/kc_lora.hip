@@ -3,10 +3,11 @@
 // for the rows of adapter a; A_a is [rank, in], B_a [out, rank].  The caller's plan groups
 // the rows: a tile is up to 64 rows of one adapter.
 //
-// Two launches, bound by bytes: the adapters' factors where rows are few (64 adapters of 64
-// rows, 2048 -> 11008, ranks 8 to 64, 53 MB: 5.4 + 17 us, 2.4 TB/s), else the base rows and
-// the results (2000 rows of one adapter, 8.2 + 88 MB: 7.4 + 25.9 us, 2.9 TB/s); one row is
-// the latency of two launches (3.5 + 4.7 us).
+// Two launches, bound by bytes: the adapters' factors where rows are few (64 adapters of a
+// row each, 2048 -> 11008, ranks 8 to 64, 53 MB: 6.4 + 16.3 us, 2.3 TB/s), else the inputs,
+// the base rows and the results (2000 rows of one adapter, 2048 -> 11008, 96 MB: 7.5 + 23.8
+// us, 3.1 TB/s; 8 chunks of 2996 rows, 11008 -> 2048, 90 MB: 18.5 + 13.7, 2.8 TB/s); one
+// row is the latency of two launches (3.5 + 4.5 us).
 //
 // The first forms u = x A^T, a tile's rows by up to 64 ranks a block, over a share of `in`
 // (few tiles are split so that the adapters' bytes come through all CUs); the four waves
@@ -14,9 +15,10 @@
 // u into two 16-bit parts (normalised by a power of two a row, so that fp16 keeps 22 bits
 // of it and bf16 16) and takes 64 outputs a wave: up to rank 16 both parts lie along one
 // product's inner axis of 32, above the factor meets one after the other.  Operands come
-// straight from memory: both factors' rows are contiguous along the inner axis.  Nothing
-// is stored through or kept past the caches: streamed (nontemporal) factors cost 22 %,
-// since several loads touch a line.
+// straight from memory: both factors' rows are contiguous along the inner axis.  (Lanes
+// that read them in their order in memory, as rows through LDS would, gain a tenth of the
+// first launch before the exchange is paid for.)  Loads are plain: streamed (nontemporal)
+// factors cost 22 %, since several loads touch a line.
 #include <type_traits>
 
 #include "kc_device.h"
@@ -32,6 +34,10 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kStep = 32;            // of the inner axis, a matrix instruction
 constexpr int kBlockStep = 4 * kStep;  // of the four waves
+// Blocks of the first launch that tiles are split into.  More shorten it and lengthen the
+// second, which sums the shares in each of its blocks: the 8 chunks above 19.3 + 11.7 us with
+// 256, 18.5 + 13.7 with 512, 15.8 + 16.9 with 1024; 4 chunks of 2000, rank 64, 66 + 31, 62 +
+// 35, 61 + 42.
 constexpr int64_t kBlocks = 512;
 
 __device__ __forceinline__ floatx4 mfma16(Bf16, uint4 a, uint4 b, floatx4 c) {
@@ -284,13 +290,21 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
             if (row < t.count && rank < t.rank) {
                 const float* const p = a.partials + static_cast<int64_t>(t.first + row) * a.pitch + rank;
                 const int64_t share = a.tokens * a.pitch;
-#pragma unroll 8
-                for (int s = 0; s < splits; ++s) {
-                    const float4 v = *reinterpret_cast<const float4*>(p + s * share);
-                    sum.x += v.x;
-                    sum.y += v.y;
-                    sum.z += v.z;
-                    sum.w += v.w;
+                constexpr int kTogether = 8;  // shares on their way (past the last one it is read again)
+                for (int s0 = 0; s0 < splits; s0 += kTogether) {
+                    float4 v[kTogether];
+#pragma unroll
+                    for (int n = 0; n < kTogether; ++n) {
+                        v[n] = *reinterpret_cast<const float4*>(p + (s0 + n < splits ? s0 + n : splits - 1) * share);
+                    }
+#pragma unroll
+                    for (int n = 0; n < kTogether; ++n) {
+                        const bool more = s0 + n < splits;
+                        sum.x = more ? sum.x + v[n].x : sum.x;
+                        sum.y = more ? sum.y + v[n].y : sum.y;
+                        sum.z = more ? sum.z + v[n].z : sum.z;
+                        sum.w = more ? sum.w + v[n].w : sum.w;
+                    }
                 }
                 sum.y = rank + 1 < t.rank ? sum.y : 0.0f;
                 sum.z = rank + 2 < t.rank ? sum.z : 0.0f;
@@ -444,7 +458,7 @@ hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
     // One group of 64 outputs a wave, more where there are blocks enough without.  Few rows a
     // tile are bound by what a block does before its first product, and the groups after the
     // first come while others are multiplied: 64 adapters, 64 rows of 11008 outputs, ranks 8
-    // to 64 -- one group 27.5 us, two 21.7, four 17.2, six 20.5; one adapter and row 4.7 with
+    // to 64 -- one group 27.5 us, two 21.7, four 17.2 (16.3 now), six 20.5; one adapter and row 4.7 with
     // one.  Tiles of 64 rows are bound by their rows: 2000 rows of 11008 outputs -- one
     // group 25.9 us, four 29.
     constexpr int kSets = outer_sets(RT, SUBS);

@@ -50,6 +50,8 @@ def _check(batch, out, rows=None):
     ([33, 200, 1, 64], [33, 500, 77, 64], 8, 4, 16),
     ([250, 5], [1300, 5], 7, 7, 128),
     ([1, 130, 1], [900, 131, 2], 16, 2, 4096),
+    # chunks behind a past as long and longer, tiles enough for blocks of one K-group and splits
+    ([300, 1, 200, 64, 130], [2700, 900, 3000, 64, 131], 24, 12, 16),
     # sequences without new tokens, without cache rows, and rows that see no key
     ([0, 4, 0, 1, 40], [9, 4, 0, 0, 13], 4, 2, 16),
     ([2, 60], [0, 1], 4, 4, 16),
