@@ -126,6 +126,8 @@ class LoraAdapters:
 
     def _capturing(self) -> bool:
         cuda = self.torch.cuda
+        if cuda.current_device() == self.device.index:
+            return cuda.is_current_stream_capturing()
         with cuda.device(self.device):
             return cuda.is_current_stream_capturing()
 
@@ -135,6 +137,8 @@ class LoraAdapters:
         out = base if out is None else out
         if batch.most >= self.count:
             raise IndexError(f"adapter {batch.most} of {self.count}")
+        if batch.order.device != self.device:
+            raise ValueError(f"a plan on {batch.order.device} for adapters on {self.device}")
         x_stride = self._rows("x", x, batch.tokens, self.in_features)
         base_stride = self._rows("base", base, batch.tokens, self.out_features)
         out_stride = self._rows("out", out, batch.tokens, self.out_features)

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+from kudacuda_amd._native import Native
 from kudacuda_amd.lora import LoraAdapters, lora_batch
 from kudacuda_amd.paged_cache import PagedKvCache
 from tests import _mx_ref as mx
@@ -128,3 +129,20 @@ def test_factors_lie_in_rows_of_their_rank():
             pool.load(index, x, y)
     with pytest.raises(IndexError):
         pool.load(3, a, b)
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda:1"])
+def test_adapters_lie_on_their_handles_device(device):
+    native = Native.__new__(Native)
+    native.handle, native.device_id = None, 0
+    with pytest.raises(ValueError, match="cuda:0"):
+        LoraAdapters(native, torch, in_features=8, out_features=8, adapters=1, max_rank=8, device=device)
+
+
+def test_a_plan_of_another_device_or_of_more_adapters_is_refused():
+    pool = LoraAdapters(None, torch, in_features=8, out_features=8, adapters=2, max_rank=8, device="cpu")
+    x, y = torch.zeros((3, 8), dtype=torch.bfloat16), torch.zeros((3, 8), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="plan on meta"):
+        pool.add(lora_batch(torch, [1], [3], device="meta"), x, y)
+    with pytest.raises(IndexError):
+        pool.add(lora_batch(torch, [2], [3], device="cpu"), x, y)
