@@ -3,11 +3,11 @@
 // for the rows of adapter a; A_a is [rank, in], B_a [out, rank].  The caller's plan groups
 // the rows: a tile is up to 64 rows of one adapter.
 //
-// Two launches, bound by bytes: the adapters' factors where rows are few (64 adapters of a
+// Two launches (one where both are small), bound by bytes: the adapters' factors where rows are few (64 adapters of a
 // row each, 2048 -> 11008, ranks 8 to 64, 53 MB: 6.4 + 16.3 us, 2.3 TB/s), else the inputs,
 // the base rows and the results (2000 rows of one adapter, 2048 -> 11008, 96 MB: 7.5 + 23.8
 // us, 3.1 TB/s; 8 chunks of 2996 rows, 11008 -> 2048, 90 MB: 18.5 + 13.7, 2.8 TB/s); one
-// row is the latency of two launches (3.5 + 4.5 us).
+// row is latency: 6.8 us, places, two products and their sums one after the other.
 //
 // The first forms u = x A^T, a tile's rows by up to 64 ranks a block, over a share of `in`
 // (few tiles are split so that the adapters' bytes come through all CUs); the four waves
@@ -85,10 +85,11 @@ __device__ __forceinline__ int row_of(const LoraArgs& a, const Tile& t, int i) {
 }
 
 // ------------------------------------------------------------------- x A^T
-// RT tiles of 16 ranks from rank0 on, SUBS of 16 rows.
-template <typename T, int RT, int SUBS>
-__device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int rank0, int k_begin, int k_end,
-                                           float* partials, float (*s_u)[16][RT * 16 + 4]) {
+// RT tiles of 16 ranks from rank0 on, SUBS of 16 rows: a wave's share, its part of every
+// kBlockStep.  acc[s][i][e]: rank 16 i + 4 q + e of row 16 s + r.
+template <typename T, int RT, int SUBS, int AHEAD>
+__device__ __forceinline__ void inner_sums(const LoraArgs& a, const Tile& t, int rank0, int k_begin, int k_end,
+                                           floatx4 (&acc)[SUBS][RT]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int r = lane & 15;
@@ -106,7 +107,6 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
         const int row = row_of(a, t, 16 * i + r);
         xrow[i] = a.x + static_cast<int64_t>(row < 0 ? 0 : row) * a.x_stride;
     }
-    floatx4 acc[SUBS][RT];
 #pragma unroll
     for (int s = 0; s < SUBS; ++s) {
 #pragma unroll
@@ -116,8 +116,7 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
     }
     const int tiles = (t.rank - rank0 + 15) / 16;
     // steps on their way while others are multiplied
-    constexpr int kAhead = RT * SUBS <= 2 ? 4 : 2;
-    uint4 av[kAhead][RT], xv[kAhead][SUBS];
+    uint4 av[AHEAD][RT], xv[AHEAD][SUBS];
     const auto request = [&](int n, int k0) __attribute__((always_inline)) {
         const int k = k0 + 8 * q;
         const bool in = k < k_end;
@@ -138,12 +137,12 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
     };
     int k0 = k_begin + wave * kStep;
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) {
+    for (int n = 0; n < AHEAD; ++n) {
         request(n, k0 + n * kBlockStep);
     }
-    for (; k0 < k_end; k0 += kAhead * kBlockStep) {
+    for (; k0 < k_end; k0 += AHEAD * kBlockStep) {
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n) {
+        for (int n = 0; n < AHEAD; ++n) {
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
 #pragma unroll
@@ -151,10 +150,21 @@ __device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int
                     acc[s][i] = mfma16(T{}, av[n][i], xv[n][s], acc[s][i]);
                 }
             }
-            request(n, k0 + (n + kAhead) * kBlockStep);
+            request(n, k0 + (n + AHEAD) * kBlockStep);
         }
     }
-    // acc[s][i][e]: rank 16 i + 4 q + e of row 16 s + r; the waves' shares meet in LDS
+}
+
+template <typename T, int RT, int SUBS>
+__device__ __forceinline__ void inner_tile(const LoraArgs& a, const Tile& t, int rank0, int k_begin, int k_end,
+                                           float* partials, float (*s_u)[16][RT * 16 + 4]) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int r = lane & 15;
+    const int q = lane >> 4;
+    floatx4 acc[SUBS][RT];
+    inner_sums<T, RT, SUBS, RT * SUBS <= 2 ? 4 : 2>(a, t, rank0, k_begin, k_end, acc);
+    // the waves' shares meet in LDS
 #pragma unroll
     for (int s = 0; s < SUBS; ++s) {
         if (16 * s >= t.count) {
@@ -229,9 +239,9 @@ __global__ __launch_bounds__(kThreads) void lora_inner_kernel(LoraArgs a, int sp
 // first and then the second parts.
 constexpr int outer_sets(int rank_tiles, int subs) { return subs == 1 && rank_tiles <= 4 ? 2 : 1; }
 
-template <typename T, int RT, int SUBS>
+template <typename T, int RT, int SUBS, bool WHOLE>
 __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int splits, int column0, int groups,
-                                           uint8_t* s_row, float* s_factor) {
+                                           uint8_t* s_row, float* s_factor, float (*s_u)[16][RT * 16 + 4]) {
     constexpr int kRowBytes = RT * 64 + 16;
     constexpr int kFactors = (RT + 1) / 2;  // of 32 ranks
     constexpr int kSets = outer_sets(RT, SUBS);
@@ -283,11 +293,33 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
     };
     request(0, column0 + wave * 64);
     if (t.rank > 0) {
+        if constexpr (WHOLE) {
+            floatx4 acc[SUBS][RT];
+            inner_sums<T, RT, SUBS, RT <= 2 ? 8 : 4>(a, t, 0, 0, static_cast<int>(a.in_features), acc);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                *reinterpret_cast<float4*>(&s_u[wave][r][16 * i + 4 * q]) =
+                    make_float4(acc[0][i][0], acc[0][i][1], acc[0][i][2], acc[0][i][3]);
+            }
+            __syncthreads();
+        }
         for (int i = tid; i < 16 * SUBS * RT * 4; i += kThreads) {
             const int row = i / (RT * 4);
             const int rank = i % (RT * 4) * 4;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (row < t.count && rank < t.rank) {
+            if constexpr (WHOLE) {
+                if (row < t.count && rank < t.rank) {
+                    sum = *reinterpret_cast<const float4*>(&s_u[0][row][rank]);
+#pragma unroll
+                    for (int w = 1; w < 4; ++w) {
+                        const float4 v = *reinterpret_cast<const float4*>(&s_u[w][row][rank]);
+                        sum.x += v.x;
+                        sum.y += v.y;
+                        sum.z += v.z;
+                        sum.w += v.w;
+                    }
+                }
+            } else if (row < t.count && rank < t.rank) {
                 const float* const p = a.partials + static_cast<int64_t>(t.first + row) * a.pitch + rank;
                 const int64_t share = a.tokens * a.pitch;
                 constexpr int kTogether = 8;  // shares on their way (past the last one it is read again)
@@ -306,10 +338,10 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
                         sum.w = more ? sum.w + v[n].w : sum.w;
                     }
                 }
-                sum.y = rank + 1 < t.rank ? sum.y : 0.0f;
-                sum.z = rank + 2 < t.rank ? sum.z : 0.0f;
-                sum.w = rank + 3 < t.rank ? sum.w : 0.0f;
             }
+            sum.y = rank + 1 < t.rank ? sum.y : 0.0f;
+            sum.z = rank + 2 < t.rank ? sum.z : 0.0f;
+            sum.w = rank + 3 < t.rank ? sum.w : 0.0f;
             *reinterpret_cast<float4*>(s_row + row * kRowBytes + rank * 4) = sum;
         }
         __syncthreads();
@@ -431,8 +463,9 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
     }
 }
 
-template <typename T, int RT, int SUBS>
+template <typename T, int RT, int SUBS, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void lora_outer_kernel(LoraArgs a, int splits, int blocks, int groups) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_u[WHOLE ? 4 * 16 * (RT * 16 + 4) * 4 : 16];
     __shared__ __attribute__((aligned(16))) uint8_t s_row[16 * SUBS * (RT * 64 + 16)];
     __shared__ float s_factor[16 * SUBS];
     const Tile t = tile_of(a, static_cast<int>(blockIdx.x) / blocks);
@@ -441,34 +474,47 @@ __global__ __launch_bounds__(kThreads) void lora_outer_kernel(LoraArgs a, int sp
         return;
     }
     rows_of_tile(t, 16 * SUBS, [&](const Tile& part) __attribute__((always_inline)) {
-        outer_tile<T, RT, SUBS>(a, part, splits, column0, groups, s_row, s_factor);
+        outer_tile<T, RT, SUBS, WHOLE>(a, part, splits, column0, groups, s_row, s_factor,
+                                         reinterpret_cast<float (*)[16][RT * 16 + 4]>(s_u));
     });
 }
 
-template <typename T, int RT, int SUBS>
-hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
-    constexpr int kChunk = RT < 4 ? RT : 4;  // ranks of 16 that a block of the first product takes
-    const int64_t chunks = (a.pitch / 16 + kChunk - 1) / kChunk;
-    hipLaunchKernelGGL((lora_inner_kernel<T, kChunk, SUBS>), dim3(static_cast<unsigned>(a.tile_count * plan.splits * chunks)),
-                       dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits), static_cast<int>(chunks));
-    const hipError_t status = hipGetLastError();
-    if (status != hipSuccess) {
-        return status;
-    }
+template <typename T, int RT, int SUBS, bool WHOLE>
+hipError_t launch_outer(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
     // One group of 64 outputs a wave, more where there are blocks enough without.  Few rows a
     // tile are bound by what a block does before its first product, and the groups after the
     // first come while others are multiplied: 64 adapters, 64 rows of 11008 outputs, ranks 8
-    // to 64 -- one group 27.5 us, two 21.7, four 17.2 (16.3 now), six 20.5; one adapter and row 4.7 with
-    // one.  Tiles of 64 rows are bound by their rows: 2000 rows of 11008 outputs -- one
+    // to 64 -- one group 27.5 us, two 21.7, four 17.2 (16.3 now), six 20.5; one adapter and row
+    // 4.7 with one.  Tiles of 64 rows are bound by their rows: 2000 rows of 11008 outputs -- one
     // group 25.9 us, four 29.
     constexpr int kSets = outer_sets(RT, SUBS);
     const int64_t columns = (a.out_features + 255) / 256;
     int64_t groups = a.tile_count * columns / (kSets == 2 ? 640 : 4 * kBlocks);
     groups = groups < 2 ? 1 : (groups < 16 ? groups / kSets * kSets : 16);
     const int64_t blocks = (columns + groups - 1) / groups;
-    hipLaunchKernelGGL((lora_outer_kernel<T, RT, SUBS>), dim3(static_cast<unsigned>(a.tile_count * blocks)), dim3(kThreads), 0,
-                       stream, a, static_cast<int>(plan.splits), static_cast<int>(blocks), static_cast<int>(groups));
+    hipLaunchKernelGGL((lora_outer_kernel<T, RT, SUBS, WHOLE>), dim3(static_cast<unsigned>(a.tile_count * blocks)),
+                       dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits), static_cast<int>(blocks),
+                       static_cast<int>(groups));
     return hipGetLastError();
+}
+
+template <typename T, int RT, int SUBS>
+hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
+    if constexpr (SUBS == 1 && RT <= 4) {
+        // Small factors and few blocks: each forms u for itself, and a launch is saved, 4 us of
+        // a call (one row, 2048 -> 2048: rank 16 6.8 us and 3.6 + 4.6 in two launches, rank 32
+        // 8.9 and 4.1 + 5.1; but rank 64 13.3 and 5.0 + 6.6, 11008 -> 2048 with rank 16 16.4 and
+        // 4.0 + 5.7; rank 16, 16 adapters 8.5 and 4.0 + 4.7, 64 11.4 and 4.6 + 5.6).
+        if (a.pitch * a.in_features <= 65536 && a.tile_count * ((a.out_features + 255) / 256) <= 128) {
+            return launch_outer<T, RT, SUBS, true>(a, plan, stream);
+        }
+    }
+    constexpr int kChunk = RT < 4 ? RT : 4;  // ranks of 16 that a block of the first product takes
+    const int64_t chunks = (a.pitch / 16 + kChunk - 1) / kChunk;
+    hipLaunchKernelGGL((lora_inner_kernel<T, kChunk, SUBS>), dim3(static_cast<unsigned>(a.tile_count * plan.splits * chunks)),
+                       dim3(kThreads), 0, stream, a, static_cast<int>(plan.splits), static_cast<int>(chunks));
+    const hipError_t status = hipGetLastError();
+    return status != hipSuccess ? status : launch_outer<T, RT, SUBS, false>(a, plan, stream);
 }
 
 template <typename T, int SUBS>

@@ -85,6 +85,12 @@ class Round:
     ([2, 3, 2], [(1, 8), (0, 16), (1, 8)], 32, 40, 96),
     ([1] * 300, [(i % 50, 12) for i in range(300)], 128, 64, None),
     ([129] * 9, [(i, 16) for i in range(9)], 2048, 2560, None),
+    # few rows a tile: one launch where factors and blocks are few, two otherwise
+    ([40, 1, 1, 1, 2], [(0, 24), (1, 8), (2, 3), (3, 16), None], 2048, 520, None),
+    ([40, 1, 1, 1, 2], [(0, 24), (1, 8), (2, 3), (3, 16), None], 11008, 520, None),
+    ([1, 4, 1], [(0, 64), (1, 50), (2, 33)], 1024, 1000, None),
+    ([1, 4, 1], [(0, 64), (1, 50), (2, 33)], 1032, 1000, None),
+    ([2, 1, 33], [(0, 128), (1, 100), (2, 65)], 520, 264, None),
 ])
 def test_matches_fp64(torch_gpu, native, dtype, chunks, ranks, inner, outer, max_rank):
     print(f"adapters {ranks[:9]} for {chunks[:9]} rows, {inner} -> {outer}, {dtype}", flush=True)
