@@ -85,6 +85,30 @@ __device__ __forceinline__ void get_words(uint32_t (&w)[WORDS], const uint8_t* p
     }
 }
 
+// A page's first `bytes` bytes, of the whole wave's page: a load behind them reads nothing and
+// gives zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_buffer(const uint8_t* page, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(page), 0, bytes, 0x00027000);
+}
+template <int WORDS>
+__device__ __forceinline__ void get_words(uint32_t (&w)[WORDS], __amdgpu_buffer_rsrc_t page, int offset) {
+    static_assert(WORDS == 2 || WORDS == 4 || WORDS == 8, "whole loads");
+    if constexpr (WORDS == 2) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(page, offset, 0, 0);
+        w[0] = v[0];
+        w[1] = v[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(page, offset + 4 * i, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                w[i + k] = v[k];
+            }
+        }
+    }
+}
+
 // -------------------------------------------------------------------- packing
 // The byte of a block whose largest magnitude has these bits (sign off), 255 if it is no
 // number: the least exponent e with magnitude < 7 * 2^e (4 bits), 464 * 2^e (8 bits), so

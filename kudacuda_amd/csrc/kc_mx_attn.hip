@@ -195,10 +195,12 @@ struct MxFewTile {
         const int pos = s.kv_len - s.q_len + column / G;  // the last key that the column sees
         const int first_pos = s.kv_len - s.q_len + c0 / G;
         const int ends = s.kv_len - s.q_len + (c0 + count - 1) / G + 1;
-        const int keys = ends > 0 ? ends : 0;
+        // (the wave's, and told to be: the loop and the pages' buffers take them as scalars)
+        const int keys = __builtin_amdgcn_readfirstlane(ends > 0 ? ends : 0);
         const int units = (keys + kUnit - 1) / kUnit;
-        const int u_end = end * 4 < units ? end * 4 : units;
-        int unit = begin * 4 + wave;
+        const int u_end = __builtin_amdgcn_readfirstlane(end * 4 < units ? end * 4 : units);
+        int unit = __builtin_amdgcn_readfirstlane(begin * 4 + wave);
+        const int head = __builtin_amdgcn_readfirstlane(g << a.page_shift);
 
         // Pages of the wave's next 64 tiles, one a lane: read in the loop, their ids would come
         // behind the rows that are on their way, since loads return in order.
@@ -218,43 +220,42 @@ struct MxFewTile {
         const int b_lane = q * (D / 4) / kMxBlock;
         const uint8_t* const kpool = reinterpret_cast<const uint8_t*>(a.k);
         const uint8_t* const vpool = reinterpret_cast<const uint8_t*>(a.v);
+        // A unit behind the wave's last one is asked for like the others, from a page of no bytes:
+        // loads under a condition would be waited for all together.
         const auto fetch = [&](int u, Raw& raw) __attribute__((always_inline)) {
-            if (u == pages_from + 4 * 32) {
+            if (u == pages_from + 4 * 32 && u < u_end) {
                 look(u);
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int id = __builtin_amdgcn_readlane(pages, (u - pages_from) / 2 + t);
+                const int id = __builtin_amdgcn_readlane(pages, ((u - pages_from) / 2 + t) & 63);
                 const bool out = static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.num_pages);
-                bad |= out;
+                bad |= out && u < u_end;
                 int key = u * kUnit + 16 * t;
                 key = key < last_tile ? key : last_tile;
                 // (rows past the end read the last one)
                 const int row = r < keys - 1 - key ? r : keys - 1 - key;
                 const int64_t at = static_cast<int64_t>(out ? 0 : id) * a.page_stride;
-                const int64_t first = (static_cast<int64_t>(g) << a.page_shift) + (key & page_mask);
-                const uint8_t* const k_at = kpool + at + first * kRowBytes;
-                const uint8_t* const v_at = vpool + at + first * kRowBytes;
-                const int64_t blocks = at + a.block_offset + first * (D / kMxBlock);
-                const uint32_t offset = static_cast<uint32_t>(row * kRowBytes);
-                const uint32_t block = static_cast<uint32_t>(row * (D / kMxBlock) + b_lane);
+                const int bytes = out || u >= u_end ? 0 : static_cast<int>(a.page_stride);
+                const auto k_page = page_buffer(kpool + at, bytes);
+                const auto v_page = page_buffer(vpool + at, bytes);
+                const int first = head + (key & page_mask) + row;
+                const int elements = first * kRowBytes;
+                const int block = static_cast<int>(a.block_offset) + first * (D / kMxBlock) + b_lane;
                 if constexpr (D == 128 && BITS == 8) {
-                    const uint4 x = load_stream(reinterpret_cast<const uint4*>(k_at + (offset + k_lane0)));
-                    const uint4 y = load_stream(reinterpret_cast<const uint4*>(k_at + (offset + k_lane0 + 64)));
-                    raw.k[t][0] = x.x;
-                    raw.k[t][1] = x.y;
-                    raw.k[t][2] = x.z;
-                    raw.k[t][3] = x.w;
-                    raw.k[t][4] = y.x;
-                    raw.k[t][5] = y.y;
-                    raw.k[t][6] = y.z;
-                    raw.k[t][7] = y.w;
+                    uint32_t half[2][4];
+                    get_words(half[0], k_page, elements + k_lane0);
+                    get_words(half[1], k_page, elements + k_lane0 + 64);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        raw.k[t][i] = half[i / 4][i % 4];
+                    }
                 } else {
-                    get_words(raw.k[t], k_at + (offset + k_lane0));
+                    get_words(raw.k[t], k_page, elements + k_lane0);
                 }
-                get_words(raw.v[t], v_at + (offset + v_lane));
-                raw.k_byte[t] = (kpool + blocks)[block];
-                raw.v_byte[t] = (vpool + blocks)[block];
+                get_words(raw.v[t], v_page, elements + v_lane);
+                raw.k_byte[t] = __builtin_amdgcn_raw_buffer_load_b8(k_page, block, 0, 0);
+                raw.v_byte[t] = __builtin_amdgcn_raw_buffer_load_b8(v_page, block, 0, 0);
             }
         };
 
@@ -262,13 +263,11 @@ struct MxFewTile {
         MxQuery<T, D, BITS> query;
         query.load(a.q + static_cast<int64_t>(s.first + column / G) * a.q_stride + (g * G + column % G) * D, q);
         Raw raw[kDepth];
-        if (unit < u_end) {
-            look(unit);
-            fetch(unit, raw[0]);
-            if (unit + 4 < u_end) {
-                fetch(unit + 4, raw[1]);
-            }
-        }
+        look(unit);
+        fetch(unit, raw[0]);
+        asm volatile("" ::: "memory");  // (asked for in this order and before the query's parts)
+        fetch(unit + 4, raw[1]);
+        asm volatile("" ::: "memory");
         query.form(q);
         floatx4 acc[D / 16];
 #pragma unroll
@@ -296,9 +295,7 @@ struct MxFewTile {
                         mx_unpack8<T, BITS>(now.v[t] + i * (BITS / 4), power);
                 }
             }
-            if (unit + 4 * kDepth < u_end) {
-                fetch(unit + 4 * kDepth, now);
-            }
+            fetch(unit + 4 * kDepth, now);
             // sc[t][i]: key 16 t + 4 q + i of the unit
             if (unit * kUnit + kUnit > first_pos + 1) {
                 const int rel = pos - unit * kUnit - 4 * q;
@@ -360,14 +357,16 @@ struct MxFewTile {
                 acc[i] = mfma16(T{}, vt, pl, acc[i]);
             }
         };
-        while (unit < u_end) {
+        // (no way out between the two, which would come back to the first as far as the counts of
+        // loads on their way are concerned)
+        while (unit + 4 < u_end) {
             step(raw[0]);
             unit += 4;
-            if (unit >= u_end) {
-                break;
-            }
             step(raw[1]);
             unit += 4;
+        }
+        if (unit < u_end) {
+            step(raw[0]);
         }
         join_waves<T, D, MxRow<T, D, BITS>>(a, s, table, g, c0, count, begin * kRound, u_end * kUnit, split, splits, acc, m_run,
                                             l_run, bad, s_mem, s_ml, s_redo);
