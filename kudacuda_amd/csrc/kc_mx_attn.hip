@@ -405,6 +405,20 @@ __device__ __forceinline__ int block_sum(int (*s_part)[N], int i) {
     return __builtin_amdgcn_readfirstlane(s_part[0][i] + s_part[1][i] + s_part[2][i] + s_part[3][i]);
 }
 
+// Of a batch's pieces: candidates for the longest's rounds, from an even share of all on in
+// steps to where every tile may have a short last piece.
+constexpr int kTries = 4;
+__device__ __forceinline__ int least_piece(int rounds, int tiles, int most, int splits, int& step) {
+    const int at_once = static_cast<int>(kFewAtOnce);
+    const int spare = at_once - tiles > at_once / 4 ? at_once - tiles : at_once / 4;
+    int least = (rounds + at_once - 1) / at_once;
+    const int allowed = (most + splits - 1) / splits;
+    least = least > allowed ? least : allowed;
+    const int enough = (rounds + spare - 1) / spare;
+    step = enough > least ? (enough - least + kTries - 2) / (kTries - 1) : 1;
+    return least;
+}
+
 // ceil(n / d) for n < 2^23: the quotient of the nearest floats is at most one off.
 __device__ __forceinline__ int parts_of(int n, int d) {
     const int up = n + d - 1;
@@ -417,7 +431,6 @@ template <typename T, int D, int BITS>
 __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, int splits, int few_rows) {
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kUnit * D * 2];
     __shared__ float s_ml[4][16][2];
-    constexpr int kTries = 4;
     __shared__ int s_total[4][2], s_most[4], s_tries[4][kTries];
     __shared__ int s_found[6];
     __shared__ int s_redo;
@@ -442,6 +455,40 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
         const int parts = share < 1 ? 1 : (share < splits ? share : splits);
         longest = (line.rounds + parts - 1) / parts;
         pieces = pieces_of(line, longest);
+    } else if (sequences <= 64) {
+        // a lane a sequence, in every wave alike: no wave waits for another
+        const int lane = tid & 63;
+        const auto add = [](int x, int y) { return x + y; };
+        const auto last = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(v, 63); };
+        Line line = {};
+        bool descending = false;
+        if (lane < sequences) {
+            own = sequence(a, lane);
+            descending = a.starts[lane + 1] < a.starts[lane];
+            line = line_of(a, own, few_rows, splits);
+        }
+        const int rounds = last(wave_scan(length_of(a, line), add));
+        const int tiles = last(wave_scan(kv_heads * line.tiles, add));
+        const int most = last(wave_scan(line.tiles > 0 && line.rounds > 1 ? line.rounds : 1, [](int x, int y) { return x > y ? x : y; }));
+        if (__any(descending) || rounds == 0) {
+            return;
+        }
+        int step;
+        const int least = least_piece(rounds, tiles, most, splits, step);
+        longest = 0;
+        pieces = 0;
+#pragma unroll
+        for (int t = kTries - 1; t >= 0; --t) {
+            const int mine = pieces_of(line, least + t * step);
+            const int after = wave_scan(mine, add);
+            const int sum = last(after);
+            if (sum <= static_cast<int>(kFewAtOnce) || t == kTries - 1) {
+                longest = least + t * step;
+                pieces = sum;
+                own_pieces = mine;
+                before = after - mine;
+            }
+        }
     } else {
         const int run_end = run + per_thread < sequences ? run + per_thread : sequences;
         Line line = {};
@@ -467,15 +514,8 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
         if (most == 0x7fffffff || total[0] == 0) {
             return;
         }
-        // candidates from an even share of the rounds on, to where every tile may have a
-        // short last piece
-        const int at_once = static_cast<int>(kFewAtOnce);
-        const int spare = at_once - total[1] > at_once / 4 ? at_once - total[1] : at_once / 4;
-        int least = (total[0] + at_once - 1) / at_once;
-        const int allowed = (most + splits - 1) / splits;
-        least = least > allowed ? least : allowed;
-        const int enough = (total[0] + spare - 1) / spare;
-        const int step = enough > least ? (enough - least + kTries - 2) / (kTries - 1) : 1;
+        int step;
+        const int least = least_piece(total[0], total[1], most, splits, step);
         int tries[kTries] = {};
         for (int i = run; i < run_end; ++i) {
             if (per_thread > 1) {
@@ -497,7 +537,7 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
 #pragma unroll
         for (int t = kTries - 1; t >= 0; --t) {
             const int sum = block_sum(s_tries, t);
-            if (sum <= at_once || t == kTries - 1) {  // (more tiles than fit at once: the last)
+            if (sum <= static_cast<int>(kFewAtOnce) || t == kTries - 1) {  // (more tiles than fit at once: the last)
                 longest = least + t * step;
                 pieces = sum;
                 own_pieces = mine[t];
@@ -515,7 +555,15 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
     int index = 0;
     int first = 0;  // the first piece of the sequence
     Sequence s = own;
-    if (sequences > 1) {
+    if (sequences > 1 && sequences <= 64) {
+        const uint64_t found = __ballot(before <= piece && piece < before + own_pieces);
+        index = __builtin_amdgcn_readfirstlane(__builtin_ctzll(found));  // (pieces are all somebody's)
+        first = __builtin_amdgcn_readlane(before, index);
+        s.first = __builtin_amdgcn_readlane(own.first, index);
+        s.q_len = __builtin_amdgcn_readlane(own.q_len, index);
+        s.kv_len = __builtin_amdgcn_readlane(own.kv_len, index);
+        s.bad = __builtin_amdgcn_readlane(static_cast<int>(own.bad), index) != 0;
+    } else if (sequences > 1) {
         // the thread whose sequences the piece is of tells which
         if (before <= piece && piece < before + own_pieces) {
             int i = run;
