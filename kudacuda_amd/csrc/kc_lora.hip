@@ -254,8 +254,16 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
     const bool one = pieces <= 2;
     const int half = one ? 2 : (pieces + 3) / 4 * 4;
     const int factors = t.rank > 0 ? (pieces + 3) / 4 : 0;
-    const uint16_t* const factor = a.b + static_cast<int64_t>(t.adapter < 0 ? 0 : t.adapter) * a.max_rank * a.out_features;
     const int out = static_cast<int>(a.out_features);
+    // Loads without conditions, which would be waited for all together: a factor's rows are a
+    // buffer of their bytes (past it and for pieces that are none a load reads nothing), and
+    // base rows that are none are read from another (base is output where there is none).
+    const uint16_t* const rows_b = a.b + static_cast<int64_t>(t.adapter < 0 ? 0 : t.adapter) * a.max_rank * a.out_features;
+    const int row_bytes = 16 * pieces;
+    const __amdgpu_buffer_rsrc_t factor =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(rows_b), 0, out * row_bytes, 0x00027000);
+    const uint16_t* const base_rows = a.base != nullptr ? a.base : a.out;
+    const int64_t base_stride = a.base != nullptr ? a.base_stride : a.out_stride;
     const float scale = t.rank > 0 ? a.scales[t.adapter] : 0.0f;
     int rows[SUBS];
 #pragma unroll
@@ -269,14 +277,11 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int o = o0 + 32 * (i >> 1) + 8 * (r >> 2) + 4 * (i & 1) + (r & 3);
-            const uint16_t* const brow = factor + static_cast<int64_t>(o < out ? o : out - 1) * (8 * pieces);
 #pragma unroll
             for (int f = 0; f < kFactors; ++f) {
                 const int piece = one ? q & 1 : 4 * f + q;
-                bv[set][f][i] = make_uint4(0, 0, 0, 0);
-                if (piece < pieces) {
-                    bv[set][f][i] = *reinterpret_cast<const uint4*>(brow + 8 * piece);
-                }
+                bv[set][f][i] = __builtin_bit_cast(
+                    uint4, __builtin_amdgcn_raw_buffer_load_b128(factor, piece < pieces ? o * row_bytes + 16 * piece : 0x7ffffff0, 0, 0));
             }
         }
 #pragma unroll
@@ -284,10 +289,8 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int o = o0 + 32 * h + 8 * q;
-                base[set][s][h] = make_uint4(0, 0, 0, 0);
-                if (a.base != nullptr && rows[s] >= 0 && o < out) {
-                    base[set][s][h] = *reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(rows[s]) * a.base_stride + o);
-                }
+                base[set][s][h] = *reinterpret_cast<const uint4*>(base_rows + static_cast<int64_t>(rows[s] < 0 ? 0 : rows[s]) * base_stride +
+                                                                  (o < out ? o : 0));
             }
         }
     };
@@ -428,8 +431,10 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
             for (int h = 0; h < 2; ++h) {
                 const int o = o0 + 32 * h + 8 * q;
                 if (o < out) {
-                    float v[8];
-                    unpack8<T>(base[set][s][h], v);
+                    float v[8] = {};
+                    if (a.base != nullptr) {
+                        unpack8<T>(base[set][s][h], v);
+                    }
                     if (t.rank > 0) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
@@ -442,29 +447,32 @@ __device__ __forceinline__ void outer_tile(const LoraArgs& a, const Tile& t, int
             }
         }
     };
-    // (a group past the end requests the last factors again)
     int o0 = column0 + wave * 64;
-    for (int n = 0; n < groups; n += kSets) {
-        if constexpr (kSets == 2) {
+    if constexpr (kSets == 2) {
+        // (a group past the block's last asks for none)
+        int n = 0;
+        for (; n + 1 < groups; n += 2) {
             request(1, o0 + 256);
+            multiply(0, o0);
+            request(0, n + 2 < groups ? o0 + 512 : out);
+            multiply(1, o0 + 256);
+            o0 += 512;
         }
+        if (n < groups) {
+            multiply(0, o0);
+        }
+    } else {
         multiply(0, o0);
-        o0 += 256;
-        if (n + 1 >= groups) {
-            break;
-        }
-        if constexpr (kSets == 2) {
-            request(0, o0 + 256);
-            multiply(1, o0);
+        for (int n = 1; n < groups; ++n) {
             o0 += 256;
-        } else {
             request(0, o0);
+            multiply(0, o0);
         }
     }
 }
 
 template <typename T, int RT, int SUBS, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void lora_outer_kernel(LoraArgs a, int splits, int blocks, int groups) {
+__global__ __launch_bounds__(kThreads, SUBS == 1 && !WHOLE ? 3 : 2) void lora_outer_kernel(LoraArgs a, int splits, int blocks, int groups) {
     __shared__ __attribute__((aligned(16))) uint8_t s_u[WHOLE ? 4 * 16 * (RT * 16 + 4) * 4 : 16];
     __shared__ __attribute__((aligned(16))) uint8_t s_row[16 * SUBS * (RT * 64 + 16)];
     __shared__ float s_factor[16 * SUBS];
