@@ -59,6 +59,9 @@ def _check(batch, out, rows=None):
     ([2048], [2100], 32, 32, 16),
     ([40, 0, 7, 100] * 70, [41, 5, 30, 100] * 70, 2, 2, 16),
     ([1] * 300, list(range(1, 301)), 4, 2, 16),
+    # as many sequences as a wave has lanes, and one more
+    ([1, 2, 0, 1] * 16, [(i * 37) % 900 for i in range(64)], 8, 2, 16),
+    ([1, 2, 0, 1] * 16 + [3], [(i * 37) % 900 for i in range(64)] + [1500], 8, 2, 16),
     # one tile a KV head: more than 64 splits, splits that even out lengths, with empty ones among them
     ([4], [20000], 16, 2, 16),
     ([1, 1], [30000, 31], 32, 1, 64),
