@@ -388,9 +388,7 @@ KUDACUDA_API int kudacuda_paged_read_mx(void* handle, uint64_t key_pages, uint64
 
 /* kudacuda_paged_attention over such a cache: the same rows, masks, sums and workspace
  * rules, on the numbers that the cache holds (kudacuda_paged_read_mx with the same dtype);
- * a row that sees a NaN block is NaN where that block weighs in.  (In heads of 128, where a
- * sequence has at most 32 rows a KV head, the query meets the keys in parts of 4 bits: exact
- * but for what lies below 2^-21 (bf16) or 2^-25 (fp16) of the largest of 32 dims.) */
+ * a row that sees a NaN block is NaN where that block weighs in. */
 KUDACUDA_API int kudacuda_paged_attention_mx(void* handle, uint64_t query, uint64_t key_pages, uint64_t value_pages,
                                              uint64_t page_table, uint64_t query_starts, uint64_t kv_lens,
                                              uint64_t output, uint64_t workspace, int64_t workspace_bytes, int64_t dtype,

@@ -39,51 +39,22 @@ struct MxRow {
 
 // ------------------------------------------------------------------ few rows
 // The two tiles of 16 keys that a wave takes next: their rows lie in one page each, whose
-// place is the wave's; K straight into the first product's operand, V through LDS.
+// place is the wave's; K unpacked into the first product's operand, V through LDS.
 //
-// Heads of 128 meet K as it is stored: the scaled matrix instruction takes a row of 128
-// elements with its four blocks' bytes, and the query as e4m3 numbers in PARTS parts with a
-// power of two a block -- 4 bits each, so that two parts are a bf16 query exactly and
-// three an fp16 one, down to 2^-21 and 2^-25 of the largest of a block's 32 dims.  Unpacking
-// K costs more than that in vector instructions, and these are what bounds the kernel
-// beside memory.  Heads of 64 would leave half of the instruction empty: they unpack K.
-typedef int intx8 __attribute__((ext_vector_type(8)));
-
-// The exponent that makes the largest of a block 128 .. 255.
-__device__ __forceinline__ int query_exponent(float most) {
-    const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127 - 7;
-    return e > -110 ? (e < 120 ? e : 120) : -110;
-}
-// Four numbers' e4m3 parts of this exponent; what is left of the numbers stays.
-__device__ __forceinline__ int query_part(float* x, int exponent) {
-    typedef short shortx2 __attribute__((ext_vector_type(2)));
-    typedef float floatx2 __attribute__((ext_vector_type(2)));
-    const float power = __uint_as_float(static_cast<uint32_t>(exponent + 127) << 23);
-    shortx2 w = {0, 0};
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[0], x[1], power, false);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[2], x[3], power, true);
-    const int word = __builtin_bit_cast(int, w);
-    const floatx2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, power, false);
-    const floatx2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, power, true);
-    x[0] -= lo[0];
-    x[1] -= lo[1];
-    x[2] -= hi[0];
-    x[3] -= hi[1];
-    return word;
-}
-
+// (The scaled matrix instructions would meet K as it is stored, the query as e4m3 numbers
+// in parts, and save the unpacking.  But they align the products of neighbouring dims to
+// the largest of them and drop what lies below 2^-13 of it, where the 16-bit instructions
+// keep 2^-23: small dims beside large ones vanish.)
 template <typename T, int D, int BITS>
-struct MxQuery {  // heads of 64
+struct MxQuery {
     static constexpr int kSteps = D / 32;
     uint4 part[kSteps];
-    static __device__ __forceinline__ int key_offset(int q, int i) { return (D / 4 * q + 16 * i) * BITS / 8; }
     __device__ __forceinline__ void load(const uint16_t* row, int q) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             part[i] = *reinterpret_cast<const uint4*>(row + D / 4 * q + 8 * i);
         }
     }
-    __device__ __forceinline__ void form(int) {}
     template <int WORDS>
     __device__ __forceinline__ floatx4 scores(const uint32_t (&key)[WORDS], uint32_t byte) const {
         floatx4 sc = floatx4{};
@@ -91,74 +62,6 @@ struct MxQuery {  // heads of 64
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             sc = mfma16(T{}, mx_unpack8<T, BITS>(key + i * (BITS / 4), power), part[i], sc);
-        }
-        return sc;
-    }
-};
-
-template <typename T, int BITS>
-struct MxQuery<T, 128, BITS> {
-    static constexpr int kParts = std::is_same<T, Bf16>::value ? 2 : 3;
-    intx8 part[kParts];
-    int byte[kParts];
-    // 8 bits: the instruction's lane q has dims 16 q .. and 64 + 16 q .., 4 bits: 32 q ..
-    static __device__ __forceinline__ int key_offset(int q, int i) { return BITS == 4 ? 16 * q : 16 * q + 64 * i; }
-    uint4 raw[4];
-    __device__ __forceinline__ void load(const uint16_t* row, int q) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            raw[i] = *reinterpret_cast<const uint4*>(row + 64 * (i / 2) + 16 * q + 8 * (i % 2));
-        }
-    }
-    __device__ __forceinline__ void form(int q) {
-        float x[2][16];
-        int e[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float half[8];
-            unpack8<T>(raw[2 * h], half);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[h][i] = half[i];
-            }
-            unpack8<T>(raw[2 * h + 1], half);
-            float most = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[h][8 + i] = half[i];
-                most = fmaxf(most, fmaxf(fabsf(x[h][i]), fabsf(half[i])));
-            }
-            most = fmaxf(most, __shfl_xor(most, 16, 64));  // a block is two lanes' halves
-            e[h] = query_exponent(most);
-        }
-        const int lane = static_cast<int>(threadIdx.x) & 15;
-        const int low_block = __shfl(e[0], lane + (q == 1 ? 32 : 0), 64);
-        const int high_block = __shfl(e[1], lane + (q == 3 ? 48 : 0), 64);
-        const int block = q < 2 ? low_block : high_block;
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-            byte[p] = block - 4 * p + 127;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    part[p][4 * h + i] = query_part(x[h] + 4 * i, e[h] - 4 * p);
-                }
-            }
-        }
-    }
-    template <int WORDS>
-    __device__ __forceinline__ floatx4 scores(const uint32_t (&key)[WORDS], uint32_t power) const {
-        intx8 k;  // (of 4 bits the first half is read)
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            k[i] = static_cast<int>(key[i]);
-        }
-        floatx4 sc = floatx4{};
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-            sc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, part[p], sc, BITS == 4 ? 4 : 0, 0, 0,
-                                                                  static_cast<int>(power), 0, byte[p]);
         }
         return sc;
     }
@@ -215,8 +118,7 @@ struct MxFewTile {
             asm volatile("" : "+v"(pages));  // (waited for here, once in 32 units, not wherever it is read)
             pages_from = u;
         };
-        const int k_lane0 = MxQuery<T, D, BITS>::key_offset(q, 0);
-        const int v_lane = q * (kRowBytes / 4);
+        const int lane_bytes = q * (kRowBytes / 4);
         const int b_lane = q * (D / 4) / kMxBlock;
         const uint8_t* const kpool = reinterpret_cast<const uint8_t*>(a.k);
         const uint8_t* const vpool = reinterpret_cast<const uint8_t*>(a.v);
@@ -242,18 +144,8 @@ struct MxFewTile {
                 const int first = head + (key & page_mask) + row;
                 const int elements = first * kRowBytes;
                 const int block = static_cast<int>(a.block_offset) + first * (D / kMxBlock) + b_lane;
-                if constexpr (D == 128 && BITS == 8) {
-                    uint32_t half[2][4];
-                    get_words(half[0], k_page, elements + k_lane0);
-                    get_words(half[1], k_page, elements + k_lane0 + 64);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        raw.k[t][i] = half[i / 4][i % 4];
-                    }
-                } else {
-                    get_words(raw.k[t], k_page, elements + k_lane0);
-                }
-                get_words(raw.v[t], v_page, elements + v_lane);
+                get_words(raw.k[t], k_page, elements + lane_bytes);
+                get_words(raw.v[t], v_page, elements + lane_bytes);
                 raw.k_byte[t] = __builtin_amdgcn_raw_buffer_load_b8(k_page, block, 0, 0);
                 raw.v_byte[t] = __builtin_amdgcn_raw_buffer_load_b8(v_page, block, 0, 0);
             }
@@ -265,10 +157,8 @@ struct MxFewTile {
         Raw raw[kDepth];
         look(unit);
         fetch(unit, raw[0]);
-        asm volatile("" ::: "memory");  // (asked for in this order and before the query's parts)
+        asm volatile("" ::: "memory");  // (asked for in this order)
         fetch(unit + 4, raw[1]);
-        asm volatile("" ::: "memory");
-        query.form(q);
         floatx4 acc[D / 16];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -378,7 +268,7 @@ struct MxFewTile {
 // the least number for which the pieces of the batch fit on the chip at once.  (Blocks of
 // equal stretches of all sequences' rounds, as over 16-bit rows, end together, but most of
 // them then begin and end two pieces, and what a piece costs beside its rows -- places
-// found one after the other, a query's parts, the waves' meeting -- is as long as two or
+// found one after the other, the query, the waves' meeting -- is as long as two or
 // three rounds here.)  Bound by memory once rows flow: a round more on 512 blocks of heads of
 // 128 in 4 bits is 1.5 us, 5.8 TB/s; beside it 7 us of launch, places, query and meeting.  64
 // sequences of up to 8192 keys, 82 MB, 21.7 us; 120000 keys of one in 8 bits, 63 MB, 16.5.
@@ -623,8 +513,8 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
 // arithmetic and LDS are each about as busy there, and unpacking adds to two of them: a
 // prompt of 8192 tokens takes 279 to 285 us, 980 TFLOP/s, 7 % longer than over 16-bit rows.  (Measured instead: the
 // same behind the barrier, a window later, 5 % slower; K kept packed, its products by scaled
-// instructions with the query in parts, as above for few rows, 1 % faster in bf16 heads of
-// 128 in 4 bits, 2 % slower in 8, 9 % in fp16, with three parts, and 18 % in heads of 64.)
+// instructions, whose sums are coarse as told above, 1 % faster in bf16 heads of
+// 128 in 4 bits, 2 % slower in 8, 9 % in fp16 and 18 % in heads of 64.)
 template <typename T, int D, int BITS>
 struct MxWindow {
     using Rows = MxRow<T, D, BITS>;
