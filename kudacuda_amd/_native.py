@@ -120,6 +120,7 @@ class Native:
     def __init__(self, device_id: int = 0, lib: ctypes.CDLL | None = None) -> None:
         self.lib = lib or load_library()
         self.device_id = int(device_id)
+        self.workspaces: dict[Any, Any] = {}  # scratch that the handle's callers share, by use and stream
         self.handle = self.lib.kudacuda_create(self.device_id)
         if not self.handle:
             raise NativeError("kudacuda_create returned a null handle")
@@ -140,6 +141,7 @@ class Native:
         if self.handle:
             self.lib.kudacuda_destroy(self.handle)
             self.handle = None
+            self.workspaces.clear()
 
     def __del__(self) -> None:
         try:

@@ -85,7 +85,6 @@ class LoraAdapters:
         self.ranks = torch.zeros(adapters, dtype=torch.int32, device=device)
         self.scales = torch.zeros(adapters, dtype=torch.float32, device=device)
         self.device = self.a.device  # with its number, whichever device is current later
-        self._workspaces: dict[Any, Any] = {}
 
     def _index(self, index: int) -> int:
         if not 0 <= index < self.count:
@@ -148,13 +147,14 @@ class LoraAdapters:
                 rows.record_stream(stream)
         nbytes = self.native.lib.kudacuda_lora_workspace_bytes(batch.tokens, batch.tile_count, self.max_rank,
                                                                self.in_features)
-        # a workspace a stream: calls on one stream follow one another; a captured call
-        # gets its own, from its graph's memory
-        workspace = None if capturing else self._workspaces.get(stream.cuda_stream)
+        # a workspace a stream for all adapters of the handle: calls on one stream follow one
+        # another; a captured call gets its own, from its graph's memory
+        shared, use = self.native.workspaces, ("adapters", stream.cuda_stream)
+        workspace = None if capturing else shared.get(use)
         if workspace is None or workspace.numel() < nbytes:
             workspace = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
             if not capturing:
-                self._workspaces[stream.cuda_stream] = workspace
+                shared[use] = workspace
         self.native.call("kudacuda_lora_add", x.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.ranks.data_ptr(),
                          self.scales.data_ptr(), batch.order.data_ptr(), batch.tiles.data_ptr(), base.data_ptr(),
                          out.data_ptr(), workspace.data_ptr(), nbytes, 1 if self.dtype == self.torch.bfloat16 else 2,
