@@ -359,7 +359,7 @@ KUDACUDA_API int64_t kudacuda_paged_attention_workspace_bytes(int64_t tokens, in
  * head_dim / 32], 127 + the exponent, 255 for NaN; page p begins page_stride * p BYTES
  * into the pool.  What a page of zero bytes holds is zeros.  copy_pages copies such pages.
  * Contract: head_dim 64 or 128, page_size a power of two, 16..4096, kv_heads 1..1024,
- * pools and page_stride on 16-byte boundaries.
+ * pools and page_stride on 16-byte boundaries, page_stride below 2^31.
  *
  * kudacuda_rope_paged_append_mx is kudacuda_rope_paged_append into such pages: a key row is
  * turned (in 64 bits) and rounded to the type, then it and the value row are rounded to

@@ -929,8 +929,11 @@ int64_t mx_elements(Handle* h, const char* symbol, int64_t bits, int64_t kv_head
         return no("kv_heads 1..1024, num_pages>=1 and a page_size that is a power of two, 16..4096");
     }
     const int64_t elements = kv_heads * page_size * head_dim * bits / 8;
+    if (page_stride > kInt32Max) {
+        return no("a page_stride below 2^31 bytes");
+    }
     if (page_stride < elements + kv_heads * page_size * (head_dim / 32) || page_stride % 16 != 0 ||
-        page_stride > kInt32Max || ((key_pages | value_pages) & 15) != 0) {
+        ((key_pages | value_pages) & 15) != 0) {
         return no("pages on 16-byte boundaries and a page_stride of at least kv_heads * page_size * "
                   "(head_dim * bits / 8 + head_dim / 32) bytes");
     }
