@@ -419,8 +419,8 @@ struct MxReadArgs {
 };
 hipError_t launch_mx_read(Act act, const MxReadArgs& args, hipStream_t stream);
 
-// Attention over such a cache: of the arguments, k and v are its pools, page_stride,
-// head_stride and token_stride the bytes between pages, heads and tokens of elements.
+// Attention over such a cache: of the arguments, k and v are its pools, page_stride the
+// bytes between pages; head_stride and token_stride are not used.
 PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_query_len, int64_t max_kv_len,
                                 int64_t max_keys, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                 int64_t workspace_bytes);

@@ -2089,8 +2089,6 @@ int kudacuda_paged_attention_mx(void* raw, uint64_t query, uint64_t key_pages, u
     a.num_pages = num_pages;
     a.table_stride = table_stride;
     a.page_stride = page_stride;
-    a.token_stride = head_dim * bits / 8;
-    a.head_stride = page_size * a.token_stride;
     a.block_offset = elements;
     a.page_shift = shift;
     a.scale_log2 = scale * kc::kLog2e;
