@@ -34,11 +34,16 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kStep = 32;            // of the inner axis, a matrix instruction
 constexpr int kBlockStep = 4 * kStep;  // of the four waves
+// Tiles of 16 rows on average or fewer have kernels for 16 rows at a time (calls with 64
+// adapters, 2048 -> 11008: a row each of ranks 8 to 64 20.1 us, with room for 64 rows 26.9;
+// 16 rows each of rank 16 18.4 and 22.6).
+inline bool few_rows(int64_t tokens, int64_t tile_count) { return tokens <= 16 * tile_count; }
 // Blocks of the first launch that tiles are split into.  More shorten it and lengthen the
-// second, which sums the shares in each of its blocks: the 8 chunks above 19.3 + 11.7 us with
-// 256, 18.5 + 13.7 with 512, 15.8 + 16.9 with 1024; 4 chunks of 2000, rank 64, 66 + 31, 62 +
-// 35, 61 + 42.
-constexpr int64_t kBlocks = 512;
+// second, which sums the shares in each of its blocks.  Calls with 256, 512 and 1024, us,
+// 11008 -> 2048: few rows a tile, 64 adapters of a row, ranks 8 to 64, 24.2, 21.6, 23.3, 16 of
+// rank 64 14.6, 15.1, 15.3; more rows, the 8 chunks above 29.3, 30.5, 32.2, 16 chunks of 100,
+// rank 32, 22.4, 25.1, 27.1, 4 of 700, rank 128, 68, 74, 90, 4 of 2000, rank 64, 97, 94, 101.
+inline int64_t inner_blocks(int64_t tokens, int64_t tile_count) { return few_rows(tokens, tile_count) ? 512 : 256; }
 
 __device__ __forceinline__ floatx4 mfma16(Bf16, uint4 a, uint4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -498,7 +503,7 @@ hipError_t launch_outer(const LoraArgs& a, const LoraPlan& plan, hipStream_t str
     // group 25.9 us, four 29.
     constexpr int kSets = outer_sets(RT, SUBS);
     const int64_t columns = (a.out_features + 255) / 256;
-    int64_t groups = a.tile_count * columns / (kSets == 2 ? 640 : 4 * kBlocks);
+    int64_t groups = a.tile_count * columns / (kSets == 2 ? 640 : 2048);
     groups = groups < 2 ? 1 : (groups < 16 ? groups / kSets * kSets : 16);
     const int64_t blocks = (columns + groups - 1) / groups;
     hipLaunchKernelGGL((lora_outer_kernel<T, RT, SUBS, WHOLE>), dim3(static_cast<unsigned>(a.tile_count * blocks)),
@@ -536,9 +541,7 @@ hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
 
 template <typename T>
 hipError_t launch(const LoraArgs& a, const LoraPlan& plan, hipStream_t stream) {
-    // tiles of 16 rows on average or fewer: kernels for 16 rows at a time (64 adapters of one
-    // row each 17 us in the second kernel; with room for 64 rows 28)
-    return a.tokens <= 16 * a.tile_count ? launch<T, 1>(a, plan, stream) : launch<T, kLoraTile / 16>(a, plan, stream);
+    return few_rows(a.tokens, a.tile_count) ? launch<T, 1>(a, plan, stream) : launch<T, kLoraTile / 16>(a, plan, stream);
 }
 
 }  // namespace
@@ -547,7 +550,7 @@ LoraPlan lora_plan(int64_t tokens, int64_t tile_count, int64_t max_rank, int64_t
     LoraPlan p;
     p.pitch = (max_rank + 15) / 16 * 16;
     const int64_t steps = (in_features + kBlockStep - 1) / kBlockStep;
-    const int64_t wanted = tile_count > 0 ? kBlocks / tile_count : 1;
+    const int64_t wanted = tile_count > 0 ? inner_blocks(tokens, tile_count) / tile_count : 1;
     // (at least four steps a split: their loads are on their way together)
     const int64_t most = (steps + 3) / 4;
     p.splits = wanted < 1 ? 1 : (wanted < most ? wanted : most);
