@@ -657,8 +657,10 @@ PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_q
     const int64_t windows = (max_kv_len + kWindow - 1) / kWindow;
     const int64_t rounds = (max_kv_len + kRound - 1) / kRound;
     const bool few = rows <= kMxFewRows;
+    int64_t even_splits = 1;  // of tiles, as for 16-bit rows
     if (!few) {
         plan_tiles(p, tokens, sequences, group, rows, windows, kv_heads, head_dim);
+        even_splits = p.tile_splits;
         // Tiles of one K-group here are two blocks a CU (heads of 64: three), of two K-groups one
         // (kc_paged_attn.hip's are two of heads of 64).  So sequences of one tile each, whose
         // lengths splits even out, take one group where there are blocks enough for it (heads of
@@ -668,7 +670,9 @@ PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_q
         // heads of 128, 16 over 2: 1200 after 2000 62 and 51, 2500 after 3000 138 and 129).
         // Shorter and fewer ones would lose by the merge what they gain: 3 chunks of 800 after
         // 1000 27 (heads of 128 60) and 36 (64), 1200 of heads of 64 after 2000 31 and 34, whole
-        // prompts likewise.
+        // prompts likewise.  (The longest past may be another sequence's than the longest chunk:
+        // a whole prompt of 2000 beside a token after 6000 63 us so and 71 with two groups, beside
+        // 8 after up to 8000 59 and 63; 1500 of heads of 64 beside 8 36 and 36.)
         const int64_t tiles = p.slots * kv_heads;
         if (sequences > 1 && rows <= kTileRows) {
             p.tile_groups = tiles * p.tile_splits > 256 ? 1 : p.tile_groups;
@@ -678,8 +682,13 @@ PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_q
             p.tile_splits = head_dim == 64 ? (511 + tiles) / tiles : (tiles <= 256 ? 512 : 1024) / tiles;
         }
     }
+    // Beside longer sequences few rows go to their kernel where a tile would take more than 50
+    // windows, of the splits that even out lengths: those of the chunks above are no help to a
+    // token that is one of them (2000 beside a token after 6000 63 us, in tiles 87; 1500 of heads
+    // of 64 beside 8 after up to 8000 36 and 56; but 2000 after 3000 beside 16 after up to 4000
+    // 115 and 103).
     int64_t few_splits = 0;
-    if (few || (tokens != sequences * longest && windows > 50 * p.tile_splits)) {
+    if (few || (tokens != sequences * longest && windows > 50 * even_splits)) {
         // Where no other sequence is split: up to 5 rounds in one piece (a token over 512
         // keys 9.1 us so, 10.7 split and merged; over 768 11.2 and 10.7).
         const int64_t tiles = sequences * kv_heads * ((cap(rows, kMxFewRows) + 15) / 16);
