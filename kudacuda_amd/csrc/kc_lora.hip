@@ -4,9 +4,9 @@
 // the rows: a tile is up to 64 rows of one adapter.
 //
 // Two launches (one where both are small), bound by bytes: the adapters' factors where rows are few (64 adapters of a
-// row each, 2048 -> 11008, ranks 8 to 64, 53 MB: 7.0 + 14.3 us, 2.5 TB/s), else the inputs,
-// the base rows and the results (2000 rows of one adapter, 2048 -> 11008, 96 MB: 7.5 + 23.8
-// us, 3.1 TB/s; 8 chunks of 2996 rows, 11008 -> 2048, 79 MB: 18.7 + 12.6, 2.5 TB/s); one
+// row each, 2048 -> 11008, ranks 8 to 64, 53 MB: 7.0 + 14.4 us, 2.5 TB/s), else the inputs,
+// the base rows and the results (2000 rows of one adapter of rank 16, 2048 -> 11008, 97 MB:
+// 7.6 + 23.1 us, 3.2 TB/s; 8 chunks of 2996 rows, 11008 -> 2048, 79 MB: 19.9 + 10.4, 2.6 TB/s); one
 // row is latency: 6.7 us, places, two products and their sums one after the other.
 //
 // The first forms u = x A^T, a tile's rows by up to 64 ranks a block, over a share of `in`
@@ -499,8 +499,9 @@ hipError_t launch_outer(const LoraArgs& a, const LoraPlan& plan, hipStream_t str
     // first come while others are multiplied: 64 adapters, 64 rows of 11008 outputs, ranks 8
     // to 64 -- two groups 16.1 us, four 14.1, six 16.9, rank 16 alone 9.8, 8.0 and 8.0 (with
     // loads under conditions, waited for all together, four took 16.8 and 11.0); one adapter
-    // and row 4.7 with one.  Tiles of 64 rows are bound by their rows: 2000 rows of 11008 outputs -- one
-    // group 25.9 us, four 29.
+    // and row 4.7 with one.  Tiles of 64 rows are bound by their rows: 2000 rows of
+    // 11008 outputs -- one group 25.9 us, four 29 (with twice the shares that the first launch
+    // makes now: one 23.1).
     constexpr int kSets = outer_sets(RT, SUBS);
     const int64_t columns = (a.out_features + 255) / 256;
     int64_t groups = a.tile_count * columns / (kSets == 2 ? 640 : 2048);

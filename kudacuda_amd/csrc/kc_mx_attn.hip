@@ -270,8 +270,9 @@ struct MxFewTile {
 // them then begin and end two pieces, and what a piece costs beside its rows -- places
 // found one after the other, the query, the waves' meeting -- is as long as two or
 // three rounds here.)  Bound by memory once rows flow: a round more on 512 blocks of heads of
-// 128 in 4 bits is 1.5 us, 5.8 TB/s; beside it 7 us of launch, places, query and meeting.  64
-// sequences of up to 8192 keys, 82 MB, 21.7 us; 120000 keys of one in 8 bits, 63 MB, 16.5.
+// 128 in 4 bits is 1.6 us, 5.4 TB/s; beside it 7 us of launch, places, query and meeting.  64
+// sequences of up to 8192 keys, 82 MB, 23.5 us, of heads of 64, 41 MB, 18.2; 120000 keys of one
+// in 8 bits, 63 MB, 16.9.
 constexpr int64_t kFewAtOnce = 512;  // two blocks a CU
 constexpr int kMxFewRows = 32;
 
@@ -511,10 +512,12 @@ __global__ __launch_bounds__(kThreads, 2) void mx_few_kernel(PagedAttnArgs a, in
 // both (D = 64: lanes 0 .. 31 K's, the others V's).  V's rows are dealt so that 16 lanes'
 // stores, and the transposed reads of 4 rows, lie in different banks.  The products, the
 // arithmetic and LDS are each about as busy there, and unpacking adds to two of them: a
-// prompt of 8192 tokens takes 279 to 285 us, 980 TFLOP/s, 7 % longer than over 16-bit rows.  (Measured instead: the
-// same behind the barrier, a window later, 5 % slower; K kept packed, its products by scaled
-// instructions, whose sums are coarse as told above, 1 % faster in bf16 heads of
-// 128 in 4 bits, 2 % slower in 8, 9 % in fp16 and 18 % in heads of 64.)
+// prompt of 8192 tokens takes 283 us in 4 bits and 291 in 8, 970 and 945 TFLOP/s, where it
+// takes 279 over 16-bit rows.  In 8 bits the rows' words do not fit beside the rest: 2 to 10
+// registers a lane are spilled, in heads of 128 and in heads of 64 with one K-group; none in
+// 4 bits.  (Measured instead: the same behind the barrier, a window later, 5 % slower; K kept
+// packed, its products by scaled instructions, whose sums are coarse as told above, 1 % faster
+// in bf16 heads of 128 in 4 bits, 2 % slower in 8, 9 % in fp16 and 18 % in heads of 64.)
 template <typename T, int D, int BITS>
 struct MxWindow {
     using Rows = MxRow<T, D, BITS>;
@@ -689,8 +692,9 @@ PagedAttnPlan mx_attention_plan(int64_t tokens, int64_t sequences, int64_t max_q
     // 115 and 103).
     int64_t few_splits = 0;
     if (few || (tokens != sequences * longest && windows > 50 * even_splits)) {
-        // Where no other sequence is split: up to 5 rounds in one piece (a token over 512
-        // keys 9.1 us so, 10.7 split and merged; over 768 11.2 and 10.7).
+        // Where no other sequence is split: up to 5 rounds in one piece (a call of a token over
+        // 640 keys 10.4 us so, 13.0 split and merged, replayed 8.8 and 7.6; over 768 replayed
+        // 10.0 and 7.6).
         const int64_t tiles = sequences * kv_heads * ((cap(rows, kMxFewRows) + 15) / 16);
         few_splits = p.tile_splits <= 1 && rounds <= 5 ? 1 : cap(2 * ((kFewAtOnce + tiles - 1) / tiles) + 1, cap(rounds, 256));
     }

@@ -8,7 +8,7 @@
 // steps away; the queries' are fp32 as there.
 //
 // Bound by the bytes of the projections' rows: 19999 tokens of 16 and 2 heads of 128 into
-// 8 bits, 216 MB, 41 us, 5.2 TB/s; 8 tokens 4.4 us, a launch and the angles.  Four lanes
+// 8 bits, 195 MB, 41 us, 4.7 TB/s; 8 tokens 4.4 us, a launch and the angles.  Four lanes
 // share a block, 8 dims each: 16 bytes in, 4 or 8 out, the largest magnitude by two
 // exchanges.  A key's lane also loads the 8 dims that its own are paired with.
 #include <type_traits>

@@ -258,7 +258,7 @@ __device__ __forceinline__ void tell_splits(const PagedAttnArgs& a, const Sequen
 // says which): single tokens, bound by the cache's bytes.  All blocks share the cached
 // rows of all sequences evenly: the work is the line of (sequence, KV head, tile of 16
 // rows, round of 128 keys), cut into one stretch a block, so a batch of unequal lengths
-// ends everywhere at once (64 sequences of up to 8192 tokens, 307 MB: 70 us, 4.4 TB/s;
+// ends everywhere at once (64 sequences of up to 8192 tokens, 307 MB: 68 us, 4.5 TB/s;
 // with a fixed number of splits a sequence 88).  A stretch is whole rounds: 9.25 of them
 // a block, as there, are 10 for 474 blocks and none for 38.  In a round the four waves
 // take 32 keys each, K straight from memory into the first product's operand, V through
@@ -400,7 +400,7 @@ __device__ __forceinline__ int wave_scan(int v, Join join) {
 // 346 us at first, 318 with loads that bypass the compiler's waits, 293 with operands
 // read ahead and the maximum allowed to lag, 287 with page bases as scalars, 262 with the
 // waves' priorities and the order of blocks, 266 with the second loop that follows here
-// in one kernel (1035 TFLOP/s; a library product of 8192^3 1405).  Forming the next
+// in one kernel (1035 TFLOP/s; a library product of 8192^3 1405; 257 to 279 over boxes).  Forming the next
 // window's scores between this window's weights (250 VGPRs) took 293.
 //
 // Sequences of at most kFineRows rows a KV head (single tokens, drafts) are one wave's
